@@ -257,6 +257,115 @@ int exl3_finish_and_reduce(const float* raw, const uint16_t* svh, const void* sc
                            int32_t scores_type, int64_t rows, int32_t top_k, int32_t width,
                            void* y, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Between a layer's q/k/v projections and its output projection: rotary
+ * positions, the paged key/value cache, attention over it.  (No counterpart
+ * in the reference's EXL3 operators; its engine has kernels per model.)
+ * ------------------------------------------------------------------------ */
+
+/* What a cache stores: f16 or bf16 values, or 8- or 4-bit codes with one f16
+ * scale per 32 neighbouring channels of a head. */
+typedef enum {
+  EXL3_KV_Q4 = 4,
+  EXL3_KV_Q8 = 8,
+  EXL3_KV_F16 = EXL3_F16,
+  EXL3_KV_BF16 = EXL3_BF16
+} exl3_kv_format;
+
+/* A pool of pages of page_tokens tokens (a power of two, 16 to 1024) of
+ * kv_heads heads of head_dim channels (64, 128 or 256).  Like the other
+ * handles it borrows its buffers, which are 16-byte aligned, keys and values
+ * alike:
+ *   16-bit  [pages][kv_heads][page_tokens][head_dim] f16 or bf16
+ *   8-bit   [pages][kv_heads][page_tokens][head_dim] bytes, code + 128
+ *   4-bit   [pages][kv_heads][page_tokens][head_dim / 2] bytes, code + 8, the
+ *           even channel in the low half
+ *   scales  [pages][kv_heads][head_dim / 32][page_tokens] f16 (8 and 4 bits;
+ *           NULL for 16-bit formats)
+ * A stored value is code * scale, scale = f16(max|x| / 127) of its group
+ * (4 bits: / 7; at most 65504), code = x / scale rounded to nearest even and
+ * clipped to +-127 (+-7).  A group that holds a NaN or an infinity reads back
+ * as NaN. */
+typedef struct exl3_kv_cache exl3_kv_cache;
+int exl3_kv_cache_create(void* k, void* v, uint16_t* k_scales, uint16_t* v_scales,
+                         int32_t format, int64_t pages, int32_t page_tokens, int32_t kv_heads,
+                         int32_t head_dim, exl3_kv_cache** out_handle);
+void exl3_kv_cache_destroy(exl3_kv_cache* handle);
+
+/* The sequences of a call.  Rows [q_starts[b], q_starts[b + 1]) of the call's
+ * tensors are the newest tokens of sequence b, which has kv_lens[b] tokens
+ * with them; row r is at position kv_lens[b] - q_starts[b + 1] + r, and
+ * position t lies in page block_table[b][t / page_tokens].  The arrays are
+ * device memory that the host does not read, so a captured graph can be
+ * replayed for other lengths.  What they say is checked on the device: rows
+ * outside every sequence are left as they were; a token whose position or page
+ * lies outside the table or the pool is not written, reads as zeros and is
+ * not attended to.  max_q and max_kv bound the new tokens of a sequence and
+ * its length (max_kv <= 0: the table's room): rows past max_q are left as they
+ * were by exl3_attention; max_kv only shapes the launch. */
+typedef struct {
+  const int32_t* q_starts;    /* [seqs + 1], ascending */
+  const int32_t* kv_lens;     /* [seqs] */
+  const int32_t* block_table; /* [seqs][table_pages] */
+  int32_t seqs;
+  int32_t table_pages;
+  int32_t max_q;
+  int32_t max_kv;
+} exl3_kv_batch;
+
+/* Rotary positions: channels (a, b) of a head become (a c - b s, a s + b c)
+ * with c, s = scale * (cos, sin)(position * inv_freq[i]), pair i being
+ * channels (2i, 2i + 1) (interleaved != 0) or (i, i + rotary_dim / 2), i <
+ * rotary_dim / 2; channels from rotary_dim on are kept.  Angles are formed and
+ * their cosines and sines taken in 64 bits, the products in 32.  inv_freq is
+ * device memory; scale is 1, or the attention factor of a scaled context.
+ * A negative position turns back. */
+typedef struct {
+  const float* inv_freq; /* [rotary_dim / 2] */
+  int32_t rotary_dim;    /* even, at most head_dim */
+  int32_t interleaved;
+  double scale;
+} exl3_rope_spec;
+
+/* y[tokens][heads][head_dim] = x rotated; x_type and y_type f16, bf16 or f32
+ * (rounded once), token strides in elements, heads contiguous (head_dim at
+ * most 256).  Positions come from `positions` [tokens] or, where that is NULL,
+ * from `batch` (whose block table is not used).  y may be x. */
+int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_type, int64_t tokens,
+              int32_t heads, int32_t head_dim, int64_t x_stride, const int32_t* positions,
+              const exl3_kv_batch* batch, void* y, int32_t y_type, int64_t y_stride,
+              void* stream);
+
+/* Writes the batch's new tokens, k and v [tokens][kv_heads][head_dim] of
+ * `type` (f16, bf16 or f32; token strides in elements), to their pages, keys
+ * rotated first where rope is not NULL (as exl3_rope, but rounded only to the
+ * cache's format).  A sequence is listed once. */
+int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const void* k,
+                   int64_t k_stride, const void* v, int64_t v_stride, int32_t type,
+                   int64_t tokens, const exl3_rope_spec* rope, void* stream);
+
+/* The reverse: the batch's newest tokens from their pages to k and v
+ * [tokens][kv_heads][head_dim] of `type`, 16-byte aligned.  A batch whose
+ * sequences are all new (q_starts from kv_lens) reads whole sequences. */
+int exl3_kv_read(const exl3_kv_cache* cache, const exl3_kv_batch* batch, void* k, void* v,
+                 int32_t type, int64_t tokens, void* stream);
+
+/* y[tokens][heads][head_dim]: every new token's query heads (head h reads
+ * cache head h / (heads / kv_heads)) over its sequence's cache, which holds
+ * the new tokens' keys and values already: softmax(scale q.k) v over the
+ * tokens t < kv_lens[b], with causal != 0 only t <= the token's position, with
+ * window > 0 only t > its position - window.  A token that sees none gives
+ * zeros.  q_type is f16 or bf16 and the cache's where that is 16-bit; y has
+ * q_type; token strides in elements.  Workspace:
+ * exl3_attention_workspace_bytes, not initialised and not shared between
+ * calls that run concurrently. */
+size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                                      int64_t tokens, int32_t heads);
+int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const void* q,
+                   int32_t q_type, int64_t tokens, int32_t heads, int64_t q_stride, float scale,
+                   int32_t causal, int32_t window, void* y, int64_t y_stride, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 /* Decode hook, the reference's `metal-decode` codec op (exl3.metal:102-109,
  * main.rs:945-967): for every tile, states[t*256 + i] (nullable) and the f16
  * bits values[t*256 + i] of state index i, in the tile's stored order. */

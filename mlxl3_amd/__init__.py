@@ -11,6 +11,8 @@ behaviour:
   dense SwiGLU MLP (qwen35.rs:303-307) with the SwiGLU fused into the gate/up epilogue
 * :class:`Exl3SwitchGlu` -- ``Exl3SwitchGlu::new`` / ``forward`` (native/src/moe.rs:809-975)
 * :func:`decode_tiles`  -- the ``metal-decode`` codec op (exl3.metal:102-109)
+* :class:`Rope`, :class:`KvCache`, :class:`KvBatch`, :func:`attention` (``kv.py``) -- rotary
+  positions, the paged key/value cache and attention over it
 * :class:`Checkpoint`   -- ``checkpoint::inspect`` / ``TensorInfo`` (native/src/checkpoint.rs),
   with ``Exl3Linear.from_checkpoint`` and ``Exl3SwitchGlu.from_checkpoint``
 
@@ -42,6 +44,11 @@ __all__ = [
     "Exl3Linear",
     "Exl3Group",
     "Exl3SwitchGlu",
+    "KvBatch",
+    "KvCache",
+    "Rope",
+    "attention",
+    "rope_frequencies",
     "decode_tiles",
     "load_library",
     "LIB_PATH",
@@ -114,6 +121,21 @@ _SIGNATURES = {
         _i32,
         [_vp, _i32, _i32, _i32, _i32, _vp, _i32, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp,
          _i32, _vp, _vp, _sz, _vp],
+    ),
+    "exl3_kv_cache_create": (
+        _i32, [_vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, ctypes.POINTER(_vp)],
+    ),
+    "exl3_kv_cache_destroy": (None, [_vp]),
+    "exl3_rope": (
+        _i32, [_vp, _vp, _i32, _i64, _i32, _i32, _i64, _vp, _vp, _vp, _i32, _i64, _vp],
+    ),
+    "exl3_kv_append": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _i64, _vp, _vp]),
+    "exl3_kv_read": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _vp]),
+    "exl3_attention_workspace_bytes": (_sz, [_vp, _vp, _i64, _i32]),
+    "exl3_attention": (
+        _i32,
+        [_vp, _vp, _vp, _i32, _i64, _i32, _i64, ctypes.c_float, _i32, _i32, _vp, _i64, _vp, _sz,
+         _vp],
     ),
     "exl3_decode_tiles": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp]),
     "exl3_codewords": (_i32, [_vp, _i64, _i32, _vp, _vp]),
@@ -903,3 +925,6 @@ def decode_tiles(packed, k: int, cb: int, with_states: bool = True):
         )
     )
     return states, values
+
+
+from .kv import KvBatch, KvCache, Rope, attention, rope_frequencies  # noqa: E402

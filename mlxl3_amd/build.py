@@ -24,7 +24,7 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libexl3_hip.so"
 CODEC = HERE / "exl3_codec"  # the codec JSON-lines driver (links LIB)
 SOURCES = ["exl3_api.hip", "exl3_qmv.hip", "exl3_qmm.hip", "exl3_wide.hip", "exl3_moe.hip", "exl3_moe_wide.hip",
-           "exl3_mapped.hip",
+           "exl3_mapped.hip", "exl3_kv.hip", "exl3_attn.hip",
            "exl3_checkpoint.cpp"]
 ARCH = "gfx950"
 

@@ -1,0 +1,346 @@
+"""What lies between a layer's q/k/v projections and its output projection: rotary
+positions, the paged key/value cache and attention over it (``exl3_rope``,
+``exl3_kv_append``, ``exl3_kv_read``, ``exl3_attention`` of ``include/exl3_hip.h``).
+
+* :class:`KvBatch`   -- the sequences of a call: new tokens, lengths, block table
+* :class:`Rope`, :func:`rope_frequencies` -- rotary positions and their frequencies
+* :class:`KvCache`   -- pages of f16, bf16, 8- or 4-bit values; append and read
+* :func:`attention`  -- new tokens over their sequences' pages
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+from . import Exl3Error, _check, _dtype_code, _ptr, _stream_ptr, _torch, _vp, load_library
+
+_FORMATS = {8: 8, 4: 4}
+
+
+class _KvBatchC(ctypes.Structure):
+    _fields_ = [
+        ("q_starts", _vp),
+        ("kv_lens", _vp),
+        ("block_table", _vp),
+        ("seqs", ctypes.c_int32),
+        ("table_pages", ctypes.c_int32),
+        ("max_q", ctypes.c_int32),
+        ("max_kv", ctypes.c_int32),
+    ]
+
+
+class _RopeC(ctypes.Structure):
+    _fields_ = [
+        ("inv_freq", _vp),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("scale", ctypes.c_double),
+    ]
+
+
+class _On:
+    """Makes `device` the current one for a call (launches go to the current device)."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        torch = _torch()
+        self.guard = None
+        if device.index is not None and torch.cuda.current_device() != device.index:
+            self.guard = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _device_tensor(t, name: str, dtypes, dims: int):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise Exl3Error(-1, f"{name} must be a device tensor")
+    if t.dtype not in dtypes:
+        raise Exl3Error(-1, f"{name} has dtype {t.dtype}, expected one of {tuple(dtypes)}")
+    if t.dim() != dims:
+        raise Exl3Error(-1, f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
+    return t
+
+
+def _same_device(device, *named):
+    for name, t in named:
+        if t is not None and t.device != device:
+            raise Exl3Error(-1, f"{name} is on {t.device}, expected {device}")
+
+
+def _plain(t, name: str, dtypes, dims: int):
+    """A tensor that the kernels read in place: contiguous."""
+    t = _device_tensor(t, name, dtypes, dims)
+    if not t.is_contiguous():
+        raise Exl3Error(-1, f"{name} must be contiguous")
+    return t
+
+
+def _heads(t, name: str, dtypes):
+    """[tokens, heads, channels] with contiguous heads; copied where its strides are others."""
+    t = _device_tensor(t, name, dtypes, 3)
+    n, h, d = t.shape
+    if n and not (t.stride(2) == 1 and (h == 1 or t.stride(1) == d) and (n == 1 or t.stride(0) >= h * d)):
+        t = t.contiguous()
+    return t
+
+
+def _floats():
+    torch = _torch()
+    return (torch.float16, torch.bfloat16, torch.float32)
+
+
+class KvBatch:
+    """The sequences of a call (``exl3_kv_batch``).
+
+    q_starts int32 [seqs + 1]: rows [q_starts[b], q_starts[b + 1]) of the call's tensors
+    are the newest tokens of sequence b; kv_lens int32 [seqs]: its tokens with them;
+    block_table int32 [seqs, pages]: the page of every page_tokens positions.  The
+    tensors are read on the device at every call (a captured graph can be replayed after
+    they were changed in place).  max_q and max_kv bound a sequence's new tokens and its
+    length (max_kv None: what the table has room for).
+    """
+
+    def __init__(self, q_starts, kv_lens, block_table=None, max_q: int = 1, max_kv: Optional[int] = None):
+        i32 = (_torch().int32,)
+        self.q_starts = _plain(q_starts, "q_starts", i32, 1)
+        self.kv_lens = _plain(kv_lens, "kv_lens", i32, 1)
+        self.block_table = None if block_table is None else _plain(block_table, "block_table", i32, 2)
+        self.seqs = int(self.kv_lens.numel())
+        if self.seqs < 1 or self.q_starts.numel() != self.seqs + 1:
+            raise Exl3Error(-1, "q_starts has one entry more than kv_lens, which has at least one")
+        if block_table is not None and self.block_table.shape[0] != self.seqs:
+            raise Exl3Error(-1, "block_table has one row per sequence")
+        if int(max_q) < 1:
+            raise Exl3Error(-1, "max_q must be positive")
+        self.device = self.kv_lens.device
+        _same_device(self.device, ("q_starts", self.q_starts), ("block_table", self.block_table))
+        pages = 0 if block_table is None else int(self.block_table.shape[1])
+        self._c = _KvBatchC(_ptr(self.q_starts), _ptr(self.kv_lens), _ptr(self.block_table), self.seqs, pages,
+                            int(max_q), 0 if max_kv is None else int(max_kv))
+        self._ref = ctypes.byref(self._c)
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None):
+    """(inv_freq f32 [rotary_dim / 2], scale) of rotary positions: base^(-2i / rotary_dim),
+    changed for a context longer than the trained one as `scaling` says (the keys of a
+    checkpoint's rope_scaling):
+
+    * ``{"rope_type": "linear", "factor": s}``: every frequency / s;
+    * ``"llama3"`` with factor, low_freq_factor, high_freq_factor and
+      original_max_position_embeddings n: wavelengths above n / low are stretched by
+      factor, those below n / high kept, in between a linear mix in n / wavelength;
+    * ``"yarn"`` with factor, original_max_position_embeddings n and optionally
+      beta_fast (32), beta_slow (1), attention_factor: pairs that turn more than
+      beta_fast times in n positions are kept, those that turn less than beta_slow times
+      stretched, in between a linear mix in the pair's index; scale is attention_factor,
+      0.1 ln(factor) + 1 by default.
+    """
+    torch = _torch()
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise Exl3Error(-1, f"rotary dimension {rotary_dim}")
+    half = rotary_dim // 2
+    freq = [base ** (-2.0 * i / rotary_dim) for i in range(half)]
+    scale = 1.0
+    if scaling:
+        kind = scaling.get("rope_type", scaling.get("type"))
+        s = float(scaling.get("factor", 1.0))
+        n = scaling.get("original_max_position_embeddings")
+        if kind == "linear":
+            freq = [f / s for f in freq]
+        elif kind == "llama3":
+            low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+            mixed = []
+            for f in freq:
+                turns = n * f / (2 * math.pi)
+                keep = min(1.0, max(0.0, (turns - low) / (high - low)))
+                mixed.append(keep * f + (1.0 - keep) * f / s)
+            freq = mixed
+        elif kind == "yarn":
+            def pair(turns):
+                return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+            first = max(0, math.floor(pair(float(scaling.get("beta_fast", 32.0)))))
+            last = min(rotary_dim - 1, math.ceil(pair(float(scaling.get("beta_slow", 1.0)))))
+            mixed = []
+            for i, f in enumerate(freq):
+                stretch = min(1.0, max(0.0, (i - first) / max(last - first, 1e-3)))
+                mixed.append((1.0 - stretch) * f + stretch * f / s)
+            freq = mixed
+            scale = scaling.get("attention_factor")
+            scale = 0.1 * math.log(s) + 1.0 if scale is None and s > 1 else 1.0 if scale is None else float(scale)
+        elif kind not in (None, "default"):
+            raise Exl3Error(-1, f"unknown rotary scaling {kind!r}")
+    return torch.tensor(freq, dtype=torch.float64).float(), scale
+
+
+class Rope:
+    """Rotary positions (``exl3_rope``): inv_freq f32 [rotary_dim / 2] on the device,
+    pairs (2i, 2i + 1) with interleaved, else (i, i + rotary_dim / 2); cosines and sines
+    times `scale`."""
+
+    def __init__(self, inv_freq, interleaved: bool = False, scale: float = 1.0):
+        self.inv_freq = _plain(inv_freq, "inv_freq", (_torch().float32,), 1)
+        if self.inv_freq.numel() < 1:
+            raise Exl3Error(-1, "empty rotary frequencies")
+        self.device = self.inv_freq.device
+        self.rotary_dim = 2 * int(self.inv_freq.numel())
+        self._c = _RopeC(_ptr(self.inv_freq), self.rotary_dim, int(bool(interleaved)), float(scale))
+        self._ref = ctypes.byref(self._c)
+
+    def apply(self, x, positions=None, batch: Optional[KvBatch] = None, out=None, dtype=None):
+        """x [tokens, heads, channels] (f16, bf16 or f32) rotated by its tokens' positions
+        (int32 [tokens], or the batch's) into `out` (x itself: in place) or a new tensor
+        of `dtype` (default x's)."""
+        torch = _torch()
+        if out is x and not (x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == x.shape[2])):
+            raise Exl3Error(-1, "rotation in place needs contiguous heads")
+        src = _heads(x, "x", _floats())
+        n, heads, dim = src.shape
+        if out is None:
+            out = torch.empty((n, heads, dim), dtype=dtype or src.dtype, device=src.device)
+        else:
+            _device_tensor(out, "out", _floats(), 3)
+            if out.shape != src.shape or _heads(out, "out", _floats()) is not out:
+                raise Exl3Error(-1, "out must have x's shape and contiguous heads")
+        if positions is not None:
+            _plain(positions, "positions", (torch.int32,), 1)
+            if positions.numel() != n:
+                raise Exl3Error(-1, f"{positions.numel()} positions for {n} tokens")
+        _same_device(src.device, ("inv_freq", self.inv_freq), ("positions", positions), ("out", out),
+                     ("batch", None if batch is None else batch.kv_lens))
+        with _On(src.device):
+            _check(load_library().exl3_rope(
+                self._ref, _ptr(src), _dtype_code(src.dtype), n, heads, dim, src.stride(0), _ptr(positions),
+                None if batch is None else batch._ref, _ptr(out), _dtype_code(out.dtype), out.stride(0),
+                _stream_ptr(src.device)))
+        return out
+
+
+class KvCache:
+    """A pool of pages of keys and values (``exl3_kv_cache``).
+
+    k, v: [pages, kv_heads, page_tokens, head_dim] f16 or bf16 (bits=16), or uint8 codes
+    of head_dim bytes (bits=8) or head_dim / 2 bytes (bits=4) with k_scales, v_scales f16
+    [pages, kv_heads, head_dim / 32, page_tokens].  The tensors are used in place.
+    """
+
+    def __init__(self, k, v, k_scales=None, v_scales=None, bits: int = 16):
+        torch = _torch()
+        if bits not in (16, 8, 4):
+            raise Exl3Error(-1, f"KV caches hold 16, 8 or 4 bits a value, got {bits}")
+        kinds = (torch.float16, torch.bfloat16) if bits == 16 else (torch.uint8,)
+        self.k, self.v = _plain(k, "k", kinds, 4), _plain(v, "v", kinds, 4)
+        if self.k.shape != self.v.shape or self.k.dtype != self.v.dtype:
+            raise Exl3Error(-1, "keys and values of a cache have one shape and type")
+        self.pages, self.kv_heads, self.page_tokens, width = (int(d) for d in self.k.shape)
+        self.head_dim = 2 * width if bits == 4 else width
+        self.bits, self.device = bits, self.k.device
+        self.k_scales, self.v_scales = k_scales, v_scales
+        if bits == 16:
+            if k_scales is not None or v_scales is not None:
+                raise Exl3Error(-1, "16-bit KV caches have no scales")
+        else:
+            want = (self.pages, self.kv_heads, self.head_dim // 32, self.page_tokens)
+            for name, s in (("k_scales", k_scales), ("v_scales", v_scales)):
+                if tuple(_plain(s, name, (torch.float16,), 4).shape) != want:
+                    raise Exl3Error(-1, f"{name} must have shape {want}")
+        _same_device(self.device, ("v", v), ("k_scales", k_scales), ("v_scales", v_scales))
+        fmt = _FORMATS.get(bits) or _dtype_code(self.k.dtype)
+        h = _vp()
+        lib = load_library()
+        self._destroy = lib.exl3_kv_cache_destroy
+        _check(lib.exl3_kv_cache_create(
+            _ptr(self.k), _ptr(self.v), _ptr(k_scales), _ptr(v_scales), fmt, self.pages, self.page_tokens,
+            self.kv_heads, self.head_dim, ctypes.byref(h)))
+        self._handle = h
+
+    @classmethod
+    def zeros(cls, pages: int, page_tokens: int, kv_heads: int, head_dim: int, dtype=None, bits: int = 16,
+              device="cuda") -> "KvCache":
+        """A new pool of zeros: `dtype` (default float16) with bits=16, else codes and scales."""
+        torch = _torch()
+        shape = (pages, kv_heads, page_tokens)
+        if bits == 16:
+            dtype = dtype or torch.float16
+            return cls(*(torch.zeros(*shape, head_dim, dtype=dtype, device=device) for _ in range(2)))
+        codes = [torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.zeros(pages, kv_heads, head_dim // 32, page_tokens, dtype=torch.float16, device=device)
+                  for _ in range(2)]
+        return cls(*codes, *scales, bits=bits)
+
+    @property
+    def handle(self):
+        return self._handle
+
+    def __del__(self):
+        h = getattr(self, "_handle", None)
+        if h is not None and h.value:
+            self._destroy(h)
+            self._handle = None
+
+    def append(self, batch: KvBatch, k, v, rope: Optional[Rope] = None) -> None:
+        """Writes the batch's new tokens, k and v [tokens, kv_heads, head_dim] (f16, bf16
+        or f32), to their pages, keys rotated by `rope` first."""
+        k, v = _heads(k, "k", _floats()), _heads(v, "v", (k.dtype,))
+        if k.shape != v.shape or tuple(k.shape[1:]) != (self.kv_heads, self.head_dim):
+            raise Exl3Error(-1, f"new keys and values have shape [tokens, {self.kv_heads}, {self.head_dim}]")
+        _same_device(self.device, ("k", k), ("v", v), ("batch", batch.kv_lens),
+                     ("rope", None if rope is None else rope.inv_freq))
+        with _On(self.device):
+            _check(load_library().exl3_kv_append(
+                self._handle, batch._ref, _ptr(k), k.stride(0), _ptr(v), v.stride(0), _dtype_code(k.dtype),
+                k.shape[0], None if rope is None else rope._ref, _stream_ptr(self.device)))
+
+    def read(self, batch: KvBatch, tokens: int, dtype=None):
+        """(k, v) [tokens, kv_heads, head_dim] of the batch's newest tokens in `dtype`
+        (default: the cache's, float16 for codes).  Rows behind the last sequence are not
+        written."""
+        torch = _torch()
+        dtype = dtype or (self.k.dtype if self.bits == 16 else torch.float16)
+        _same_device(self.device, ("batch", batch.kv_lens))
+        k, v = (torch.empty(int(tokens), self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
+                for _ in range(2))
+        with _On(self.device):
+            _check(load_library().exl3_kv_read(self._handle, batch._ref, _ptr(k), _ptr(v), _dtype_code(dtype),
+                                               int(tokens), _stream_ptr(self.device)))
+        return k, v
+
+
+def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, causal: bool = True,
+              window: int = 0, out=None, workspace=None):
+    """Attention of the batch's new tokens over the cache (``exl3_attention``): q
+    [tokens, heads, head_dim] (f16 or bf16, the cache's type where it is 16-bit) -> the
+    same shape and type.  scale defaults to 1 / sqrt(head_dim); causal: a token sees the
+    positions up to its own; window > 0: only the last `window` of them.  Rows outside
+    every sequence are not written."""
+    torch = _torch()
+    q = _heads(q, "q", (torch.float16, torch.bfloat16))
+    n, heads, dim = q.shape
+    if dim != cache.head_dim:
+        raise Exl3Error(-1, f"queries of {dim} channels over a cache of {cache.head_dim}")
+    if out is None:
+        out = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or _heads(out, "out", (q.dtype,)) is not out:
+        raise Exl3Error(-1, "out must have q's shape and type and contiguous heads")
+    _same_device(cache.device, ("q", q), ("out", out), ("batch", batch.kv_lens), ("workspace", workspace))
+    lib = load_library()
+    with _On(cache.device):
+        if workspace is None:
+            need = lib.exl3_attention_workspace_bytes(cache._handle, batch._ref, n, heads)
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _check(lib.exl3_attention(
+            cache._handle, batch._ref, _ptr(q), _dtype_code(q.dtype), n, heads, q.stride(0),
+            1.0 / math.sqrt(dim) if scale is None else float(scale), int(bool(causal)), int(window), _ptr(out),
+            out.stride(0), _ptr(workspace), 0 if workspace is None else workspace.numel(),
+            _stream_ptr(q.device)))
+    return out
