@@ -5,100 +5,80 @@
 // over the tokens t that the row sees: t < kv_len, causal t <= its position, window
 // t > its position - window.  m is the largest score so far: one pass over the cache
 // with a running maximum and sum, both f32.  A row that sees nothing gives zeros.
+//
+// The rows of a launch are (token, query head of a group) pairs: all heads that read one
+// cache head share its bytes.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
 
 #include "../../include/exl3_hip.h"
+#include "exl3_attn_few.hpp"
 #include "exl3_kv_host.hpp"
 #include "exl3_launch.hpp"
 
 namespace exl3 {
 
-struct AttnParams {
-  KvCacheView cache;
-  KvBatchView batch;
-  const void* q;
-  void* y;
-  int64_t tokens, q_stride, y_stride;
-  int heads, group, q_type, causal, window;
-  float scale2;  // scale * log2(e): scores in units of a factor of two
-};
-
-__device__ __forceinline__ float wave_sum(float v) {
-  v += xor_lanes<1>(v);
-  v += xor_lanes<2>(v);
-  v += xor_lanes<4>(v);
-  v += xor_lanes<8>(v);
-  v += xor_lanes<16>(v);
-  v += xor_lanes<32>(v);
-  return v;
-}
-
-// One wave per (token row, query head), the head's channels spread over its lanes.
+// One wave per (token row, query head).
 template <int E>
 __global__ __launch_bounds__(64) void attn_row_kernel(AttnParams p) {
   const int64_t token = blockIdx.x;
   const int head = blockIdx.y, lane = threadIdx.x;
   const int seq = kv_sequence(p.batch, token);
   if (seq < 0) return;
-  const KvCacheView& c = p.cache;
-  const int D = 64 * E;
-  const int64_t pos = kv_position(p.batch, seq, token);
-  const int64_t room = (int64_t)p.batch.table_pages << c.page_shift;
-  int64_t hi = min((int64_t)p.batch.kv_lens[seq], room), lo = 0;
-  if (p.causal) hi = min(hi, pos + 1);
-  if (p.window > 0) lo = max(lo, pos - p.window + 1);
-  float q[E], acc[E], m = -__builtin_inff(), l = 0.0f;
-  for (int e = 0; e < E; ++e) {
-    q[e] = load1(p.q, p.q_type, (size_t)token * p.q_stride + (size_t)head * D + E * lane + e);
-    acc[e] = 0.0f;
-  }
-  const int kvh = head / p.group;
-  for (int64_t t = lo; t < hi; ++t) {
-    const int64_t page = kv_page(c, p.batch, seq, t);
-    if (page < 0) continue;
-    const size_t h = (size_t)page * c.kv_heads + kvh;
-    const int slot = (int)(t & ((1 << c.page_shift) - 1));
-    const size_t row = kv_bytes(c.format, ((h << c.page_shift) + slot) * D);
-    float s = 0.0f, v[E], ks = 1.0f, vs = 1.0f;
-    if (c.ks) {
-      const size_t g = ((h * (D / 32) + E * lane / 32) << c.page_shift) + slot;
-      ks = h2f(c.ks[g]);
-      vs = h2f(c.vs[g]);
-    }
-    for (int e = 0; e < E; ++e) {
-      const int d = E * lane + e;
-      float k;
-      if (c.format == KV_Q8) {
-        k = (float)((int)c.k[row + d] - 128) * ks;
-        v[e] = (float)((int)c.v[row + d] - 128) * vs;
-      } else if (c.format == KV_Q4) {
-        k = (float)(((int)c.k[row + d / 2] >> (4 * (d & 1)) & 15) - 8) * ks;
-        v[e] = (float)(((int)c.v[row + d / 2] >> (4 * (d & 1)) & 15) - 8) * vs;
-      } else {
-        k = load1(c.k + row, c.format, d);
-        v[e] = load1(c.v + row, c.format, d);
-      }
-      s += q[e] * k;
-    }
-    s = wave_sum(s) * p.scale2;
-    const float n = fmaxf(m, s);
-    const float base = n == -__builtin_inff() ? 0.0f : n;
-    const float f = exp2f(m - base), w = exp2f(s - base);
-    l = l * f + w;
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * f + w * v[e];
-    m = n;
-  }
+  const Work w = sequence_work(p, seq);
+  const int kvh = head / p.group, row = (int)(token - w.start) * p.group + head % p.group;
+  if (row >= w.rows) return;
+  const Seen see = row_sees(p, w.first, w.len, row);
+  float m, l, acc[E];
+  row_pass<E>(p, w, kvh, row, see.lo, see.hi, lane, m, l, acc);
   for (int e = 0; e < E; ++e)
-    store1(p.y, p.q_type, (size_t)token * p.y_stride + (size_t)head * D + E * lane + e,
-           l > 0.0f || l != l ? acc[e] / l : 0.0f);
+    store1(p.y, p.q_type, (size_t)token * p.y_stride + (size_t)head * 64 * E + E * lane + e,
+           l != 0.0f ? acc[e] / l : 0.0f);
 }
-
 template __global__ void attn_row_kernel<1>(AttnParams);
 template __global__ void attn_row_kernel<2>(AttnParams);
 template __global__ void attn_row_kernel<4>(AttnParams);
+
+// The splits of a row joined in their order: grid (rows / 4, kv heads, sequences), a wave
+// per row.  A split that saw nothing has a maximum of -inf, and its sums are not read.
+template <int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int kvh = blockIdx.y, seq = blockIdx.z;
+  const Work w = sequence_work(p, seq);
+  if (row >= w.rows) return;
+  const size_t slot = (size_t)(seq * p.cache.kv_heads + kvh) * p.splits * rows + row;
+  float most = -__builtin_inff();
+  for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.stats[(slot + (size_t)s * rows) * 2]);
+  const float base = most == -__builtin_inff() ? 0.0f : most;
+  float total = 0.0f, acc[E] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const size_t at = slot + (size_t)s * rows;
+    const float m = p.stats[at * 2], l = p.stats[at * 2 + 1];
+    if (m == -__builtin_inff() && l == 0.0f) continue;
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    total += l * f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += p.part[at * D + E * lane + e] * f;
+  }
+  const size_t yi = (size_t)(w.start + row / p.group) * p.y_stride +
+                    (size_t)(kvh * p.group + row % p.group) * D + E * lane;
+#pragma unroll
+  for (int e = 0; e < E; ++e) store1(p.y, p.q_type, yi + e, total != 0.0f ? acc[e] / total : 0.0f);
+}
+template __global__ void attn_join_kernel<64>(AttnParams, int);
+template __global__ void attn_join_kernel<128>(AttnParams, int);
+template __global__ void attn_join_kernel<256>(AttnParams, int);
+
+#define EXL3_FEW_D(M, FMT, T) \
+  M(FMT, T, 64, 1) M(FMT, T, 64, 2) M(FMT, T, 128, 1) M(FMT, T, 128, 2) M(FMT, T, 256, 1)
+#define EXL3_FEW(M) \
+  EXL3_FEW_D(M, KV_F16, F16) EXL3_FEW_D(M, KV_BF16, BF16) EXL3_FEW_D(M, KV_Q8, F16) EXL3_FEW_D(M, KV_Q4, F16)
+#define EXL3_FEW_INST(FMT, T, D, RT) template __global__ void attn_few_kernel<FMT, T, D, RT>(AttnParams);
+EXL3_FEW(EXL3_FEW_INST)
 
 }  // namespace exl3
 
@@ -106,11 +86,57 @@ using namespace exl3;
 
 #ifndef __HIP_DEVICE_COMPILE__
 
+namespace {
+
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+struct Shape {
+  bool few;    // attn_few_kernel, else attn_row_kernel
+  int rows;    // rows of a workgroup
+  int splits;  // ranges of each sequence's tokens
+};
+
+Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int heads) {
+  const int64_t rows = (int64_t)b.max_q * (heads / c.kv_heads);
+  if (rows > (c.head_dim == 256 ? 16 : 32)) return Shape{false, 1, 1};
+  Shape s{true, rows > 16 ? 32 : 16, 1};
+  const int64_t room = (int64_t)b.table_pages << c.page_shift;
+  const int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;
+  const int64_t groups = (int64_t)b.seqs * c.kv_heads;
+  const int64_t want = (512 + groups - 1) / groups;
+  s.splits = (int)std::max<int64_t>(1, std::min(std::min<int64_t>(want, 64), (most + 127) / 128));
+  return s;
+}
+
+template <int FMT, typename T, int D, int RT>
+void launch_few(const AttnParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.splits, (unsigned)p.cache.kv_heads, (unsigned)p.batch.seqs);
+  constexpr size_t lds = 4 * (Few<FMT, T, D, RT>::kWaveLds);
+  hipLaunchKernelGGL((attn_few_kernel<FMT, T, D, RT>), grid, dim3(256), lds, s, p);
+}
+template <int FMT, typename T>
+void launch_few(const AttnParams& p, int rows, hipStream_t s) {
+  const int d = p.cache.head_dim;
+  if (rows == 16) {
+    d == 64 ? launch_few<FMT, T, 64, 1>(p, s) : d == 128 ? launch_few<FMT, T, 128, 1>(p, s)
+                                                         : launch_few<FMT, T, 256, 1>(p, s);
+  } else {
+    d == 64 ? launch_few<FMT, T, 64, 2>(p, s) : launch_few<FMT, T, 128, 2>(p, s);
+  }
+}
+
+}  // namespace
+
 extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
                                                  const exl3_kv_batch* batch, int64_t tokens,
                                                  int32_t heads) {
-  if (!cache || !batch || tokens <= 0 || heads <= 0) return 0;
-  return 0;
+  if (!cache || !batch || tokens <= 0 || heads <= 0 || batch->seqs <= 0 || batch->max_q <= 0 ||
+      batch->table_pages <= 0 || heads % cache->view.kv_heads)
+    return 0;
+  const Shape sh = choose(cache->view, *batch, heads);
+  if (sh.splits == 1) return 0;
+  const size_t slots = (size_t)batch->seqs * cache->view.kv_heads * sh.splits * sh.rows;
+  return align256(slots * cache->view.head_dim * 4) + align256(slots * 8);
 }
 
 extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
@@ -133,6 +159,8 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
     return fail(EXL3_EINVAL, "attention scale must be positive and finite");
   if (window < 0) return fail(EXL3_EINVAL, "negative attention window %d", window);
   if (batch->max_q < 1) return fail(EXL3_EINVAL, "max_q must be positive");
+  if (batch->seqs > 65535)
+    return fail(EXL3_EUNSUPPORTED, "attention takes up to 65535 sequences, got %d", batch->seqs);
   const int64_t width = (int64_t)heads * p.cache.head_dim;
   if (tokens > 1 && (q_stride < width || y_stride < width))
     return fail(EXL3_EINVAL, "token strides are at least heads * head_dim");
@@ -142,9 +170,11 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   const size_t need = exl3_attention_workspace_bytes(cache, batch, tokens, heads);
   if (need && (!workspace || workspace_bytes < need))
     return fail(EXL3_EINVAL, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  if (need && !aligned16(workspace))
+    return fail(EXL3_EINVAL, "attention workspace must be 16-byte aligned");
+  const Shape sh = choose(p.cache, *batch, heads);
   p.q = q;
   p.y = y;
-  p.tokens = tokens;
   p.q_stride = q_stride;
   p.y_stride = y_stride;
   p.heads = heads;
@@ -152,17 +182,43 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   p.q_type = q_type;
   p.causal = causal != 0;
   p.window = window;
+  p.max_q = batch->max_q;
+  p.splits = sh.splits;
+  p.q_vec = aligned16(q) && (tokens == 1 || q_stride % 8 == 0);
   p.scale2 = scale * 1.4426950408889634f;
-  if (int rc = launch_gate("attention")) return rc;
-  const dim3 grid((unsigned)tokens, (unsigned)heads);
+  const size_t slots = (size_t)batch->seqs * p.cache.kv_heads * sh.splits * sh.rows;
+  p.part = (float*)workspace;
+  p.stats = (float*)((uint8_t*)workspace + align256(slots * p.cache.head_dim * 4));
+  const int D = p.cache.head_dim;
   hipStream_t s = (hipStream_t)stream;
-  if (p.cache.head_dim == 64)
-    hipLaunchKernelGGL(attn_row_kernel<1>, grid, dim3(64), 0, s, p);
-  else if (p.cache.head_dim == 128)
-    hipLaunchKernelGGL(attn_row_kernel<2>, grid, dim3(64), 0, s, p);
+  if (int rc = launch_gate("attention")) return rc;
+  if (!sh.few) {
+    const dim3 grid((unsigned)tokens, (unsigned)heads);
+    if (D == 64)
+      hipLaunchKernelGGL(attn_row_kernel<1>, grid, dim3(64), 0, s, p);
+    else if (D == 128)
+      hipLaunchKernelGGL(attn_row_kernel<2>, grid, dim3(64), 0, s, p);
+    else
+      hipLaunchKernelGGL(attn_row_kernel<4>, grid, dim3(64), 0, s, p);
+    return check_launch("attention");
+  }
+  switch (p.cache.format) {
+    case EXL3_KV_F16: launch_few<KV_F16, F16>(p, sh.rows, s); break;
+    case EXL3_KV_BF16: launch_few<KV_BF16, BF16>(p, sh.rows, s); break;
+    case EXL3_KV_Q8: launch_few<KV_Q8, F16>(p, sh.rows, s); break;
+    default: launch_few<KV_Q4, F16>(p, sh.rows, s);
+  }
+  if (int rc = check_launch("attention")) return rc;
+  if (sh.splits == 1) return EXL3_OK;
+  if (int rc = launch_gate("attention join")) return rc;
+  const dim3 grid((unsigned)(sh.rows / 4), (unsigned)p.cache.kv_heads, (unsigned)batch->seqs);
+  if (D == 64)
+    hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(256), 0, s, p, sh.rows);
+  else if (D == 128)
+    hipLaunchKernelGGL(attn_join_kernel<128>, grid, dim3(256), 0, s, p, sh.rows);
   else
-    hipLaunchKernelGGL(attn_row_kernel<4>, grid, dim3(64), 0, s, p);
-  return check_launch("attention");
+    hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(256), 0, s, p, sh.rows);
+  return check_launch("attention join");
 }
 
 #endif  // __HIP_DEVICE_COMPILE__

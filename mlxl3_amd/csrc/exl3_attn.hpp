@@ -1,0 +1,225 @@
+// Device code shared by the attention kernels: element types, fragments of the paged
+// cache, the running softmax.
+#pragma once
+
+#include "exl3_kv.hpp"
+
+namespace exl3 {
+
+struct AttnParams {
+  KvCacheView cache;
+  KvBatchView batch;
+  const void* q;
+  void* y;
+  float* part;   // [slots][splits][rows][D] sums, then [slots][splits][rows][2] (max, sum)
+  float* stats;
+  int64_t q_stride, y_stride;
+  int heads, group, q_type, causal, window;
+  int max_q, splits;
+  int q_vec;      // rows of q are 16-byte aligned
+  float scale2;   // scale * log2(e): scores in units of a factor of two
+};
+
+// Matrix operands of eight 16-bit values, and what an attention kernel does with them.
+struct F16 {
+  typedef half8 V8;
+  typedef _Float16 E;
+  static __device__ __forceinline__ float4v mfma16(V8 a, V8 b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+struct BF16 {
+  typedef bf8 V8;
+  typedef __bf16 E;
+  static __device__ __forceinline__ float4v mfma16(V8 a, V8 b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+// Four rows of 16 16-bit values in LDS, transposed on the way to registers: of each 16
+// lanes, lane 4j + c names values 4c .. 4c + 3 of row j, and lane i gets value i of rows
+// 0 .. 3.
+__device__ __forceinline__ u32x2 lds_transpose4(const uint8_t* p) {
+  typedef __attribute__((address_space(3))) short4v* LdsPtr;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(size_t)lds_offset(p)));
+}
+
+// Eight 8-bit codes (code + 128) times a scale: byte b between 0x64 and itself is the f16
+// 1024 + b, and 1024 + b - 1152 is exact.
+__device__ __forceinline__ u32x4 decode8(uint32_t w0, uint32_t w1, half2v s) {
+  const half2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+  u32x4 r;
+  r[0] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u);
+  r[1] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u);
+  r[2] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u);
+  r[3] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = r[i];
+    r[i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, x) + off) * s);
+  }
+  return r;
+}
+
+// Eight 4-bit codes (code + 8) times a scale, in the order 0 4 1 5 2 6 3 7: a nibble in
+// the lowest or second-lowest place of an f16's mantissa under the exponent of 1024 is
+// 1024 + n or 1024 + 16 n.
+__device__ __forceinline__ u32x4 decode4(uint32_t w, half2v s) {
+  const half2v off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+  const half2v part = {(_Float16)0.0625f, (_Float16)0.0625f}, off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t v = w >> (8 * i);
+    const uint32_t lo = (v & 0x000f000fu) | 0x64006400u, hi = (v & 0x00f000f0u) | 0x64006400u;
+    r[2 * i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, lo) + off) * s);
+    r[2 * i + 1] = __builtin_bit_cast(
+        uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, hi), part, off16) * s);
+  }
+  return r;
+}
+// Where channel e of eight lies in decode4's order, and which channel lies at place e.
+__device__ __forceinline__ constexpr int place4(int e) { return e < 4 ? 2 * e : 2 * e - 7; }
+__device__ __forceinline__ constexpr int channel4(int e) { return (e >> 1) | ((e & 1) << 2); }
+
+// f16 of a query of a coded cache; a bf16 beyond f16's range takes its largest value.
+__device__ __forceinline__ uint16_t f2h_sat(float v) {
+  const float a = fabsf(v);
+  return f2h(a > 65504.0f && a <= 3.402823466e38f ? copysignf(65504.0f, v) : v);
+}
+
+// Eight query channels from element i on, as T: T is the queries' own type for 16-bit
+// caches, f16 for coded ones (4 bits: in decode4's order).
+template <int FMT, typename T>
+__device__ __forceinline__ typename T::V8 load_q8(const AttnParams& p, size_t i) {
+  const uint16_t* q = (const uint16_t*)p.q + i;
+  uint16_t h[8];
+  if (p.q_vec) {
+    const u32x4 w = *(const u32x4*)q;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = q[e];
+  }
+  if (FMT < 9 && p.q_type == DT_BF16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = f2h_sat(bf2f(h[e]));
+  }
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int a = FMT == KV_Q4 ? channel4(2 * e) : 2 * e, b = FMT == KV_Q4 ? channel4(2 * e + 1) : 2 * e + 1;
+    r[e] = (uint32_t)h[a] | ((uint32_t)h[b] << 16);
+  }
+  return __builtin_bit_cast(typename T::V8, r);
+}
+
+// The tokens that row `row` (token row / group of the sequence) may see: [lo, hi).
+struct Seen {
+  int lo, hi;
+};
+__device__ __forceinline__ Seen row_sees(const AttnParams& p, int first, int len, int row) {
+  const int64_t pos = (int64_t)first + row / p.group;
+  Seen s{0, len};
+  if (p.causal) s.hi = (int)max((int64_t)0, min((int64_t)len, pos + 1));
+  if (p.window > 0) s.lo = (int)min((int64_t)len, max((int64_t)0, pos - p.window + 1));
+  return s;
+}
+
+// What a workgroup works on: sequence, its first row of the call's tensors, rows
+// (tokens x heads of the group), first new position, length cut to the table's room.
+struct Work {
+  int seq, start, rows, first, len;
+};
+__device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
+  Work w;
+  w.seq = seq;
+  w.start = p.batch.q_starts[seq];
+  const int64_t n = (int64_t)p.batch.q_starts[seq + 1] - w.start;
+  w.rows = (int)max((int64_t)0, min(n, (int64_t)p.max_q)) * p.group;
+  const int kv = p.batch.kv_lens[seq];
+  const int64_t room = (int64_t)p.batch.table_pages << p.cache.page_shift;
+  w.len = (int)max((int64_t)0, min(min((int64_t)kv, room), (int64_t)INT32_MAX - 4095));
+  w.first = (int)max((int64_t)INT32_MIN, (int64_t)kv - n);
+  return w;
+}
+
+// The page that holds the 16 tokens from t (a multiple of 16) on, or -1.
+__device__ __forceinline__ int block_page(const AttnParams& p, const Work& w, int t, int hi) {
+  if (t >= hi) return -1;
+  const int32_t page = p.batch.table[(int64_t)w.seq * p.batch.table_pages + (t >> p.cache.page_shift)];
+  return page >= 0 && page < p.cache.pages ? page : -1;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+  v += xor_lanes<1>(v);
+  v += xor_lanes<2>(v);
+  v += xor_lanes<4>(v);
+  v += xor_lanes<8>(v);
+  v += xor_lanes<16>(v);
+  v += xor_lanes<32>(v);
+  return v;
+}
+
+// One row over the tokens [lo, hi) by one wave, its channels spread over the lanes (lane
+// l holds channels E l ..): running maximum m, sum l and weighted values acc.  Touches
+// only tokens that the row sees.
+template <int E>
+__device__ __forceinline__ void row_pass(const AttnParams& p, const Work& w, int kvh, int row, int lo, int hi,
+                                         int lane, float& m, float& l, float (&acc)[E]) {
+  const KvCacheView& c = p.cache;
+  constexpr int D = 64 * E;
+  const size_t qi = (size_t)(w.start + row / p.group) * p.q_stride +
+                    (size_t)(kvh * p.group + row % p.group) * D + E * lane;
+  float q[E];
+  m = -__builtin_inff();
+  l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    q[e] = load1(p.q, p.q_type, qi + e);
+    acc[e] = 0.0f;
+  }
+  for (int t = lo; t < hi; ++t) {
+    const int64_t page = kv_page(c, p.batch, w.seq, t);
+    if (page < 0) continue;
+    const size_t h = (size_t)page * c.kv_heads + kvh;
+    const int slot = t & ((1 << c.page_shift) - 1);
+    const size_t row0 = kv_bytes(c.format, ((h << c.page_shift) + slot) * D);
+    float s = 0.0f, v[E], ks = 1.0f, vs = 1.0f;
+    if (c.ks) {
+      const size_t g = ((h * (D / 32) + E * lane / 32) << c.page_shift) + slot;
+      ks = h2f(c.ks[g]);
+      vs = h2f(c.vs[g]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = E * lane + e;
+      float k;
+      if (c.format == KV_Q8) {
+        k = (float)((int)c.k[row0 + d] - 128) * ks;
+        v[e] = (float)((int)c.v[row0 + d] - 128) * vs;
+      } else if (c.format == KV_Q4) {
+        k = (float)(((int)c.k[row0 + d / 2] >> (4 * (d & 1)) & 15) - 8) * ks;
+        v[e] = (float)(((int)c.v[row0 + d / 2] >> (4 * (d & 1)) & 15) - 8) * vs;
+      } else {
+        k = load1(c.k + row0, c.format, d);
+        v[e] = load1(c.v + row0, c.format, d);
+      }
+      s += q[e] * k;
+    }
+    s = wave_sum(s) * p.scale2;
+    const float n = fmaxf(m, s);
+    const float base = n == -__builtin_inff() ? 0.0f : n;
+    const float f = exp2f(m - base), x = exp2f(s - base);
+    l = l * f + x;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = acc[e] * f + x * v[e];
+    m = n;
+  }
+}
+
+}  // namespace exl3

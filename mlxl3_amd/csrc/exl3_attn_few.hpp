@@ -1,0 +1,408 @@
+// Attention of few rows (tokens x heads of a group, at most 16 RT) over the cache:
+// decode and short drafts.  The cache's bytes bound it, so every byte is read once, by
+// one wave, straight into registers.
+//
+// A workgroup (4 waves) takes a range of one sequence's tokens for one cache head; wave w
+// takes steps of 32 tokens w, w + 4, ...  A step:
+//   S^T = K Q^T   16x16x32 MFMAs, K rows (tokens) as the A operand as they lie in the
+//                 cache, the group's queries as the B operand.  Lane l then holds, of
+//                 query l % 16, tokens 4 (l / 16) + i of both 16-token blocks;
+//   P   = exp2(S - m), rounded to 16 bits: already the B operand of the next product,
+//                 eight tokens a lane, so no lane exchange;
+//   O^T += V^T P^T  with V^T read from LDS transposed (four tokens of a channel a read),
+//                 in the token order that P has.  V goes through the wave's own LDS, so
+//                 there is no barrier in the loop.
+// m moves only when some score passes it by kSlack (a factor of 256: P and its sums stay
+// far inside 16 bits' and f32's range), so a step usually has no exchange between lanes
+// at all; the sum l is kept per lane and reduced once at the end.
+// The waves' results meet in LDS; with more than one range per sequence they are joined
+// by attn_join_kernel.
+#pragma once
+
+#include "exl3_attn.hpp"
+
+namespace exl3 {
+
+constexpr float kSlack = 8.0f;  // in factors of two
+
+template <int FMT, typename T, int D, int RT>
+struct Few {
+  static constexpr bool kRaw = FMT >= 9;
+  static constexpr int kSteps = D / 32;                                 // MFMAs over the channels
+  static constexpr int kRow = kRaw ? 2 * D : FMT == KV_Q8 ? D : D / 2;  // bytes of a cached head
+  // keys: channels of a lane's vector load, and loads per 16 tokens
+  static constexpr int kVec = kRaw ? 8 : FMT == KV_Q8 || D == 64 ? 16 : 32;
+  static constexpr int kKeyLoads = D / 4 / kVec;
+  static constexpr int kKeyWords = kVec * kRow / D / 4;
+  // values: 16-byte loads, lanes per row, rows per load
+  static constexpr int kLanes = kRow / 16, kRows = 64 / kLanes, kValueLoads = 32 / kRows;
+  static constexpr int kWaveLds = 32 * D * 2 > 16 * RT * D * 4 ? 32 * D * 2 : 16 * RT * D * 4;
+
+  // First channel of lane group g's operand in MFMA step s.
+  static __device__ __forceinline__ int channel(int s, int g) {
+    constexpr int n = kVec / 8;
+    return (s / n) * 4 * kVec + g * kVec + (s % n) * 8;
+  }
+  // Byte of 16-byte chunk c of row t of the values in LDS.  The transposing read takes 32
+  // bytes of each of 8 rows at a time: pairs of chunks change places so that those fall
+  // into different banks.
+  static __device__ __forceinline__ int place(int t, int c) {
+    const int swz = D == 64 ? ((t >> 1) & 3) << 1 : (t & 7) << 1;
+    return t * D * 2 + ((c ^ swz) << 4);
+  }
+
+  struct Keys {
+    uint32_t w[2][kKeyLoads][kKeyWords];
+    uint16_t s[2][kRaw ? 1 : kKeyLoads];
+  };
+  struct Values {
+    u32x4 w[kValueLoads];
+    uint16_t s[kRaw ? 1 : kValueLoads];
+  };
+
+  static __device__ __forceinline__ void load_keys(const AttnParams& p, const int (&page)[2], int kvh, int t0,
+                                                   int lane, Keys& k) {
+    const KvCacheView& c = p.cache;
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const size_t h = (size_t)max(page[a], 0) * c.kv_heads + kvh;
+      const int slot = (t0 + 16 * a) & ((1 << c.page_shift) - 1);
+      const uint8_t* b = c.k + ((h << c.page_shift) + slot) * kRow;
+      const uint16_t* sc = kRaw ? nullptr : c.ks + ((h * (D / 32)) << c.page_shift) + slot;
+#pragma unroll
+      for (int u = 0; u < kKeyLoads; ++u) {
+        const int ch = u * 4 * kVec + g * kVec;
+        const uint8_t* from = b + r * kRow + ch * kRow / D;
+        if constexpr (kKeyWords == 4) {
+          const u32x4 v = *(const u32x4*)from;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) k.w[a][u][i] = v[i];
+        } else {
+          const u32x2 v = *(const u32x2*)from;
+          k.w[a][u][0] = v[0];
+          k.w[a][u][1] = v[1];
+        }
+        if constexpr (!kRaw) k.s[a][u] = sc[((ch / 32) << c.page_shift) + r];
+      }
+    }
+  }
+  static __device__ __forceinline__ typename T::V8 key(const Keys& k, int a, int s) {
+    constexpr int n = kVec / 8;
+    const int u = s / n, i = s % n;
+    u32x4 r;
+    if constexpr (kRaw) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = k.w[a][u][e];
+    } else {
+      const _Float16 sc = __builtin_bit_cast(_Float16, k.s[a][u]);
+      const half2v s2 = {sc, sc};
+      if constexpr (FMT == KV_Q8)
+        r = decode8(k.w[a][u][2 * i], k.w[a][u][2 * i + 1], s2);
+      else
+        r = decode4(k.w[a][u][i], s2);
+    }
+    return __builtin_bit_cast(typename T::V8, r);
+  }
+
+  static __device__ __forceinline__ void load_values(const AttnParams& p, const int (&page)[2], int kvh, int t0,
+                                                     int lane, Values& v) {
+    const KvCacheView& c = p.cache;
+    const uint8_t* b[2];
+    const uint16_t* sc[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const size_t h = (size_t)max(page[a], 0) * c.kv_heads + kvh;
+      const int slot = (t0 + 16 * a) & ((1 << c.page_shift) - 1);
+      b[a] = c.v + ((h << c.page_shift) + slot) * kRow;
+      sc[a] = kRaw ? nullptr : c.vs + ((h * (D / 32)) << c.page_shift) + slot;
+    }
+    const int r = lane / kLanes, ch = lane % kLanes;
+#pragma unroll
+    for (int u = 0; u < kValueLoads; ++u) {
+      const int t = u * kRows + r;
+      const bool second = kRows > 16 ? t >= 16 : u * kRows >= 16;
+      v.w[u] = *(const u32x4*)((second ? b[1] : b[0]) + (t & 15) * kRow + ch * 16);
+      if constexpr (!kRaw) {
+        const int group = ch * (16 * D / kRow) / 32;
+        v.s[u] = (second ? sc[1] : sc[0])[(group << c.page_shift) + (t & 15)];
+      }
+    }
+  }
+  // Values to LDS as 16-bit rows (4 bits: channels in decode4's order); rows outside
+  // [live_lo, live_hi) or of a block without a page become zeros.
+  template <bool EDGE>
+  static __device__ __forceinline__ void put_values(const Values& v, uint8_t* lds, int lane, int live_lo, int live_hi,
+                                                    bool on0, bool on1) {
+    const int r = lane / kLanes, ch = lane % kLanes;
+#pragma unroll
+    for (int u = 0; u < kValueLoads; ++u) {
+      const int t = u * kRows + r;
+      const bool live = !EDGE || (t >= live_lo && t < live_hi && (t < 16 ? on0 : on1));
+      constexpr int n = kRaw ? 1 : FMT == KV_Q8 ? 2 : 4;  // 16-byte chunks of the decoded row
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        u32x4 x = v.w[u];
+        if constexpr (!kRaw) {
+          const _Float16 sc = __builtin_bit_cast(_Float16, v.s[u]);
+          const half2v s2 = {sc, sc};
+          if constexpr (FMT == KV_Q8) {
+            const uint32_t w0 = v.w[u][2 * i], w1 = v.w[u][2 * i + 1];
+            x = decode8(w0, w1, s2);
+          } else {
+            const uint32_t w0 = v.w[u][i];
+            x = decode4(w0, s2);
+          }
+        }
+        if (!live) x = u32x4{0, 0, 0, 0};
+        *(u32x4*)(lds + place(t, ch * n + i)) = x;
+      }
+    }
+  }
+  static __device__ __forceinline__ typename T::V8 value(const uint8_t* lds, int dt, int lane) {
+    const int g = lane >> 4, j = (lane >> 2) & 3, c = lane & 3;
+    const int t = 4 * g + j, chunk = dt * 2 + (c >> 1), half = (c & 1) * 8;
+    const u32x2 lo = lds_transpose4(lds + place(t, chunk) + half);
+    const u32x2 hi = lds_transpose4(lds + place(t + 16, chunk) + half);
+    const u32x4 r = {lo[0], lo[1], hi[0], hi[1]};
+    return __builtin_bit_cast(typename T::V8, r);
+  }
+};
+
+// Whether any 16-bit value of the lane's share is not finite.
+template <typename F, typename T>
+__device__ __forceinline__ bool not_finite(const typename F::Values& v) {
+  constexpr uint32_t mask = sizeof(typename T::E) == 2 && __is_same(T, BF16) ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t lo = mask & 0xffffu, hi = mask & 0xffff0000u;
+  bool bad = false;
+#pragma unroll
+  for (int u = 0; u < F::kValueLoads; ++u) {
+    if constexpr (F::kRaw) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = v.w[u][i];
+        bad = bad || (w & lo) == lo || (w & hi) == hi;
+      }
+    } else {
+      bad = bad || (v.s[u] & 0x7c00) == 0x7c00;
+    }
+  }
+  return bad;
+}
+
+// The tokens [t0, t1) of split `split`: 16-aligned ranges of [lo, hi), a multiple of 128
+// tokens each so that the four waves' steps come out even.
+__device__ __forceinline__ void split_range(int lo, int hi, int splits, int split, int& t0, int& t1) {
+  lo &= ~15;
+  const int n = max(hi - lo, 0);
+  const int each = ((n + splits - 1) / splits + 127) / 128 * 128;
+  const int64_t a = (int64_t)lo + (int64_t)split * each;
+  t0 = (int)min(a, (int64_t)hi);
+  t1 = (int)min(a + each, (int64_t)hi);
+}
+
+// grid (splits, kv heads, sequences)
+template <int FMT, typename T, int D, int RT>
+__global__ __launch_bounds__(256, D == 256 || RT == 2 ? 1 : 2) void attn_few_kernel(AttnParams p) {
+  typedef Few<FMT, T, D, RT> F;
+  typedef typename T::V8 V8;
+  extern __shared__ __align__(16) uint8_t lds[];  // 4 kWaveLds
+  __shared__ float wave_m[4][16 * RT], wave_l[4][16 * RT];
+  __shared__ int retry;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const Work w = sequence_work(p, seq);
+  if (w.rows == 0) return;
+  const Seen top = row_sees(p, w.first, w.len, 0), end = row_sees(p, w.first, w.len, w.rows - 1);
+  // rows see later tokens the later they are: the union is [top.lo, end.hi), what all see
+  // [end.lo, top.hi)
+  int t0, t1;
+  split_range(top.lo, end.hi, p.splits, split, t0, t1);
+  if (p.splits > 1 && t0 >= t1) {
+    const size_t slot = ((size_t)(seq * p.cache.kv_heads + kvh) * p.splits + split) * (16 * RT);
+    for (int e = threadIdx.x; e < 2 * w.rows; e += 256)
+      p.stats[slot * 2 + e] = e & 1 ? 0.0f : -__builtin_inff();
+    return;
+  }
+  if (threadIdx.x == 0) retry = 0;
+  __syncthreads();
+
+  const int n = lane & 15, g = lane >> 4;
+  uint8_t* my = lds + wave * F::kWaveLds;
+  V8 q[RT][F::kSteps];
+  Seen see[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = rt * 16 + n;
+    const int r = row < w.rows ? row : 0;  // rows past the last repeat the first; nobody reads them
+    see[rt] = row_sees(p, w.first, w.len, r);
+    const size_t qi =
+        (size_t)(w.start + r / p.group) * p.q_stride + (size_t)(kvh * p.group + r % p.group) * D;
+#pragma unroll
+    for (int s = 0; s < F::kSteps; ++s) q[rt][s] = load_q8<FMT, T>(p, qi + F::channel(s, g));
+  }
+  float4v o[RT][D / 16];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -__builtin_inff();
+    l[rt] = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = float4v{0, 0, 0, 0};
+  }
+  bool again = false;
+
+  typename F::Keys k;
+  typename F::Values v;
+  int t = t0 + 32 * wave;
+  int page[2], next[2];
+  if (t < t1) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) page[a] = block_page(p, w, t + 16 * a, t1);
+    F::load_keys(p, page, kvh, t, lane, k);
+    F::load_values(p, page, kvh, t, lane, v);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) next[a] = block_page(p, w, t + 128 + 16 * a, t1);
+  }
+  for (; t < t1; t += 128) {
+    const bool edge = t < end.lo || t + 32 > min(top.hi, t1) || page[0] < 0 || page[1] < 0;
+    float4v s[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) s[rt][a] = float4v{0, 0, 0, 0};
+#pragma unroll
+    for (int st = 0; st < F::kSteps; ++st)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const V8 key = F::key(k, a, st);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][a] = T::mfma16(key, q[rt][st], s[rt][a]);
+      }
+    // values that some rows see and others do not must be finite for the product below (a
+    // zero weight times an infinity is no zero); where they are not, the rows are done one
+    // by one at the end
+    const bool on0 = page[0] >= 0, on1 = page[1] >= 0;
+    if (edge) {
+      if ((t < end.lo || t + 32 > top.hi) && (top.lo < end.lo || top.hi < end.hi))
+        again = again || not_finite<F, T>(v);
+      F::template put_values<true>(v, my, lane, top.lo - t, min(end.hi, t1) - t, on0, on1);
+    } else {
+      F::template put_values<false>(v, my, lane, 0, 32, true, true);
+    }
+    if (t + 128 < t1) {
+      F::load_keys(p, next, kvh, t + 128, lane, k);
+      F::load_values(p, next, kvh, t + 128, lane, v);
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        page[a] = next[a];
+        next[a] = block_page(p, w, t + 256 + 16 * a, t1);
+      }
+    }
+    V8 w8[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float x[8], most = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = s[rt][i >> 2][i & 3];
+        if (edge) {
+          const int at = t + (i >> 2) * 16 + 4 * g + (i & 3);
+          const bool live = at >= see[rt].lo && at < min(see[rt].hi, t1) && ((i >> 2) ? on1 : on0);
+          x[i] = live ? x[i] : -__builtin_inff();
+        }
+        most = fmaxf(most, x[i]);
+      }
+      most *= p.scale2;
+      if (__any(most > m[rt] + kSlack)) {
+        most = fmaxf(most, xor_lanes<16>(most));
+        most = fmaxf(most, xor_lanes<32>(most));
+        const float up = fmaxf(m[rt], most);
+        const float f = up == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - up);
+        m[rt] = up;
+        l[rt] *= f;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
+      }
+      const float base = m[rt] == -__builtin_inff() ? 0.0f : m[rt];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], p.scale2, -base));
+        l[rt] += x[i];
+        w8[rt][i] = (typename T::E)x[i];
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      const V8 val = F::value(my, dt, lane);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) o[rt][dt] = T::mfma16(val, w8[rt], o[rt][dt]);
+    }
+  }
+
+  // the waves' results: maxima and sums, then weighted sums [row][channel] in LDS
+  if (again) retry = 1;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] += xor_lanes<16>(l[rt]);
+    l[rt] += xor_lanes<32>(l[rt]);
+    if (g == 0) {
+      wave_m[wave][rt * 16 + n] = m[rt];
+      wave_l[wave][rt * 16 + n] = l[rt];
+    }
+    float* out = (float*)my + (rt * 16 + n) * D;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) *(float4v*)(out + dt * 16 + 4 * g) = o[rt][dt];
+  }
+  __syncthreads();
+  if (retry) {
+    // one row at a time, by the wave that then stands for all four
+    __syncthreads();
+    constexpr int E = D / 64;
+    for (int row = wave; row < 16 * RT; row += 4) {
+      float rm = -__builtin_inff(), rl = 0.0f, acc[E] = {};
+      if (row < w.rows) {
+        const Seen s = row_sees(p, w.first, w.len, row);
+        row_pass<E>(p, w, kvh, row, max(s.lo, t0), min(s.hi, t1), lane, rm, rl, acc);
+      }
+      for (int o4 = 0; o4 < 4; ++o4) {
+        if (lane == 0) {
+          wave_m[o4][row] = o4 ? -__builtin_inff() : rm;
+          wave_l[o4][row] = o4 ? 0.0f : rl;
+        }
+        for (int e = 0; e < E; ++e) {
+          const int d = E * lane + e;
+          const int at = FMT == KV_Q4 ? (d & ~7) | place4(d & 7) : d;
+          ((float*)(lds + o4 * F::kWaveLds))[row * D + at] = o4 ? 0.0f : acc[e];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int e = threadIdx.x; e < w.rows * D; e += 256) {
+    const int row = e / D, d = e % D;
+    const int at = row * D + (FMT == KV_Q4 ? (d & ~7) | place4(d & 7) : d);
+    float most = wave_m[0][row];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) most = fmaxf(most, wave_m[i][row]);
+    const float base = most == -__builtin_inff() ? 0.0f : most;
+    float sum = 0.0f, total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = __builtin_amdgcn_exp2f(wave_m[i][row] - base);
+      total += wave_l[i][row] * f;
+      sum += ((const float*)(lds + i * F::kWaveLds))[at] * f;
+    }
+    if (p.splits == 1) {
+      const size_t yi = (size_t)(w.start + row / p.group) * p.y_stride +
+                        (size_t)(kvh * p.group + row % p.group) * D + d;
+      store1(p.y, p.q_type, yi, total != 0.0f ? sum / total : 0.0f);
+    } else {
+      const size_t slot = ((size_t)(seq * p.cache.kv_heads + kvh) * p.splits + split) * (16 * RT) + row;
+      p.part[slot * D + d] = sum;
+      if (d < 2) p.stats[slot * 2 + d] = d ? total : most;
+    }
+  }
+}
+
+}  // namespace exl3
