@@ -15,42 +15,24 @@
 
 #include "../../include/exl3_hip.h"
 #include "exl3_attn_few.hpp"
+#include "exl3_attn_many.hpp"
 #include "exl3_kv_host.hpp"
 #include "exl3_launch.hpp"
 
 namespace exl3 {
 
-// One wave per (token row, query head).
-template <int E>
-__global__ __launch_bounds__(64) void attn_row_kernel(AttnParams p) {
-  const int64_t token = blockIdx.x;
-  const int head = blockIdx.y, lane = threadIdx.x;
-  const int seq = kv_sequence(p.batch, token);
-  if (seq < 0) return;
-  const Work w = sequence_work(p, seq);
-  const int kvh = head / p.group, row = (int)(token - w.start) * p.group + head % p.group;
-  if (row >= w.rows) return;
-  const Seen see = row_sees(p, w.first, w.len, row);
-  float m, l, acc[E];
-  row_pass<E>(p, w, kvh, row, see.lo, see.hi, lane, m, l, acc);
-  for (int e = 0; e < E; ++e)
-    store1(p.y, p.q_type, (size_t)token * p.y_stride + (size_t)head * 64 * E + E * lane + e,
-           l != 0.0f ? acc[e] / l : 0.0f);
-}
-template __global__ void attn_row_kernel<1>(AttnParams);
-template __global__ void attn_row_kernel<2>(AttnParams);
-template __global__ void attn_row_kernel<4>(AttnParams);
-
-// The splits of a row joined in their order: grid (rows / 4, kv heads, sequences), a wave
+// The splits of a row joined in their order: grid (rows / 4, kv heads, tiles), a wave
 // per row.  A split that saw nothing has a maximum of -inf, and its sums are not read.
 template <int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows) {
   constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int kvh = blockIdx.y, seq = blockIdx.z;
-  const Work w = sequence_work(p, seq);
+  const int lane = threadIdx.x & 63, in_tile = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int kvh = blockIdx.y, tile = blockIdx.z;
+  int row0;
+  const Work w = tile_work(p, tile, rows, row0);
+  const int row = row0 + in_tile;
   if (row >= w.rows) return;
-  const size_t slot = (size_t)(seq * p.cache.kv_heads + kvh) * p.splits * rows + row;
+  const size_t slot = (size_t)(tile * p.cache.kv_heads + kvh) * p.splits * rows + in_tile;
   float most = -__builtin_inff();
   for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.stats[(slot + (size_t)s * rows) * 2]);
   const float base = most == -__builtin_inff() ? 0.0f : most;
@@ -80,6 +62,12 @@ template __global__ void attn_join_kernel<256>(AttnParams, int);
 #define EXL3_FEW_INST(FMT, T, D, RT) template __global__ void attn_few_kernel<FMT, T, D, RT>(AttnParams);
 EXL3_FEW(EXL3_FEW_INST)
 
+#define EXL3_MANY_D(M, FMT, T) M(FMT, T, 64) M(FMT, T, 128) M(FMT, T, 256)
+#define EXL3_MANY(M) \
+  EXL3_MANY_D(M, KV_F16, F16) EXL3_MANY_D(M, KV_BF16, BF16) EXL3_MANY_D(M, KV_Q8, F16) EXL3_MANY_D(M, KV_Q4, F16)
+#define EXL3_MANY_INST(FMT, T, D) template __global__ void attn_many_kernel<FMT, T, D>(AttnParams, int);
+EXL3_MANY(EXL3_MANY_INST)
+
 }  // namespace exl3
 
 using namespace exl3;
@@ -91,21 +79,33 @@ namespace {
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Shape {
-  bool few;    // attn_few_kernel, else attn_row_kernel
-  int rows;    // rows of a workgroup
-  int splits;  // ranges of each sequence's tokens
+  bool few;       // attn_few_kernel, else attn_many_kernel
+  int rows;       // rows of a workgroup
+  bool one_tile;  // every sequence's rows fit one workgroup
+  int64_t tiles;  // at most; the device counts the tiles that there are
+  int splits;     // ranges of the tokens that a tile sees
 };
 
-Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int heads) {
-  const int64_t rows = (int64_t)b.max_q * (heads / c.kv_heads);
-  if (rows > (c.head_dim == 256 ? 16 : 32)) return Shape{false, 1, 1};
-  Shape s{true, rows > 16 ? 32 : 16, 1};
+Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int heads) {
+  const int group = heads / c.kv_heads;
+  const int64_t rows = (int64_t)b.max_q * group;
+  Shape s;
+  s.few = rows <= (c.head_dim == 256 ? 16 : 32);
+  s.rows = s.few ? rows > 16 ? 32 : 16 : kManyRows;
+  s.one_tile = rows <= s.rows;
+  s.tiles = s.one_tile ? b.seqs
+                       : std::min((rows + s.rows - 1) / s.rows * b.seqs, tokens * group / s.rows + b.seqs);
   const int64_t room = (int64_t)b.table_pages << c.page_shift;
   const int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;
-  const int64_t groups = (int64_t)b.seqs * c.kv_heads;
+  const int64_t groups = s.tiles * c.kv_heads;
   const int64_t want = (512 + groups - 1) / groups;
-  s.splits = (int)std::max<int64_t>(1, std::min(std::min<int64_t>(want, 64), (most + 127) / 128));
+  s.splits = (int)std::max<int64_t>(
+      1, std::min(std::min<int64_t>(want, 64), (most + 127) / (s.few ? 128 : 256)));
   return s;
+}
+
+size_t slots_of(const Shape& s, const KvCacheView& c) {
+  return (size_t)s.tiles * c.kv_heads * s.splits * s.rows;
 }
 
 template <int FMT, typename T, int D, int RT>
@@ -125,6 +125,22 @@ void launch_few(const AttnParams& p, int rows, hipStream_t s) {
   }
 }
 
+template <int FMT, typename T, int D>
+void launch_many(const AttnParams& p, int tiles, hipStream_t s) {
+  constexpr size_t lds = Many<FMT, T, D>::kLds;
+  const dim3 grid((unsigned)tiles * p.splits * p.cache.kv_heads);
+  hipLaunchKernelGGL((attn_many_kernel<FMT, T, D>), grid, dim3(256), lds, s, p, tiles);
+}
+template <int FMT, typename T>
+void launch(const AttnParams& p, const Shape& sh, hipStream_t s) {
+  const int d = p.cache.head_dim, tiles = (int)sh.tiles;
+  if (sh.few)
+    launch_few<FMT, T>(p, sh.rows, s);
+  else
+    d == 64 ? launch_many<FMT, T, 64>(p, tiles, s) : d == 128 ? launch_many<FMT, T, 128>(p, tiles, s)
+                                                              : launch_many<FMT, T, 256>(p, tiles, s);
+}
+
 }  // namespace
 
 extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
@@ -133,9 +149,9 @@ extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
   if (!cache || !batch || tokens <= 0 || heads <= 0 || batch->seqs <= 0 || batch->max_q <= 0 ||
       batch->table_pages <= 0 || heads % cache->view.kv_heads)
     return 0;
-  const Shape sh = choose(cache->view, *batch, heads);
+  const Shape sh = choose(cache->view, *batch, tokens, heads);
   if (sh.splits == 1) return 0;
-  const size_t slots = (size_t)batch->seqs * cache->view.kv_heads * sh.splits * sh.rows;
+  const size_t slots = slots_of(sh, cache->view);
   return align256(slots * cache->view.head_dim * 4) + align256(slots * 8);
 }
 
@@ -172,7 +188,9 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
     return fail(EXL3_EINVAL, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
   if (need && !aligned16(workspace))
     return fail(EXL3_EINVAL, "attention workspace must be 16-byte aligned");
-  const Shape sh = choose(p.cache, *batch, heads);
+  const Shape sh = choose(p.cache, *batch, tokens, heads);
+  if (sh.tiles * sh.splits * p.cache.kv_heads > INT32_MAX)
+    return fail(EXL3_EUNSUPPORTED, "attention of %lld tokens needs too many workgroups", (long long)tokens);
   p.q = q;
   p.y = y;
   p.q_stride = q_stride;
@@ -184,34 +202,26 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   p.window = window;
   p.max_q = batch->max_q;
   p.splits = sh.splits;
+  p.one_tile = sh.one_tile;
   p.q_vec = aligned16(q) && (tokens == 1 || q_stride % 8 == 0);
+  p.y_vec = ((uintptr_t)y & 7) == 0 && (tokens == 1 || y_stride % 4 == 0);
   p.scale2 = scale * 1.4426950408889634f;
-  const size_t slots = (size_t)batch->seqs * p.cache.kv_heads * sh.splits * sh.rows;
+  const size_t slots = slots_of(sh, p.cache);
   p.part = (float*)workspace;
   p.stats = (float*)((uint8_t*)workspace + align256(slots * p.cache.head_dim * 4));
   const int D = p.cache.head_dim;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = launch_gate("attention")) return rc;
-  if (!sh.few) {
-    const dim3 grid((unsigned)tokens, (unsigned)heads);
-    if (D == 64)
-      hipLaunchKernelGGL(attn_row_kernel<1>, grid, dim3(64), 0, s, p);
-    else if (D == 128)
-      hipLaunchKernelGGL(attn_row_kernel<2>, grid, dim3(64), 0, s, p);
-    else
-      hipLaunchKernelGGL(attn_row_kernel<4>, grid, dim3(64), 0, s, p);
-    return check_launch("attention");
-  }
   switch (p.cache.format) {
-    case EXL3_KV_F16: launch_few<KV_F16, F16>(p, sh.rows, s); break;
-    case EXL3_KV_BF16: launch_few<KV_BF16, BF16>(p, sh.rows, s); break;
-    case EXL3_KV_Q8: launch_few<KV_Q8, F16>(p, sh.rows, s); break;
-    default: launch_few<KV_Q4, F16>(p, sh.rows, s);
+    case EXL3_KV_F16: launch<KV_F16, F16>(p, sh, s); break;
+    case EXL3_KV_BF16: launch<KV_BF16, BF16>(p, sh, s); break;
+    case EXL3_KV_Q8: launch<KV_Q8, F16>(p, sh, s); break;
+    default: launch<KV_Q4, F16>(p, sh, s);
   }
   if (int rc = check_launch("attention")) return rc;
   if (sh.splits == 1) return EXL3_OK;
   if (int rc = launch_gate("attention join")) return rc;
-  const dim3 grid((unsigned)(sh.rows / 4), (unsigned)p.cache.kv_heads, (unsigned)batch->seqs);
+  const dim3 grid((unsigned)(sh.rows / 4), (unsigned)p.cache.kv_heads, (unsigned)sh.tiles);
   if (D == 64)
     hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(256), 0, s, p, sh.rows);
   else if (D == 128)

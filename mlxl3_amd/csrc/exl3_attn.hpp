@@ -16,9 +16,12 @@ struct AttnParams {
   int64_t q_stride, y_stride;
   int heads, group, q_type, causal, window;
   int max_q, splits;
-  int q_vec;      // rows of q are 16-byte aligned
+  int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
+  int q_vec, y_vec;  // rows of q are 16-byte, rows of y 8-byte aligned
   float scale2;   // scale * log2(e): scores in units of a factor of two
 };
+
+typedef float float16v __attribute__((ext_vector_type(16)));
 
 // Matrix operands of eight 16-bit values, and what an attention kernel does with them.
 struct F16 {
@@ -27,6 +30,9 @@ struct F16 {
   static __device__ __forceinline__ float4v mfma16(V8 a, V8 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float16v mfma32(V8 a, V8 b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
 };
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 struct BF16 {
@@ -34,6 +40,9 @@ struct BF16 {
   typedef __bf16 E;
   static __device__ __forceinline__ float4v mfma16(V8 a, V8 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float16v mfma32(V8 a, V8 b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
 
@@ -45,6 +54,20 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x2 lds_transpose4(const uint8_t* p) {
   typedef __attribute__((address_space(3))) short4v* LdsPtr;
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(size_t)lds_offset(p)));
+}
+
+// Whether any of eight 16-bit values is a NaN or an infinity.
+template <typename T>
+__device__ __forceinline__ bool not_finite(const u32x4& v) {
+  constexpr uint32_t mask = __is_same(T, BF16) ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t lo = mask & 0xffffu, hi = mask & 0xffff0000u;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = v[i];
+    bad = bad || (w & lo) == lo || (w & hi) == hi;
+  }
+  return bad;
 }
 
 // Eight 8-bit codes (code + 128) times a scale: byte b between 0x64 and itself is the f16
@@ -80,6 +103,13 @@ __device__ __forceinline__ u32x4 decode4(uint32_t w, half2v s) {
         uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, hi), part, off16) * s);
   }
   return r;
+}
+// decode4 in the channels' own order.
+__device__ __forceinline__ u32x4 decode4_plain(uint32_t w, half2v s) {
+  const u32x4 d = decode4(w, s);
+  const uint32_t a = d[0], b = d[1], c = d[2], e = d[3];
+  return u32x4{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(e, c, 0x05040100u),
+               __builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(e, c, 0x07060302u)};
 }
 // Where channel e of eight lies in decode4's order, and which channel lies at place e.
 __device__ __forceinline__ constexpr int place4(int e) { return e < 4 ? 2 * e : 2 * e - 7; }
@@ -148,10 +178,39 @@ __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
   return w;
 }
 
-// The page that holds the 16 tokens from t (a multiple of 16) on, or -1.
+// Sequence and first row of tile `tile`, sequences cut into tiles of `rows` rows; a tile
+// behind the last has no rows.  Every lane of a wave calls it.
+__device__ __forceinline__ Work tile_work(const AttnParams& p, int tile, int rows, int& row0) {
+  row0 = 0;
+  if (p.one_tile) return sequence_work(p, tile);
+  const int lane = threadIdx.x & 63;
+  for (int s0 = 0; s0 < p.batch.seqs; s0 += 64) {
+    const int seq = s0 + lane;
+    const int mine = seq < p.batch.seqs ? (sequence_work(p, seq).rows + rows - 1) / rows : 0;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int other = __shfl_up(upto, d);
+      if (lane >= d) upto += other;
+    }
+    const uint64_t past = __ballot(upto > tile);
+    if (past) {
+      const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
+      row0 = (tile - __shfl(upto - mine, at)) * rows;
+      row0 = __builtin_amdgcn_readfirstlane(row0);
+      return sequence_work(p, s0 + at);
+    }
+    tile -= __shfl(upto, 63);
+  }
+  return Work{0, 0, 0, 0, 0};
+}
+
+// The page that holds the 16 tokens from t (a multiple of 16) on, or -1.  Wave-uniform: a
+// scalar load (no kernel writes the table).
 __device__ __forceinline__ int block_page(const AttnParams& p, const Work& w, int t, int hi) {
+  typedef const __attribute__((address_space(4))) int32_t* ScalarPtr;
   if (t >= hi) return -1;
-  const int32_t page = p.batch.table[(int64_t)w.seq * p.batch.table_pages + (t >> p.cache.page_shift)];
+  const int32_t page = ((ScalarPtr)(size_t)p.batch.table)[(int64_t)w.seq * p.batch.table_pages + (t >> p.cache.page_shift)];
   return page >= 0 && page < p.cache.pages ? page : -1;
 }
 
@@ -164,6 +223,21 @@ __device__ __forceinline__ float wave_sum(float v) {
   v += xor_lanes<32>(v);
   return v;
 }
+
+// The tokens [t0, t1) of split `split`: 16-aligned ranges of [lo, hi), a multiple of 128
+// tokens each.
+__device__ __forceinline__ void split_range(int lo, int hi, int splits, int split, int& t0, int& t1) {
+  lo &= ~15;
+  const int n = max(hi - lo, 0);
+  const int each = ((n + splits - 1) / splits + 127) / 128 * 128;
+  const int64_t a = (int64_t)lo + (int64_t)split * each;
+  t0 = (int)min(a, (int64_t)hi);
+  t1 = (int)min(a + each, (int64_t)hi);
+}
+
+// A score above the running maximum by no more than this (in factors of two) does not
+// move it: weights stay below 256 and far inside 16 bits' range, their sums inside f32's.
+constexpr float kSlack = 8.0f;
 
 // One row over the tokens [lo, hi) by one wave, its channels spread over the lanes (lane
 // l holds channels E l ..): running maximum m, sum l and weighted values acc.  Touches

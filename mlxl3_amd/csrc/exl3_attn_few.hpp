@@ -23,8 +23,6 @@
 
 namespace exl3 {
 
-constexpr float kSlack = 8.0f;  // in factors of two
-
 template <int FMT, typename T, int D, int RT>
 struct Few {
   static constexpr bool kRaw = FMT >= 9;
@@ -130,15 +128,18 @@ struct Few {
     }
   }
   // Values to LDS as 16-bit rows (4 bits: channels in decode4's order); rows outside
-  // [live_lo, live_hi) or of a block without a page become zeros.
+  // [live_lo, live_hi) or of a block without a page become zeros.  Returns whether an
+  // edge's other rows hold a value that is not finite.
   template <bool EDGE>
-  static __device__ __forceinline__ void put_values(const Values& v, uint8_t* lds, int lane, int live_lo, int live_hi,
+  static __device__ __forceinline__ bool put_values(const Values& v, uint8_t* lds, int lane, int live_lo, int live_hi,
                                                     bool on0, bool on1) {
     const int r = lane / kLanes, ch = lane % kLanes;
+    bool bad = false;
 #pragma unroll
     for (int u = 0; u < kValueLoads; ++u) {
       const int t = u * kRows + r;
       const bool live = !EDGE || (t >= live_lo && t < live_hi && (t < 16 ? on0 : on1));
+      if (EDGE && live) bad = bad || (kRaw ? not_finite<T>(v.w[u]) : (v.s[kRaw ? 0 : u] & 0x7c00) == 0x7c00);
       constexpr int n = kRaw ? 1 : FMT == KV_Q8 ? 2 : 4;  // 16-byte chunks of the decoded row
 #pragma unroll
       for (int i = 0; i < n; ++i) {
@@ -158,6 +159,7 @@ struct Few {
         *(u32x4*)(lds + place(t, ch * n + i)) = x;
       }
     }
+    return bad;
   }
   static __device__ __forceinline__ typename T::V8 value(const uint8_t* lds, int dt, int lane) {
     const int g = lane >> 4, j = (lane >> 2) & 3, c = lane & 3;
@@ -168,38 +170,6 @@ struct Few {
     return __builtin_bit_cast(typename T::V8, r);
   }
 };
-
-// Whether any 16-bit value of the lane's share is not finite.
-template <typename F, typename T>
-__device__ __forceinline__ bool not_finite(const typename F::Values& v) {
-  constexpr uint32_t mask = sizeof(typename T::E) == 2 && __is_same(T, BF16) ? 0x7f807f80u : 0x7c007c00u;
-  constexpr uint32_t lo = mask & 0xffffu, hi = mask & 0xffff0000u;
-  bool bad = false;
-#pragma unroll
-  for (int u = 0; u < F::kValueLoads; ++u) {
-    if constexpr (F::kRaw) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t w = v.w[u][i];
-        bad = bad || (w & lo) == lo || (w & hi) == hi;
-      }
-    } else {
-      bad = bad || (v.s[u] & 0x7c00) == 0x7c00;
-    }
-  }
-  return bad;
-}
-
-// The tokens [t0, t1) of split `split`: 16-aligned ranges of [lo, hi), a multiple of 128
-// tokens each so that the four waves' steps come out even.
-__device__ __forceinline__ void split_range(int lo, int hi, int splits, int split, int& t0, int& t1) {
-  lo &= ~15;
-  const int n = max(hi - lo, 0);
-  const int each = ((n + splits - 1) / splits + 127) / 128 * 128;
-  const int64_t a = (int64_t)lo + (int64_t)split * each;
-  t0 = (int)min(a, (int64_t)hi);
-  t1 = (int)min(a + each, (int64_t)hi);
-}
 
 // grid (splits, kv heads, sequences)
 template <int FMT, typename T, int D, int RT>
@@ -284,9 +254,8 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 1 : 2) void attn_few_ker
     // by one at the end
     const bool on0 = page[0] >= 0, on1 = page[1] >= 0;
     if (edge) {
-      if ((t < end.lo || t + 32 > top.hi) && (top.lo < end.lo || top.hi < end.hi))
-        again = again || not_finite<F, T>(v);
-      F::template put_values<true>(v, my, lane, top.lo - t, min(end.hi, t1) - t, on0, on1);
+      const bool bad = F::template put_values<true>(v, my, lane, top.lo - t, min(end.hi, t1) - t, on0, on1);
+      again = again || (bad && (top.lo < end.lo || top.hi < end.hi));
     } else {
       F::template put_values<false>(v, my, lane, 0, 32, true, true);
     }

@@ -1,0 +1,318 @@
+// Attention of many rows (tokens x heads of a group) over the cache: prefill chunks.
+// The matrix cores bound it.
+//
+// A workgroup (4 waves) takes 128 rows of one sequence and cache head, 32 per wave, and
+// walks the cache in tiles of TK tokens that its waves share in LDS (16-bit rows; codes
+// are decoded once per workgroup on the way in).  Per tile and wave:
+//   S^T = K Q^T   32x32x16 MFMAs, K from LDS as the A operand, the wave's queries in
+//                 registers as the B operand.  Lane l holds scores of query l % 32 only, so
+//                 a row's maximum and sum stay in the lane (its other half in lane l ^ 32);
+//   P             as in the kernel for few rows: already the next product's B operand;
+//   O^T += V^T P^T  V read from LDS transposed.
+// The next tile's loads are in flight in registers meanwhile, and go to the other half of
+// LDS behind the products: one barrier per tile.  Two workgroups share a CU, so that
+// one's exponentials run beside the other's products.
+#pragma once
+
+#include "exl3_attn.hpp"
+
+namespace exl3 {
+
+constexpr int kManyRows = 128;
+
+template <int FMT, typename T, int D>
+struct Many {
+  static constexpr bool kRaw = FMT >= 9;
+  static constexpr int kTokens = D == 256 ? 32 : 64;                    // of a tile
+  static constexpr int kRow = kRaw ? 2 * D : FMT == KV_Q8 ? D : D / 2;  // bytes of a cached head
+  static constexpr int kLanes = kRow / 16;                              // lanes that load a row
+  static constexpr int kRows = 64 / kLanes;                             // rows of a wave's load
+  static constexpr int kMine = kTokens / 4;                             // a wave's rows of a tile
+  static constexpr int kLoads = kMine > kRows ? kMine / kRows : 1;
+  static constexpr int kTile = kTokens * D * 2;                         // bytes in LDS
+  static constexpr int kLds = 4 * kTile;                                // keys and values, twice
+
+  struct Loads {
+    u32x4 k[kLoads], v[kLoads];
+    uint16_t ks[kRaw ? 1 : kLoads], vs[kRaw ? 1 : kLoads];
+  };
+
+  // Byte of 16-byte chunk c of row t.  A key read takes one chunk of 16 rows at a time, a
+  // value read 64 bytes of 4 rows: both fall into different banks.
+  static __device__ __forceinline__ int key_place(int t, int c) {
+    return t * D * 2 + ((c ^ (D == 64 ? (t >> 1) & 7 : t & 15)) << 4);
+  }
+  static __device__ __forceinline__ int value_place(int t, int c) {
+    return t * D * 2 + ((c ^ (D == 64 ? ((t >> 1) & 1) << 2 : (t & 3) << 2)) << 4);
+  }
+
+  // Wave w loads rows kMine w .. of a tile, all of one page: its row of load u.
+  static __device__ __forceinline__ int row_of(int u, int lane) { return u * kRows + lane / kLanes; }
+
+  // The wave's rows of the tile at t0, from page `page`.
+  static __device__ __forceinline__ void load(const AttnParams& p, int kvh, int page, int t, int lane, Loads& x) {
+    const KvCacheView& c = p.cache;
+    const int ch = lane % kLanes;
+    const size_t h = (size_t)max(page, 0) * c.kv_heads + kvh;
+    const int slot = t & ((1 << c.page_shift) - 1);
+    const uint8_t* k = c.k + ((h << c.page_shift) + slot) * kRow;
+    const uint8_t* v = c.v + ((h << c.page_shift) + slot) * kRow;
+    const size_t s = ((h * (D / 32)) << c.page_shift) + slot;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int r = kRows > kMine ? row_of(u, lane) & (kMine - 1) : row_of(u, lane);
+      x.k[u] = *(const u32x4*)(k + r * kRow + ch * 16);
+      x.v[u] = *(const u32x4*)(v + r * kRow + ch * 16);
+      if constexpr (!kRaw) {
+        const int g = ((ch * (16 * D / kRow) / 32) << c.page_shift) + r;
+        x.ks[u] = (c.ks + s)[g];
+        x.vs[u] = (c.vs + s)[g];
+      }
+    }
+  }
+  // One loaded chunk as 16-bit values, n 16-byte chunks in LDS.
+  static __device__ __forceinline__ u32x4 decoded(const u32x4& w, uint16_t scale, int i) {
+    if constexpr (kRaw) return w;
+    const _Float16 s = __builtin_bit_cast(_Float16, scale);
+    const half2v s2 = {s, s};
+    if constexpr (FMT == KV_Q8) {
+      const uint32_t a = w[2 * i], b = w[2 * i + 1];
+      return decode8(a, b, s2);
+    }
+    const uint32_t a = w[i & 3];
+    return decode4_plain(a, s2);
+  }
+  // To LDS from row `first` on; on an edge, values of rows outside [lo, hi) become zeros.
+  // Returns whether an edge's other rows hold a value that is not finite.
+  static __device__ __forceinline__ bool put(const Loads& x, uint8_t* keys, uint8_t* values, int first, int lane,
+                                             bool edge, int lo, int hi) {
+    constexpr int n = kRaw ? 1 : FMT == KV_Q8 ? 2 : 4;
+    const int ch = lane % kLanes;
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int t = first + row_of(u, lane);
+      if (kRows > kMine && row_of(u, lane) >= kMine) continue;
+      const bool live = !edge || (t >= lo && t < hi);
+      if (edge && live) bad = bad || (kRaw ? not_finite<T>(x.v[u]) : (x.vs[kRaw ? 0 : u] & 0x7c00) == 0x7c00);
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        *(u32x4*)(keys + key_place(t, ch * n + i)) = decoded(x.k[u], kRaw ? 0 : x.ks[kRaw ? 0 : u], i);
+        u32x4 v = decoded(x.v[u], kRaw ? 0 : x.vs[kRaw ? 0 : u], i);
+        if (!live) v = u32x4{0, 0, 0, 0};
+        *(u32x4*)(values + value_place(t, ch * n + i)) = v;
+      }
+    }
+    return bad;
+  }
+};
+
+// One-dimensional grid of tiles x splits x kv heads, the heads fastest (blocks go to the
+// XCDs in turn, so a head's tiles share few L2s), a sequence's last and longest tiles first.
+template <int FMT, typename T, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnParams p, int tiles) {
+  typedef Many<FMT, T, D> F;
+  typedef typename T::V8 V8;
+  constexpr int TK = F::kTokens, NT = TK / 32;
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ int retry, page_on[2][4];  // [half of LDS][wave whose rows they are]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = blockIdx.x % p.cache.kv_heads, rest = blockIdx.x / p.cache.kv_heads;
+  const int split = rest % p.splits, tile = tiles - 1 - rest / p.splits;
+  int row0;
+  const Work w = tile_work(p, tile, kManyRows, row0);
+  const int rows = min(w.rows - row0, kManyRows);
+  if (rows <= 0) return;
+  const Seen top = row_sees(p, w.first, w.len, row0), end = row_sees(p, w.first, w.len, row0 + rows - 1);
+  int t0, t1;
+  split_range(top.lo, end.hi, p.splits, split, t0, t1);
+  const size_t slot0 = ((size_t)(tile * p.cache.kv_heads + kvh) * p.splits + split) * kManyRows;
+  if (p.splits > 1 && t0 >= t1) {
+    for (int e = threadIdx.x; e < 2 * rows; e += 256)
+      p.stats[slot0 * 2 + e] = e & 1 ? 0.0f : -__builtin_inff();
+    return;
+  }
+  if (threadIdx.x == 0) retry = 0;
+
+  const int n = lane & 31, h = lane >> 5;
+  // this wave's rows, what all of them see and what any of them sees
+  const int wrow = row0 + 32 * wave;
+  const bool busy = 32 * wave < rows;
+  const int mine = min(wrow + n, row0 + rows - 1);  // rows past the last repeat it; nobody reads them
+  const Seen see = row_sees(p, w.first, w.len, mine);
+  const Seen wtop = row_sees(p, w.first, w.len, min(wrow, row0 + rows - 1));
+  const Seen wend = row_sees(p, w.first, w.len, min(wrow + 31, row0 + rows - 1));
+  V8 q[D / 16];
+  {
+    const size_t qi = (size_t)(w.start + mine / p.group) * p.q_stride +
+                      (size_t)(kvh * p.group + mine % p.group) * D;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) q[s] = load_q8<FMT == KV_Q4 ? KV_Q8 : FMT, T>(p, qi + 16 * s + 8 * h);
+  }
+  float16v o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
+  float m = -__builtin_inff(), l = 0.0f;
+  bool again = false;
+
+  typename F::Loads x;
+  const int off = F::kMine * wave;  // of this wave's rows in a tile
+  auto page_at = [&](int t) { return block_page(p, w, (t + off) & ~15, t1); };
+  auto stage = [&](int t, int page, int half) {
+    uint8_t* buf = lds + half * 2 * F::kTile;
+    // an edge: some row of the workgroup does not see some token of the tile
+    const bool edge = t < end.lo || t + TK > min(top.hi, t1) || page < 0;
+    const bool bad =
+        F::put(x, buf, buf + F::kTile, off, lane, edge, top.lo - t, page < 0 ? 0 : min(end.hi, t1) - t);
+    again = again || (bad && (top.lo < end.lo || top.hi < end.hi));
+    if (lane == 0) page_on[half][wave] = page >= 0;
+  };
+  int page = -1, next = -1;  // of the tile to load next and of the one behind it
+  if (t0 < t1) {
+    const int first = page_at(t0);
+    F::load(p, kvh, first, t0 + off, lane, x);
+    page = page_at(t0 + TK);
+    stage(t0, first, 0);
+  }
+  int cur = 0;
+  for (int t = t0; t < t1; t += TK, cur ^= 1) {
+    __syncthreads();
+    const uint8_t* keys = lds + cur * 2 * F::kTile;
+    const uint8_t* values = keys + F::kTile;
+    const bool more = t + TK < t1;
+    if (more) {
+      next = page_at(t + 2 * TK);
+      F::load(p, kvh, page, t + TK + off, lane, x);
+    }
+    if (busy && t < wend.hi && t + TK > wtop.lo) {
+      float16v s[NT];
+#pragma unroll
+      for (int a = 0; a < NT; ++a) {
+        s[a] = float16v{};
+#pragma unroll
+        for (int st = 0; st < D / 16; ++st) {
+          const V8 key = *(const V8*)(keys + F::key_place(32 * a + n, 2 * st + h));
+          s[a] = T::mfma32(key, q[st], s[a]);
+        }
+      }
+      const int on0 = page_on[cur][0], on1 = page_on[cur][1], on2 = page_on[cur][2], on3 = page_on[cur][3];
+      const bool whole = __builtin_amdgcn_readfirstlane(on0 & on1 & on2 & on3);
+      if (t < wend.lo || t + TK > min(wtop.hi, t1) || !whole) {
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = 32 * a + 8 * (i / 4) + 4 * h + i % 4, at = t + r;
+            const bool live = at >= see.lo && at < min(see.hi, t1) && (F::kMine == 16 ? (a ? (i / 8 ? on3 : on2) : (i / 8 ? on1 : on0)) : (i / 8 ? on2 : on0));
+            s[a][i] = live ? s[a][i] : -__builtin_inff();
+          }
+      }
+      float most = s[0][0];
+#pragma unroll
+      for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, s[a][i]);
+      most *= p.scale2;
+      if (__any(most > m + kSlack)) {
+        most = fmaxf(most, xor_lanes<32>(most));
+        const float up = fmaxf(m, most);
+        const float f = up == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) o[dt] *= f;
+      }
+      const float base = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+      for (int a = 0; a < NT; ++a)
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+          V8 w8;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(s[a][8 * k2 + i], p.scale2, -base));
+            l += e;
+            w8[i] = (typename T::E)e;
+          }
+          const int tok = 32 * a + 16 * k2 + 4 * h + ((lane >> 2) & 3);
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) {
+            const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), half = (lane & 1) * 8;
+            const u32x2 lo = lds_transpose4(values + F::value_place(tok, chunk) + half);
+            const u32x2 hi = lds_transpose4(values + F::value_place(tok + 8, chunk) + half);
+            const u32x4 r = {lo[0], lo[1], hi[0], hi[1]};
+            o[dt] = T::mfma32(__builtin_bit_cast(V8, r), w8, o[dt]);
+          }
+        }
+    }
+    if (more) {
+      stage(t + TK, page, cur ^ 1);
+      page = next;
+    }
+  }
+  if (again) retry = 1;
+  __syncthreads();
+  l += xor_lanes<32>(l);
+  if (retry) {
+    // values that some rows see and others do not were not finite (a zero weight times an
+    // infinity is no zero): one row at a time, touching only what it sees
+    constexpr int E = D / 64;
+    for (int r = wave; r < rows; r += 4) {
+      const int row = row0 + r;
+      const Seen s = row_sees(p, w.first, w.len, row);
+      float rm, rl, acc[E];
+      row_pass<E>(p, w, kvh, row, max(s.lo, t0), min(s.hi, t1), lane, rm, rl, acc);
+      const size_t yi = (size_t)(w.start + row / p.group) * p.y_stride +
+                        (size_t)(kvh * p.group + row % p.group) * D + E * lane;
+      for (int e = 0; e < E; ++e) {
+        if (p.splits == 1)
+          store1(p.y, p.q_type, yi + e, rl != 0.0f ? acc[e] / rl : 0.0f);
+        else
+          p.part[(slot0 + r) * D + E * lane + e] = acc[e];
+      }
+      if (p.splits > 1 && lane == 0) {
+        p.stats[(slot0 + r) * 2] = rm;
+        p.stats[(slot0 + r) * 2 + 1] = rl;
+      }
+    }
+    return;
+  }
+  if (32 * wave + n >= rows) return;
+  if (p.splits > 1) {
+    float* out = p.part + (slot0 + 32 * wave + n) * D;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(float4v*)(out + 32 * dt + 8 * i + 4 * h) =
+            float4v{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
+    if (h == 0) {
+      p.stats[(slot0 + 32 * wave + n) * 2] = m;
+      p.stats[(slot0 + 32 * wave + n) * 2 + 1] = l;
+    }
+    return;
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  const size_t yi = (size_t)(w.start + mine / p.group) * p.y_stride +
+                    (size_t)(kvh * p.group + mine % p.group) * D;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint16_t y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = o[dt][4 * i + e] * inv;
+        y[e] = p.q_type == DT_F16 ? f2h(v) : f2bf(v);
+      }
+      uint16_t* to = (uint16_t*)p.y + yi + 32 * dt + 8 * i + 4 * h;
+      if (p.y_vec) {
+        *(u32x2*)to = u32x2{(uint32_t)y[0] | (uint32_t)y[1] << 16, (uint32_t)y[2] | (uint32_t)y[3] << 16};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = y[e];
+      }
+    }
+}
+
+}  // namespace exl3
