@@ -21,39 +21,80 @@
 
 namespace exl3 {
 
-// The splits of a row joined in their order: grid (rows / 4, kv heads, tiles), a wave
-// per row.  A split that saw nothing has a maximum of -inf, and its sums are not read.
+// The splits of a row joined: grid (rows / rows per workgroup, kv heads, tiles).  D / 4
+// lanes hold a row's sums, four channels each; 2^shift such groups share the splits of
+// one row, so that a row's loads are in flight together, and meet in LDS in a fixed order.
+// A split that saw nothing has a maximum of -inf and a sum of 0, and its sums, which are
+// not written, are not read.
 template <int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63, in_tile = blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows, int shift) {
+  constexpr int L = D / 4, kGroups = 256 / L, kBatch = 8;
+  __shared__ float4v sums[kGroups][L];
+  __shared__ float totals[kGroups];
+  const int group = threadIdx.x / L, lane = threadIdx.x % L;
+  const int per = 1 << shift, part = group & (per - 1);  // groups of a row, which of them
+  const int in_tile = blockIdx.x * (kGroups >> shift) + (group >> shift);
   const int kvh = blockIdx.y, tile = blockIdx.z;
   int row0;
   const Work w = tile_work(p, tile, rows, row0);
   const int row = row0 + in_tile;
-  if (row >= w.rows) return;
+  const bool live = in_tile < rows && row < w.rows;
   const size_t slot = (size_t)(tile * p.cache.kv_heads + kvh) * p.splits * rows + in_tile;
-  float most = -__builtin_inff();
-  for (int s = 0; s < p.splits; ++s) most = fmaxf(most, p.stats[(slot + (size_t)s * rows) * 2]);
-  const float base = most == -__builtin_inff() ? 0.0f : most;
-  float total = 0.0f, acc[E] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const size_t at = slot + (size_t)s * rows;
-    const float m = p.stats[at * 2], l = p.stats[at * 2 + 1];
-    if (m == -__builtin_inff() && l == 0.0f) continue;
-    const float f = __builtin_amdgcn_exp2f(m - base);
-    total += l * f;
+  float4v acc = {0, 0, 0, 0};
+  float total = 0.0f;
+  if (live) {
+    float most = -__builtin_inff();
+    for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
+      float m[kBatch];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += p.part[at * D + E * lane + e] * f;
+      for (int i = 0; i < kBatch; ++i) {
+        const int s = min(s0 + i, p.splits - 1);
+        m[i] = p.stats[(slot + (size_t)s * rows) * 2];
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) most = fmaxf(most, m[i]);
+    }
+    const float base = most == -__builtin_inff() ? 0.0f : most;
+    for (int s0 = part; s0 < p.splits; s0 += per * kBatch) {
+      float f[kBatch], l[kBatch];
+      bool saw[kBatch];
+      float4v v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int s = s0 + i * per;
+        const size_t at = slot + (size_t)min(s, p.splits - 1) * rows;
+        const float m = p.stats[at * 2];
+        l[i] = p.stats[at * 2 + 1];
+        const bool on = s < p.splits && !(m == -__builtin_inff() && l[i] == 0.0f);
+        saw[i] = on;
+        f[i] = on ? __builtin_amdgcn_exp2f(m - base) : 0.0f;
+        l[i] = on ? l[i] : 0.0f;
+        v[i] = *(const float4v*)(p.part + at * D + 4 * lane);  // may be unwritten: see below
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        total += l[i] * f[i];
+        const float4v sum = acc + v[i] * f[i];
+        acc = saw[i] ? sum : acc;
+      }
+    }
+  }
+  sums[group][lane] = acc;
+  if (lane == 0) totals[group] = total;
+  __syncthreads();
+  if (!live || part) return;
+  for (int g = 1; g < per; ++g) {
+    acc += sums[group + g][lane];
+    total += totals[group + g];
   }
   const size_t yi = (size_t)(w.start + row / p.group) * p.y_stride +
-                    (size_t)(kvh * p.group + row % p.group) * D + E * lane;
+                    (size_t)(kvh * p.group + row % p.group) * D + 4 * lane;
 #pragma unroll
-  for (int e = 0; e < E; ++e) store1(p.y, p.q_type, yi + e, total != 0.0f ? acc[e] / total : 0.0f);
+  for (int e = 0; e < 4; ++e) store1(p.y, p.q_type, yi + e, total != 0.0f ? acc[e] / total : 0.0f);
 }
-template __global__ void attn_join_kernel<64>(AttnParams, int);
-template __global__ void attn_join_kernel<128>(AttnParams, int);
-template __global__ void attn_join_kernel<256>(AttnParams, int);
+template __global__ void attn_join_kernel<64>(AttnParams, int, int);
+template __global__ void attn_join_kernel<128>(AttnParams, int, int);
+template __global__ void attn_join_kernel<256>(AttnParams, int, int);
 
 #define EXL3_FEW_D(M, FMT, T) \
   M(FMT, T, 64, 1) M(FMT, T, 64, 2) M(FMT, T, 128, 1) M(FMT, T, 128, 2) M(FMT, T, 256, 1)
@@ -98,9 +139,10 @@ Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int h
   const int64_t room = (int64_t)b.table_pages << c.page_shift;
   const int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;
   const int64_t groups = s.tiles * c.kv_heads;
-  const int64_t want = (512 + groups - 1) / groups;
+  static const int tgt = getenv("DEV_TGT") ? atoi(getenv("DEV_TGT")) : 512;
+  const int64_t want = (tgt + groups - 1) / groups;
   s.splits = (int)std::max<int64_t>(
-      1, std::min(std::min<int64_t>(want, 64), (most + 127) / (s.few ? 128 : 256)));
+      1, std::min(std::min<int64_t>(want, getenv("DEV_MAX") ? atoi(getenv("DEV_MAX")) : 64), (most + 127) / (s.few ? 128 : 256)));
   return s;
 }
 
@@ -221,13 +263,20 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   if (int rc = check_launch("attention")) return rc;
   if (sh.splits == 1) return EXL3_OK;
   if (int rc = launch_gate("attention join")) return rc;
-  const dim3 grid((unsigned)(sh.rows / 4), (unsigned)p.cache.kv_heads, (unsigned)sh.tiles);
+  const int rows_most = (int)std::min<int64_t>(sh.rows, (int64_t)batch->max_q * p.group);
+  // as many groups of lanes per row as there are batches of splits to share
+  const int groups = 1024 / D;
+  int shift = 0;
+  while ((2 << shift) <= groups && (1 << shift) < sh.splits) ++shift;
+  const int per_block = groups >> shift;
+  const dim3 grid((unsigned)((rows_most + per_block - 1) / per_block), (unsigned)p.cache.kv_heads,
+                  (unsigned)sh.tiles);
   if (D == 64)
-    hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(256), 0, s, p, sh.rows);
+    hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(256), 0, s, p, sh.rows, shift);
   else if (D == 128)
-    hipLaunchKernelGGL(attn_join_kernel<128>, grid, dim3(256), 0, s, p, sh.rows);
+    hipLaunchKernelGGL(attn_join_kernel<128>, grid, dim3(256), 0, s, p, sh.rows, shift);
   else
-    hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(256), 0, s, p, sh.rows);
+    hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(256), 0, s, p, sh.rows, shift);
   return check_launch("attention join");
 }
 

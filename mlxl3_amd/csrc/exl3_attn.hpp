@@ -70,47 +70,6 @@ __device__ __forceinline__ bool not_finite(const u32x4& v) {
   return bad;
 }
 
-// Eight 8-bit codes (code + 128) times a scale: byte b between 0x64 and itself is the f16
-// 1024 + b, and 1024 + b - 1152 is exact.
-__device__ __forceinline__ u32x4 decode8(uint32_t w0, uint32_t w1, half2v s) {
-  const half2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-  u32x4 r;
-  r[0] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u);
-  r[1] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u);
-  r[2] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u);
-  r[3] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t x = r[i];
-    r[i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, x) + off) * s);
-  }
-  return r;
-}
-
-// Eight 4-bit codes (code + 8) times a scale, in the order 0 4 1 5 2 6 3 7: a nibble in
-// the lowest or second-lowest place of an f16's mantissa under the exponent of 1024 is
-// 1024 + n or 1024 + 16 n.
-__device__ __forceinline__ u32x4 decode4(uint32_t w, half2v s) {
-  const half2v off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-  const half2v part = {(_Float16)0.0625f, (_Float16)0.0625f}, off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
-  u32x4 r;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t v = w >> (8 * i);
-    const uint32_t lo = (v & 0x000f000fu) | 0x64006400u, hi = (v & 0x00f000f0u) | 0x64006400u;
-    r[2 * i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, lo) + off) * s);
-    r[2 * i + 1] = __builtin_bit_cast(
-        uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, hi), part, off16) * s);
-  }
-  return r;
-}
-// decode4 in the channels' own order.
-__device__ __forceinline__ u32x4 decode4_plain(uint32_t w, half2v s) {
-  const u32x4 d = decode4(w, s);
-  const uint32_t a = d[0], b = d[1], c = d[2], e = d[3];
-  return u32x4{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(e, c, 0x05040100u),
-               __builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(e, c, 0x07060302u)};
-}
 // Where channel e of eight lies in decode4's order, and which channel lies at place e.
 __device__ __forceinline__ constexpr int place4(int e) { return e < 4 ? 2 * e : 2 * e - 7; }
 __device__ __forceinline__ constexpr int channel4(int e) { return (e >> 1) | ((e & 1) << 2); }
@@ -205,13 +164,16 @@ __device__ __forceinline__ Work tile_work(const AttnParams& p, int tile, int row
   return Work{0, 0, 0, 0, 0};
 }
 
-// The page that holds the 16 tokens from t (a multiple of 16) on, or -1.  Wave-uniform: a
-// scalar load (no kernel writes the table).
-__device__ __forceinline__ int block_page(const AttnParams& p, const Work& w, int t, int hi) {
+// The table's entry for the 16 tokens from t (a multiple of 16) on, hi > 0 the end of the
+// tokens in use.  Wave-uniform: a scalar load (no kernel writes the table), not waited for
+// here; page_ok says later whether it names a page.
+__device__ __forceinline__ int table_entry(const AttnParams& p, const Work& w, int t, int hi) {
   typedef const __attribute__((address_space(4))) int32_t* ScalarPtr;
-  if (t >= hi) return -1;
-  const int32_t page = ((ScalarPtr)(size_t)p.batch.table)[(int64_t)w.seq * p.batch.table_pages + (t >> p.cache.page_shift)];
-  return page >= 0 && page < p.cache.pages ? page : -1;
+  const int at = min(t, hi - 1) >> p.cache.page_shift;
+  return ((ScalarPtr)(size_t)p.batch.table)[(int64_t)w.seq * p.batch.table_pages + at];
+}
+__device__ __forceinline__ int page_ok(const AttnParams& p, int entry, int t, int hi) {
+  return t < hi && entry >= 0 && entry < p.cache.pages ? entry : -1;
 }
 
 __device__ __forceinline__ float wave_sum(float v) {

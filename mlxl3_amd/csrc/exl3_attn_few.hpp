@@ -36,26 +36,32 @@ struct Few {
   static constexpr int kLanes = kRow / 16, kRows = 64 / kLanes, kValueLoads = 32 / kRows;
   static constexpr int kWaveLds = 32 * D * 2 > 16 * RT * D * 4 ? 32 * D * 2 : 16 * RT * D * 4;
 
+  // steps whose loads are in flight (16-bit caches: one has 16 KB of a wave in flight)
+  static constexpr int kAhead = 1;
+
   // First channel of lane group g's operand in MFMA step s.
   static __device__ __forceinline__ int channel(int s, int g) {
     constexpr int n = kVec / 8;
     return (s / n) * 4 * kVec + g * kVec + (s % n) * 8;
   }
   // Byte of 16-byte chunk c of row t of the values in LDS.  The transposing read takes 32
-  // bytes of each of 8 rows at a time: pairs of chunks change places so that those fall
-  // into different banks.
+  // bytes (a pair of chunks) of each of 8 rows at a time: pairs change places so that
+  // those fall into different banks.  A write of decoded codes takes every 2nd or 4th
+  // chunk of one to eight rows: the two of a pair change places too so that those do.
   static __device__ __forceinline__ int place(int t, int c) {
-    const int swz = D == 64 ? ((t >> 1) & 3) << 1 : (t & 7) << 1;
-    return t * D * 2 + ((c ^ swz) << 4);
+    const int r = D == 64 ? t >> 1 : t;  // rows that start in the same bank
+    const int odd = kRaw ? 0 : D == 256 ? c >> 4 : FMT == KV_Q8 ? r : r >> 1;
+    const int swz = D == 64 ? (r & 3) << 1 : (r & 7) << 1;
+    return t * D * 2 + ((c ^ swz ^ (odd & 1)) << 4);
   }
 
   struct Keys {
     uint32_t w[2][kKeyLoads][kKeyWords];
-    uint16_t s[2][kRaw ? 1 : kKeyLoads];
+    uint32_t s[2][kRaw ? 1 : kKeyLoads];  // (16-bit elements would go through scratch)
   };
   struct Values {
     u32x4 w[kValueLoads];
-    uint16_t s[kRaw ? 1 : kValueLoads];
+    uint32_t s[kRaw ? 1 : kValueLoads];
   };
 
   static __device__ __forceinline__ void load_keys(const AttnParams& p, const int (&page)[2], int kvh, int t0,
@@ -93,7 +99,7 @@ struct Few {
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[e] = k.w[a][u][e];
     } else {
-      const _Float16 sc = __builtin_bit_cast(_Float16, k.s[a][u]);
+      const _Float16 sc = __builtin_bit_cast(_Float16, (uint16_t)k.s[a][u]);
       const half2v s2 = {sc, sc};
       if constexpr (FMT == KV_Q8)
         r = decode8(k.w[a][u][2 * i], k.w[a][u][2 * i + 1], s2);
@@ -145,7 +151,7 @@ struct Few {
       for (int i = 0; i < n; ++i) {
         u32x4 x = v.w[u];
         if constexpr (!kRaw) {
-          const _Float16 sc = __builtin_bit_cast(_Float16, v.s[u]);
+          const _Float16 sc = __builtin_bit_cast(_Float16, (uint16_t)v.s[u]);
           const half2v s2 = {sc, sc};
           if constexpr (FMT == KV_Q8) {
             const uint32_t w0 = v.w[u][2 * i], w1 = v.w[u][2 * i + 1];
@@ -173,7 +179,7 @@ struct Few {
 
 // grid (splits, kv heads, sequences)
 template <int FMT, typename T, int D, int RT>
-__global__ __launch_bounds__(256, D == 256 || RT == 2 ? 1 : 2) void attn_few_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnParams p) {
   typedef Few<FMT, T, D, RT> F;
   typedef typename T::V8 V8;
   extern __shared__ __align__(16) uint8_t lds[];  // 4 kWaveLds
@@ -222,19 +228,33 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 1 : 2) void attn_few_ker
   }
   bool again = false;
 
-  typename F::Keys k;
-  typename F::Values v;
-  int t = t0 + 32 * wave;
-  int page[2], next[2];
-  if (t < t1) {
+  constexpr int A = F::kAhead;
+  typename F::Keys keys[A];
+  typename F::Values vals[A];
+  int pages[A][2], next[A][2];  // of the steps loaded; the table's entries for those behind them
+  const int first = t0 + 32 * wave;
+  auto find = [&](int t, int (&entry)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) page[a] = block_page(p, w, t + 16 * a, t1);
+    for (int a = 0; a < 2; ++a) entry[a] = table_entry(p, w, t + 16 * a, max(t1, 1));
+  };
+  // always, so that the wait for one step's loads can leave the later ones in flight
+  // (behind the end they read the pool's first page, and nobody uses that)
+  auto load = [&](int t, const int (&entry)[2], int (&page)[2], typename F::Keys& k,
+                  typename F::Values& v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) page[a] = page_ok(p, entry[a], t + 16 * a, t1);
     F::load_keys(p, page, kvh, t, lane, k);
     F::load_values(p, page, kvh, t, lane, v);
+  };
+  if (w.len > 0) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) next[a] = block_page(p, w, t + 128 + 16 * a, t1);
+    for (int j = 0; j < A; ++j) find(first + 128 * j, next[j]);
+#pragma unroll
+    for (int j = 0; j < A; ++j) load(first + 128 * j, next[j], pages[j], keys[j], vals[j]);
+#pragma unroll
+    for (int j = 0; j < A; ++j) find(first + 128 * (j + A), next[j]);
   }
-  for (; t < t1; t += 128) {
+  auto step = [&](const int t, typename F::Keys& k, typename F::Values& v, int (&page)[2], int (&next)[2]) __attribute__((always_inline)) {
     const bool edge = t < end.lo || t + 32 > min(top.hi, t1) || page[0] < 0 || page[1] < 0;
     float4v s[RT][2];
 #pragma unroll
@@ -259,15 +279,7 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 1 : 2) void attn_few_ker
     } else {
       F::template put_values<false>(v, my, lane, 0, 32, true, true);
     }
-    if (t + 128 < t1) {
-      F::load_keys(p, next, kvh, t + 128, lane, k);
-      F::load_values(p, next, kvh, t + 128, lane, v);
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        page[a] = next[a];
-        next[a] = block_page(p, w, t + 256 + 16 * a, t1);
-      }
-    }
+    load(t + 128 * A, next, page, k, v);
     V8 w8[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -307,7 +319,15 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 1 : 2) void attn_few_ker
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) o[rt][dt] = T::mfma16(val, w8[rt], o[rt][dt]);
     }
-  }
+    // here, where no LDS read is waited for before the next step's keys are (a wait for one
+    // waits for scalar loads as well)
+    find(t + 256 * A, next);
+  };
+  for (int t = first; t < t1; t += 128 * A)
+    static_for<A>([&](auto j_) {
+      constexpr int j = decltype(j_)::value;
+      if (t + 128 * j < t1) step(t + 128 * j, keys[j], vals[j], pages[j], next[j]);
+    });
 
   // the waves' results: maxima and sums, then weighted sums [row][channel] in LDS
   if (again) retry = 1;
@@ -348,28 +368,58 @@ __global__ __launch_bounds__(256, D == 256 || RT == 2 ? 1 : 2) void attn_few_ker
     }
     __syncthreads();
   }
-  for (int e = threadIdx.x; e < w.rows * D; e += 256) {
-    const int row = e / D, d = e % D;
-    const int at = row * D + (FMT == KV_Q4 ? (d & ~7) | place4(d & 7) : d);
+  // per row: the common maximum, the waves' weights against it, their sum
+  if (threadIdx.x < 16 * RT) {
+    const int row = threadIdx.x;
     float most = wave_m[0][row];
 #pragma unroll
     for (int i = 1; i < 4; ++i) most = fmaxf(most, wave_m[i][row]);
     const float base = most == -__builtin_inff() ? 0.0f : most;
-    float sum = 0.0f, total = 0.0f;
+    float total = 0.0f, f[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float f = __builtin_amdgcn_exp2f(wave_m[i][row] - base);
-      total += wave_l[i][row] * f;
-      sum += ((const float*)(lds + i * F::kWaveLds))[at] * f;
+      f[i] = __builtin_amdgcn_exp2f(wave_m[i][row] - base);
+      total += wave_l[i][row] * f[i];
+    }
+    const float norm = p.splits > 1 ? 1.0f : total != 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wave_l[i][row] = f[i] * norm;
+    if (p.splits > 1 && row < w.rows) {
+      const size_t slot = ((size_t)(seq * p.cache.kv_heads + kvh) * p.splits + split) * (16 * RT) + row;
+      p.stats[slot * 2] = most;
+      p.stats[slot * 2 + 1] = total;
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < w.rows * (D / 4); e += 256) {
+    const int row = e / (D / 4), d = e % (D / 4) * 4;
+    float sum[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = wave_l[i][row];
+      const float* from = (const float*)(lds + i * F::kWaveLds) + row * D;
+      if constexpr (FMT == KV_Q4) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] += from[(d & ~7) | place4((d & 4) + c)] * f;
+      } else {
+        const float4v v = *(const float4v*)(from + d);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] += v[c] * f;
+      }
     }
     if (p.splits == 1) {
-      const size_t yi = (size_t)(w.start + row / p.group) * p.y_stride +
-                        (size_t)(kvh * p.group + row % p.group) * D + d;
-      store1(p.y, p.q_type, yi, total != 0.0f ? sum / total : 0.0f);
+      uint16_t* to = (uint16_t*)p.y + (size_t)(w.start + row / p.group) * p.y_stride +
+                     (size_t)(kvh * p.group + row % p.group) * D + d;
+      const u32x2 y = {pack2(p.q_type, sum[0], sum[1]), pack2(p.q_type, sum[2], sum[3])};
+      if (p.y_vec) {
+        *(u32x2*)to = y;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) to[c] = (uint16_t)(y[c / 2] >> (16 * (c & 1)));
+      }
     } else {
       const size_t slot = ((size_t)(seq * p.cache.kv_heads + kvh) * p.splits + split) * (16 * RT) + row;
-      p.part[slot * D + d] = sum;
-      if (d < 2) p.stats[slot * 2 + d] = d ? total : most;
+      *(float4v*)(p.part + slot * D + d) = float4v{sum[0], sum[1], sum[2], sum[3]};
     }
   }
 }

@@ -34,7 +34,7 @@ struct Many {
 
   struct Loads {
     u32x4 k[kLoads], v[kLoads];
-    uint16_t ks[kRaw ? 1 : kLoads], vs[kRaw ? 1 : kLoads];
+    uint32_t ks[kRaw ? 1 : kLoads], vs[kRaw ? 1 : kLoads];  // (16-bit elements would go through scratch)
   };
 
   // Byte of 16-byte chunk c of row t.  A key read takes one chunk of 16 rows at a time, a
@@ -71,9 +71,9 @@ struct Many {
     }
   }
   // One loaded chunk as 16-bit values, n 16-byte chunks in LDS.
-  static __device__ __forceinline__ u32x4 decoded(const u32x4& w, uint16_t scale, int i) {
+  static __device__ __forceinline__ u32x4 decoded(const u32x4& w, uint32_t scale, int i) {
     if constexpr (kRaw) return w;
-    const _Float16 s = __builtin_bit_cast(_Float16, scale);
+    const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)scale);
     const half2v s2 = {s, s};
     if constexpr (FMT == KV_Q8) {
       const uint32_t a = w[2 * i], b = w[2 * i + 1];
@@ -157,7 +157,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnPa
 
   typename F::Loads x;
   const int off = F::kMine * wave;  // of this wave's rows in a tile
-  auto page_at = [&](int t) { return block_page(p, w, (t + off) & ~15, t1); };
+  auto entry_at = [&](int t) { return table_entry(p, w, (t + off) & ~15, t1); };
+  auto page_at = [&](int entry, int t) { return page_ok(p, entry, (t + off) & ~15, t1); };
   auto stage = [&](int t, int page, int half) {
     uint8_t* buf = lds + half * 2 * F::kTile;
     // an edge: some row of the workgroup does not see some token of the tile
@@ -167,12 +168,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnPa
     again = again || (bad && (top.lo < end.lo || top.hi < end.hi));
     if (lane == 0) page_on[half][wave] = page >= 0;
   };
-  int page = -1, next = -1;  // of the tile to load next and of the one behind it
+  int page = -1, next = -1;  // of the tile in flight; the table's entry for the one behind it
   if (t0 < t1) {
-    const int first = page_at(t0);
-    F::load(p, kvh, first, t0 + off, lane, x);
-    page = page_at(t0 + TK);
-    stage(t0, first, 0);
+    next = entry_at(t0);
+    page = page_at(next, t0);
+    F::load(p, kvh, page, t0 + off, lane, x);
+    next = entry_at(t0 + TK);
+    stage(t0, page, 0);
   }
   int cur = 0;
   for (int t = t0; t < t1; t += TK, cur ^= 1) {
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnPa
     const uint8_t* values = keys + F::kTile;
     const bool more = t + TK < t1;
     if (more) {
-      next = page_at(t + 2 * TK);
+      page = page_at(next, t + TK);
       F::load(p, kvh, page, t + TK + off, lane, x);
     }
     if (busy && t < wend.hi && t + TK > wtop.lo) {
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnPa
     }
     if (more) {
       stage(t + TK, page, cur ^ 1);
-      page = next;
+      next = entry_at(t + 2 * TK);
     }
   }
   if (again) retry = 1;

@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 #include "../../include/exl3_hip.h"
 #include "exl3_kv_host.hpp"
@@ -50,7 +51,7 @@ __device__ __forceinline__ void sincos64(double t, double* s_out, double* c_out)
   c = fma(c, z, 1.0 / 24.0);
   c = fma(c, z, -0.5);
   c = fma(c, z, 1.0);
-  const int q = (int)((int64_t)k & 3);
+  const int q = (int)(k - 4.0 * floor(0.25 * k));
   const double a = q & 1 ? c : s, b = q & 1 ? s : c;
   *s_out = q & 2 ? -a : a;
   *c_out = (q + 1) & 2 ? -b : b;
@@ -69,8 +70,7 @@ __device__ __forceinline__ float2 rope_cs(const RopeView& r, int64_t pos, int i)
   return make_float2((float)(c * r.scale), (float)(s * r.scale));
 }
 
-constexpr int kMaxDim = 256;        // largest head
-constexpr int kRopeTokens = 4;      // tokens per workgroup of the kernels below
+constexpr int kBatch = 4;     // heads whose loads a thread has in flight
 
 struct RopeParams {
   const void* x;
@@ -80,94 +80,118 @@ struct RopeParams {
   RopeView rope;
   int64_t tokens, x_stride, y_stride;
   int heads, head_dim, x_type, y_type;
+  int lanes;  // per token: a thread's channels (below) are the same in all heads
+  int per;    // heads of a workgroup
 };
 
-// grid ceil(tokens / kRopeTokens).  VEC: a work item is eight pairs (two chunks of
-// eight channels, or one chunk of neighbours) or a chunk behind the rotated
-// channels; else one pair or one channel.  An item loads all it needs before it
-// stores, so y may be x.
-template <bool VEC>
+// grid (tokens / (256 / lanes), heads / per).  A thread has, of one token's heads in turn,
+// VEC: eight pairs (two chunks of eight channels, or one chunk of neighbours) or a chunk
+// behind the rotated channels; else one pair or one channel.  Its cosines and sines stay in
+// registers.  It loads all it needs of a head before it stores, so y may be x.  BYTES: of a
+// value of x (VEC).
+template <bool VEC, int BYTES>
 __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
-  __shared__ float2 cs[kRopeTokens][kMaxDim / 2];
-  __shared__ int live[kRopeTokens];
-  const int64_t t0 = (int64_t)blockIdx.x * kRopeTokens;
-  const int nt = (int)min((int64_t)kRopeTokens, p.tokens - t0);
-  const int r = p.rope.pairs;
-  for (int e = threadIdx.x; e < nt * r; e += 256) {
-    const int t = e / r, i = e - t * r;
-    int64_t pos = 0;
-    bool on = true;
-    if (p.positions) {
-      pos = p.positions[t0 + t];
-    } else {
-      const int seq = kv_sequence(p.batch, t0 + t);
-      on = seq >= 0;
-      if (on) pos = kv_position(p.batch, seq, t0 + t);
+  __shared__ float2 cs[2048];        // [tokens][pairs]: at most 8 pairs a lane
+  __shared__ int64_t position[256];
+  constexpr int W = VEC ? 8 : 1;
+  const int L = p.lanes, most = 256 / L, r = p.rope.pairs;
+  const int64_t t0 = (int64_t)blockIdx.x * most;
+  const int nt = (int)min((int64_t)most, p.tokens - t0);
+  const int t = threadIdx.x / L, c = threadIdx.x - t * L;
+  const bool two = !p.rope.interleaved;  // the pair's second half lies r channels further
+  const int turned = VEC && !two ? 2 * r / W : r / W;
+  const bool tail = c >= turned;
+  bool on = t < nt;
+  int64_t pos = 0;
+  if (p.positions) {
+    if (on) pos = p.positions[t0 + t];
+  } else {
+    // the wave's tokens, one by one
+    const int first = __builtin_amdgcn_readfirstlane(t), last = min(__builtin_amdgcn_readlane(t, 63), nt - 1);
+    int seq = -1;
+    for (int i = first; i <= last; ++i) {
+      const KvToken at = kv_locate(p.batch, t0 + i);
+      if (t == i) {
+        seq = at.seq;
+        pos = at.pos;
+      }
     }
-    cs[t][i] = rope_cs(p.rope, pos, i);
-    if (i == 0) live[t] = on;
+    on = on && seq >= 0;
+  }
+  const int h0 = blockIdx.y * p.per, h1 = min(h0 + p.per, p.heads);
+  const int da = tail ? 2 * r + (c - turned) * W : !two ? c * (VEC ? 8 : 2) : c * W;
+  const int db = two ? da + r : da + 1;  // db: not with neighbours of a chunk
+  const size_t xr = (size_t)(t0 + t) * p.x_stride, yr = (size_t)(t0 + t) * p.y_stride;
+  Raw8<BYTES> a[VEC ? kBatch : 1], b[VEC ? kBatch : 1];
+  float fa[VEC ? 1 : kBatch], fb[VEC ? 1 : kBatch];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (!on || h + u >= h1) continue;
+      const size_t row = xr + (size_t)(h + u) * p.head_dim;
+      if constexpr (VEC) {
+        a[u].load(p.x, row + da, true);
+        if (two && !tail) b[u].load(p.x, row + db, true);
+      } else {
+        fa[u] = load1(p.x, p.x_type, row + da);
+        if (!tail) fb[u] = load1(p.x, p.x_type, row + db);
+      }
+    }
+  };
+  load(h0);
+  if (c == 0 && t < nt) position[t] = pos;
+  __syncthreads();
+  for (int j = threadIdx.x; j < nt * r; j += 256) {
+    const int i = j / r;
+    cs[j] = rope_cs(p.rope, position[i], j - i * r);
   }
   __syncthreads();
-  const int W = VEC ? 8 : 1;
-  // items of a head: rotated ones, then the channels behind them
-  const int turned = p.rope.interleaved && VEC ? 2 * r / W : r / W;
-  const int per_head = turned + (p.head_dim - 2 * r) / W;
-  const int per_token = per_head * p.heads;
-  for (int e = threadIdx.x; e < nt * per_token; e += 256) {
-    const int t = e / per_token, i = e - t * per_token;
-    const int h = i / per_head, c = i - h * per_head;
-    if (!live[t]) continue;
-    const size_t xr = (size_t)(t0 + t) * p.x_stride + (size_t)h * p.head_dim;
-    const size_t yr = (size_t)(t0 + t) * p.y_stride + (size_t)h * p.head_dim;
-    if (c >= turned) {
-      const int d = 2 * r + (c - turned) * W;
-      if (p.x == p.y) continue;
+  if (!on || (tail && p.x == p.y)) return;
+  constexpr int N = VEC ? 8 : 1;
+  float2 f[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) f[n] = cs[tail ? 0 : min(t * r + (two ? c * W : c * (VEC ? 4 : 1)) + n, 2047)];
+  for (int h = h0; h < h1; h += kBatch) {
+    if (h > h0) load(h);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (h + u >= h1) continue;
+      const size_t row = yr + (size_t)(h + u) * p.head_dim;
       if constexpr (VEC) {
-        float v[8];
-        load8(p.x, p.x_type, xr + d, true, v);
-        store8(p.y, p.y_type, yr + d, true, v);
-      } else {
-        store1(p.y, p.y_type, yr + d, load1(p.x, p.x_type, xr + d));
-      }
-    } else if constexpr (VEC) {
-      if (p.rope.interleaved) {
-        float v[8];
-        load8(p.x, p.x_type, xr + 8 * c, true, v);
+        float x[8], z[8];
+        a[u].get(p.x_type, x);
+        if (!tail && two) {
+          b[u].get(p.x_type, z);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float2 f = cs[t][4 * c + n];
-          const float a = v[2 * n], b = v[2 * n + 1];
-          v[2 * n] = a * f.x - b * f.y;
-          v[2 * n + 1] = a * f.y + b * f.x;
-        }
-        store8(p.y, p.y_type, yr + 8 * c, true, v);
-      } else {
-        float a[8], b[8];
-        load8(p.x, p.x_type, xr + 8 * c, true, a);
-        load8(p.x, p.x_type, xr + r + 8 * c, true, b);
+          for (int n = 0; n < 8; ++n) {
+            const float v = x[n], w = z[n];
+            x[n] = v * f[n].x - w * f[n].y;
+            z[n] = v * f[n].y + w * f[n].x;
+          }
+          store8(p.y, p.y_type, row + db, z);
+        } else if (!tail) {
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 f = cs[t][8 * c + n];
-          const float u = a[n], w = b[n];
-          a[n] = u * f.x - w * f.y;
-          b[n] = u * f.y + w * f.x;
+          for (int n = 0; n < 4; ++n) {
+            const float v = x[2 * n], w = x[2 * n + 1];
+            x[2 * n] = v * f[n].x - w * f[n].y;
+            x[2 * n + 1] = v * f[n].y + w * f[n].x;
+          }
         }
-        store8(p.y, p.y_type, yr + 8 * c, true, a);
-        store8(p.y, p.y_type, yr + r + 8 * c, true, b);
+        store8(p.y, p.y_type, row + da, x);
+      } else if (tail) {
+        store1(p.y, p.y_type, row + da, fa[u]);
+      } else {
+        store1(p.y, p.y_type, row + da, fa[u] * f[0].x - fb[u] * f[0].y);
+        store1(p.y, p.y_type, row + db, fa[u] * f[0].y + fb[u] * f[0].x);
       }
-    } else {
-      const int da = p.rope.interleaved ? 2 * c : c, db = p.rope.interleaved ? 2 * c + 1 : c + r;
-      const float a = load1(p.x, p.x_type, xr + da), b = load1(p.x, p.x_type, xr + db);
-      const float2 f = cs[t][c];
-      store1(p.y, p.y_type, yr + da, a * f.x - b * f.y);
-      store1(p.y, p.y_type, yr + db, a * f.y + b * f.x);
     }
   }
 }
 
 // The host code below is left out of the device pass, which needs the instances spelled out.
-template __global__ void rope_kernel<true>(RopeParams);
-template __global__ void rope_kernel<false>(RopeParams);
+template __global__ void rope_kernel<true, 2>(RopeParams);
+template __global__ void rope_kernel<true, 4>(RopeParams);
+template __global__ void rope_kernel<false, 2>(RopeParams);
 
 // The scale of a group whose largest magnitude is `most` (NaN where it is not finite).
 __device__ __forceinline__ uint16_t group_scale(float most, float levels) {
@@ -191,117 +215,161 @@ struct AppendParams {
   RopeView rope;
   const void *k, *v;
   int64_t tokens, k_stride, v_stride;
-  int type, vec;  // vec: rows of k and v are 16-byte aligned
+  int type, vec;     // vec: rows of k and v are 16-byte aligned
+  int heads, parts;  // heads of a workgroup, and workgroups for all heads of a side
 };
 
-// grid ceil(tokens / kRopeTokens): a work item is eight channels of one head of one
-// token's key or value; a quantised group is the items of four neighbouring lanes.
+// The workgroups of an append or a read: 256 / (D / 8) tokens each (a thread has eight
+// channels of one token), blockIdx.y the keys' or values' side and a few heads.
+template <int D>
+struct Tile {
+  static constexpr int kLanes = D / 8, kTokens = 256 / kLanes;
+  int token, d0;     // the thread's token in the workgroup and its first channel
+  bool value;
+  int h0, h1;
+  __device__ __forceinline__ Tile(int heads, int parts, int kv_heads) {
+    token = threadIdx.x / kLanes;
+    d0 = (threadIdx.x % kLanes) * 8;
+    value = (int)blockIdx.y >= parts;
+    h0 = ((int)blockIdx.y - (value ? parts : 0)) * heads;
+    h1 = min(h0 + heads, kv_heads);
+  }
+  // The thread's token, or seq = -1 behind the last.
+  __device__ __forceinline__ KvToken locate(const KvBatchView& b, int64_t t0, int64_t tokens) const {
+    constexpr int n = 64 / kLanes;  // tokens of a wave
+    const int wave = threadIdx.x >> 6;
+    KvToken mine{-1, 0};
+    for (int i = 0; i < n; ++i) {
+      const int64_t t = t0 + wave * n + i;
+      if (t >= tokens) break;
+      const KvToken at = kv_locate(b, t);
+      if (token == wave * n + i) mine = at;
+    }
+    return mine;
+  }
+};
+
+// grid (tokens, sides x parts): a quantised group is the channels of four neighbouring
+// lanes.
+template <int FMT, int D, int BYTES>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
-  __shared__ float2 cs[kRopeTokens][kMaxDim / 2];
-  __shared__ int64_t page_of[kRopeTokens];
-  __shared__ int64_t pos_of[kRopeTokens];
+  typedef Tile<D> W;
+  __shared__ float2 cs[W::kTokens][D / 2];
+  __shared__ int64_t positions[W::kTokens];
   const KvCacheView& c = p.cache;
-  const int64_t t0 = (int64_t)blockIdx.x * kRopeTokens;
-  const int nt = (int)min((int64_t)kRopeTokens, p.tokens - t0);
-  if ((int)threadIdx.x < nt) {
-    const int seq = kv_sequence(p.batch, t0 + threadIdx.x);
-    const int64_t pos = seq < 0 ? -1 : kv_position(p.batch, seq, t0 + threadIdx.x);
-    page_of[threadIdx.x] = seq < 0 ? -1 : kv_page(c, p.batch, seq, pos);
-    pos_of[threadIdx.x] = pos;
-  }
-  __syncthreads();
-  const int r = p.rope.freq ? p.rope.pairs : 0;
-  for (int e = threadIdx.x; e < nt * r; e += 256) {
-    const int t = e / r, i = e - t * r;
-    cs[t][i] = rope_cs(p.rope, pos_of[t], i);
-  }
-  if (r) __syncthreads();
-  const int D = c.head_dim, chunks = D / 8, per_side = chunks * c.kv_heads;
-  const int pmask = (1 << c.page_shift) - 1;
-  for (int e = threadIdx.x; e < nt * 2 * per_side; e += 256) {
-    const int t = e / (2 * per_side), i = e - t * 2 * per_side;
-    const bool value = i >= per_side;
-    const int j = value ? i - per_side : i, h = j / chunks, d0 = (j - h * chunks) * 8;
-    if (page_of[t] < 0) continue;  // the four lanes of a group leave together
-    const void* src = value ? p.v : p.k;
-    const size_t row =
-        (size_t)(t0 + t) * (value ? p.v_stride : p.k_stride) + (size_t)h * D;
-    float x[8];
-    load8(src, p.type, row + d0, p.vec, x);
-    if (!value && d0 < 2 * r) {
-      if (p.rope.interleaved) {
+  const W w(p.heads, p.parts, c.kv_heads);
+  const int64_t t0 = (int64_t)blockIdx.x * W::kTokens;
+  const int nt = (int)min((int64_t)W::kTokens, p.tokens - t0);
+  const int r = p.rope.freq && !w.value ? p.rope.pairs : 0;
+  const bool half = !p.rope.interleaved && r % 8 == 0 && w.d0 < 2 * r, second = w.d0 >= r;
+  const void* src = w.value ? p.v : p.k;
+  const size_t row = (size_t)(t0 + w.token) * (w.value ? p.v_stride : p.k_stride) + w.d0;
+  Raw8<BYTES> x[kBatch], other[kBatch];
+  auto load = [&](int h0) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          if (d0 / 2 + n < r) {
-            const float2 f = cs[t][d0 / 2 + n];
-            const float a = x[2 * n], b = x[2 * n + 1];
-            x[2 * n] = a * f.x - b * f.y;
-            x[2 * n + 1] = a * f.y + b * f.x;
+    for (int u = 0; u < kBatch; ++u) {
+      if (h0 + u >= w.h1 || w.token >= nt) continue;
+      const size_t at = row + (size_t)(h0 + u) * D;
+      x[u].load(src, at, p.vec);
+      if (half) other[u].load(src, second ? at - r : at + r, p.vec);
+    }
+  };
+  load(w.h0);
+  const KvToken at = w.locate(p.batch, t0, p.tokens);
+  if (r) {
+    if (w.d0 == 0) positions[w.token] = at.pos;
+    __syncthreads();
+    for (int j = threadIdx.x; j < nt * r; j += 256) {
+      const int t = j / r;
+      cs[t][j - t * r] = rope_cs(p.rope, positions[t], j - t * r);
+    }
+    __syncthreads();
+  }
+  const int64_t page = at.seq < 0 ? -1 : kv_page(c, p.batch, at.seq, at.pos);
+  if (page < 0) return;  // all lanes of a token leave together
+  const int slot = (int)(at.pos & ((1 << c.page_shift) - 1));
+  const float2* f = cs[w.token];
+  for (int h0 = w.h0; h0 < w.h1; h0 += kBatch) {
+    if (h0 > w.h0) load(h0);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (h0 + u >= w.h1) continue;
+      float v[8];
+      x[u].get(p.type, v);
+      if (w.d0 < 2 * r) {
+        if (p.rope.interleaved) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            if (w.d0 / 2 + n < r) {
+              const float2 g = f[w.d0 / 2 + n];
+              const float a = v[2 * n], b = v[2 * n + 1];
+              v[2 * n] = a * g.x - b * g.y;
+              v[2 * n + 1] = a * g.y + b * g.x;
+            }
           }
-        }
-      } else if (r % 8 == 0) {
-        const bool second = d0 >= r;
-        const int i0 = second ? d0 - r : d0;
-        float o[8];
-        load8(src, p.type, row + (second ? d0 - r : d0 + r), p.vec, o);
+        } else if (half) {
+          float o[8];
+          other[u].get(p.type, o);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const float2 f = cs[t][i0 + n];
-          x[n] = second ? o[n] * f.y + x[n] * f.x : x[n] * f.x - o[n] * f.y;
-        }
-      } else {
+          for (int n = 0; n < 8; ++n) {
+            const float2 g = f[second ? w.d0 - r + n : w.d0 + n];
+            v[n] = second ? o[n] * g.y + v[n] * g.x : v[n] * g.x - o[n] * g.y;
+          }
+        } else {
+#pragma unroll 1
+          for (int n = 0; n < 8; ++n) {
+            const int d = w.d0 + n;
+            if (d >= 2 * r) break;
+            const bool back = d >= r;
+            const float2 g = f[back ? d - r : d];
+            const size_t i = row - w.d0 + (size_t)(h0 + u) * D;
+            const float a = load1(src, p.type, i + d), o = load1(src, p.type, i + (back ? d - r : d + r));
+            const float turned = back ? o * g.y + a * g.x : a * g.x - o * g.y;
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const int d = d0 + n;
-          if (d < 2 * r) {
-            const bool second = d >= r;
-            const float2 f = cs[t][second ? d - r : d];
-            const float o = load1(src, p.type, row + (second ? d - r : d + r));
-            x[n] = second ? o * f.y + x[n] * f.x : x[n] * f.x - o * f.y;
+            for (int e = 0; e < 8; ++e) v[e] = e == n ? turned : v[e];
           }
         }
       }
-    }
-    const size_t head = (size_t)page_of[t] * c.kv_heads + h;
-    const int slot = (int)(pos_of[t] & pmask);
-    const size_t token = (head << c.page_shift) + slot;  // row of D values
-    uint8_t* base = value ? c.v : c.k;
-    if (c.format == KV_F16 || c.format == KV_BF16) {
-      store8(base, c.format, token * D + d0, true, x);
-      continue;
-    }
-    float most = 0.0f;
-    bool whole = true;  // fmaxf drops a NaN
+      const size_t head = (size_t)page * c.kv_heads + h0 + u;
+      const size_t token = (head << c.page_shift) + slot;  // row of D values
+      uint8_t* base = w.value ? c.v : c.k;
+      if constexpr (FMT >= 9) {
+        store8(base, FMT, token * D + w.d0, v);
+      } else {
+        float most = 0.0f;
+        bool whole = true;  // fmaxf drops a NaN
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      most = fmaxf(most, fabsf(x[n]));
-      whole = whole && fabsf(x[n]) <= 3.402823466e38f;
-    }
-    if (!whole) most = __builtin_inff();
-    most = fmaxf(most, xor_lanes<1>(most));
-    most = fmaxf(most, xor_lanes<2>(most));
-    const float levels = c.format == KV_Q8 ? 127.0f : 7.0f;
-    const uint16_t sh = group_scale(most, levels);
-    const float s = h2f(sh);
-    const bool on = s > 0.0f;
-    const float inv = on ? 1.0f / s : 0.0f;
-    int code[8];
+        for (int n = 0; n < 8; ++n) {
+          most = fmaxf(most, fabsf(v[n]));
+          whole = whole && fabsf(v[n]) <= 3.402823466e38f;
+        }
+        if (!whole) most = __builtin_inff();
+        most = fmaxf(most, xor_lanes<1>(most));
+        most = fmaxf(most, xor_lanes<2>(most));
+        constexpr float levels = FMT == KV_Q8 ? 127.0f : 7.0f;
+        const uint16_t sh = group_scale(most, levels);
+        const float s = h2f(sh);
+        const bool on = s > 0.0f;
+        const float inv = on ? 1.0f / s : 0.0f;
+        int code[8];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) { code[n] = on ? group_code(x[n], s, inv, levels) : 0; }
-    if (c.format == KV_Q8) {
-      u32x2 w = {0, 0};
+        for (int n = 0; n < 8; ++n) code[n] = on ? group_code(v[n], s, inv, levels) : 0;
+        if constexpr (FMT == KV_Q8) {
+          u32x2 o = {0, 0};
 #pragma unroll
-      for (int n = 0; n < 8; ++n) { w[n / 4] |= (uint32_t)(code[n] + 128) << (8 * (n & 3)); }
-      *(u32x2*)(base + token * D + d0) = w;
-    } else {
-      uint32_t w = 0;
+          for (int n = 0; n < 8; ++n) o[n / 4] |= (uint32_t)(code[n] + 128) << (8 * (n & 3));
+          *(u32x2*)(base + token * D + w.d0) = o;
+        } else {
+          uint32_t o = 0;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) { w |= (uint32_t)(code[n] + 8) << (4 * n); }
-      *(uint32_t*)(base + (token * D + d0) / 2) = w;
-    }
-    if ((d0 & 31) == 0) {
-      uint16_t* sc = value ? c.vs : c.ks;
-      sc[((head * (D / 32) + d0 / 32) << c.page_shift) + slot] = sh;
+          for (int n = 0; n < 8; ++n) o |= (uint32_t)(code[n] + 8) << (4 * n);
+          *(uint32_t*)(base + (token * D + w.d0) / 2) = o;
+        }
+        if ((w.d0 & 31) == 0) {
+          uint16_t* sc = w.value ? c.vs : c.ks;
+          sc[((head * (D / 32) + w.d0 / 32) << c.page_shift) + slot] = sh;
+        }
+      }
     }
   }
 }
@@ -311,43 +379,94 @@ struct ReadParams {
   KvBatchView batch;
   void *k, *v;
   int64_t tokens;
-  int type;
+  int type, heads, parts;
 };
 
-// grid ceil(tokens / kRopeTokens): the items of kv_append_kernel, the other way.
+// The workgroups of kv_append_kernel, the other way.
+template <int FMT, int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadParams p) {
-  __shared__ int64_t page_of[kRopeTokens];
-  __shared__ int slot_of[kRopeTokens];  // -1: behind the last sequence
+  typedef Tile<D> W;
+  constexpr int kWords = FMT >= 9 ? 4 : FMT == KV_Q8 ? 2 : 1;
   const KvCacheView& c = p.cache;
-  const int64_t t0 = (int64_t)blockIdx.x * kRopeTokens;
-  const int nt = (int)min((int64_t)kRopeTokens, p.tokens - t0);
-  const int pmask = (1 << c.page_shift) - 1;
-  if ((int)threadIdx.x < nt) {
-    const int seq = kv_sequence(p.batch, t0 + threadIdx.x);
-    const int64_t pos = seq < 0 ? 0 : kv_position(p.batch, seq, t0 + threadIdx.x);
-    page_of[threadIdx.x] = seq < 0 ? -1 : kv_page(c, p.batch, seq, pos);
-    slot_of[threadIdx.x] = seq < 0 ? -1 : (int)(pos & pmask);
-  }
-  __syncthreads();
-  const int D = c.head_dim, chunks = D / 8, per_side = chunks * c.kv_heads;
-  for (int e = threadIdx.x; e < nt * 2 * per_side; e += 256) {
-    const int t = e / (2 * per_side), i = e - t * 2 * per_side;
-    const bool value = i >= per_side;
-    const int j = value ? i - per_side : i, h = j / chunks, d0 = (j - h * chunks) * 8;
-    const int slot = slot_of[t];
-    if (slot < 0) continue;
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};  // a token without a page reads as zeros
-    if (page_of[t] >= 0) {
-      const size_t head = (size_t)page_of[t] * c.kv_heads + h;
+  const W w(p.heads, p.parts, c.kv_heads);
+  const int64_t t0 = (int64_t)blockIdx.x * W::kTokens;
+  const KvToken at = w.locate(p.batch, t0, p.tokens);
+  if (at.seq < 0) return;
+  const int64_t page = kv_page(c, p.batch, at.seq, at.pos);  // a token without one reads as zeros
+  const int slot = (int)(at.pos & ((1 << c.page_shift) - 1));
+  const uint8_t* base = w.value ? c.v : c.k;
+  const uint16_t* scales = w.value ? c.vs : c.ks;
+  for (int h0 = w.h0; h0 < w.h1; h0 += kBatch) {
+    uint32_t x[kBatch][kWords];
+    uint16_t scale[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const size_t head = (size_t)max(page, (int64_t)0) * c.kv_heads + min(h0 + u, w.h1 - 1);
       const size_t token = (head << c.page_shift) + slot;
-      float s = 1.0f;
-      if (c.ks)
-        s = h2f((value ? c.vs : c.ks)[((head * (D / 32) + d0 / 32) << c.page_shift) + slot]);
-      kv_load8((value ? c.v : c.k) + kv_bytes(c.format, token * D), c.format, d0, s, x);
+      const uint8_t* from = base + (token * D + w.d0) * kWords / 2;
+      if constexpr (kWords == 4) {
+        const u32x4 q = *(const u32x4*)from;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) x[u][n] = q[n];
+      } else if constexpr (kWords == 2) {
+        const u32x2 q = *(const u32x2*)from;
+        x[u][0] = q[0];
+        x[u][1] = q[1];
+      } else {
+        x[u][0] = *(const uint32_t*)from;
+      }
+      if constexpr (FMT < 9) scale[u] = scales[((head * (D / 32) + w.d0 / 32) << c.page_shift) + slot];
     }
-    store8(value ? p.v : p.k, p.type, ((size_t)(t0 + t) * c.kv_heads + h) * D + d0, true, x);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (h0 + u >= w.h1) continue;
+      void* out = w.value ? p.v : p.k;
+      const size_t at = ((size_t)(t0 + w.token) * c.kv_heads + h0 + u) * D + w.d0;
+      if (p.type == DT_F16) {
+        // code * scale is rounded once either way: in f16 arithmetic, two at a time
+        u32x4 o;
+        if constexpr (FMT == KV_F16) {
+          o = u32x4{x[u][0], x[u][1], x[u][2], x[u][3]};
+        } else if constexpr (FMT == KV_BF16) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) o[n] = pack2(DT_F16, bf2f((uint16_t)x[u][n]), bf2f((uint16_t)(x[u][n] >> 16)));
+        } else {
+          const _Float16 s = __builtin_bit_cast(_Float16, scale[u]);
+          const half2v s2 = {s, s};
+          if constexpr (FMT == KV_Q8)
+            o = decode8(x[u][0], x[u][1], s2);
+          else
+            o = decode4_plain(x[u][0], s2);
+        }
+        if (page < 0) o = u32x4{0, 0, 0, 0};
+        *(u32x4*)((uint16_t*)out + at) = o;
+        continue;
+      }
+      float y[8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        if constexpr (FMT == KV_Q8) {
+          y[n] = (float)((int)((x[u][n / 4] >> (8 * (n & 3))) & 255) - 128) * h2f(scale[u]);
+        } else if constexpr (FMT == KV_Q4) {
+          y[n] = (float)((int)((x[u][0] >> (4 * n)) & 15) - 8) * h2f(scale[u]);
+        } else {
+          const uint16_t v = (uint16_t)(x[u][n / 2] >> (16 * (n & 1)));
+          y[n] = FMT == KV_F16 ? h2f(v) : bf2f(v);
+        }
+        y[n] = page >= 0 ? y[n] : 0.0f;
+      }
+      store8(out, p.type, at, y);
+    }
   }
 }
+
+#define EXL3_KV_D(M, FMT) M(FMT, 64) M(FMT, 128) M(FMT, 256)
+#define EXL3_KV(M) EXL3_KV_D(M, KV_F16) EXL3_KV_D(M, KV_BF16) EXL3_KV_D(M, KV_Q8) EXL3_KV_D(M, KV_Q4)
+#define EXL3_KV_INST(FMT, D)                                        \
+  template __global__ void kv_append_kernel<FMT, D, 2>(AppendParams); \
+  template __global__ void kv_append_kernel<FMT, D, 4>(AppendParams); \
+  template __global__ void kv_read_kernel<FMT, D>(ReadParams);
+EXL3_KV(EXL3_KV_INST)
 
 }  // namespace exl3
 
@@ -434,11 +553,36 @@ static int check_rope(const exl3_rope_spec* rope, int head_dim, RopeView* view) 
   return EXL3_OK;
 }
 
-static int token_blocks(int64_t tokens, unsigned* blocks) {
-  const int64_t n = (tokens + kRopeTokens - 1) / kRopeTokens;
+// Heads per workgroup of an append or a read: a batch of loads each while that leaves
+// four workgroups per CU.
+static int head_parts(int64_t tokens, const KvCacheView& c, dim3* grid, int* heads, int* parts) {
+  const int64_t n = (tokens + 2048 / c.head_dim - 1) / (2048 / c.head_dim);
   if (n > INT32_MAX) return fail(EXL3_EINVAL, "too many tokens: %lld", (long long)tokens);
-  *blocks = (unsigned)n;
+  int per = kBatch;
+  while (per > 1 && n * 2 * ((c.kv_heads + per - 1) / per) < 1024) per /= 2;
+  *heads = per;
+  *parts = (c.kv_heads + per - 1) / per;
+  *grid = dim3((unsigned)n, 2u * (unsigned)*parts);
   return EXL3_OK;
+}
+
+// f(format, head width) as template arguments of f.
+template <typename F>
+static void by_format(const KvCacheView& c, F&& f) {
+  auto width = [&](auto fmt) {
+    if (c.head_dim == 64)
+      f(fmt, std::integral_constant<int, 64>{});
+    else if (c.head_dim == 128)
+      f(fmt, std::integral_constant<int, 128>{});
+    else
+      f(fmt, std::integral_constant<int, 256>{});
+  };
+  switch (c.format) {
+    case EXL3_KV_F16: width(std::integral_constant<int, KV_F16>{}); break;
+    case EXL3_KV_BF16: width(std::integral_constant<int, KV_BF16>{}); break;
+    case EXL3_KV_Q8: width(std::integral_constant<int, KV_Q8>{}); break;
+    default: width(std::integral_constant<int, KV_Q4>{});
+  }
 }
 
 extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_type, int64_t tokens,
@@ -449,7 +593,7 @@ extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_ty
   if (tokens < 0) return fail(EXL3_EINVAL, "negative token count");
   if (!known_type(x_type) || !known_type(y_type))
     return fail(EXL3_EINVAL, "unsupported rotary dtypes %d and %d", x_type, y_type);
-  if (heads < 1 || heads > 65536 || head_dim < 2 || head_dim > kMaxDim)
+  if (heads < 1 || heads > 65536 || head_dim < 2 || head_dim > 256)
     return fail(EXL3_EINVAL, "invalid rotary heads: %d of %d channels", heads, head_dim);
   const int64_t width = (int64_t)heads * head_dim;
   if (tokens > 1 && (x_stride < width || y_stride < width))
@@ -464,8 +608,6 @@ extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_ty
   if (!x || !y) return fail(EXL3_EINVAL, "null rotary input or output");
   if (x == y && (x_type != y_type || (tokens > 1 && x_stride != y_stride)))
     return fail(EXL3_EINVAL, "rotation in place keeps the type and the stride");
-  unsigned blocks;
-  if (int rc = token_blocks(tokens, &blocks)) return rc;
   p.x = x;
   p.y = y;
   p.positions = positions;
@@ -481,11 +623,22 @@ extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_ty
   const bool vec = head_dim % 8 == 0 && p.rope.pairs % (p.rope.interleaved ? 4 : 8) == 0 &&
                    rows_aligned(x, tokens > 1 ? x_stride : 0, x_type) &&
                    rows_aligned(y, tokens > 1 ? y_stride : 0, y_type);
+  const int pairs = p.rope.pairs, chunk = vec ? 8 : 1;
+  p.lanes = (p.rope.interleaved && vec ? 2 * pairs : pairs) / chunk + (head_dim - 2 * pairs) / chunk;
+  const int64_t blocks = (tokens + 256 / p.lanes - 1) / (256 / p.lanes);
+  if (blocks > INT32_MAX) return fail(EXL3_EINVAL, "too many tokens: %lld", (long long)tokens);
+  // two batches of loads a thread while that leaves four workgroups per CU
+  p.per = 2 * kBatch;
+  while ((p.per > 1 && blocks * ((heads + p.per - 1) / p.per) < 1024)) p.per /= 2;
+  const dim3 grid((unsigned)blocks, (unsigned)((heads + p.per - 1) / p.per));
   if (int rc = launch_gate("rotary launch")) return rc;
-  if (vec)
-    hipLaunchKernelGGL(rope_kernel<true>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, p);
+  hipStream_t s = (hipStream_t)stream;
+  if (vec && x_type == EXL3_F32)
+    hipLaunchKernelGGL((rope_kernel<true, 4>), grid, dim3(256), 0, s, p);
+  else if (vec)
+    hipLaunchKernelGGL((rope_kernel<true, 2>), grid, dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL(rope_kernel<false>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL((rope_kernel<false, 2>), grid, dim3(256), 0, s, p);
   return check_launch("rotary launch");
 }
 
@@ -505,8 +658,8 @@ extern "C" int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* b
     if (int rc = check_rope(rope, p.cache.head_dim, &p.rope)) return rc;
   if (tokens == 0) return EXL3_OK;
   if (!k || !v) return fail(EXL3_EINVAL, "null KV input");
-  unsigned blocks;
-  if (int rc = token_blocks(tokens, &blocks)) return rc;
+  dim3 grid;
+  if (int rc = head_parts(tokens, p.cache, &grid, &p.heads, &p.parts)) return rc;
   p.k = k;
   p.v = v;
   p.tokens = tokens;
@@ -516,7 +669,12 @@ extern "C" int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* b
   p.vec = rows_aligned(k, tokens > 1 ? k_stride : 0, type) &&
           rows_aligned(v, tokens > 1 ? v_stride : 0, type);
   if (int rc = launch_gate("KV append")) return rc;
-  hipLaunchKernelGGL(kv_append_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, p);
+  by_format(p.cache, [&](auto fmt, auto dim) {
+    if (type == EXL3_F32)
+      hipLaunchKernelGGL((kv_append_kernel<fmt(), dim(), 4>), grid, dim3(256), 0, (hipStream_t)stream, p);
+    else
+      hipLaunchKernelGGL((kv_append_kernel<fmt(), dim(), 2>), grid, dim3(256), 0, (hipStream_t)stream, p);
+  });
   return check_launch("KV append");
 }
 
@@ -531,14 +689,16 @@ extern "C" int exl3_kv_read(const exl3_kv_cache* cache, const exl3_kv_batch* bat
   if (!k || !v) return fail(EXL3_EINVAL, "null KV output");
   if (!aligned16(k) || !aligned16(v))
     return fail(EXL3_EINVAL, "KV outputs must be 16-byte aligned");
-  unsigned blocks;
-  if (int rc = token_blocks(tokens, &blocks)) return rc;
+  dim3 grid;
+  if (int rc = head_parts(tokens, p.cache, &grid, &p.heads, &p.parts)) return rc;
   p.k = k;
   p.v = v;
   p.tokens = tokens;
   p.type = type;
   if (int rc = launch_gate("KV read")) return rc;
-  hipLaunchKernelGGL(kv_read_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, p);
+  by_format(p.cache, [&](auto fmt, auto dim) {
+    hipLaunchKernelGGL((kv_read_kernel<fmt(), dim()>), grid, dim3(256), 0, (hipStream_t)stream, p);
+  });
   return check_launch("KV read");
 }
 

@@ -46,28 +46,31 @@ __device__ __forceinline__ int64_t kv_page(const KvCacheView& c, const KvBatchVi
   return page >= 0 && page < c.pages ? page : -1;
 }
 
-// The sequence that token row `token` belongs to (the last one that starts at or
-// before it; empty sequences share their start with the next), or -1 behind the last.
-__device__ __forceinline__ int kv_sequence(const KvBatchView& b, int64_t token) {
-  if (token < b.q_starts[0] || token >= b.q_starts[b.seqs]) return -1;
-  int lo = 0, hi = b.seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (b.q_starts[mid] <= token)
-      lo = mid;
-    else
-      hi = mid - 1;
+// Where token row `token` belongs: its sequence (the first that ends behind it; -1 in
+// front of the first or behind the last) and its position there, the new tokens being
+// the sequence's last ones.  Every lane of a wave calls it with one token: the lanes look
+// at 64 sequences at a time.
+struct KvToken {
+  int seq;
+  int64_t pos;
+};
+__device__ __forceinline__ KvToken kv_locate(const KvBatchView& b, int64_t token) {
+  const int lane = threadIdx.x & 63, first = b.q_starts[0];
+  for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+    const int at = min(s0 + lane, b.seqs - 1);
+    const int end = b.q_starts[at + 1], len = b.kv_lens[at];
+    const int n = __popcll(__ballot(s0 + lane < b.seqs && end <= token));
+    if (n < 64) {
+      const int seq = s0 + n;
+      if (seq >= b.seqs || token < first) break;
+      return KvToken{seq, (int64_t)__builtin_amdgcn_readlane(len, n) - __builtin_amdgcn_readlane(end, n) + token};
+    }
   }
-  return lo;
-}
-
-// Position of token row `token` of sequence seq: the new tokens are its last ones.
-__device__ __forceinline__ int64_t kv_position(const KvBatchView& b, int seq, int64_t token) {
-  return (int64_t)b.kv_lens[seq] - (int64_t)b.q_starts[seq + 1] + token;
+  return KvToken{-1, 0};
 }
 
 // ---------------------------------------------------------------------------
-// eight values
+// values
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float load1(const void* p, int dt, size_t i) {
   return dt == DT_F32 ? ((const float*)p)[i]
@@ -80,64 +83,120 @@ __device__ __forceinline__ void store1(void* p, int dt, size_t i, float v) {
     ((uint16_t*)p)[i] = dt == DT_F16 ? f2h(v) : f2bf(v);
 }
 
-// vec: the eight values are 16-byte aligned.
-__device__ __forceinline__ void load8(const void* p, int dt, size_t i, bool vec, float (&x)[8]) {
-  if (!vec) {
+// Eight values as they lie in memory, of 2 or 4 bytes each: loaded early, turned into
+// floats where they are needed.
+template <int BYTES>
+struct Raw8 {
+  u32x4 w[BYTES / 2];
+  // vec: the values are 16-byte aligned.
+  __device__ __forceinline__ void load(const void* p, size_t i, bool vec) {
+    const uint8_t* from = (const uint8_t*)p + i * BYTES;
+    if (vec) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { x[e] = load1(p, dt, i + e); }
-  } else if (dt == DT_F32) {
-    const float4v a = *(const float4v*)((const float*)p + i);
-    const float4v b = *(const float4v*)((const float*)p + i + 4);
+      for (int j = 0; j < BYTES / 2; ++j) w[j] = ((const u32x4*)from)[j];
+    } else if constexpr (BYTES == 4) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[e + 4] = b[e]; }
-  } else {
-    const u32x4 w = *(const u32x4*)((const uint16_t*)p + i);
+      for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = ((const uint32_t*)from)[e];
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint16_t h = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-      x[e] = dt == DT_F16 ? h2f(h) : bf2f(h);
+      for (int e = 0; e < 4; ++e)
+        w[0][e] = (uint32_t)((const uint16_t*)from)[2 * e] | (uint32_t)((const uint16_t*)from)[2 * e + 1] << 16;
     }
   }
-}
-__device__ __forceinline__ void store8(void* p, int dt, size_t i, bool vec, const float (&x)[8]) {
-  if (!vec) {
+  __device__ __forceinline__ void get(int dt, float (&x)[8]) const {
+    if constexpr (BYTES == 4) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { store1(p, dt, i + e, x[e]); }
-  } else if (dt == DT_F32) {
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t v = w[e / 4][e % 4];
+        x[e] = __builtin_bit_cast(float, v);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t h = (uint16_t)(w[0][e / 2] >> (16 * (e & 1)));
+        x[e] = dt == DT_F16 ? h2f(h) : bf2f(h);
+      }
+    }
+  }
+};
+
+// Two floats as 16-bit values of type dt, rounded to nearest even.
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack2(int dt, float a, float b) {
+  const float2v v = {a, b};
+  return dt == DT_F16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2v))
+                      : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf2v));
+}
+
+// Eight values to 16-byte aligned memory.
+__device__ __forceinline__ void store8(void* p, int dt, size_t i, const float (&x)[8]) {
+  if (dt == DT_F32) {
     float4v a, b;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { a[e] = x[e]; b[e] = x[e + 4]; }
+    for (int e = 0; e < 4; ++e) {
+      a[e] = x[e];
+      b[e] = x[e + 4];
+    }
     *(float4v*)((float*)p + i) = a;
     *(float4v*)((float*)p + i + 4) = b;
   } else {
     u32x4 w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint16_t lo = dt == DT_F16 ? f2h(x[2 * e]) : f2bf(x[2 * e]);
-      const uint16_t hi = dt == DT_F16 ? f2h(x[2 * e + 1]) : f2bf(x[2 * e + 1]);
-      w[e] = (uint32_t)lo | ((uint32_t)hi << 16);
-    }
+    for (int e = 0; e < 4; ++e) w[e] = pack2(dt, x[2 * e], x[2 * e + 1]);
     *(u32x4*)((uint16_t*)p + i) = w;
   }
 }
 
-// Eight cached values as floats: `row` is the head's row of D values, d0 the first
-// channel (a multiple of 8), `scale` its group's (8- and 4-bit formats).
-__device__ __forceinline__ void kv_load8(const uint8_t* row, int format, int d0, float scale,
-                                         float (&x)[8]) {
-  if (format == KV_Q8) {
-    const u32x2 w = *(const u32x2*)(row + d0);
+// ---------------------------------------------------------------------------
+// codes
+// ---------------------------------------------------------------------------
+// Eight 8-bit codes (code + 128) times a scale: byte b between 0x64 and itself is the f16
+// 1024 + b, and 1024 + b - 1152 is exact.
+__device__ __forceinline__ u32x4 decode8(uint32_t w0, uint32_t w1, half2v s) {
+  const half2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+  u32x4 r;
+  r[0] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u);
+  r[1] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u);
+  r[2] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u);
+  r[3] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = (float)((int)((w[e / 4] >> (8 * (e & 3))) & 255) - 128) * scale;
-    }
-  } else if (format == KV_Q4) {
-    const uint32_t w = *(const uint32_t*)(row + d0 / 2);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { x[e] = (float)((int)((w >> (4 * e)) & 15) - 8) * scale; }
-  } else {
-    load8(row, format, (size_t)d0, true, x);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = r[i];
+    r[i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, x) + off) * s);
   }
+  return r;
 }
 
+// (a & m) | b in one instruction (the compiler makes two of it with literal operands).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t m, uint32_t b) {
+  uint32_t d;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "s"(m), "v"(b));
+  return d;
+}
+
+// Eight 4-bit codes (code + 8) times a scale, in the order 0 4 1 5 2 6 3 7: a nibble in
+// the lowest or second-lowest place of an f16's mantissa under the exponent of 1024 is
+// 1024 + n or 1024 + 16 n.
+__device__ __forceinline__ u32x4 decode4(uint32_t w, half2v s) {
+  const half2v off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+  const half2v part = {(_Float16)0.0625f, (_Float16)0.0625f}, off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t v = w >> (8 * i);
+    const uint32_t lo = and_or(v, 0x000f000fu, 0x64006400u), hi = and_or(v, 0x00f000f0u, 0x64006400u);
+    r[2 * i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, lo) + off) * s);
+    r[2 * i + 1] = __builtin_bit_cast(
+        uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, hi), part, off16) * s);
+  }
+  return r;
+}
+// decode4 in the channels' own order.
+__device__ __forceinline__ u32x4 decode4_plain(uint32_t w, half2v s) {
+  const u32x4 d = decode4(w, s);
+  const uint32_t a = d[0], b = d[1], c = d[2], e = d[3];
+  return u32x4{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(e, c, 0x05040100u),
+               __builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(e, c, 0x07060302u)};
+}
 }  // namespace exl3

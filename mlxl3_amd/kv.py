@@ -40,24 +40,16 @@ class _RopeC(ctypes.Structure):
     ]
 
 
-class _On:
-    """Makes `device` the current one for a call (launches go to the current device)."""
+_FLOATS: dict = {}  # f16, bf16, f32 -> code, and the 16-bit ones: filled on first use
+_HALVES: dict = {}
 
-    __slots__ = ("guard",)
 
-    def __init__(self, device):
+def _floats() -> dict:
+    if not _FLOATS:
         torch = _torch()
-        self.guard = None
-        if device.index is not None and torch.cuda.current_device() != device.index:
-            self.guard = torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+        _FLOATS.update({t: _dtype_code(t) for t in (torch.float16, torch.bfloat16, torch.float32)})
+        _HALVES.update({t: _dtype_code(t) for t in (torch.float16, torch.bfloat16)})
+    return _FLOATS
 
 
 def _device_tensor(t, name: str, dtypes, dims: int):
@@ -71,12 +63,6 @@ def _device_tensor(t, name: str, dtypes, dims: int):
     return t
 
 
-def _same_device(device, *named):
-    for name, t in named:
-        if t is not None and t.device != device:
-            raise Exl3Error(-1, f"{name} is on {t.device}, expected {device}")
-
-
 def _plain(t, name: str, dtypes, dims: int):
     """A tensor that the kernels read in place: contiguous."""
     t = _device_tensor(t, name, dtypes, dims)
@@ -85,18 +71,35 @@ def _plain(t, name: str, dtypes, dims: int):
     return t
 
 
+def _rows_ok(t) -> bool:
+    """Whether the kernels read [tokens, heads, channels] as it is: contiguous heads, tokens
+    any distance apart."""
+    if t.is_contiguous():
+        return True
+    n, h, d = t.shape
+    return t.stride(2) == 1 and (h == 1 or t.stride(1) == d) and (n == 1 or t.stride(0) >= h * d)
+
+
 def _heads(t, name: str, dtypes):
     """[tokens, heads, channels] with contiguous heads; copied where its strides are others."""
     t = _device_tensor(t, name, dtypes, 3)
-    n, h, d = t.shape
-    if n and not (t.stride(2) == 1 and (h == 1 or t.stride(1) == d) and (n == 1 or t.stride(0) >= h * d)):
-        t = t.contiguous()
-    return t
+    return t if _rows_ok(t) else t.contiguous()
 
 
-def _floats():
+def _same(device, t, name: str):
+    if t.device != device:
+        raise Exl3Error(-1, f"{name} is on {t.device}, expected {device}")
+
+
+def _launch(device, entry, *args):
+    """entry(*args, stream) on the current stream of `device`, which is made the current one
+    (launches go to the current device)."""
     torch = _torch()
-    return (torch.float16, torch.bfloat16, torch.float32)
+    if torch.cuda.current_device() == device.index:
+        _check(entry(*args, _stream_ptr(device)))
+    else:
+        with torch.cuda.device(device):
+            _check(entry(*args, _stream_ptr(device)))
 
 
 class KvBatch:
@@ -123,11 +126,21 @@ class KvBatch:
         if int(max_q) < 1:
             raise Exl3Error(-1, "max_q must be positive")
         self.device = self.kv_lens.device
-        _same_device(self.device, ("q_starts", self.q_starts), ("block_table", self.block_table))
+        _same(self.device, self.q_starts, "q_starts")
+        if block_table is not None:
+            _same(self.device, self.block_table, "block_table")
         pages = 0 if block_table is None else int(self.block_table.shape[1])
         self._c = _KvBatchC(_ptr(self.q_starts), _ptr(self.kv_lens), _ptr(self.block_table), self.seqs, pages,
                             int(max_q), 0 if max_kv is None else int(max_kv))
         self._ref = ctypes.byref(self._c)
+        self._sized = (None, 0)  # the last attention's (cache, tokens, heads) and workspace
+
+    def _workspace_bytes(self, cache: "KvCache", tokens: int, heads: int) -> int:
+        key = (cache, tokens, heads)
+        if self._sized[0] != key:
+            need = load_library().exl3_attention_workspace_bytes(cache.handle, self._ref, tokens, heads)
+            self._sized = (key, int(need))
+        return self._sized[1]
 
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None):
@@ -201,28 +214,31 @@ class Rope:
         """x [tokens, heads, channels] (f16, bf16 or f32) rotated by its tokens' positions
         (int32 [tokens], or the batch's) into `out` (x itself: in place) or a new tensor
         of `dtype` (default x's)."""
-        torch = _torch()
-        if out is x and not (x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == x.shape[2])):
+        if out is x and not _rows_ok(x):
             raise Exl3Error(-1, "rotation in place needs contiguous heads")
         src = _heads(x, "x", _floats())
         n, heads, dim = src.shape
+        device = src.device
         if out is None:
-            out = torch.empty((n, heads, dim), dtype=dtype or src.dtype, device=src.device)
-        else:
-            _device_tensor(out, "out", _floats(), 3)
-            if out.shape != src.shape or _heads(out, "out", _floats()) is not out:
+            out = _torch().empty((n, heads, dim), dtype=dtype or src.dtype, device=device)
+        elif out is not x:
+            _device_tensor(out, "out", _FLOATS, 3)
+            if out.shape != src.shape or not _rows_ok(out):
                 raise Exl3Error(-1, "out must have x's shape and contiguous heads")
+            _same(device, out, "out")
+        where = None
         if positions is not None:
-            _plain(positions, "positions", (torch.int32,), 1)
+            _plain(positions, "positions", (_torch().int32,), 1)
             if positions.numel() != n:
                 raise Exl3Error(-1, f"{positions.numel()} positions for {n} tokens")
-        _same_device(src.device, ("inv_freq", self.inv_freq), ("positions", positions), ("out", out),
-                     ("batch", None if batch is None else batch.kv_lens))
-        with _On(src.device):
-            _check(load_library().exl3_rope(
-                self._ref, _ptr(src), _dtype_code(src.dtype), n, heads, dim, src.stride(0), _ptr(positions),
-                None if batch is None else batch._ref, _ptr(out), _dtype_code(out.dtype), out.stride(0),
-                _stream_ptr(src.device)))
+            _same(device, positions, "positions")
+            where = positions.data_ptr()
+        if batch is not None:
+            _same(device, batch.kv_lens, "batch")
+        _same(device, self.inv_freq, "inv_freq")
+        _launch(device, load_library().exl3_rope, self._ref, src.data_ptr(), _FLOATS[src.dtype], n, heads, dim,
+                src.stride(0), where, None if batch is None else batch._ref, out.data_ptr(), _FLOATS[out.dtype],
+                out.stride(0))
         return out
 
 
@@ -254,7 +270,9 @@ class KvCache:
             for name, s in (("k_scales", k_scales), ("v_scales", v_scales)):
                 if tuple(_plain(s, name, (torch.float16,), 4).shape) != want:
                     raise Exl3Error(-1, f"{name} must have shape {want}")
-        _same_device(self.device, ("v", v), ("k_scales", k_scales), ("v_scales", v_scales))
+        for name, t in (("v", v), ("k_scales", k_scales), ("v_scales", v_scales)):
+            if t is not None:
+                _same(self.device, t, name)
         fmt = _FORMATS.get(bits) or _dtype_code(self.k.dtype)
         h = _vp()
         lib = load_library()
@@ -292,14 +310,16 @@ class KvCache:
         """Writes the batch's new tokens, k and v [tokens, kv_heads, head_dim] (f16, bf16
         or f32), to their pages, keys rotated by `rope` first."""
         k, v = _heads(k, "k", _floats()), _heads(v, "v", (k.dtype,))
-        if k.shape != v.shape or tuple(k.shape[1:]) != (self.kv_heads, self.head_dim):
+        if k.shape != v.shape or k.shape[1] != self.kv_heads or k.shape[2] != self.head_dim:
             raise Exl3Error(-1, f"new keys and values have shape [tokens, {self.kv_heads}, {self.head_dim}]")
-        _same_device(self.device, ("k", k), ("v", v), ("batch", batch.kv_lens),
-                     ("rope", None if rope is None else rope.inv_freq))
-        with _On(self.device):
-            _check(load_library().exl3_kv_append(
-                self._handle, batch._ref, _ptr(k), k.stride(0), _ptr(v), v.stride(0), _dtype_code(k.dtype),
-                k.shape[0], None if rope is None else rope._ref, _stream_ptr(self.device)))
+        device = self.device
+        _same(device, k, "k")
+        _same(device, v, "v")
+        _same(device, batch.kv_lens, "batch")
+        if rope is not None:
+            _same(device, rope.inv_freq, "rope")
+        _launch(device, load_library().exl3_kv_append, self._handle, batch._ref, k.data_ptr(), k.stride(0),
+                v.data_ptr(), v.stride(0), _FLOATS[k.dtype], k.shape[0], None if rope is None else rope._ref)
 
     def read(self, batch: KvBatch, tokens: int, dtype=None):
         """(k, v) [tokens, kv_heads, head_dim] of the batch's newest tokens in `dtype`
@@ -307,12 +327,14 @@ class KvCache:
         written."""
         torch = _torch()
         dtype = dtype or (self.k.dtype if self.bits == 16 else torch.float16)
-        _same_device(self.device, ("batch", batch.kv_lens))
-        k, v = (torch.empty(int(tokens), self.kv_heads, self.head_dim, dtype=dtype, device=self.device)
-                for _ in range(2))
-        with _On(self.device):
-            _check(load_library().exl3_kv_read(self._handle, batch._ref, _ptr(k), _ptr(v), _dtype_code(dtype),
-                                               int(tokens), _stream_ptr(self.device)))
+        if dtype not in _floats():
+            raise Exl3Error(-1, f"unsupported KV output dtype {dtype}")
+        device, tokens = self.device, int(tokens)
+        _same(device, batch.kv_lens, "batch")
+        shape = (tokens, self.kv_heads, self.head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+        _launch(device, load_library().exl3_kv_read, self._handle, batch._ref, k.data_ptr(), v.data_ptr(),
+                _FLOATS[dtype], tokens)
         return k, v
 
 
@@ -324,23 +346,32 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     positions up to its own; window > 0: only the last `window` of them.  Rows outside
     every sequence are not written."""
     torch = _torch()
-    q = _heads(q, "q", (torch.float16, torch.bfloat16))
+    _floats()
+    q = _heads(q, "q", _HALVES)
     n, heads, dim = q.shape
+    device = cache.device
     if dim != cache.head_dim:
         raise Exl3Error(-1, f"queries of {dim} channels over a cache of {cache.head_dim}")
+    _same(device, q, "q")
+    _same(device, batch.kv_lens, "batch")
     if out is None:
-        out = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or _heads(out, "out", (q.dtype,)) is not out:
+        out = torch.empty((n, heads, dim), dtype=q.dtype, device=device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda or not _rows_ok(out):
         raise Exl3Error(-1, "out must have q's shape and type and contiguous heads")
-    _same_device(cache.device, ("q", q), ("out", out), ("batch", batch.kv_lens), ("workspace", workspace))
-    lib = load_library()
-    with _On(cache.device):
-        if workspace is None:
-            need = lib.exl3_attention_workspace_bytes(cache._handle, batch._ref, n, heads)
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _check(lib.exl3_attention(
-            cache._handle, batch._ref, _ptr(q), _dtype_code(q.dtype), n, heads, q.stride(0),
-            1.0 / math.sqrt(dim) if scale is None else float(scale), int(bool(causal)), int(window), _ptr(out),
-            out.stride(0), _ptr(workspace), 0 if workspace is None else workspace.numel(),
-            _stream_ptr(q.device)))
+    else:
+        _same(device, out, "out")
+    space, room = None, 0
+    if workspace is None:
+        room = batch._workspace_bytes(cache, n, heads)
+        if room:
+            workspace = torch.empty(room, dtype=torch.uint8, device=device)
+    else:
+        _plain(workspace, "workspace", (torch.uint8,), 1)
+        _same(device, workspace, "workspace")
+        room = workspace.numel()
+    if workspace is not None:
+        space = workspace.data_ptr()
+    _launch(device, load_library().exl3_attention, cache._handle, batch._ref, q.data_ptr(), _HALVES[q.dtype], n, heads,
+            q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, int(window),
+            out.data_ptr(), out.stride(0), space, room)
     return out
