@@ -139,10 +139,9 @@ Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int h
   const int64_t room = (int64_t)b.table_pages << c.page_shift;
   const int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;
   const int64_t groups = s.tiles * c.kv_heads;
-  static const int tgt = getenv("DEV_TGT") ? atoi(getenv("DEV_TGT")) : 512;
-  const int64_t want = (tgt + groups - 1) / groups;
+  const int64_t want = (512 + groups - 1) / groups;
   s.splits = (int)std::max<int64_t>(
-      1, std::min(std::min<int64_t>(want, getenv("DEV_MAX") ? atoi(getenv("DEV_MAX")) : 64), (most + 127) / (s.few ? 128 : 256)));
+      1, std::min(std::min<int64_t>(want, 32), (most + 127) / (s.few ? 128 : 256)));
   return s;
 }
 

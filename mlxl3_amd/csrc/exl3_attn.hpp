@@ -56,6 +56,9 @@ __device__ __forceinline__ u32x2 lds_transpose4(const uint8_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(size_t)lds_offset(p)));
 }
 
+// The compiler moves no instruction across this.
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
+
 // Whether any of eight 16-bit values is a NaN or an infinity.
 template <typename T>
 __device__ __forceinline__ bool not_finite(const u32x4& v) {
@@ -123,6 +126,7 @@ __device__ __forceinline__ Seen row_sees(const AttnParams& p, int first, int len
 // (tokens x heads of the group), first new position, length cut to the table's room.
 struct Work {
   int seq, start, rows, first, len;
+  const int32_t* table;  // the sequence's row of the block table
 };
 __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
   Work w;
@@ -134,6 +138,7 @@ __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
   const int64_t room = (int64_t)p.batch.table_pages << p.cache.page_shift;
   w.len = (int)max((int64_t)0, min(min((int64_t)kv, room), (int64_t)INT32_MAX - 4095));
   w.first = (int)max((int64_t)INT32_MIN, (int64_t)kv - n);
+  w.table = p.batch.table + (int64_t)seq * p.batch.table_pages;
   return w;
 }
 
@@ -161,7 +166,7 @@ __device__ __forceinline__ Work tile_work(const AttnParams& p, int tile, int row
     }
     tile -= __shfl(upto, 63);
   }
-  return Work{0, 0, 0, 0, 0};
+  return Work{};
 }
 
 // The table's entry for the 16 tokens from t (a multiple of 16) on, hi > 0 the end of the
@@ -169,11 +174,10 @@ __device__ __forceinline__ Work tile_work(const AttnParams& p, int tile, int row
 // here; page_ok says later whether it names a page.
 __device__ __forceinline__ int table_entry(const AttnParams& p, const Work& w, int t, int hi) {
   typedef const __attribute__((address_space(4))) int32_t* ScalarPtr;
-  const int at = min(t, hi - 1) >> p.cache.page_shift;
-  return ((ScalarPtr)(size_t)p.batch.table)[(int64_t)w.seq * p.batch.table_pages + at];
+  return ((ScalarPtr)(size_t)w.table)[(uint32_t)min(t, hi - 1) >> p.cache.page_shift];
 }
 __device__ __forceinline__ int page_ok(const AttnParams& p, int entry, int t, int hi) {
-  return t < hi && entry >= 0 && entry < p.cache.pages ? entry : -1;
+  return t < hi && (uint32_t)entry < (uint32_t)p.cache.pages ? entry : -1;  // pages < 2^31
 }
 
 __device__ __forceinline__ float wave_sum(float v) {

@@ -9,8 +9,9 @@
 //                 a row's maximum and sum stay in the lane (its other half in lane l ^ 32);
 //   P             as in the kernel for few rows: already the next product's B operand;
 //   O^T += V^T P^T  V read from LDS transposed.
-// The next tile's loads are in flight in registers meanwhile, and go to the other half of
-// LDS behind the products: one barrier per tile.  Two workgroups share a CU, so that
+// The next tile's loads are in flight meanwhile, straight into the other half of LDS or,
+// coded ones, into registers and from there decoded behind the products: one barrier per
+// tile.  Two workgroups share a CU, so that
 // one's exponentials run beside the other's products.
 #pragma once
 
@@ -32,24 +33,55 @@ struct Many {
   static constexpr int kTile = kTokens * D * 2;                         // bytes in LDS
   static constexpr int kLds = 4 * kTile;                                // keys and values, twice
 
-  struct Loads {
+  struct Loads {  // of coded caches
     u32x4 k[kLoads], v[kLoads];
-    uint32_t ks[kRaw ? 1 : kLoads], vs[kRaw ? 1 : kLoads];  // (16-bit elements would go through scratch)
+    uint32_t ks[kLoads], vs[kLoads];  // (16-bit elements would go through scratch)
   };
 
   // Byte of 16-byte chunk c of row t.  A key read takes one chunk of 16 rows at a time, a
   // value read 64 bytes of 4 rows: both fall into different banks.
-  static __device__ __forceinline__ int key_place(int t, int c) {
-    return t * D * 2 + ((c ^ (D == 64 ? (t >> 1) & 7 : t & 15)) << 4);
-  }
-  static __device__ __forceinline__ int value_place(int t, int c) {
-    return t * D * 2 + ((c ^ (D == 64 ? ((t >> 1) & 1) << 2 : (t & 3) << 2)) << 4);
-  }
+  static __device__ __forceinline__ int key_swizzle(int t) { return D == 64 ? (t >> 1) & 7 : t & 15; }
+  static __device__ __forceinline__ int value_swizzle(int t) { return D == 64 ? ((t >> 1) & 1) << 2 : (t & 3) << 2; }
+  static __device__ __forceinline__ int key_place(int t, int c) { return t * D * 2 + ((c ^ key_swizzle(t)) << 4); }
+  static __device__ __forceinline__ int value_place(int t, int c) { return t * D * 2 + ((c ^ value_swizzle(t)) << 4); }
 
   // Wave w loads rows kMine w .. of a tile, all of one page: its row of load u.
   static __device__ __forceinline__ int row_of(int u, int lane) { return u * kRows + lane / kLanes; }
 
-  // The wave's rows of the tile at t0, from page `page`.
+  // 16-bit caches: the wave's rows of the tile at t0 from page `page` straight into LDS
+  // (keys and values of rows `first` on); whoever waits for them waits with vmcnt.  A load
+  // fills 1 KB in lane order, so a lane fetches the chunk that belongs at its place.
+  static __device__ __forceinline__ void copy(const AttnParams& p, int kvh, int page, int t, int first, int lane,
+                                              uint8_t* keys, uint8_t* values) {
+    const KvCacheView& c = p.cache;
+    const int ch = lane % kLanes;
+    const size_t h = (size_t)max(page, 0) * c.kv_heads + kvh;
+    const size_t at = ((h << c.page_shift) + (t & ((1 << c.page_shift) - 1))) * kRow;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int r = row_of(u, lane), to = (first + u * kRows) * D * 2;
+      lds_dma16_s(c.k + at, r * kRow + ((ch ^ key_swizzle(first + r)) << 4), lds_offset(keys) + to);
+      lds_dma16_s(c.v + at, r * kRow + ((ch ^ value_swizzle(first + r)) << 4), lds_offset(values) + to);
+    }
+  }
+  // Their values on an edge, once they are there: rows outside [lo, hi) become zeros.
+  // Returns whether the others hold a value that is not finite.
+  static __device__ __forceinline__ bool clear(uint8_t* values, int first, int lane, int lo, int hi) {
+    bool bad = false;
+#pragma unroll 1
+    for (int u = 0; u < kLoads; ++u) {
+      const int t = first + row_of(u, lane);
+      u32x4* at = (u32x4*)(values + (first + u * kRows) * D * 2 + lane * 16);
+      const u32x4 v = *at;
+      if (t >= lo && t < hi)
+        bad = bad || not_finite<T>(v);
+      else
+        *at = u32x4{0, 0, 0, 0};
+    }
+    return bad;
+  }
+
+  // Coded caches: the same rows into registers.
   static __device__ __forceinline__ void load(const AttnParams& p, int kvh, int page, int t, int lane, Loads& x) {
     const KvCacheView& c = p.cache;
     const int ch = lane % kLanes;
@@ -61,18 +93,14 @@ struct Many {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       const int r = kRows > kMine ? row_of(u, lane) & (kMine - 1) : row_of(u, lane);
+      const int g = ((ch * (16 * D / kRow) / 32) << c.page_shift) + r;
       x.k[u] = *(const u32x4*)(k + r * kRow + ch * 16);
       x.v[u] = *(const u32x4*)(v + r * kRow + ch * 16);
-      if constexpr (!kRaw) {
-        const int g = ((ch * (16 * D / kRow) / 32) << c.page_shift) + r;
-        x.ks[u] = (c.ks + s)[g];
-        x.vs[u] = (c.vs + s)[g];
-      }
+      x.ks[u] = (c.ks + s)[g];
+      x.vs[u] = (c.vs + s)[g];
     }
   }
-  // One loaded chunk as 16-bit values, n 16-byte chunks in LDS.
   static __device__ __forceinline__ u32x4 decoded(const u32x4& w, uint32_t scale, int i) {
-    if constexpr (kRaw) return w;
     const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)scale);
     const half2v s2 = {s, s};
     if constexpr (FMT == KV_Q8) {
@@ -82,11 +110,10 @@ struct Many {
     const uint32_t a = w[i & 3];
     return decode4_plain(a, s2);
   }
-  // To LDS from row `first` on; on an edge, values of rows outside [lo, hi) become zeros.
-  // Returns whether an edge's other rows hold a value that is not finite.
+  // And decoded to LDS, with what clear() does on an edge.
   static __device__ __forceinline__ bool put(const Loads& x, uint8_t* keys, uint8_t* values, int first, int lane,
                                              bool edge, int lo, int hi) {
-    constexpr int n = kRaw ? 1 : FMT == KV_Q8 ? 2 : 4;
+    constexpr int n = FMT == KV_Q8 ? 2 : 4;  // 16-byte chunks of a lane's load
     const int ch = lane % kLanes;
     bool bad = false;
 #pragma unroll
@@ -94,11 +121,11 @@ struct Many {
       const int t = first + row_of(u, lane);
       if (kRows > kMine && row_of(u, lane) >= kMine) continue;
       const bool live = !edge || (t >= lo && t < hi);
-      if (edge && live) bad = bad || (kRaw ? not_finite<T>(x.v[u]) : (x.vs[kRaw ? 0 : u] & 0x7c00) == 0x7c00);
+      if (edge && live) bad = bad || (x.vs[u] & 0x7c00) == 0x7c00;
 #pragma unroll
       for (int i = 0; i < n; ++i) {
-        *(u32x4*)(keys + key_place(t, ch * n + i)) = decoded(x.k[u], kRaw ? 0 : x.ks[kRaw ? 0 : u], i);
-        u32x4 v = decoded(x.v[u], kRaw ? 0 : x.vs[kRaw ? 0 : u], i);
+        *(u32x4*)(keys + key_place(t, ch * n + i)) = decoded(x.k[u], x.ks[u], i);
+        u32x4 v = decoded(x.v[u], x.vs[u], i);
         if (!live) v = u32x4{0, 0, 0, 0};
         *(u32x4*)(values + value_place(t, ch * n + i)) = v;
       }
@@ -110,7 +137,7 @@ struct Many {
 // One-dimensional grid of tiles x splits x kv heads, the heads fastest (blocks go to the
 // XCDs in turn, so a head's tiles share few L2s), a sequence's last and longest tiles first.
 template <int FMT, typename T, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnParams p, int tiles) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(256 / D > 3 ? 3 : 256 / D, 256 / D > 3 ? 3 : 256 / D))) void attn_many_kernel(AttnParams p, int tiles) {
   typedef Many<FMT, T, D> F;
   typedef typename T::V8 V8;
   constexpr int TK = F::kTokens, NT = TK / 32;
@@ -159,12 +186,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnPa
   const int off = F::kMine * wave;  // of this wave's rows in a tile
   auto entry_at = [&](int t) { return table_entry(p, w, (t + off) & ~15, t1); };
   auto page_at = [&](int entry, int t) { return page_ok(p, entry, (t + off) & ~15, t1); };
-  auto stage = [&](int t, int page, int half) {
+  // starts the loads of the tile at t, and ends them in half `half` of LDS
+  auto fetch = [&](int t, int page, int half) __attribute__((always_inline)) {
+    uint8_t* buf = lds + half * 2 * F::kTile;
+    if constexpr (F::kRaw)
+      F::copy(p, kvh, page, t + off, off, lane, buf, buf + F::kTile);
+    else
+      F::load(p, kvh, page, t + off, lane, x);
+  };
+  auto stage = [&](int t, int page, int half) __attribute__((always_inline)) {
     uint8_t* buf = lds + half * 2 * F::kTile;
     // an edge: some row of the workgroup does not see some token of the tile
     const bool edge = t < end.lo || t + TK > min(top.hi, t1) || page < 0;
-    const bool bad =
-        F::put(x, buf, buf + F::kTile, off, lane, edge, top.lo - t, page < 0 ? 0 : min(end.hi, t1) - t);
+    const int lo = top.lo - t, hi = page < 0 ? 0 : min(end.hi, t1) - t;
+    bool bad = false;
+    if constexpr (F::kRaw) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (edge) bad = F::clear(buf + F::kTile, off, lane, lo, hi);
+    } else {
+      bad = F::put(x, buf, buf + F::kTile, off, lane, edge, lo, hi);
+    }
     again = again || (bad && (top.lo < end.lo || top.hi < end.hi));
     if (lane == 0) page_on[half][wave] = page >= 0;
   };
@@ -172,42 +213,76 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnPa
   if (t0 < t1) {
     next = entry_at(t0);
     page = page_at(next, t0);
-    F::load(p, kvh, page, t0 + off, lane, x);
+    fetch(t0, page, 0);
     next = entry_at(t0 + TK);
     stage(t0, page, 0);
   }
+  // the queries are here before the loop: a wait for them inside it would be one for the
+  // tile in flight
+#pragma unroll
+  for (int st = 0; st < D / 16; ++st) asm volatile("" : "+v"(q[st]));
   int cur = 0;
   for (int t = t0; t < t1; t += TK, cur ^= 1) {
     __syncthreads();
     const uint8_t* keys = lds + cur * 2 * F::kTile;
     const uint8_t* values = keys + F::kTile;
-    const bool more = t + TK < t1;
-    if (more) {
-      page = page_at(next, t + TK);
-      F::load(p, kvh, page, t + TK + off, lane, x);
-    }
+    // always, so that no later wait has to count both ways (behind the end: the pool's first
+    // page, and nobody uses it)
+    page = page_at(next, t + TK);
+    fetch(t + TK, page, cur ^ 1);
     if (busy && t < wend.hi && t + TK > wtop.lo) {
+      // The compiler orders these reads and products for few registers, each product right
+      // behind its read; pin() keeps kDepth reads ahead of the products.
+            constexpr int QK = NT * (D / 16), kDepth = 4;
       float16v s[NT];
+      auto key = [&](int i) __attribute__((always_inline)) {
+        return *(const V8*)(keys + F::key_place(32 * (i % NT) + n, 2 * (i / NT) + h));
+      };
+      V8 kf[kDepth];
 #pragma unroll
-      for (int a = 0; a < NT; ++a) {
-        s[a] = float16v{};
+      for (int i = 0; i < kDepth; ++i) kf[i] = key(i);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int st = 0; st < D / 16; ++st) {
-          const V8 key = *(const V8*)(keys + F::key_place(32 * a + n, 2 * st + h));
-          s[a] = T::mfma32(key, q[st], s[a]);
-        }
+      for (int i = 0; i < QK; ++i) {
+        pin();
+        const int a = i % NT, st = i / NT;
+        if (st == 0) s[a] = float16v{};
+        s[a] = T::mfma32(kf[i % kDepth], q[st], s[a]);
+        if (i + kDepth < QK) kf[i % kDepth] = key(i + kDepth);
       }
-      const int on0 = page_on[cur][0], on1 = page_on[cur][1], on2 = page_on[cur][2], on3 = page_on[cur][3];
-      const bool whole = __builtin_amdgcn_readfirstlane(on0 & on1 & on2 & on3);
-      if (t < wend.lo || t + TK > min(wtop.hi, t1) || !whole) {
+      constexpr int KS = TK / 16, DT = D / 32;
+      auto value = [&](int ks, int dt) __attribute__((always_inline)) {
+        const int tok = 16 * ks + 4 * h + ((lane >> 2) & 3);
+        const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), half = (lane & 1) * 8;
+        const u32x2 lo = lds_transpose4(values + F::value_place(tok, chunk) + half);
+        const u32x2 hi = lds_transpose4(values + F::value_place(tok + 8, chunk) + half);
+        const u32x4 r = {lo[0], lo[1], hi[0], hi[1]};
+        return __builtin_bit_cast(V8, r);
+      };
+      V8 vf[DT];
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vf[dt] = value(0, dt);
+      pin();
+      __builtin_amdgcn_s_setprio(0);
+      if (t < wend.lo || t + TK > min(wtop.hi, t1)) {
+        // token r of the tile is one of the row's `n` from `lo` on
+        const int lo = see.lo - t - 4 * h, n = max(min(see.hi, t1) - see.lo, 0);
 #pragma unroll
         for (int a = 0; a < NT; ++a)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int r = 32 * a + 8 * (i / 4) + 4 * h + i % 4, at = t + r;
-            const bool live = at >= see.lo && at < min(see.hi, t1) && (F::kMine == 16 ? (a ? (i / 8 ? on3 : on2) : (i / 8 ? on1 : on0)) : (i / 8 ? on2 : on0));
-            s[a][i] = live ? s[a][i] : -__builtin_inff();
+            const int r = 32 * a + 8 * (i / 4) + i % 4;
+            s[a][i] = (uint32_t)(r - lo) < (uint32_t)n ? s[a][i] : -__builtin_inff();
           }
+      }
+      // where a page is missing, so are its tokens
+      const int* on = page_on[cur];
+      if (!__builtin_amdgcn_readfirstlane(on[0] & on[1] & on[2] & on[3])) {
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[a][i] = on[(2 * a + i / 8) * 16 / F::kMine] ? s[a][i] : -__builtin_inff();
       }
       float most = s[0][0];
 #pragma unroll
@@ -225,32 +300,37 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_many_kernel(AttnPa
         for (int dt = 0; dt < D / 32; ++dt) o[dt] *= f;
       }
       const float base = m == -__builtin_inff() ? 0.0f : m;
+      V8 w8, following;
+      auto weight = [&](int ks, int i) __attribute__((always_inline)) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[ks / 2][8 * (ks & 1) + i], p.scale2, -base));
+        l += e;
+        return (typename T::E)e;
+      };
 #pragma unroll
-      for (int a = 0; a < NT; ++a)
+      for (int i = 0; i < 8; ++i) following[i] = weight(0, i);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-          V8 w8;
+      for (int ks = 0; ks < KS; ++ks) {
+        w8 = following;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(s[a][8 * k2 + i], p.scale2, -base));
-            l += e;
-            w8[i] = (typename T::E)e;
-          }
-          const int tok = 32 * a + 16 * k2 + 4 * h + ((lane >> 2) & 3);
+        for (int dt = 0; dt < DT; ++dt) {
+          pin();
+          o[dt] = T::mfma32(vf[dt], w8, o[dt]);
+          if (ks + 1 < KS) {  // beside it the next 16 tokens' values and weights
+            vf[dt] = value(ks + 1, dt);
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) {
-            const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), half = (lane & 1) * 8;
-            const u32x2 lo = lds_transpose4(values + F::value_place(tok, chunk) + half);
-            const u32x2 hi = lds_transpose4(values + F::value_place(tok + 8, chunk) + half);
-            const u32x4 r = {lo[0], lo[1], hi[0], hi[1]};
-            o[dt] = T::mfma32(__builtin_bit_cast(V8, r), w8, o[dt]);
+            for (int i = 0; i < 8 / DT; ++i) following[dt * (8 / DT) + i] = weight(ks + 1, dt * (8 / DT) + i);
           }
         }
+      }
+      pin();
+      __builtin_amdgcn_s_setprio(0);
     }
-    if (more) {
+    if (t + TK < t1)
       stage(t + TK, page, cur ^ 1);
-      next = entry_at(t + 2 * TK);
-    }
+    else if (F::kRaw)
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // LDS is not left to loads in flight
+    next = entry_at(t + 2 * TK);
   }
   if (again) retry = 1;
   __syncthreads();
