@@ -356,15 +356,37 @@ int exl3_kv_read(const exl3_kv_cache* cache, const exl3_kv_batch* batch, void* k
  * tokens t < kv_lens[b], with causal != 0 only t <= the token's position, with
  * window > 0 only t > its position - window.  A token that sees none gives
  * zeros.  q_type is f16 or bf16 and the cache's where that is 16-bit; y has
- * q_type; token strides in elements.  Workspace:
- * exl3_attention_workspace_bytes, not initialised and not shared between
- * calls that run concurrently. */
+ * q_type; token strides in elements; y may be q (with its stride).  Rows are
+ * equal bit for bit in repeated calls; the same row in a call of other sizes
+ * may differ in the order of its f32 sums.  Workspace:
+ * exl3_attention_workspace_bytes, 16-byte aligned, not initialised and not
+ * shared between calls that run concurrently. */
 size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
                                       int64_t tokens, int32_t heads);
 int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const void* q,
                    int32_t q_type, int64_t tokens, int32_t heads, int64_t q_stride, float scale,
                    int32_t causal, int32_t window, void* y, int64_t y_stride, void* workspace,
                    size_t workspace_bytes, void* stream);
+
+/* The attention block of a decoder layer, next to exl3_mlp_forward: q, k, v =
+ * exl3_group_forward of x; k and v appended and q rotated (rope may be NULL);
+ * exl3_attention with causal masking; y[rows][o.out] = exl3_linear_forward of
+ * it with o, in exl3_linear_output_dtype(o, x_type).  x_type is f16 or bf16
+ * (the cache's type where that is 16-bit).  q.out = o.in = heads * head_dim,
+ * k.out = v.out = kv_heads * head_dim.  Bit-identical to the calls it stands
+ * for.  Rows outside every sequence get unspecified values.  Biased
+ * projections under bf16 give f32 queries, which are rounded to bf16 by the
+ * rotation: without one they are refused.  Workspace:
+ * exl3_attn_block_workspace_bytes, zero-filled once like the others. */
+size_t exl3_attn_block_workspace_bytes(const exl3_linear* q, const exl3_linear* k,
+                                       const exl3_linear* v, const exl3_linear* o,
+                                       const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                                       int32_t x_type, int64_t rows);
+int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* k, const exl3_linear* v,
+                            const exl3_linear* o, const exl3_kv_cache* cache,
+                            const exl3_kv_batch* batch, const exl3_rope_spec* rope, float scale,
+                            int32_t window, const void* x, int32_t x_type, int64_t rows, void* y,
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 /* Decode hook, the reference's `metal-decode` codec op (exl3.metal:102-109,
  * main.rs:945-967): for every tile, states[t*256 + i] (nullable) and the f16

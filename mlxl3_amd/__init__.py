@@ -12,7 +12,8 @@ behaviour:
 * :class:`Exl3SwitchGlu` -- ``Exl3SwitchGlu::new`` / ``forward`` (native/src/moe.rs:809-975)
 * :func:`decode_tiles`  -- the ``metal-decode`` codec op (exl3.metal:102-109)
 * :class:`Rope`, :class:`KvCache`, :class:`KvBatch`, :func:`attention` (``kv.py``) -- rotary
-  positions, the paged key/value cache and attention over it
+  positions, the paged key/value cache and attention over it; :class:`Exl3Attention` -- the
+  attention block of a decoder layer around them
 * :class:`Checkpoint`   -- ``checkpoint::inspect`` / ``TensorInfo`` (native/src/checkpoint.rs),
   with ``Exl3Linear.from_checkpoint`` and ``Exl3SwitchGlu.from_checkpoint``
 
@@ -44,6 +45,7 @@ __all__ = [
     "Exl3Linear",
     "Exl3Group",
     "Exl3SwitchGlu",
+    "Exl3Attention",
     "KvBatch",
     "KvCache",
     "Rope",
@@ -135,6 +137,12 @@ _SIGNATURES = {
     "exl3_attention": (
         _i32,
         [_vp, _vp, _vp, _i32, _i64, _i32, _i64, ctypes.c_float, _i32, _i32, _vp, _i64, _vp, _sz,
+         _vp],
+    ),
+    "exl3_attn_block_workspace_bytes": (_sz, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64]),
+    "exl3_attn_block_forward": (
+        _i32,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _i32, _vp, _i32, _i64, _vp, _vp, _sz,
          _vp],
     ),
     "exl3_decode_tiles": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp]),
@@ -931,4 +939,4 @@ def decode_tiles(packed, k: int, cb: int, with_states: bool = True):
     return states, values
 
 
-from .kv import KvBatch, KvCache, Rope, attention, rope_frequencies  # noqa: E402
+from .kv import Exl3Attention, KvBatch, KvCache, Rope, attention, rope_frequencies  # noqa: E402

@@ -223,6 +223,8 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
     return fail(EXL3_EINVAL, "token strides are at least heads * head_dim");
   if (tokens == 0) return EXL3_OK;
   if (!q || !y) return fail(EXL3_EINVAL, "null attention input or output");
+  if (q == y && tokens > 1 && q_stride != y_stride)
+    return fail(EXL3_EINVAL, "attention in place keeps the stride");
   if (tokens > INT32_MAX) return fail(EXL3_EINVAL, "too many tokens: %lld", (long long)tokens);
   const size_t need = exl3_attention_workspace_bytes(cache, batch, tokens, heads);
   if (need && (!workspace || workspace_bytes < need))
@@ -277,6 +279,101 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   else
     hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(256), 0, s, p, sh.rows, shift);
   return check_launch("attention join");
+}
+
+namespace {
+
+// Workspace of an attention block: the projections' (its counters first), then q, k, v as
+// projected, q as attention takes it where that is another type, attention's own.
+struct Block {
+  int heads, types[3];      // output types of q, k and v
+  size_t linear, part[3], rounded, attention, total;
+};
+
+int plan_block(const exl3_linear* q, const exl3_linear* k, const exl3_linear* v, const exl3_linear* o,
+               const exl3_kv_cache* cache, const exl3_kv_batch* batch, int32_t x_type, int64_t rows,
+               Block* b) {
+  if (!q || !k || !v || !o) return fail(EXL3_EINVAL, "null EXL3 linear handle");
+  if (!cache) return fail(EXL3_EINVAL, "null KV cache");
+  KvBatchView view;
+  if (int rc = check_batch(cache, batch, rows, &view)) return rc;
+  if (rows < 1) return fail(EXL3_EINVAL, "empty attention block input");
+  if (x_type != EXL3_F16 && x_type != EXL3_BF16)
+    return fail(EXL3_EINVAL, "attention blocks take f16 or bf16 activations, got dtype %d", x_type);
+  const int D = cache->view.head_dim;
+  const exl3_linear* parts[3] = {q, k, v};
+  const int32_t wide = exl3_linear_out_features(q), narrow = cache->view.kv_heads * D;
+  if (wide % D || (wide / D) % cache->view.kv_heads || exl3_linear_out_features(k) != narrow ||
+      exl3_linear_out_features(v) != narrow || exl3_linear_in_features(o) != wide)
+    return fail(EXL3_EINVAL, "attention block widths differ from the cache's heads");
+  b->heads = wide / D;
+  const size_t group = exl3_group_workspace_bytes(parts, 3, rows);
+  if (!group) return fail(EXL3_EINVAL, "incompatible grouped projections");
+  b->linear = align256(std::max(group, exl3_linear_workspace_bytes(o, rows)));
+  size_t at = b->linear;
+  for (int i = 0; i < 3; ++i) {
+    b->types[i] = exl3_linear_output_dtype(parts[i], x_type);
+    b->part[i] = at;
+    at += align256((size_t)rows * (i ? narrow : wide) * (b->types[i] == EXL3_F32 ? 4 : 2));
+  }
+  b->rounded = at;
+  if (b->types[0] != x_type) at += align256((size_t)rows * wide * 2);
+  b->attention = at;
+  b->total = at + exl3_attention_workspace_bytes(cache, batch, rows, b->heads);
+  return EXL3_OK;
+}
+
+}  // namespace
+
+extern "C" size_t exl3_attn_block_workspace_bytes(const exl3_linear* q, const exl3_linear* k,
+                                                  const exl3_linear* v, const exl3_linear* o,
+                                                  const exl3_kv_cache* cache,
+                                                  const exl3_kv_batch* batch, int32_t x_type,
+                                                  int64_t rows) {
+  Block b;
+  return plan_block(q, k, v, o, cache, batch, x_type, rows, &b) ? 0 : b.total;
+}
+
+extern "C" int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* k,
+                                       const exl3_linear* v, const exl3_linear* o,
+                                       const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                                       const exl3_rope_spec* rope, float scale, int32_t window,
+                                       const void* x, int32_t x_type, int64_t rows, void* y,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+  Block b;
+  if (int rc = plan_block(q, k, v, o, cache, batch, x_type, rows, &b)) return rc;
+  if (!x || !y) return fail(EXL3_EINVAL, "null attention block input or output");
+  if (!workspace || workspace_bytes < b.total)
+    return fail(EXL3_EINVAL, "workspace too small: need %zu bytes, got %zu", b.total, workspace_bytes);
+  if (!aligned16(workspace)) return fail(EXL3_EINVAL, "attention workspace must be 16-byte aligned");
+  if (b.types[1] != b.types[2])
+    return fail(EXL3_EUNSUPPORTED, "keys and values of an attention block have one type: both biased or neither");
+  if (!rope && b.types[0] != x_type)
+    return fail(EXL3_EUNSUPPORTED, "biased bf16 queries need a rotation, which rounds them");
+  uint8_t* ws = (uint8_t*)workspace;
+  const exl3_linear* parts[3] = {q, k, v};
+  void* qkv[3] = {ws + b.part[0], ws + b.part[1], ws + b.part[2]};
+  void* query = b.types[0] == x_type ? qkv[0] : ws + b.rounded;
+  const int D = cache->view.head_dim;
+  const int64_t wide = (int64_t)b.heads * D, narrow = (int64_t)cache->view.kv_heads * D;
+  // what a later call would refuse is refused before the first launch
+  if (int rc = exl3_kv_append(cache, batch, nullptr, narrow, nullptr, narrow, b.types[1], 0, rope, stream))
+    return rc;
+  if (int rc = exl3_attention(cache, batch, nullptr, x_type, 0, b.heads, wide, scale, 1, window, nullptr, wide,
+                              nullptr, 0, stream))
+    return rc;
+  if (int rc = exl3_group_forward(parts, 3, x, x_type, rows, qkv, ws, b.linear, stream)) return rc;
+  if (rope)
+    if (int rc = exl3_rope(rope, qkv[0], b.types[0], rows, b.heads, D, wide, nullptr, batch, query, x_type, wide,
+                           stream))
+      return rc;
+  if (int rc = exl3_kv_append(cache, batch, qkv[1], narrow, qkv[2], narrow, b.types[1], rows, rope, stream))
+    return rc;
+  if (int rc = exl3_attention(cache, batch, query, x_type, rows, b.heads, wide, scale, 1, window, query, wide,
+                              ws + b.attention, b.total - b.attention, stream))
+    return rc;
+  return exl3_linear_forward(o, query, x_type, rows, y, exl3_linear_output_dtype(o, x_type), ws, b.linear,
+                             stream);
 }
 
 #endif  // __HIP_DEVICE_COMPILE__

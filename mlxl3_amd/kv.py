@@ -6,6 +6,8 @@ positions, the paged key/value cache and attention over it (``exl3_rope``,
 * :class:`Rope`, :func:`rope_frequencies` -- rotary positions and their frequencies
 * :class:`KvCache`   -- pages of f16, bf16, 8- or 4-bit values; append and read
 * :func:`attention`  -- new tokens over their sequences' pages
+* :class:`Exl3Attention` -- the attention block of a decoder layer
+  (``exl3_attn_block_forward``)
 """
 
 from __future__ import annotations
@@ -14,7 +16,9 @@ import ctypes
 import math
 from typing import Optional
 
-from . import Exl3Error, _check, _dtype_code, _ptr, _stream_ptr, _torch, _vp, load_library
+from . import (
+    Exl3Error, Exl3Linear, _check, _code_dtype, _dtype_code, _ptr, _stream_ptr, _torch, _vp, _Workspace, load_library,
+)
 
 _FORMATS = {8: 8, 4: 4}
 
@@ -375,3 +379,55 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
             q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, int(window),
             out.data_ptr(), out.stride(0), space, room)
     return out
+
+
+class Exl3Attention:
+    """The attention block of a decoder layer (``exl3_attn_block_forward``): the q/k/v
+    projections of x as a group, keys rotated and appended with the values, queries rotated,
+    causal attention over the cache, the o projection."""
+
+    def __init__(self, q: Exl3Linear, k: Exl3Linear, v: Exl3Linear, o: Exl3Linear, rope: Optional[Rope] = None,
+                 scale: Optional[float] = None, window: int = 0):
+        if len({(m.in_features, m.k, m.cb) for m in (q, k, v)}) != 1:
+            raise Exl3Error(-1, "incompatible grouped projections")
+        if o.in_features != q.out_features or k.out_features != v.out_features:
+            raise Exl3Error(-1, "attention block widths differ")
+        self.q, self.k, self.v, self.o = q, k, v, o
+        self.rope, self.scale, self.window = rope, scale, int(window)
+        self._ws = _Workspace()
+
+    def workspace_bytes(self, cache: KvCache, batch: KvBatch, rows: int, dtype) -> int:
+        return int(load_library().exl3_attn_block_workspace_bytes(
+            self.q.handle, self.k.handle, self.v.handle, self.o.handle, cache.handle, batch._ref, _dtype_code(dtype),
+            int(rows)))
+
+    def forward(self, x, cache: KvCache, batch: KvBatch, workspace=None):
+        """x [rows, in] (f16 or bf16) -> [rows, out] in the o projection's result dtype;
+        the cache's pages get the rows' keys and values.  `workspace`: a zero-filled uint8
+        tensor of :meth:`workspace_bytes`; by default one that the block keeps, so that two
+        calls must not run concurrently (two captured graphs: give each its own)."""
+        torch = _torch()
+        _floats()
+        x = _device_tensor(x, "x", _HALVES, 2).contiguous()
+        rows, device = x.shape[0], cache.device
+        if x.shape[1] != self.q.in_features or rows < 1:
+            raise Exl3Error(-1, f"invalid attention block input for {self.q.in_features} inputs")
+        _same(device, x, "x")
+        _same(device, batch.kv_lens, "batch")
+        if self.rope is not None:
+            _same(device, self.rope.inv_freq, "rope")
+        lib, code = load_library(), _HALVES[x.dtype]
+        y = torch.empty(rows, self.o.out_features, device=device,
+                        dtype=_code_dtype(lib.exl3_linear_output_dtype(self.o.handle, code)))
+        if workspace is None:
+            workspace = self._ws.get(self.workspace_bytes(cache, batch, rows, x.dtype), device)
+        else:
+            _plain(workspace, "workspace", (torch.uint8,), 1)
+            _same(device, workspace, "workspace")
+        scale = cache.head_dim**-0.5 if self.scale is None else float(self.scale)
+        _launch(device, lib.exl3_attn_block_forward, self.q.handle, self.k.handle, self.v.handle, self.o.handle,
+                cache.handle, batch._ref, None if self.rope is None else self.rope._ref, scale, self.window,
+                x.data_ptr(), code, rows, y.data_ptr(), workspace.data_ptr(), workspace.numel())
+        return y
+
+    __call__ = forward

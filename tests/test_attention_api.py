@@ -210,6 +210,72 @@ def test_armed_launches_fail_before_anything_is_issued(name, call):
         lib.exl3_kv_cache_destroy(h)
 
 
+def block(**kw):
+    """exl3_attn_block_forward with host-only handles; nothing is launched."""
+    lib, h = calls()
+    made = []
+
+    def linear(n_in, n_out, k=4, bias=None):
+        p = ctypes.c_void_p()
+        assert lib.exl3_linear_create(FAKE, n_in, n_out, k, 0, FAKE, FAKE, bias, ctypes.byref(p)) == 0
+        made.append(p)
+        return p
+
+    a = dict(q=(512, 512), k=(512, 256), v=(512, 256), o=(512, 512), kk=4, bias=(None, None, None), r=rope(), scale=0.1,
+             window=0, x=FAKE, t=9, rows=5, y=FAKE, ws=FAKE, bytes=1 << 40, b={})
+    a.update(kw)
+    q, k, v = (linear(*a[n], k=a["kk"] if n == "k" else 4, bias=b) for n, b in zip("qkv", a["bias"]))
+    o = linear(*a["o"])
+    try:
+        b = ref(batch(**a["b"]))
+        need = lib.exl3_attn_block_workspace_bytes(q, k, v, o, h, b, a["t"], a["rows"])
+        rc = lib.exl3_attn_block_forward(q, k, v, o, h, b, ref(a["r"]), a["scale"], a["window"], a["x"], a["t"], a["rows"],
+                                         a["y"], a["ws"], min(a["bytes"], max(need, 1) - 1) if a["bytes"] < 0 else a["bytes"],
+                                         None)
+        return rc, lib.exl3_last_error().decode(), need
+    finally:
+        for p in made:
+            lib.exl3_linear_destroy(p)
+        lib.exl3_kv_cache_destroy(h)
+
+
+@pytest.mark.parametrize("kw, rc, msg", [
+    (dict(k=(512, 384)), -1, "widths differ from the cache's heads"),
+    (dict(v=(512, 512)), -1, "widths differ from the cache's heads"),
+    (dict(q=(512, 384), o=(384, 512)), -1, "widths differ from the cache's heads"),
+    (dict(o=(256, 512)), -1, "widths differ from the cache's heads"),
+    (dict(kk=3), -1, "incompatible grouped projections"),
+    (dict(t=10), -1, "f16 or bf16 activations, got dtype 10"),
+    (dict(t=12), -1, "queries of a 16-bit KV cache have its type"),
+    (dict(rows=0), -1, "empty attention block input"),
+    (dict(x=None), -1, "null attention block input or output"),
+    (dict(y=None), -1, "null attention block input or output"),
+    (dict(ws=None), -1, "workspace too small"),
+    (dict(bytes=64), -1, "workspace too small"),
+    (dict(ws=FAKE + 8), -1, "16-byte aligned"),
+    (dict(scale=0.0), -1, "positive and finite"),
+    (dict(window=-4), -1, "negative attention window"),
+    (dict(r=rope(rotary_dim=256)), -1, "rotary dimension 256"),
+    (dict(b=dict(block_table=None)), -1, "needs a block table"),
+    (dict(b=dict(max_q=0)), -1, "max_q must be positive"),
+    (dict(t=12, bias=(None, FAKE, None)), -4, "both biased or neither"),
+    (dict(t=12, bias=(FAKE, FAKE, FAKE), r=None), -4, "need a rotation"),
+])
+def test_attention_block_refusals(kw, rc, msg):
+    got, err, _ = block(**kw)
+    assert got == rc and msg in err
+
+
+def test_attention_block_fails_before_anything_is_issued():
+    lib = mlxl3_amd.load_library()
+    lib.exl3_debug_fail_launch(b"EXL3 QMV launch")
+    try:
+        rc, err, need = block()
+        assert rc == -2 and "forced launch failure" in err and need > 65536
+    finally:
+        lib.exl3_debug_fail_launch(None)
+
+
 def test_python_refuses_host_tensors():
     i = torch.zeros(3, dtype=torch.int32)
     with pytest.raises(mlxl3_amd.Exl3Error, match="q_starts must be a device tensor"):

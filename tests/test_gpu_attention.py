@@ -483,6 +483,108 @@ def test_captured_graphs_follow_the_device_arrays():
             assert torch.equal(s.cache.k, eager.cache.k) and torch.equal(s.cache.v_scales, eager.cache.v_scales)
 
 
+# ---------------------------------------------------------------------------
+# the attention block
+# ---------------------------------------------------------------------------
+def projections(seed, hidden, heads, kv_heads, dim, k, cb, bias):
+    from mlxl3_amd import synth
+
+    def one(i, n_in, n_out, with_bias):
+        tr, suh, svh, b = synth.linear_layer(seed, i, n_in, n_out, k, bias=with_bias)
+        dev = lambda a: None if a is None else torch.from_numpy(a.view("int16") if a.dtype.name == "uint16" else a).cuda()
+        return mlxl3_amd.Exl3Linear(dev(tr), dev(suh), dev(svh), dev(b) if with_bias else None, k, cb)
+
+    return [one(0, hidden, heads * dim, bias), one(1, hidden, kv_heads * dim, bias), one(2, hidden, kv_heads * dim, bias),
+            one(3, heads * dim, hidden, False)]
+
+
+@pytest.mark.parametrize("dtype, bits, bias", [(F16, 16, False), (BF16, 16, True), (BF16, 8, True), (F16, 4, True)])
+@pytest.mark.parametrize("dim, heads, kv_heads, new, old", [
+    (128, 8, 2, [1, 1, 1], [70, 0, 300]), (64, 6, 2, [3, 40], [9, 0]), (256, 2, 1, [2], [33]),
+])
+def test_attention_block_equals_its_calls(dtype, bits, bias, dim, heads, kv_heads, new, old):
+    hidden, rows = 512, sum(new)
+    q, k, v, o = projections(3, hidden, heads, kv_heads, dim, 4, 0, bias)
+    lens = [n + m for n, m in zip(new, old)]
+    pool = Pool(73, lens, kv_heads, dim, 16, bits, dtype, loud=1.0)
+    b = kv_ref.batch(mlxl3_amd, new, lens, pool.table)
+    rope = mlxl3_amd.Rope(mlxl3_amd.rope_frequencies(dim)[0].cuda())
+    x = (torch.randn(rows, hidden, generator=torch.Generator().manual_seed(1)) / 8).to(dtype).cuda()
+    block = mlxl3_amd.Exl3Attention(q, k, v, o, rope=rope, window=100)
+    one, two = pool.cuda(mlxl3_amd), pool.cuda(mlxl3_amd)
+    for _ in range(2):
+        y = block(x, one, b)
+    qs, ks, vs = mlxl3_amd.Exl3Group([q, k, v])(x)
+    qr = rope.apply(qs.view(rows, heads, dim), batch=b, dtype=dtype)
+    two.append(b, ks.view(rows, kv_heads, dim), vs.view(rows, kv_heads, dim), rope=rope)
+    a = mlxl3_amd.attention(qr, two, b, window=100)
+    want = o(a.view(rows, heads * dim))
+    assert y.dtype == want.dtype and torch.equal(y, want) and bool(y.isfinite().all())
+    for name in ("k", "v", "k_scales", "v_scales"):
+        if getattr(one, name) is not None:
+            assert torch.equal(getattr(one, name).view(torch.uint8), getattr(two, name).view(torch.uint8)), name
+    # and the attention inside against 64 bits, from the cache as it now is
+    pool.k, pool.v = two.k.cpu(), two.v.cpu()
+    pool.ks, pool.vs = (None if t is None else t.cpu() for t in (two.k_scales, two.v_scales))
+    check(pool, new, qr.cpu(), a, window=100)
+
+
+def test_attention_block_in_graphs():
+    """Two blocks' steps captured with a workspace each and replayed in turn as the
+    sequences grow, against eager calls."""
+    hidden, heads, kv_heads, dim = 256, 4, 2, 64
+    q, k, v, o = projections(5, hidden, heads, kv_heads, dim, 3, 1, False)
+    rope = mlxl3_amd.Rope(mlxl3_amd.rope_frequencies(dim)[0].cuda())
+    lens, steps = [40, 3, 260], 4
+    pool = Pool(79, [n + steps for n in lens], kv_heads, dim, 16, 4, None, poison=False, loud=1.0)
+    table, starts = pool.table.cuda(), torch.arange(4, dtype=torch.int32).cuda()
+    block = mlxl3_amd.Exl3Attention(q, k, v, o, rope=rope)
+
+    class Side:
+        def __init__(self):
+            self.cache = pool.cuda(mlxl3_amd)
+            self.lens = torch.tensor(lens, dtype=torch.int32).cuda()
+            self.batch = mlxl3_amd.KvBatch(starts, self.lens, table, max_q=1, max_kv=300)
+            self.x = torch.zeros(3, hidden, dtype=F16, device="cuda")
+            self.ws = torch.zeros(block.workspace_bytes(self.cache, self.batch, 3, F16), dtype=torch.uint8, device="cuda")
+
+        def step(self):
+            return block(self.x, self.cache, self.batch, workspace=self.ws)
+
+    eager, sides, graphs, outs = Side(), [Side(), Side()], [], []
+    eager.step()
+    for s in sides:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            s.step()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s.step())
+        graphs.append(g)
+    gen = torch.Generator().manual_seed(11)
+    for step in range(steps):
+        x = torch.randn(3, hidden, generator=gen).half().cuda()
+        for s in [eager] + sides:
+            s.lens.copy_(torch.tensor([n + step + 1 for n in lens], dtype=torch.int32))
+            s.x.copy_(x)
+        want = eager.step()
+        for g, out, s in zip(graphs, outs, sides):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), step
+            assert torch.equal(s.cache.v, eager.cache.v)
+
+
+def test_attention_in_place():
+    for new in ([1, 2], [40, 33]):
+        pool = Pool(83, [900, 55], 2, 128, 16, 16, F16)
+        q, cache, b, y = run(pool, new, 8, F16)
+        x = q.cuda()
+        assert mlxl3_amd.attention(x, cache, b, out=x) is x and torch.equal(x, y)
+
+
 def test_python_refusals():
     pool = Pool(71, [20], 2, 128, 16, 16, F16)
     cache = pool.cuda(mlxl3_amd)
