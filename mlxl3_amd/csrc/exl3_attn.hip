@@ -96,11 +96,14 @@ template __global__ void attn_join_kernel<64>(AttnParams, int, int);
 template __global__ void attn_join_kernel<128>(AttnParams, int, int);
 template __global__ void attn_join_kernel<256>(AttnParams, int, int);
 
-#define EXL3_FEW_D(M, FMT, T) \
-  M(FMT, T, 64, 1) M(FMT, T, 64, 2) M(FMT, T, 128, 1) M(FMT, T, 128, 2) M(FMT, T, 256, 1)
-#define EXL3_FEW(M) \
-  EXL3_FEW_D(M, KV_F16, F16) EXL3_FEW_D(M, KV_BF16, BF16) EXL3_FEW_D(M, KV_Q8, F16) EXL3_FEW_D(M, KV_Q4, F16)
-#define EXL3_FEW_INST(FMT, T, D, RT) template __global__ void attn_few_kernel<FMT, T, D, RT>(AttnParams);
+#define EXL3_FEW_D(M, FMT, T, PARTS)                                                      \
+  M(FMT, T, 64, 1, PARTS) M(FMT, T, 64, 2, PARTS) M(FMT, T, 128, 1, PARTS) M(FMT, T, 128, 2, PARTS) \
+  M(FMT, T, 256, 1, PARTS)
+#define EXL3_FEW(M)                                                                       \
+  EXL3_FEW_D(M, KV_F16, F16, 1) EXL3_FEW_D(M, KV_BF16, BF16, 1) EXL3_FEW_D(M, KV_Q8, F16, 1) \
+  EXL3_FEW_D(M, KV_Q8, F16, 2) EXL3_FEW_D(M, KV_Q4, F16, 1) EXL3_FEW_D(M, KV_Q4, F16, 2)
+#define EXL3_FEW_INST(FMT, T, D, RT, PARTS) \
+  template __global__ void attn_few_kernel<FMT, T, D, RT, PARTS>(AttnParams);
 EXL3_FEW(EXL3_FEW_INST)
 
 #define EXL3_MANY_D(M, FMT, T) M(FMT, T, 64) M(FMT, T, 128) M(FMT, T, 256)
@@ -125,9 +128,11 @@ struct Shape {
   bool one_tile;  // every sequence's rows fit one workgroup
   int64_t tiles;  // at most; the device counts the tiles that there are
   int splits;     // ranges of the tokens that a tile sees
+  int split_tokens;
 };
 
-Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int heads) {
+
+Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int heads, int window) {
   const int group = heads / c.kv_heads;
   const int64_t rows = (int64_t)b.max_q * group;
   Shape s;
@@ -137,11 +142,14 @@ Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int h
   s.tiles = s.one_tile ? b.seqs
                        : std::min((rows + s.rows - 1) / s.rows * b.seqs, tokens * group / s.rows + b.seqs);
   const int64_t room = (int64_t)b.table_pages << c.page_shift;
-  const int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;
+  int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;
+  if (window > 0) most = std::min<int64_t>(most, (int64_t)window + b.max_q);
   const int64_t groups = s.tiles * c.kv_heads;
-  const int64_t want = (512 + groups - 1) / groups;
-  s.splits = (int)std::max<int64_t>(
-      1, std::min(std::min<int64_t>(want, 32), (most + 127) / (s.few ? 128 : 256)));
+  const int64_t slots = c.head_dim == 256 ? 256 : s.rows == 16 ? 768 : 512;
+  const int64_t want = (slots + groups - 1) / groups;
+  const int64_t least = s.few ? 128 : 256;
+  s.splits = (int)std::max<int64_t>(1, std::min(std::min<int64_t>(want, 32), (most + least / 2) / least));
+  s.split_tokens = (int)std::min<int64_t>(((most + s.splits - 1) / s.splits + 127) / 128 * 128, INT32_MAX - 255);
   return s;
 }
 
@@ -149,20 +157,20 @@ size_t slots_of(const Shape& s, const KvCacheView& c) {
   return (size_t)s.tiles * c.kv_heads * s.splits * s.rows;
 }
 
-template <int FMT, typename T, int D, int RT>
+template <int FMT, typename T, int PARTS, int D, int RT>
 void launch_few(const AttnParams& p, hipStream_t s) {
   const dim3 grid((unsigned)p.splits, (unsigned)p.cache.kv_heads, (unsigned)p.batch.seqs);
-  constexpr size_t lds = 4 * (Few<FMT, T, D, RT>::kWaveLds);
-  hipLaunchKernelGGL((attn_few_kernel<FMT, T, D, RT>), grid, dim3(256), lds, s, p);
+  constexpr size_t lds = 4 * (Few<FMT, T, D, RT, PARTS>::kWaveLds);
+  hipLaunchKernelGGL((attn_few_kernel<FMT, T, D, RT, PARTS>), grid, dim3(256), lds, s, p);
 }
-template <int FMT, typename T>
+template <int FMT, typename T, int PARTS>
 void launch_few(const AttnParams& p, int rows, hipStream_t s) {
   const int d = p.cache.head_dim;
   if (rows == 16) {
-    d == 64 ? launch_few<FMT, T, 64, 1>(p, s) : d == 128 ? launch_few<FMT, T, 128, 1>(p, s)
-                                                         : launch_few<FMT, T, 256, 1>(p, s);
+    d == 64 ? launch_few<FMT, T, PARTS, 64, 1>(p, s) : d == 128 ? launch_few<FMT, T, PARTS, 128, 1>(p, s)
+                                                                : launch_few<FMT, T, PARTS, 256, 1>(p, s);
   } else {
-    d == 64 ? launch_few<FMT, T, 64, 2>(p, s) : launch_few<FMT, T, 128, 2>(p, s);
+    d == 64 ? launch_few<FMT, T, PARTS, 64, 2>(p, s) : launch_few<FMT, T, PARTS, 128, 2>(p, s);
   }
 }
 
@@ -175,8 +183,10 @@ void launch_many(const AttnParams& p, int tiles, hipStream_t s) {
 template <int FMT, typename T>
 void launch(const AttnParams& p, const Shape& sh, hipStream_t s) {
   const int d = p.cache.head_dim, tiles = (int)sh.tiles;
-  if (sh.few)
-    launch_few<FMT, T>(p, sh.rows, s);
+  if (sh.few && FMT < 9 && p.q_type == DT_F16)
+    launch_few<FMT, T, FMT < 9 ? 2 : 1>(p, sh.rows, s);
+  else if (sh.few)
+    launch_few<FMT, T, 1>(p, sh.rows, s);
   else
     d == 64 ? launch_many<FMT, T, 64>(p, tiles, s) : d == 128 ? launch_many<FMT, T, 128>(p, tiles, s)
                                                               : launch_many<FMT, T, 256>(p, tiles, s);
@@ -190,7 +200,7 @@ extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
   if (!cache || !batch || tokens <= 0 || heads <= 0 || batch->seqs <= 0 || batch->max_q <= 0 ||
       batch->table_pages <= 0 || heads % cache->view.kv_heads)
     return 0;
-  const Shape sh = choose(cache->view, *batch, tokens, heads);
+  const Shape sh = choose(cache->view, *batch, tokens, heads, 0);
   if (sh.splits == 1) return 0;
   const size_t slots = slots_of(sh, cache->view);
   return align256(slots * cache->view.head_dim * 4) + align256(slots * 8);
@@ -231,7 +241,7 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
     return fail(EXL3_EINVAL, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
   if (need && !aligned16(workspace))
     return fail(EXL3_EINVAL, "attention workspace must be 16-byte aligned");
-  const Shape sh = choose(p.cache, *batch, tokens, heads);
+  const Shape sh = choose(p.cache, *batch, tokens, heads, window);
   if (sh.tiles * sh.splits * p.cache.kv_heads > INT32_MAX)
     return fail(EXL3_EUNSUPPORTED, "attention of %lld tokens needs too many workgroups", (long long)tokens);
   p.q = q;
@@ -245,6 +255,7 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   p.window = window;
   p.max_q = batch->max_q;
   p.splits = sh.splits;
+  p.split_tokens = sh.split_tokens;
   p.one_tile = sh.one_tile;
   p.q_vec = aligned16(q) && (tokens == 1 || q_stride % 8 == 0);
   p.y_vec = ((uintptr_t)y & 7) == 0 && (tokens == 1 || y_stride % 4 == 0);

@@ -15,7 +15,7 @@ struct AttnParams {
   float* stats;
   int64_t q_stride, y_stride;
   int heads, group, q_type, causal, window;
-  int max_q, splits;
+  int max_q, splits, split_tokens;
   int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
   int q_vec, y_vec;  // rows of q are 16-byte, rows of y 8-byte aligned
   float scale2;   // scale * log2(e): scores in units of a factor of two
@@ -73,7 +73,7 @@ __device__ __forceinline__ bool not_finite(const u32x4& v) {
   return bad;
 }
 
-// Where channel e of eight lies in decode4's order, and which channel lies at place e.
+// Where channel e of eight lies in codes4's order, and which channel lies at place e.
 __device__ __forceinline__ constexpr int place4(int e) { return e < 4 ? 2 * e : 2 * e - 7; }
 __device__ __forceinline__ constexpr int channel4(int e) { return (e >> 1) | ((e & 1) << 2); }
 
@@ -84,7 +84,7 @@ __device__ __forceinline__ uint16_t f2h_sat(float v) {
 }
 
 // Eight query channels from element i on, as T: T is the queries' own type for 16-bit
-// caches, f16 for coded ones (4 bits: in decode4's order).
+// caches, f16 for coded ones (4 bits: in codes4's order).
 template <int FMT, typename T>
 __device__ __forceinline__ typename T::V8 load_q8(const AttnParams& p, size_t i) {
   const uint16_t* q = (const uint16_t*)p.q + i;
@@ -190,12 +190,14 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// The tokens [t0, t1) of split `split`: 16-aligned ranges of [lo, hi), a multiple of 128
-// tokens each.
-__device__ __forceinline__ void split_range(int lo, int hi, int splits, int split, int& t0, int& t1) {
+// The tokens [t0, t1) of split `split` of [lo, hi): 16-aligned ranges of split_tokens each,
+// the same for every sequence, so that a ragged batch's workgroups take equally long (the
+// shorter sequences' last ones have nothing to do); longer ones where that leaves too few
+// splits (a sequence longer than the host was told).
+__device__ __forceinline__ void split_range(const AttnParams& p, int lo, int hi, int split, int& t0, int& t1) {
   lo &= ~15;
   const int n = max(hi - lo, 0);
-  const int each = ((n + splits - 1) / splits + 127) / 128 * 128;
+  const int each = max(p.split_tokens, ((n + p.splits - 1) / p.splits + 127) / 128 * 128);
   const int64_t a = (int64_t)lo + (int64_t)split * each;
   t0 = (int)min(a, (int64_t)hi);
   t1 = (int)min(a + each, (int64_t)hi);

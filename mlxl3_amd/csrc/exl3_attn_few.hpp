@@ -23,7 +23,7 @@
 
 namespace exl3 {
 
-template <int FMT, typename T, int D, int RT>
+template <int FMT, typename T, int D, int RT, int PARTS>
 struct Few {
   static constexpr bool kRaw = FMT >= 9;
   static constexpr int kSteps = D / 32;                                 // MFMAs over the channels
@@ -32,12 +32,28 @@ struct Few {
   static constexpr int kVec = kRaw ? 8 : FMT == KV_Q8 || D == 64 ? 16 : 32;
   static constexpr int kKeyLoads = D / 4 / kVec;
   static constexpr int kKeyWords = kVec * kRow / D / 4;
-  // values: 16-byte loads, lanes per row, rows per load
-  static constexpr int kLanes = kRow / 16, kRows = 64 / kLanes, kValueLoads = 32 / kRows;
-  static constexpr int kWaveLds = 32 * D * 2 > 16 * RT * D * 4 ? 32 * D * 2 : 16 * RT * D * 4;
+  static constexpr int kParts = PARTS;  // f16 that a coded value is made of (below)
+  // Values go through LDS kSpan channels at a time: with two parts half a head, so that
+  // three workgroups still fit a CU (32 rows: the results at the end need as much).  16-byte loads: lanes per row, rows per load, loads.
+  static constexpr int kSpans = PARTS == 1 || D == 64 || RT == 2 ? 1 : 2, kSpan = D / kSpans;
+  static constexpr int kLanes = kRow / kSpans / 16, kRows = 64 / kLanes, kSpanLoads = 32 / kRows;
+  static constexpr int kValueLoads = kSpans * kSpanLoads;
+  static constexpr int kPart = 32 * kSpan * 2;
+  static constexpr int kWaveLds = kParts * kPart > 16 * RT * D * 4 ? kParts * kPart : 16 * RT * D * 4;
 
-  // steps whose loads are in flight (16-bit caches: one has 16 KB of a wave in flight)
-  static constexpr int kAhead = 1;
+  // code * scale needs up to 18 bits, an f16 has 11.  Rounded to those it is off by half as
+  // much as an f16 query or output is, and a large score by many times that: with f16
+  // queries a value is two f16 -- the scale's leading bits times the code, exact, and the
+  // rest (8 bits: to 2^-15) -- each with its own product.  bf16 queries' outputs are 8 times
+  // coarser, so one rounded f16 is enough there.  Same box, us: 32 decodes over 8192 8-bit
+  // tokens, f16, one part 86.4 (2-norm error 8.3e-4, 2.1e-4 of it the output's own
+  // rounding), two 94.5 (2.9e-4); four drafts of 5 over 6001 4-bit tokens, bf16, 24.3 (1.8e-3
+  // against 1.6e-3) and 27.6 (1.6e-3).
+  static __device__ __forceinline__ void scale_parts(uint32_t scale, _Float16& hi, _Float16& lo) {
+    const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)scale);
+    hi = PARTS == 1 ? s : __builtin_bit_cast(_Float16, (uint16_t)(scale & (FMT == KV_Q8 ? 0xff80u : 0xfff8u)));
+    lo = s - hi;
+  }
 
   // First channel of lane group g's operand in MFMA step s.
   static __device__ __forceinline__ int channel(int s, int g) {
@@ -49,10 +65,10 @@ struct Few {
   // those fall into different banks.  A write of decoded codes takes every 2nd or 4th
   // chunk of one to eight rows: the two of a pair change places too so that those do.
   static __device__ __forceinline__ int place(int t, int c) {
-    const int r = D == 64 ? t >> 1 : t;  // rows that start in the same bank
-    const int odd = kRaw ? 0 : D == 256 ? c >> 4 : FMT == KV_Q8 ? r : r >> 1;
-    const int swz = D == 64 ? (r & 3) << 1 : (r & 7) << 1;
-    return t * D * 2 + ((c ^ swz ^ (odd & 1)) << 4);
+    const int r = kSpan == 64 ? t >> 1 : t;  // rows that start in the same bank
+    const int odd = kRaw ? 0 : kSpan == 256 ? c >> 4 : FMT == KV_Q8 ? r : r >> 1;
+    const int swz = kSpan == 64 ? (r & 3) << 1 : (r & 7) << 1;
+    return t * kSpan * 2 + ((c ^ swz ^ (odd & 1)) << 4);
   }
 
   struct Keys {
@@ -91,22 +107,26 @@ struct Few {
       }
     }
   }
-  static __device__ __forceinline__ typename T::V8 key(const Keys& k, int a, int s) {
+  // The operand of step s for block a, in kParts parts.
+  static __device__ __forceinline__ void key(const Keys& k, int a, int s, typename T::V8 (&part)[kParts]) {
     constexpr int n = kVec / 8;
     const int u = s / n, i = s % n;
-    u32x4 r;
     if constexpr (kRaw) {
+      u32x4 r;
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[e] = k.w[a][u][e];
+      part[0] = __builtin_bit_cast(typename T::V8, r);
     } else {
-      const _Float16 sc = __builtin_bit_cast(_Float16, (uint16_t)k.s[a][u]);
-      const half2v s2 = {sc, sc};
+      _Float16 hi, lo;
+      scale_parts(k.s[a][u], hi, lo);
+      u32x4 c;
       if constexpr (FMT == KV_Q8)
-        r = decode8(k.w[a][u][2 * i], k.w[a][u][2 * i + 1], s2);
+        c = codes8(k.w[a][u][2 * i], k.w[a][u][2 * i + 1]);
       else
-        r = decode4(k.w[a][u][i], s2);
+        c = codes4(k.w[a][u][i]);
+      part[0] = __builtin_bit_cast(typename T::V8, times(c, hi));
+      if constexpr (kParts == 2) part[1] = __builtin_bit_cast(typename T::V8, times(c, lo));
     }
-    return __builtin_bit_cast(typename T::V8, r);
   }
 
   static __device__ __forceinline__ void load_values(const AttnParams& p, const int (&page)[2], int kvh, int t0,
@@ -124,45 +144,49 @@ struct Few {
     const int r = lane / kLanes, ch = lane % kLanes;
 #pragma unroll
     for (int u = 0; u < kValueLoads; ++u) {
-      const int t = u * kRows + r;
-      const bool second = kRows > 16 ? t >= 16 : u * kRows >= 16;
-      v.w[u] = *(const u32x4*)((second ? b[1] : b[0]) + (t & 15) * kRow + ch * 16);
+      const int span = u / kSpanLoads, from = (span * kLanes + ch) * 16;  // byte of the head's row
+      const int t = (u % kSpanLoads) * kRows + r;
+      const bool second = kRows > 16 ? t >= 16 : (u % kSpanLoads) * kRows >= 16;
+      v.w[u] = *(const u32x4*)((second ? b[1] : b[0]) + (t & 15) * kRow + from);
       if constexpr (!kRaw) {
-        const int group = ch * (16 * D / kRow) / 32;
+        const int group = from * D / kRow / 32;
         v.s[u] = (second ? sc[1] : sc[0])[(group << c.page_shift) + (t & 15)];
       }
     }
   }
-  // Values to LDS as 16-bit rows (4 bits: channels in decode4's order); rows outside
+  // A span's values to LDS as 16-bit rows (4 bits: channels in codes4's order); rows outside
   // [live_lo, live_hi) or of a block without a page become zeros.  Returns whether an
   // edge's other rows hold a value that is not finite.
   template <bool EDGE>
-  static __device__ __forceinline__ bool put_values(const Values& v, uint8_t* lds, int lane, int live_lo, int live_hi,
-                                                    bool on0, bool on1) {
+  static __device__ __forceinline__ bool put_values(const Values& v, int span, uint8_t* lds, int lane, int live_lo,
+                                                    int live_hi, bool on0, bool on1) {
     const int r = lane / kLanes, ch = lane % kLanes;
     bool bad = false;
 #pragma unroll
-    for (int u = 0; u < kValueLoads; ++u) {
-      const int t = u * kRows + r;
+    for (int u0 = 0; u0 < kSpanLoads; ++u0) {
+      const int u = span * kSpanLoads + u0, t = u0 * kRows + r;
       const bool live = !EDGE || (t >= live_lo && t < live_hi && (t < 16 ? on0 : on1));
       if (EDGE && live) bad = bad || (kRaw ? not_finite<T>(v.w[u]) : (v.s[kRaw ? 0 : u] & 0x7c00) == 0x7c00);
       constexpr int n = kRaw ? 1 : FMT == KV_Q8 ? 2 : 4;  // 16-byte chunks of the decoded row
 #pragma unroll
       for (int i = 0; i < n; ++i) {
-        u32x4 x = v.w[u];
-        if constexpr (!kRaw) {
-          const _Float16 sc = __builtin_bit_cast(_Float16, (uint16_t)v.s[u]);
-          const half2v s2 = {sc, sc};
+        const int at = place(t, ch * n + i);
+        if constexpr (kRaw) {
+          *(u32x4*)(lds + at) = live ? v.w[u] : u32x4{0, 0, 0, 0};
+        } else {
+          _Float16 hi, lo;
+          scale_parts(v.s[u], hi, lo);
+          u32x4 c;
           if constexpr (FMT == KV_Q8) {
             const uint32_t w0 = v.w[u][2 * i], w1 = v.w[u][2 * i + 1];
-            x = decode8(w0, w1, s2);
+            c = codes8(w0, w1);
           } else {
             const uint32_t w0 = v.w[u][i];
-            x = decode4(w0, s2);
+            c = codes4(w0);
           }
+          *(u32x4*)(lds + at) = live ? times(c, hi) : u32x4{0, 0, 0, 0};
+          if constexpr (kParts == 2) *(u32x4*)(lds + kPart + at) = live ? times(c, lo) : u32x4{0, 0, 0, 0};
         }
-        if (!live) x = u32x4{0, 0, 0, 0};
-        *(u32x4*)(lds + place(t, ch * n + i)) = x;
       }
     }
     return bad;
@@ -178,9 +202,9 @@ struct Few {
 };
 
 // grid (splits, kv heads, sequences)
-template <int FMT, typename T, int D, int RT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnParams p) {
-  typedef Few<FMT, T, D, RT> F;
+template <int FMT, typename T, int D, int RT, int PARTS>
+__global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_kernel(AttnParams p) {
+  typedef Few<FMT, T, D, RT, PARTS> F;
   typedef typename T::V8 V8;
   extern __shared__ __align__(16) uint8_t lds[];  // 4 kWaveLds
   __shared__ float wave_m[4][16 * RT], wave_l[4][16 * RT];
@@ -193,7 +217,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnPar
   // rows see later tokens the later they are: the union is [top.lo, end.hi), what all see
   // [end.lo, top.hi)
   int t0, t1;
-  split_range(top.lo, end.hi, p.splits, split, t0, t1);
+  split_range(p, top.lo, end.hi, split, t0, t1);
   if (p.splits > 1 && t0 >= t1) {
     const size_t slot = ((size_t)(seq * p.cache.kv_heads + kvh) * p.splits + split) * (16 * RT);
     for (int e = threadIdx.x; e < 2 * w.rows; e += 256)
@@ -228,33 +252,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnPar
   }
   bool again = false;
 
-  constexpr int A = F::kAhead;
-  typename F::Keys keys[A];
-  typename F::Values vals[A];
-  int pages[A][2], next[A][2];  // of the steps loaded; the table's entries for those behind them
-  const int first = t0 + 32 * wave;
-  auto find = [&](int t, int (&entry)[2]) __attribute__((always_inline)) {
+  typename F::Keys k;
+  typename F::Values v;
+  int page[2], next[2];  // of the step loaded; the table's entries for the one behind it
+  auto find = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) entry[a] = table_entry(p, w, t + 16 * a, max(t1, 1));
+    for (int a = 0; a < 2; ++a) next[a] = table_entry(p, w, t + 16 * a, max(t1, 1));
   };
-  // always, so that the wait for one step's loads can leave the later ones in flight
-  // (behind the end they read the pool's first page, and nobody uses that)
-  auto load = [&](int t, const int (&entry)[2], int (&page)[2], typename F::Keys& k,
-                  typename F::Values& v) __attribute__((always_inline)) {
+  auto check = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) page[a] = page_ok(p, entry[a], t + 16 * a, t1);
+    for (int a = 0; a < 2; ++a) page[a] = page_ok(p, next[a], t + 16 * a, t1);
+  };
+  int t = t0 + 32 * wave;
+  if (w.len > 0) {
+    find(t);
+    check(t);
     F::load_keys(p, page, kvh, t, lane, k);
     F::load_values(p, page, kvh, t, lane, v);
-  };
-  if (w.len > 0) {
-#pragma unroll
-    for (int j = 0; j < A; ++j) find(first + 128 * j, next[j]);
-#pragma unroll
-    for (int j = 0; j < A; ++j) load(first + 128 * j, next[j], pages[j], keys[j], vals[j]);
-#pragma unroll
-    for (int j = 0; j < A; ++j) find(first + 128 * (j + A), next[j]);
+    find(t + 128);
   }
-  auto step = [&](const int t, typename F::Keys& k, typename F::Values& v, int (&page)[2], int (&next)[2]) __attribute__((always_inline)) {
+  for (; t < t1; t += 128) {
     const bool edge = t < end.lo || t + 32 > min(top.hi, t1) || page[0] < 0 || page[1] < 0;
     float4v s[RT][2];
 #pragma unroll
@@ -265,21 +282,32 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnPar
     for (int st = 0; st < F::kSteps; ++st)
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        const V8 key = F::key(k, a, st);
+        V8 key[F::kParts];
+        F::key(k, a, st, key);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][a] = T::mfma16(key, q[rt][st], s[rt][a]);
+        for (int part = 0; part < F::kParts; ++part)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][a] = T::mfma16(key[part], q[rt][st], s[rt][a]);
       }
     // values that some rows see and others do not must be finite for the product below (a
     // zero weight times an infinity is no zero); where they are not, the rows are done one
     // by one at the end
     const bool on0 = page[0] >= 0, on1 = page[1] >= 0;
-    if (edge) {
-      const bool bad = F::template put_values<true>(v, my, lane, top.lo - t, min(end.hi, t1) - t, on0, on1);
-      again = again || (bad && (top.lo < end.lo || top.hi < end.hi));
-    } else {
-      F::template put_values<false>(v, my, lane, 0, 32, true, true);
-    }
-    load(t + 128 * A, next, page, k, v);
+    auto put = [&](int span) __attribute__((always_inline)) {
+      if (edge) {
+        const bool bad =
+            F::template put_values<true>(v, span, my, lane, top.lo - t, min(end.hi, t1) - t, on0, on1);
+        again = again || (bad && (top.lo < end.lo || top.hi < end.hi));
+      } else {
+        F::template put_values<false>(v, span, my, lane, 0, 32, true, true);
+      }
+    };
+    put(0);
+    // the next step's loads, always, so that a wait for them never has to count both ways
+    // (behind the end they read the pool's first page, and nobody uses that)
+    check(t + 128);
+    F::load_keys(p, page, kvh, t + 128, lane, k);
+    if (F::kSpans == 1) F::load_values(p, page, kvh, t + 128, lane, v);
     V8 w8[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -314,20 +342,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_few_kernel(AttnPar
       }
     }
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) {
-      const V8 val = F::value(my, dt, lane);
+    for (int span = 0; span < F::kSpans; ++span) {
+      if (span) {
+        put(span);
+        if (span == F::kSpans - 1) F::load_values(p, page, kvh, t + 128, lane, v);
+      }
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) o[rt][dt] = T::mfma16(val, w8[rt], o[rt][dt]);
+      for (int i = 0; i < F::kSpan / 16; ++i)
+#pragma unroll
+        for (int part = 0; part < F::kParts; ++part) {
+          const V8 val = F::value(my + part * F::kPart, i, lane);
+          const int dt = span * (F::kSpan / 16) + i;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) o[rt][dt] = T::mfma16(val, w8[rt], o[rt][dt]);
+        }
     }
     // here, where no LDS read is waited for before the next step's keys are (a wait for one
     // waits for scalar loads as well)
-    find(t + 256 * A, next);
-  };
-  for (int t = first; t < t1; t += 128 * A)
-    static_for<A>([&](auto j_) {
-      constexpr int j = decltype(j_)::value;
-      if (t + 128 * j < t1) step(t + 128 * j, keys[j], vals[j], pages[j], next[j]);
-    });
+    find(t + 256);
+  }
 
   // the waves' results: maxima and sums, then weighted sums [row][channel] in LDS
   if (again) retry = 1;

@@ -102,13 +102,12 @@ struct Many {
   }
   static __device__ __forceinline__ u32x4 decoded(const u32x4& w, uint32_t scale, int i) {
     const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)scale);
-    const half2v s2 = {s, s};
     if constexpr (FMT == KV_Q8) {
       const uint32_t a = w[2 * i], b = w[2 * i + 1];
-      return decode8(a, b, s2);
+      return decode8(a, b, s);
     }
     const uint32_t a = w[i & 3];
-    return decode4_plain(a, s2);
+    return decode4(a, s);
   }
   // And decoded to LDS, with what clear() does on an edge.
   static __device__ __forceinline__ bool put(const Loads& x, uint8_t* keys, uint8_t* values, int first, int lane,
@@ -152,7 +151,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(256 / D > 3
   if (rows <= 0) return;
   const Seen top = row_sees(p, w.first, w.len, row0), end = row_sees(p, w.first, w.len, row0 + rows - 1);
   int t0, t1;
-  split_range(top.lo, end.hi, p.splits, split, t0, t1);
+  split_range(p, top.lo, end.hi, split, t0, t1);
   const size_t slot0 = ((size_t)(tile * p.cache.kv_heads + kvh) * p.splits + split) * kManyRows;
   if (p.splits > 1 && t0 >= t1) {
     for (int e = threadIdx.x; e < 2 * rows; e += 256)

@@ -432,11 +432,10 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadParams p) {
           for (int n = 0; n < 4; ++n) o[n] = pack2(DT_F16, bf2f((uint16_t)x[u][n]), bf2f((uint16_t)(x[u][n] >> 16)));
         } else {
           const _Float16 s = __builtin_bit_cast(_Float16, scale[u]);
-          const half2v s2 = {s, s};
           if constexpr (FMT == KV_Q8)
-            o = decode8(x[u][0], x[u][1], s2);
+            o = decode8(x[u][0], x[u][1], s);
           else
-            o = decode4_plain(x[u][0], s2);
+            o = decode4(x[u][0], s);
         }
         if (page < 0) o = u32x4{0, 0, 0, 0};
         *(u32x4*)((uint16_t*)out + at) = o;

@@ -151,9 +151,9 @@ __device__ __forceinline__ void store8(void* p, int dt, size_t i, const float (&
 // ---------------------------------------------------------------------------
 // codes
 // ---------------------------------------------------------------------------
-// Eight 8-bit codes (code + 128) times a scale: byte b between 0x64 and itself is the f16
-// 1024 + b, and 1024 + b - 1152 is exact.
-__device__ __forceinline__ u32x4 decode8(uint32_t w0, uint32_t w1, half2v s) {
+// Eight 8-bit codes (code + 128) as f16: byte b between 0x64 and itself is the f16 1024 + b,
+// and 1024 + b - 1152 is exact.
+__device__ __forceinline__ u32x4 codes8(uint32_t w0, uint32_t w1) {
   const half2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
   u32x4 r;
   r[0] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u);
@@ -163,7 +163,7 @@ __device__ __forceinline__ u32x4 decode8(uint32_t w0, uint32_t w1, half2v s) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t x = r[i];
-    r[i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, x) + off) * s);
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, x) + off);
   }
   return r;
 }
@@ -175,10 +175,10 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t m, uint32_t b) {
   return d;
 }
 
-// Eight 4-bit codes (code + 8) times a scale, in the order 0 4 1 5 2 6 3 7: a nibble in
-// the lowest or second-lowest place of an f16's mantissa under the exponent of 1024 is
-// 1024 + n or 1024 + 16 n.
-__device__ __forceinline__ u32x4 decode4(uint32_t w, half2v s) {
+// Eight 4-bit codes (code + 8) as f16, in the order 0 4 1 5 2 6 3 7: a nibble in the lowest
+// or second-lowest place of an f16's mantissa under the exponent of 1024 is 1024 + n or
+// 1024 + 16 n.
+__device__ __forceinline__ u32x4 codes4(uint32_t w) {
   const half2v off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
   const half2v part = {(_Float16)0.0625f, (_Float16)0.0625f}, off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
   u32x4 r;
@@ -186,15 +186,28 @@ __device__ __forceinline__ u32x4 decode4(uint32_t w, half2v s) {
   for (int i = 0; i < 2; ++i) {
     const uint32_t v = w >> (8 * i);
     const uint32_t lo = and_or(v, 0x000f000fu, 0x64006400u), hi = and_or(v, 0x00f000f0u, 0x64006400u);
-    r[2 * i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, lo) + off) * s);
-    r[2 * i + 1] = __builtin_bit_cast(
-        uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, hi), part, off16) * s);
+    r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, lo) + off);
+    r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, hi), part, off16));
   }
   return r;
 }
-// decode4 in the channels' own order.
-__device__ __forceinline__ u32x4 decode4_plain(uint32_t w, half2v s) {
-  const u32x4 d = decode4(w, s);
+
+// Eight f16 times one.
+__device__ __forceinline__ u32x4 times(const u32x4& v, _Float16 s) {
+  const half2v s2 = {s, s};
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = v[i];
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, x) * s2);
+  }
+  return r;
+}
+__device__ __forceinline__ u32x4 decode8(uint32_t w0, uint32_t w1, _Float16 s) { return times(codes8(w0, w1), s); }
+
+// Eight 4-bit codes times a scale in the channels' own order.
+__device__ __forceinline__ u32x4 decode4(uint32_t w, _Float16 s) {
+  const u32x4 d = times(codes4(w), s);
   const uint32_t a = d[0], b = d[1], c = d[2], e = d[3];
   return u32x4{__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(e, c, 0x05040100u),
                __builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(e, c, 0x07060302u)};
