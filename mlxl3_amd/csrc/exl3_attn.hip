@@ -222,7 +222,8 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
     return fail(EXL3_EINVAL, "queries of a 16-bit KV cache have its type");
   if (heads < 1 || heads > 65535 || heads % p.cache.kv_heads)
     return fail(EXL3_EINVAL, "%d query heads over %d KV heads", heads, p.cache.kv_heads);
-  if (!(scale > 0.0f) || !std::isfinite(scale))
+  const float scale2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.0f) || !std::isfinite(scale2))
     return fail(EXL3_EINVAL, "attention scale must be positive and finite");
   if (window < 0) return fail(EXL3_EINVAL, "negative attention window %d", window);
   if (batch->max_q < 1) return fail(EXL3_EINVAL, "max_q must be positive");
@@ -235,19 +236,21 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   if (!q || !y) return fail(EXL3_EINVAL, "null attention input or output");
   if (q == y && tokens > 1 && q_stride != y_stride)
     return fail(EXL3_EINVAL, "attention in place keeps the stride");
-  if (tokens > INT32_MAX) return fail(EXL3_EINVAL, "too many tokens: %lld", (long long)tokens);
+  if (tokens * (heads / p.cache.kv_heads) > INT32_MAX)
+    return fail(EXL3_EUNSUPPORTED, "too many tokens: %lld", (long long)tokens);
   const size_t need = exl3_attention_workspace_bytes(cache, batch, tokens, heads);
   if (need && (!workspace || workspace_bytes < need))
     return fail(EXL3_EINVAL, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
   if (need && !aligned16(workspace))
     return fail(EXL3_EINVAL, "attention workspace must be 16-byte aligned");
   const Shape sh = choose(p.cache, *batch, tokens, heads, window);
-  if (sh.tiles * sh.splits * p.cache.kv_heads > INT32_MAX)
+  if (sh.tiles * sh.splits * p.cache.kv_heads > kMostBlocks)
     return fail(EXL3_EUNSUPPORTED, "attention of %lld tokens needs too many workgroups", (long long)tokens);
   p.q = q;
   p.y = y;
   p.q_stride = q_stride;
   p.y_stride = y_stride;
+  p.tokens = (int)tokens;
   p.heads = heads;
   p.group = heads / p.cache.kv_heads;
   p.q_type = q_type;
@@ -259,7 +262,7 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   p.one_tile = sh.one_tile;
   p.q_vec = aligned16(q) && (tokens == 1 || q_stride % 8 == 0);
   p.y_vec = ((uintptr_t)y & 7) == 0 && (tokens == 1 || y_stride % 4 == 0);
-  p.scale2 = scale * 1.4426950408889634f;
+  p.scale2 = scale2;
   const size_t slots = slots_of(sh, p.cache);
   p.part = (float*)workspace;
   p.stats = (float*)((uint8_t*)workspace + align256(slots * p.cache.head_dim * 4));

@@ -11,9 +11,10 @@ struct AttnParams {
   KvBatchView batch;
   const void* q;
   void* y;
-  float* part;   // [slots][splits][rows][D] sums, then [slots][splits][rows][2] (max, sum)
-  float* stats;
+  float* part;    // [tiles][kv heads][splits][rows][D] weighted sums
+  float* stats;   // [tiles][kv heads][splits][rows][2] their maximum and sum of weights
   int64_t q_stride, y_stride;
+  int tokens;     // rows of q and y
   int heads, group, q_type, causal, window;
   int max_q, splits, split_tokens;
   int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
@@ -123,7 +124,8 @@ __device__ __forceinline__ Seen row_sees(const AttnParams& p, int first, int len
 }
 
 // What a workgroup works on: sequence, its first row of the call's tensors, rows
-// (tokens x heads of the group), first new position, length cut to the table's room.
+// (tokens x heads of the group), first new position, length cut to the table's room.  Rows
+// that q does not have are not touched, whatever q_starts says.
 struct Work {
   int seq, start, rows, first, len;
   const int32_t* table;  // the sequence's row of the block table
@@ -133,7 +135,8 @@ __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
   w.seq = seq;
   w.start = p.batch.q_starts[seq];
   const int64_t n = (int64_t)p.batch.q_starts[seq + 1] - w.start;
-  w.rows = (int)max((int64_t)0, min(n, (int64_t)p.max_q)) * p.group;
+  const int64_t have = w.start < 0 ? 0 : (int64_t)p.tokens - w.start;
+  w.rows = (int)max((int64_t)0, min(min(n, have), (int64_t)p.max_q)) * p.group;
   const int kv = p.batch.kv_lens[seq];
   const int64_t room = (int64_t)p.batch.table_pages << p.cache.page_shift;
   w.len = (int)max((int64_t)0, min(min((int64_t)kv, room), (int64_t)INT32_MAX - 4095));

@@ -556,7 +556,7 @@ static int check_rope(const exl3_rope_spec* rope, int head_dim, RopeView* view) 
 // four workgroups per CU.
 static int head_parts(int64_t tokens, const KvCacheView& c, dim3* grid, int* heads, int* parts) {
   const int64_t n = (tokens + 2048 / c.head_dim - 1) / (2048 / c.head_dim);
-  if (n > INT32_MAX) return fail(EXL3_EINVAL, "too many tokens: %lld", (long long)tokens);
+  if (n > kMostBlocks) return fail(EXL3_EUNSUPPORTED, "too many tokens: %lld", (long long)tokens);
   int per = kBatch;
   while (per > 1 && n * 2 * ((c.kv_heads + per - 1) / per) < 1024) per /= 2;
   *heads = per;
@@ -625,7 +625,7 @@ extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_ty
   const int pairs = p.rope.pairs, chunk = vec ? 8 : 1;
   p.lanes = (p.rope.interleaved && vec ? 2 * pairs : pairs) / chunk + (head_dim - 2 * pairs) / chunk;
   const int64_t blocks = (tokens + 256 / p.lanes - 1) / (256 / p.lanes);
-  if (blocks > INT32_MAX) return fail(EXL3_EINVAL, "too many tokens: %lld", (long long)tokens);
+  if (blocks > kMostBlocks) return fail(EXL3_EUNSUPPORTED, "too many tokens: %lld", (long long)tokens);
   // two batches of loads a thread while that leaves four workgroups per CU
   p.per = 2 * kBatch;
   while ((p.per > 1 && blocks * ((heads + p.per - 1) / p.per) < 1024)) p.per /= 2;

@@ -10,6 +10,9 @@ struct exl3_kv_cache {
 
 namespace exl3 {
 
+// Workgroups of 256 lanes that one dimension of a launch takes (2^32 lanes).
+constexpr int64_t kMostBlocks = (1 << 24) - 1;
+
 bool aligned16(const void* p);
 
 // Checks a batch (its block table only with a cache) and fills the kernels' view.

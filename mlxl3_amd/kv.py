@@ -49,10 +49,10 @@ _HALVES: dict = {}
 
 
 def _floats() -> dict:
-    if not _FLOATS:
+    if not _FLOATS:  # the halves first: another thread goes by the floats
         torch = _torch()
-        _FLOATS.update({t: _dtype_code(t) for t in (torch.float16, torch.bfloat16, torch.float32)})
         _HALVES.update({t: _dtype_code(t) for t in (torch.float16, torch.bfloat16)})
+        _FLOATS.update({t: _dtype_code(t) for t in (torch.float16, torch.bfloat16, torch.float32)})
     return _FLOATS
 
 
@@ -127,8 +127,8 @@ class KvBatch:
             raise Exl3Error(-1, "q_starts has one entry more than kv_lens, which has at least one")
         if block_table is not None and self.block_table.shape[0] != self.seqs:
             raise Exl3Error(-1, "block_table has one row per sequence")
-        if int(max_q) < 1:
-            raise Exl3Error(-1, "max_q must be positive")
+        if not 1 <= int(max_q) < 2**31 or not 0 <= int(max_kv or 0) < 2**31:
+            raise Exl3Error(-1, "max_q must be positive, max_kv not negative, both 32 bits")
         self.device = self.kv_lens.device
         _same(self.device, self.q_starts, "q_starts")
         if block_table is not None:
@@ -137,14 +137,24 @@ class KvBatch:
         self._c = _KvBatchC(_ptr(self.q_starts), _ptr(self.kv_lens), _ptr(self.block_table), self.seqs, pages,
                             int(max_q), 0 if max_kv is None else int(max_kv))
         self._ref = ctypes.byref(self._c)
-        self._sized = (None, 0)  # the last attention's (cache, tokens, heads) and workspace
+        self._sized = (None, 0)  # the last attention's sizes and workspace
 
     def _workspace_bytes(self, cache: "KvCache", tokens: int, heads: int) -> int:
-        key = (cache, tokens, heads)
-        if self._sized[0] != key:
+        key = (cache.kv_heads, cache.head_dim, cache.page_tokens, tokens, heads)
+        sized = self._sized  # read once: another thread may replace it
+        if sized[0] != key:
             need = load_library().exl3_attention_workspace_bytes(cache.handle, self._ref, tokens, heads)
-            self._sized = (key, int(need))
-        return self._sized[1]
+            self._sized = sized = (key, int(need))
+        return sized[1]
+
+
+# rope_scaling by type: the keys it needs, and those it may have
+_SCALING = {
+    "default": (set(), set()),
+    "linear": ({"factor"}, set()),
+    "llama3": ({"factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"}, set()),
+    "yarn": ({"factor", "original_max_position_embeddings"}, {"beta_fast", "beta_slow", "attention_factor"}),
+}
 
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None):
@@ -163,40 +173,45 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
       0.1 ln(factor) + 1 by default.
     """
     torch = _torch()
-    if rotary_dim < 2 or rotary_dim % 2:
-        raise Exl3Error(-1, f"rotary dimension {rotary_dim}")
-    half = rotary_dim // 2
-    freq = [base ** (-2.0 * i / rotary_dim) for i in range(half)]
+    if rotary_dim < 2 or rotary_dim % 2 or not base > 1.0:
+        raise Exl3Error(-1, f"rotary dimension {rotary_dim} with base {base}")
+    freq = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    scaling = {key: v for key, v in (scaling or {}).items() if v is not None}
+    kind = scaling.pop("rope_type", scaling.pop("type", "default"))
+    if kind not in _SCALING:
+        raise Exl3Error(-1, f"unknown rotary scaling {kind!r}")
+    needed, more = _SCALING[kind]
+    if not needed <= set(scaling) or not set(scaling) <= needed | more:
+        raise Exl3Error(-1, f"{kind!r} rotary scaling takes {sorted(needed)}, optionally {sorted(more)}")
+    scaling = {key: float(v) for key, v in scaling.items()}
+    if any(not v > 0.0 for v in scaling.values()):
+        raise Exl3Error(-1, "rotary scaling takes positive numbers")
+    s, n = scaling.get("factor", 1.0), scaling.get("original_max_position_embeddings", 0.0)
     scale = 1.0
-    if scaling:
-        kind = scaling.get("rope_type", scaling.get("type"))
-        s = float(scaling.get("factor", 1.0))
-        n = scaling.get("original_max_position_embeddings")
-        if kind == "linear":
-            freq = [f / s for f in freq]
-        elif kind == "llama3":
-            low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
-            mixed = []
-            for f in freq:
-                turns = n * f / (2 * math.pi)
-                keep = min(1.0, max(0.0, (turns - low) / (high - low)))
-                mixed.append(keep * f + (1.0 - keep) * f / s)
-            freq = mixed
-        elif kind == "yarn":
-            def pair(turns):
-                return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+    if kind == "linear":
+        freq = [f / s for f in freq]
+    elif kind == "llama3":
+        low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
+        if not high > low:
+            raise Exl3Error(-1, "high_freq_factor must be above low_freq_factor")
+        mixed = []
+        for f in freq:
+            turns = n * f / (2 * math.pi)
+            keep = min(1.0, max(0.0, (turns - low) / (high - low)))
+            mixed.append(keep * f + (1.0 - keep) * f / s)
+        freq = mixed
+    elif kind == "yarn":
+        def pair(turns):
+            return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-            first = max(0, math.floor(pair(float(scaling.get("beta_fast", 32.0)))))
-            last = min(rotary_dim - 1, math.ceil(pair(float(scaling.get("beta_slow", 1.0)))))
-            mixed = []
-            for i, f in enumerate(freq):
-                stretch = min(1.0, max(0.0, (i - first) / max(last - first, 1e-3)))
-                mixed.append((1.0 - stretch) * f + stretch * f / s)
-            freq = mixed
-            scale = scaling.get("attention_factor")
-            scale = 0.1 * math.log(s) + 1.0 if scale is None and s > 1 else 1.0 if scale is None else float(scale)
-        elif kind not in (None, "default"):
-            raise Exl3Error(-1, f"unknown rotary scaling {kind!r}")
+        first = max(0, math.floor(pair(scaling.get("beta_fast", 32.0))))
+        last = min(rotary_dim - 1, math.ceil(pair(scaling.get("beta_slow", 1.0))))
+        mixed = []
+        for i, f in enumerate(freq):
+            stretch = min(1.0, max(0.0, (i - first) / max(last - first, 1e-3)))
+            mixed.append((1.0 - stretch) * f + stretch * f / s)
+        freq = mixed
+        scale = scaling.get("attention_factor", 0.1 * math.log(s) + 1.0 if s > 1 else 1.0)
     return torch.tensor(freq, dtype=torch.float64).float(), scale
 
 
@@ -342,6 +357,12 @@ class KvCache:
         return k, v
 
 
+def _window(window) -> int:
+    if not 0 <= int(window) < 2**31:
+        raise Exl3Error(-1, f"attention window {window}")
+    return int(window)
+
+
 def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, causal: bool = True,
               window: int = 0, out=None, workspace=None):
     """Attention of the batch's new tokens over the cache (``exl3_attention``): q
@@ -358,6 +379,7 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
         raise Exl3Error(-1, f"queries of {dim} channels over a cache of {cache.head_dim}")
     _same(device, q, "q")
     _same(device, batch.kv_lens, "batch")
+    window = _window(window)
     if out is None:
         out = torch.empty((n, heads, dim), dtype=q.dtype, device=device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda or not _rows_ok(out):
@@ -376,7 +398,7 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     if workspace is not None:
         space = workspace.data_ptr()
     _launch(device, load_library().exl3_attention, cache._handle, batch._ref, q.data_ptr(), _HALVES[q.dtype], n, heads,
-            q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, int(window),
+            q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, window,
             out.data_ptr(), out.stride(0), space, room)
     return out
 
@@ -393,7 +415,7 @@ class Exl3Attention:
         if o.in_features != q.out_features or k.out_features != v.out_features:
             raise Exl3Error(-1, "attention block widths differ")
         self.q, self.k, self.v, self.o = q, k, v, o
-        self.rope, self.scale, self.window = rope, scale, int(window)
+        self.rope, self.scale, self.window = rope, scale, _window(window)
         self._ws = _Workspace()
 
     def workspace_bytes(self, cache: KvCache, batch: KvBatch, rows: int, dtype) -> int:

@@ -145,6 +145,7 @@ def test_read_refusals():
     (dict(scale=-0.1), "positive and finite"),
     (dict(scale=math.nan), "positive and finite"),
     (dict(scale=math.inf), "positive and finite"),
+    (dict(scale=3e38), "positive and finite"),  # times log2(e) it is infinite
     (dict(window=-1), "negative attention window"),
     (dict(qs=511), "token strides are at least"),
     (dict(ys=1), "token strides are at least"),
@@ -288,6 +289,33 @@ def test_python_refuses_host_tensors():
         mlxl3_amd.KvCache(torch.zeros(1, 1, 16, 64).half(), torch.zeros(1, 1, 16, 64).half())
 
 
+def test_calls_larger_than_a_launch_are_refused():
+    lib, h = calls()
+    rc, wide, _ = cache(heads=1024)
+    assert rc == 0
+    try:
+        b = ref(batch())
+        assert lib.exl3_kv_append(h, b, FAKE, 256, FAKE, 256, 9, 1 << 29, None, None) == -4
+        assert lib.exl3_kv_read(h, b, FAKE, FAKE, 9, 1 << 29, None) == -4
+        assert lib.exl3_rope(ref(rope(rotary_dim=256)), FAKE + 2, 9, 1 << 25, 1, 256, 256, FAKE, None, FAKE, 9, 256, None) == -4
+        assert lib.exl3_attention(h, b, FAKE, 9, 1 << 31, 4, 512, 0.1, 1, 0, FAKE, 512, FAKE, 1 << 40, None) == -4
+        assert "too many tokens" in lib.exl3_last_error().decode()
+        b = ref(batch(seqs=65535, max_q=200))
+        assert lib.exl3_attention(wide, b, FAKE, 9, 65535 * 200, 1024, 1 << 17, 0.1, 1, 0, FAKE, 1 << 17, FAKE, 1 << 40, None) == -4
+        assert "too many workgroups" in lib.exl3_last_error().decode()
+        b = ref(batch(seqs=65536))
+        assert lib.exl3_attention(h, b, FAKE, 9, 65536, 4, 512, 0.1, 1, 0, FAKE, 512, FAKE, 1 << 40, None) == -4
+    finally:
+        lib.exl3_kv_cache_destroy(h)
+        lib.exl3_kv_cache_destroy(wide)
+
+
+@pytest.mark.parametrize("window", [-1, 2**31, 2**32])
+def test_windows_of_more_than_32_bits_are_refused(window):
+    with pytest.raises(mlxl3_amd.Exl3Error, match="attention window"):
+        kv._window(window)
+
+
 # ---------------------------------------------------------------------------
 # frequencies
 # ---------------------------------------------------------------------------
@@ -330,3 +358,25 @@ def test_yarn_frequencies_and_scale():
         mlxl3_amd.rope_frequencies(128, 1e6, {"rope_type": "other"})
     with pytest.raises(mlxl3_amd.Exl3Error, match="rotary dimension 7"):
         mlxl3_amd.rope_frequencies(7)
+
+
+@pytest.mark.parametrize("scaling, msg", [
+    ({"rope_type": "linear"}, "'linear' rotary scaling takes"),
+    ({"type": "llama3", "factor": 8.0}, "'llama3' rotary scaling takes"),
+    ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "mscale": 0.7}, "'yarn' rotary scaling takes"),
+    ({"rope_type": "linear", "factor": 0.0}, "positive numbers"),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 4.0, "high_freq_factor": 4.0,
+      "original_max_position_embeddings": 8192}, "high_freq_factor must be above"),
+])
+def test_scalings_that_say_too_little_or_too_much(scaling, msg):
+    with pytest.raises(mlxl3_amd.Exl3Error, match=msg):
+        mlxl3_amd.rope_frequencies(64, 10000.0, scaling)
+
+
+def test_absent_and_default_scalings():
+    f, s = mlxl3_amd.rope_frequencies(64, 10000.0)
+    for scaling in ({}, {"rope_type": "default"}, {"rope_type": None, "factor": None}):
+        g, t = mlxl3_amd.rope_frequencies(64, 10000.0, scaling)
+        assert torch.equal(f, g) and s == t == 1.0
+    with pytest.raises(mlxl3_amd.Exl3Error, match="with base 1.0"):
+        mlxl3_amd.rope_frequencies(64, 1.0)

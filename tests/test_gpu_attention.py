@@ -411,6 +411,124 @@ def test_max_q_bounds_the_rows_computed():
         within(y[at : at + 3], want[:3], bound[:3], f"sequence {s}")
 
 
+@pytest.mark.parametrize("new", [[2, 4], [20, 40]])
+def test_starts_beyond_the_tokens_are_cut(new):
+    """The last sequence claims more rows than q has: those there are right, and the memory
+    behind them is left as it was."""
+    lens = [n + 70 for n in new]
+    pool = Pool(56, lens, 1, 64, 16, 16, F16)
+    q, cache, b, _ = run(pool, new, 4, F16)
+    cut = sum(new) - 3
+    out = torch.full((sum(new), 4, 64), 9.0, dtype=F16, device="cuda")
+    mlxl3_amd.attention(q[:cut].cuda(), cache, b, out=out[:cut])
+    at = 0
+    for s, n in enumerate(new):
+        want, bound = kv_ref.attend(q[at : at + n].double(), pool.values("k", s), pool.values("v", s), 70, 64**-0.5, True, 0, dtype=F16)
+        m = min(n, cut - at)
+        within(out[at : at + m], want[:m], bound[:m], f"sequence {s}")
+        at += n
+    assert bool((out[cut:] == 9.0).all())
+
+
+@pytest.mark.parametrize("most", [1, 150])
+def test_many_sequences(most):
+    """More sequences than a wave has lanes, some without new tokens, tiles of many."""
+    g = torch.Generator().manual_seed(57)
+    new = torch.randint(0, most + 1, (203,), generator=g).tolist()
+    lens = [n + int(o) for n, o in zip(new, torch.randint(0, 60, (203,), generator=g))]
+    pool = Pool(58, lens, 1, 64, 16, 8, None)
+    q, cache, b, y = run(pool, new, 2, BF16)
+    check(pool, new, q, y)
+    loose = kv_ref.batch(mlxl3_amd, new, lens, pool.table, max_q=2**31 - 1)
+    check(pool, new, q, mlxl3_amd.attention(q.cuda(), cache, loose))
+
+
+@pytest.mark.parametrize("group, new", [(33, [1, 2]), (200, [1, 3]), (129, [2])])
+def test_groups_larger_than_a_tile(group, new):
+    """The rows of one token fall into several tiles."""
+    lens = [n + 90 for n in new]
+    pool = Pool(60, lens, 2, 64, 32, 4, None)
+    q, _, _, y = run(pool, new, 2 * group, F16)
+    check(pool, new, q, y)
+
+
+@pytest.mark.parametrize("bits, cdtype, dtype", FORMATS[:3])
+@pytest.mark.parametrize("new, old, window", [([1], [5000], 1500), ([2, 1], [700, 4000], 900), ([64, 3], [6000, 10], 2500)])
+def test_windows_over_several_ranges(bits, cdtype, dtype, new, old, window):
+    lens = [n + o for n, o in zip(new, old)]
+    pool = Pool(62, lens, 1, 128, 64, bits, cdtype)
+    q, _, _, y = run(pool, new, 4, dtype, window=window)
+    check(pool, new, q, y, window=window)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_pages_beyond_32_bits(bits):
+    """Pages that lie more than 2^32 bytes (and values) into the pool: written, read, attended."""
+    dim, heads, page = 128, 8, 64
+    pages = 2**32 // (heads * page * dim) + 8
+    shape = (pages, heads, page)
+    kw = dict(device="cuda")
+    if bits == 16:
+        cache = mlxl3_amd.KvCache(*(torch.empty(*shape, dim, dtype=F16, **kw) for _ in range(2)))
+    else:
+        codes = [torch.empty(*shape, dim, dtype=torch.uint8, **kw) for _ in range(2)]
+        scales = [torch.empty(pages, heads, dim // 32, page, dtype=F16, **kw) for _ in range(2)]
+        cache = mlxl3_amd.KvCache(*codes, *scales, bits=8)
+    table = torch.tensor([[pages - 1, 0, pages - 3], [pages - 2, 1, 5]], dtype=torch.int32)
+    lens = [150, 131]
+    g = torch.Generator().manual_seed(63)
+    k, v = (torch.randn(sum(lens), heads, dim, generator=g).to(F16) for _ in range(2))
+    cache.append(kv_ref.batch(mlxl3_amd, lens, lens, table), k.cuda(), v.cuda())
+    rk, rv = (t.cpu() for t in cache.read(kv_ref.batch(mlxl3_amd, lens, lens, table), sum(lens)))
+    for got, x in ((rk, k), (rv, v)):
+        if bits == 8:
+            c, s = kv_ref.quantise(x, 8)
+            x = (c.float() * s.float().repeat_interleave(32, -1)).half()
+        assert torch.equal(got, x)
+    for new in ([1, 2], [40, 30]):
+        q = torch.randn(sum(new), 2 * heads, dim, generator=g).to(F16)
+        y = mlxl3_amd.attention(q.cuda(), cache, kv_ref.batch(mlxl3_amd, new, lens, table))
+        at = row = 0
+        for n, length in zip(new, lens):
+            kd, vd = k[row : row + length].double(), v[row : row + length].double()
+            if bits == 8:
+                kd, vd = (c.double() * s.double().repeat_interleave(32, -1) for c, s in (kv_ref.quantise(kd, 8), kv_ref.quantise(vd, 8)))
+            want, bound = kv_ref.attend(q[at : at + n].double(), kd, vd, length - n, dim**-0.5, True, 0, coded=bits == 8, dtype=F16)
+            within(y[at : at + n], want, bound, f"{n} new")
+            at, row = at + n, row + length
+
+
+def test_threads_that_share_a_batch():
+    """Two threads, each with its stream and cache, and one batch object: a call's workspace
+    goes by its own sizes."""
+    import threading
+
+    pools = [Pool(65, [3000], 1, dim, 16, 16, F16) for dim in (64, 256)]  # the same pages
+    assert torch.equal(pools[0].table, pools[1].table)
+    caches = [p.cuda(mlxl3_amd) for p in pools]
+    b = kv_ref.batch(mlxl3_amd, [1], [3000], pools[0].table)
+    qs = [torch.randn(1, 8, p.dim, generator=torch.Generator().manual_seed(67)).to(F16).cuda() for p in pools]
+    want = [mlxl3_amd.attention(q, c, b) for q, c in zip(qs, caches)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(100):
+                    if not torch.equal(mlxl3_amd.attention(qs[i], caches[i], b), want[i]):
+                        failed.append(f"thread {i}: another result")
+        except Exception as e:  # told to the main thread
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
 def test_same_call_same_bits_and_longer_bounds_of_the_launch():
     pool = Pool(59, [3000, 17, 800], 2, 128, 32, 8, None)
     for new in ([1, 1, 1], [40, 17, 2]):
