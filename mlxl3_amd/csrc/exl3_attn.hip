@@ -128,9 +128,7 @@ struct Shape {
   bool one_tile;  // every sequence's rows fit one workgroup
   int64_t tiles;  // at most; the device counts the tiles that there are
   int splits;     // ranges of the tokens that a tile sees
-  int split_tokens;
 };
-
 
 Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int heads, int window) {
   const int group = heads / c.kv_heads;
@@ -149,7 +147,6 @@ Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int h
   const int64_t want = (slots + groups - 1) / groups;
   const int64_t least = s.few ? 128 : 256;
   s.splits = (int)std::max<int64_t>(1, std::min(std::min<int64_t>(want, 32), (most + least / 2) / least));
-  s.split_tokens = (int)std::min<int64_t>(((most + s.splits - 1) / s.splits + 127) / 128 * 128, INT32_MAX - 255);
   return s;
 }
 
@@ -258,7 +255,6 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   p.window = window;
   p.max_q = batch->max_q;
   p.splits = sh.splits;
-  p.split_tokens = sh.split_tokens;
   p.one_tile = sh.one_tile;
   p.q_vec = aligned16(q) && (tokens == 1 || q_stride % 8 == 0);
   p.y_vec = ((uintptr_t)y & 7) == 0 && (tokens == 1 || y_stride % 4 == 0);

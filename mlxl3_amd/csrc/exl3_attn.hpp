@@ -16,7 +16,7 @@ struct AttnParams {
   int64_t q_stride, y_stride;
   int tokens;     // rows of q and y
   int heads, group, q_type, causal, window;
-  int max_q, splits, split_tokens;
+  int max_q, splits;
   int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
   int q_vec, y_vec;  // rows of q are 16-byte, rows of y 8-byte aligned
   float scale2;   // scale * log2(e): scores in units of a factor of two
@@ -193,14 +193,14 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// The tokens [t0, t1) of split `split` of [lo, hi): 16-aligned ranges of split_tokens each,
-// the same for every sequence, so that a ragged batch's workgroups take equally long (the
-// shorter sequences' last ones have nothing to do); longer ones where that leaves too few
-// splits (a sequence longer than the host was told).
+// The tokens [t0, t1) of split `split` of [lo, hi): 16-aligned ranges of a multiple of 128
+// tokens.  They go by the sequence's own length, not by what the host was told: 2000 tokens
+// told as 131072 take 12.6 us so and 29.8 in ranges of the host's, 32 sequences of 100 to
+// 8192 tokens 121 and 125.
 __device__ __forceinline__ void split_range(const AttnParams& p, int lo, int hi, int split, int& t0, int& t1) {
   lo &= ~15;
   const int n = max(hi - lo, 0);
-  const int each = max(p.split_tokens, ((n + p.splits - 1) / p.splits + 127) / 128 * 128);
+  const int64_t each = max((n + p.splits - 1) / p.splits + 127, 128) / 128 * 128;
   const int64_t a = (int64_t)lo + (int64_t)split * each;
   t0 = (int)min(a, (int64_t)hi);
   t1 = (int)min(a + each, (int64_t)hi);

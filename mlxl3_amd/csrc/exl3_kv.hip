@@ -106,17 +106,10 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
   if (p.positions) {
     if (on) pos = p.positions[t0 + t];
   } else {
-    // the wave's tokens, one by one
     const int first = __builtin_amdgcn_readfirstlane(t), last = min(__builtin_amdgcn_readlane(t, 63), nt - 1);
-    int seq = -1;
-    for (int i = first; i <= last; ++i) {
-      const KvToken at = kv_locate(p.batch, t0 + i);
-      if (t == i) {
-        seq = at.seq;
-        pos = at.pos;
-      }
-    }
-    on = on && seq >= 0;
+    const KvToken at = kv_locate(p.batch, t0 + first, last - first + 1, t - first);
+    pos = at.pos;
+    on = on && at.seq >= 0;
   }
   const int h0 = blockIdx.y * p.per, h1 = min(h0 + p.per, p.heads);
   const int da = tail ? 2 * r + (c - turned) * W : !two ? c * (VEC ? 8 : 2) : c * W;
@@ -237,15 +230,8 @@ struct Tile {
   // The thread's token, or seq = -1 behind the last.
   __device__ __forceinline__ KvToken locate(const KvBatchView& b, int64_t t0, int64_t tokens) const {
     constexpr int n = 64 / kLanes;  // tokens of a wave
-    const int wave = threadIdx.x >> 6;
-    KvToken mine{-1, 0};
-    for (int i = 0; i < n; ++i) {
-      const int64_t t = t0 + wave * n + i;
-      if (t >= tokens) break;
-      const KvToken at = kv_locate(b, t);
-      if (token == wave * n + i) mine = at;
-    }
-    return mine;
+    const int first = __builtin_amdgcn_readfirstlane(token);
+    return kv_locate(b, t0 + first, (int)min((int64_t)n, tokens - t0 - first), token - first);
   }
 };
 

@@ -46,27 +46,32 @@ __device__ __forceinline__ int64_t kv_page(const KvCacheView& c, const KvBatchVi
   return page >= 0 && page < c.pages ? page : -1;
 }
 
-// Where token row `token` belongs: its sequence (the first that ends behind it; -1 in
-// front of the first or behind the last) and its position there, the new tokens being
-// the sequence's last ones.  Every lane of a wave calls it with one token: the lanes look
-// at 64 sequences at a time.
+// Where token rows belong: a row's sequence (the first that ends behind it; -1 in front of
+// the first or behind the last) and its position there, the new tokens being the sequence's
+// last ones.
 struct KvToken {
   int seq;
   int64_t pos;
 };
-__device__ __forceinline__ KvToken kv_locate(const KvBatchView& b, int64_t token) {
-  const int lane = threadIdx.x & 63, first = b.q_starts[0];
-  for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+// Of the `count` successive rows from `first` on, the lane's row `mine`.  The whole wave calls
+// it, first and count the same in all lanes: the lanes look at 64 sequences at a time, for
+// all rows that end there.
+__device__ __forceinline__ KvToken kv_locate(const KvBatchView& b, int64_t first, int count, int mine) {
+  const int lane = threadIdx.x & 63, start = b.q_starts[0];
+  KvToken r{-1, 0};
+  int i = 0;
+  for (int s0 = 0; s0 < b.seqs && i < count; s0 += 64) {
     const int at = min(s0 + lane, b.seqs - 1);
     const int end = b.q_starts[at + 1], len = b.kv_lens[at];
-    const int n = __popcll(__ballot(s0 + lane < b.seqs && end <= token));
-    if (n < 64) {
-      const int seq = s0 + n;
-      if (seq >= b.seqs || token < first) break;
-      return KvToken{seq, (int64_t)__builtin_amdgcn_readlane(len, n) - __builtin_amdgcn_readlane(end, n) + token};
+    for (; i < count; ++i) {
+      const int64_t token = first + i;
+      const int n = __popcll(__ballot(s0 + lane < b.seqs && end <= token));
+      if (n == 64 || s0 + n >= b.seqs) break;
+      const int64_t pos = (int64_t)__builtin_amdgcn_readlane(len, n) - __builtin_amdgcn_readlane(end, n) + token;
+      if (token >= start && mine == i) r = KvToken{s0 + n, pos};
     }
   }
-  return KvToken{-1, 0};
+  return r;
 }
 
 // ---------------------------------------------------------------------------
