@@ -63,12 +63,27 @@ struct RopeView {
   double scale;
 };
 
-// Cosine and sine of pair i at position pos, in f32.
-__device__ __forceinline__ float2 rope_cs(const RopeView& r, int64_t pos, int i) {
-  double s, c;
-  sincos64((double)pos * (double)r.freq[i], &s, &c);
-  return make_float2((float)(c * r.scale), (float)(s * r.scale));
-}
+// Cosines and sines of a workgroup's tokens, [tokens][stride] in LDS.  A thread has one pair:
+// its frequency is loaded once, early, beside the workgroup's other first loads.
+struct RopeTable {
+  int pair, token, step;  // the thread's pair and first token, tokens at a time
+  float freq;
+  __device__ __forceinline__ RopeTable(const RopeView& r, int pairs) {
+    step = 256 / max(pairs, 1);
+    token = threadIdx.x / max(pairs, 1);
+    pair = threadIdx.x - token * pairs;
+    freq = pairs && token < step ? r.freq[pair] : 0.0f;
+  }
+  __device__ __forceinline__ void fill(const RopeView& r, const int64_t* positions, int tokens, float2* cs,
+                                       int stride) const {
+    if (token >= step) return;
+    for (int t = token; t < tokens; t += step) {
+      double s, c;
+      sincos64((double)positions[t] * (double)freq, &s, &c);
+      cs[t * stride + pair] = make_float2((float)(c * r.scale), (float)(s * r.scale));
+    }
+  }
+};
 
 constexpr int kBatch = 4;     // heads whose loads a thread has in flight
 
@@ -101,6 +116,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
   const bool two = !p.rope.interleaved;  // the pair's second half lies r channels further
   const int turned = VEC && !two ? 2 * r / W : r / W;
   const bool tail = c >= turned;
+  const RopeTable turns(p.rope, r);
   bool on = t < nt;
   int64_t pos = 0;
   if (p.positions) {
@@ -134,10 +150,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
   load(h0);
   if (c == 0 && t < nt) position[t] = pos;
   __syncthreads();
-  for (int j = threadIdx.x; j < nt * r; j += 256) {
-    const int i = j / r;
-    cs[j] = rope_cs(p.rope, position[i], j - i * r);
-  }
+  turns.fill(p.rope, position, nt, cs, r);
   __syncthreads();
   if (!on || (tail && p.x == p.y)) return;
   constexpr int N = VEC ? 8 : 1;
@@ -260,15 +273,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
       if (half) other[u].load(src, second ? at - r : at + r, p.vec);
     }
   };
+  const RopeTable turns(p.rope, r);
   load(w.h0);
   const KvToken at = w.locate(p.batch, t0, p.tokens);
   if (r) {
     if (w.d0 == 0) positions[w.token] = at.pos;
     __syncthreads();
-    for (int j = threadIdx.x; j < nt * r; j += 256) {
-      const int t = j / r;
-      cs[t][j - t * r] = rope_cs(p.rope, positions[t], j - t * r);
-    }
+    turns.fill(p.rope, positions, nt, cs[0], D / 2);
     __syncthreads();
   }
   const int64_t page = at.seq < 0 ? -1 : kv_page(c, p.batch, at.seq, at.pos);
