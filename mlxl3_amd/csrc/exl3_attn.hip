@@ -21,8 +21,8 @@
 
 namespace exl3 {
 
-// The splits of a row joined: grid (rows / rows per workgroup, kv heads, tiles).  D / 4
-// lanes hold a row's sums, four channels each; 2^shift such groups share the splits of
+// The splits or ranges of a row joined: grid (rows / rows per workgroup, kv heads, tiles or
+// sequences).  D / 4 lanes hold a row's sums, four channels each; 2^shift such groups share the splits of
 // one row, so that a row's loads are in flight together, and meet in LDS in a fixed order.
 // A split that saw nothing has a maximum of -inf and a sum of 0, and its sums, which are
 // not written, are not read.
@@ -39,33 +39,45 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows, 
   const Work w = tile_work(p, tile, rows, row0);
   const int row = row0 + in_tile;
   const bool live = in_tile < rows && row < w.rows;
-  const size_t slot = (size_t)(tile * p.cache.kv_heads + kvh) * p.splits * rows + in_tile;
+  int count = p.splits;
+  const size_t step = (size_t)p.cache.kv_heads * rows;
+  size_t first = (size_t)tile * p.splits;
+  if (p.budget) {  // this sequence's ranges lie behind those of the ones before
+    const int size = range_tokens(p);
+    count = range_count(size, seen_tokens(p, w));
+    if (count < 2) return;
+    float before = 0.0f;
+    for (int seq = threadIdx.x & 63; seq < tile; seq += 64)
+      before += (float)range_count(size, seen_tokens(p, sequence_work(p, seq)));
+    first = (size_t)wave_sum(before);
+  }
+  const size_t slot = first * step + (size_t)kvh * rows + in_tile;
   float4v acc = {0, 0, 0, 0};
   float total = 0.0f;
   if (live) {
     float most = -__builtin_inff();
-    for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
+    for (int s0 = 0; s0 < count; s0 += kBatch) {
       float m[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int s = min(s0 + i, p.splits - 1);
-        m[i] = p.stats[(slot + (size_t)s * rows) * 2];
+        const int s = min(s0 + i, count - 1);
+        m[i] = p.stats[(slot + s * step) * 2];
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) most = fmaxf(most, m[i]);
     }
     const float base = most == -__builtin_inff() ? 0.0f : most;
-    for (int s0 = part; s0 < p.splits; s0 += per * kBatch) {
+    for (int s0 = part; s0 < count; s0 += per * kBatch) {
       float f[kBatch], l[kBatch];
       bool saw[kBatch];
       float4v v[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int s = s0 + i * per;
-        const size_t at = slot + (size_t)min(s, p.splits - 1) * rows;
+        const size_t at = slot + min(s, count - 1) * step;
         const float m = p.stats[at * 2];
         l[i] = p.stats[at * 2 + 1];
-        const bool on = s < p.splits && !(m == -__builtin_inff() && l[i] == 0.0f);
+        const bool on = s < count && !(m == -__builtin_inff() && l[i] == 0.0f);
         saw[i] = on;
         f[i] = on ? __builtin_amdgcn_exp2f(m - base) : 0.0f;
         l[i] = on ? l[i] : 0.0f;
@@ -127,7 +139,9 @@ struct Shape {
   int rows;       // rows of a workgroup
   bool one_tile;  // every sequence's rows fit one workgroup
   int64_t tiles;  // at most; the device counts the tiles that there are
-  int splits;     // ranges of the tokens that a tile sees
+  int splits;     // even ranges of the tokens that a tile sees
+  int budget;     // else ranges by the batch's sum, about (as AttnParams')
+  int64_t slots;  // of partial results to join, `rows` rows each
 };
 
 Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int heads, int window) {
@@ -142,21 +156,24 @@ Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int h
   const int64_t room = (int64_t)b.table_pages << c.page_shift;
   int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;
   if (window > 0) most = std::min<int64_t>(most, (int64_t)window + b.max_q);
-  const int64_t groups = s.tiles * c.kv_heads;
-  const int64_t slots = c.head_dim == 256 ? 256 : s.rows == 16 ? 768 : 512;
-  const int64_t want = (slots + groups - 1) / groups;
+  const int64_t resident = c.head_dim == 256 ? 256 : s.rows == 16 ? 768 : 512;
+  s.budget = 0;
+  s.slots = 0;
+  const int64_t groups = s.tiles * c.kv_heads, want = (resident + groups - 1) / groups;
   const int64_t least = s.few ? 128 : 256;
   s.splits = (int)std::max<int64_t>(1, std::min(std::min<int64_t>(want, 32), (most + least / 2) / least));
+  if (s.splits > 1) s.slots = groups * s.splits;
+  if (s.few && b.seqs > 1 && s.splits > 1 && most / s.splits >= 1024) {
+    s.budget = (int)(resident / c.kv_heads - b.seqs / 2);
+    s.slots = std::max(s.slots, (s.budget + b.seqs + 1) * (int64_t)c.kv_heads);  // a window may ask for either
+  }
   return s;
-}
-
-size_t slots_of(const Shape& s, const KvCacheView& c) {
-  return (size_t)s.tiles * c.kv_heads * s.splits * s.rows;
 }
 
 template <int FMT, typename T, int PARTS, int D, int RT>
 void launch_few(const AttnParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.splits, (unsigned)p.cache.kv_heads, (unsigned)p.batch.seqs);
+  const int ranges = p.budget ? p.budget + p.batch.seqs + 1 : p.batch.seqs * p.splits;
+  const dim3 grid((unsigned)p.cache.kv_heads, (unsigned)ranges);
   constexpr size_t lds = 4 * (Few<FMT, T, D, RT, PARTS>::kWaveLds);
   hipLaunchKernelGGL((attn_few_kernel<FMT, T, D, RT, PARTS>), grid, dim3(256), lds, s, p);
 }
@@ -198,9 +215,8 @@ extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
       batch->table_pages <= 0 || heads % cache->view.kv_heads)
     return 0;
   const Shape sh = choose(cache->view, *batch, tokens, heads, 0);
-  if (sh.splits == 1) return 0;
-  const size_t slots = slots_of(sh, cache->view);
-  return align256(slots * cache->view.head_dim * 4) + align256(slots * 8);
+  const size_t rows = (size_t)sh.slots * sh.rows;
+  return align256(rows * cache->view.head_dim * 4) + align256(rows * 8);
 }
 
 extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
@@ -255,13 +271,13 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   p.window = window;
   p.max_q = batch->max_q;
   p.splits = sh.splits;
+  p.budget = sh.budget;
   p.one_tile = sh.one_tile;
   p.q_vec = aligned16(q) && (tokens == 1 || q_stride % 8 == 0);
   p.y_vec = ((uintptr_t)y & 7) == 0 && (tokens == 1 || y_stride % 4 == 0);
   p.scale2 = scale2;
-  const size_t slots = slots_of(sh, p.cache);
   p.part = (float*)workspace;
-  p.stats = (float*)((uint8_t*)workspace + align256(slots * p.cache.head_dim * 4));
+  p.stats = (float*)((uint8_t*)workspace + align256((size_t)sh.slots * sh.rows * p.cache.head_dim * 4));
   const int D = p.cache.head_dim;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = launch_gate("attention")) return rc;
@@ -272,13 +288,13 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
     default: launch<KV_Q4, F16>(p, sh, s);
   }
   if (int rc = check_launch("attention")) return rc;
-  if (sh.splits == 1) return EXL3_OK;
+  if (!sh.slots) return EXL3_OK;
   if (int rc = launch_gate("attention join")) return rc;
   const int rows_most = (int)std::min<int64_t>(sh.rows, (int64_t)batch->max_q * p.group);
-  // as many groups of lanes per row as there are batches of splits to share
-  const int groups = 1024 / D;
+  // as many groups of lanes per row as there are splits to share
+  const int groups = 1024 / D, most = sh.budget ? kMostRanges : sh.splits;
   int shift = 0;
-  while ((2 << shift) <= groups && (1 << shift) < sh.splits) ++shift;
+  while ((2 << shift) <= groups && (1 << shift) < most) ++shift;
   const int per_block = groups >> shift;
   const dim3 grid((unsigned)((rows_most + per_block - 1) / per_block), (unsigned)p.cache.kv_heads,
                   (unsigned)sh.tiles);

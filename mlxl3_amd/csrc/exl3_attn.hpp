@@ -11,12 +11,14 @@ struct AttnParams {
   KvBatchView batch;
   const void* q;
   void* y;
-  float* part;    // [tiles][kv heads][splits][rows][D] weighted sums
-  float* stats;   // [tiles][kv heads][splits][rows][2] their maximum and sum of weights
+  float* part;    // weighted sums [slots][rows][D]; slots: [tiles][splits or ranges][kv heads]
+  float* stats;   // [slots][rows][2] their maximum and sum of weights
   int64_t q_stride, y_stride;
   int tokens;     // rows of q and y
   int heads, group, q_type, causal, window;
-  int max_q, splits;
+  int max_q;
+  int splits;     // even ranges of the tokens that a tile sees
+  int budget;     // else ranges by the batch's sum (few rows), about; 0: even ones
   int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
   int q_vec, y_vec;  // rows of q are 16-byte, rows of y 8-byte aligned
   float scale2;   // scale * log2(e): scores in units of a factor of two
@@ -145,31 +147,52 @@ __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
   return w;
 }
 
-// Sequence and first row of tile `tile`, sequences cut into tiles of `rows` rows; a tile
-// behind the last has no rows.  Every lane of a wave calls it.
-__device__ __forceinline__ Work tile_work(const AttnParams& p, int tile, int rows, int& row0) {
-  row0 = 0;
-  if (p.one_tile) return sequence_work(p, tile);
+__device__ __forceinline__ float wave_sum(float v) {
+  v += xor_lanes<1>(v);
+  v += xor_lanes<2>(v);
+  v += xor_lanes<4>(v);
+  v += xor_lanes<8>(v);
+  v += xor_lanes<16>(v);
+  v += xor_lanes<32>(v);
+  return v;
+}
+
+// The sequence that item `i` belongs to, `items` telling how many each has; i becomes its
+// number there.  Behind the last item: no rows.  Every lane of a wave calls it with one i.
+template <typename F>
+__device__ __forceinline__ Work work_of(const AttnParams& p, int& i, F&& items) {
   const int lane = threadIdx.x & 63;
   for (int s0 = 0; s0 < p.batch.seqs; s0 += 64) {
     const int seq = s0 + lane;
-    const int mine = seq < p.batch.seqs ? (sequence_work(p, seq).rows + rows - 1) / rows : 0;
+    const Work x = seq < p.batch.seqs ? sequence_work(p, seq) : Work{};
+    const int mine = seq < p.batch.seqs ? items(x) : 0;
     int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int other = __shfl_up(upto, d);
       if (lane >= d) upto += other;
     }
-    const uint64_t past = __ballot(upto > tile);
+    const uint64_t past = __ballot(upto > i);
     if (past) {
       const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
-      row0 = (tile - __shfl(upto - mine, at)) * rows;
-      row0 = __builtin_amdgcn_readfirstlane(row0);
-      return sequence_work(p, s0 + at);
+      i -= __builtin_amdgcn_readlane(upto - mine, at);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+      return Work{s0 + at, of(x.start), of(x.rows), of(x.first), of(x.len),
+                  p.batch.table + (int64_t)(s0 + at) * p.batch.table_pages};
     }
-    tile -= __shfl(upto, 63);
+    i -= __builtin_amdgcn_readlane(upto, 63);
   }
   return Work{};
+}
+
+// Sequence and first row of tile `tile`, sequences cut into tiles of `rows` rows; a tile
+// behind the last has no rows.
+__device__ __forceinline__ Work tile_work(const AttnParams& p, int tile, int rows, int& row0) {
+  row0 = 0;
+  if (p.one_tile) return sequence_work(p, tile);
+  const Work w = work_of(p, tile, [&](const Work& x) { return (x.rows + rows - 1) / rows; });
+  row0 = tile * rows;
+  return w;
 }
 
 // The table's entry for the 16 tokens from t (a multiple of 16) on, hi > 0 the end of the
@@ -183,27 +206,40 @@ __device__ __forceinline__ int page_ok(const AttnParams& p, int entry, int t, in
   return t < hi && (uint32_t)entry < (uint32_t)p.cache.pages ? entry : -1;  // pages < 2^31
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-  v += xor_lanes<1>(v);
-  v += xor_lanes<2>(v);
-  v += xor_lanes<4>(v);
-  v += xor_lanes<8>(v);
-  v += xor_lanes<16>(v);
-  v += xor_lanes<32>(v);
-  return v;
+// A tile's tokens split evenly: the length of each of p.splits ranges of `n` tokens, a multiple
+// of 128.  It goes by the sequence's own length, not by what the host was told.
+__device__ __forceinline__ int split_tokens(const AttnParams& p, int n) {
+  return (int)max(((uint32_t)(n + p.splits - 1) / p.splits + 127) & ~127u, 128u);
+}
+// The tokens that a sequence's rows see, from a multiple of 16 on; a sequence with rows has one.
+__device__ __forceinline__ int seen_tokens(const AttnParams& p, const Work& w) {
+  if (w.rows == 0) return 0;
+  const int lo = row_sees(p, w.first, w.len, 0).lo & ~15;
+  return max(row_sees(p, w.first, w.len, w.rows - 1).hi - lo, 1);
 }
 
-// The tokens [t0, t1) of split `split` of [lo, hi): 16-aligned ranges of a multiple of 128
-// tokens.  They go by the sequence's own length, not by what the host was told: 2000 tokens
-// told as 131072 take 12.6 us so and 29.8 in ranges of the host's, 32 sequences of 100 to
-// 8192 tokens 121 and 125.
-__device__ __forceinline__ void split_range(const AttnParams& p, int lo, int hi, int split, int& t0, int& t1) {
-  lo &= ~15;
-  const int n = max(hi - lo, 0);
-  const int64_t each = max((n + p.splits - 1) / p.splits + 127, 128) / 128 * 128;
-  const int64_t a = (int64_t)lo + (int64_t)split * each;
-  t0 = (int)min(a, (int64_t)hi);
-  t1 = (int)min(a + each, (int64_t)hi);
+// A batch of few rows split by its sum: ranges of equally many tokens for all sequences, longer
+// sequences in more of them, so that a ragged batch's workgroups take equally long.  Every
+// workgroup forms the sum of the tokens seen for itself and cuts them into about `budget`
+// ranges, at most budget + seqs (a sequence's last one may be short).
+constexpr int kMostRanges = 32;  // of a sequence: a row's ranges are joined by few lanes
+// The tokens of a range, by the batch (a wave calls it) and by the sequence's own.
+__device__ __forceinline__ int range_tokens(const AttnParams& p) {
+  float total = 0.0f;
+  for (int s0 = 0; s0 < p.batch.seqs; s0 += 64) {
+    const int seq = s0 + (threadIdx.x & 63);
+    if (seq < p.batch.seqs) total += (float)seen_tokens(p, sequence_work(p, seq));
+  }
+  total = wave_sum(total);
+  return __builtin_amdgcn_readfirstlane(((int)fminf(total / p.budget, 2147483392.0f) + 128) & ~127);
+}
+__device__ __forceinline__ int range_tokens(int each, int n) {
+  constexpr int unit = kMostRanges * 128;
+  return max(each, (n + unit - 1) / unit * 128);
+}
+__device__ __forceinline__ int range_count(int each, int n) {
+  const uint32_t size = range_tokens(each, n);
+  return (int)(((uint32_t)n + size - 1) / size);
 }
 
 // A score above the running maximum by no more than this (in factors of two) does not

@@ -201,7 +201,8 @@ struct Few {
   }
 };
 
-// grid (splits, kv heads, sequences)
+// grid (kv heads, sequences x splits, or ranges by the batch's sum): ranges that there are come
+// before those left over, which would take the place of others on a CU
 template <int FMT, typename T, int D, int RT, int PARTS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_kernel(AttnParams p) {
   typedef Few<FMT, T, D, RT, PARTS> F;
@@ -210,20 +211,33 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   __shared__ float wave_m[4][16 * RT], wave_l[4][16 * RT];
   __shared__ int retry;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int split = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
-  const Work w = sequence_work(p, seq);
+  const int kvh = blockIdx.x;
+  int part, size = INT32_MAX & ~127;
+  Work w;
+  if (p.budget) {
+    part = blockIdx.y;
+    size = range_tokens(p);
+    w = work_of(p, part, [&](const Work& x) { return range_count(size, seen_tokens(p, x)); });
+  } else {
+    const int seq = p.splits > 1 ? blockIdx.y / p.splits : blockIdx.y;
+    part = blockIdx.y - seq * p.splits;
+    w = sequence_work(p, seq);
+  }
   if (w.rows == 0) return;
   const Seen top = row_sees(p, w.first, w.len, 0), end = row_sees(p, w.first, w.len, w.rows - 1);
   // rows see later tokens the later they are: the union is [top.lo, end.hi), what all see
   // [end.lo, top.hi)
-  int t0, t1;
-  split_range(p, top.lo, end.hi, split, t0, t1);
-  if (p.splits > 1 && t0 >= t1) {
-    const size_t slot = ((size_t)(seq * p.cache.kv_heads + kvh) * p.splits + split) * (16 * RT);
+  const int seen = seen_tokens(p, w);
+  size = p.budget ? range_tokens(size, seen) : p.splits > 1 ? split_tokens(p, seen) : size;
+  const bool whole = p.budget ? seen <= size : p.splits == 1;  // the result is final
+  const size_t slot0 = ((size_t)blockIdx.y * p.cache.kv_heads + kvh) * (16 * RT);
+  if ((int64_t)part * size >= seen) {  // a split that a short sequence has no tokens for
     for (int e = threadIdx.x; e < 2 * w.rows; e += 256)
-      p.stats[slot * 2 + e] = e & 1 ? 0.0f : -__builtin_inff();
+      p.stats[slot0 * 2 + e] = e & 1 ? 0.0f : -__builtin_inff();
     return;
   }
+  const int t0 = (top.lo & ~15) + part * size;
+  const int t1 = (int)min((int64_t)t0 + size, (int64_t)end.hi);
   if (threadIdx.x == 0) retry = 0;
   __syncthreads();
 
@@ -414,13 +428,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
       f[i] = __builtin_amdgcn_exp2f(wave_m[i][row] - base);
       total += wave_l[i][row] * f[i];
     }
-    const float norm = p.splits > 1 ? 1.0f : total != 0.0f ? 1.0f / total : 0.0f;
+    const float norm = !whole ? 1.0f : total != 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) wave_l[i][row] = f[i] * norm;
-    if (p.splits > 1 && row < w.rows) {
-      const size_t slot = ((size_t)(seq * p.cache.kv_heads + kvh) * p.splits + split) * (16 * RT) + row;
-      p.stats[slot * 2] = most;
-      p.stats[slot * 2 + 1] = total;
+    if (!whole && row < w.rows) {
+      p.stats[(slot0 + row) * 2] = most;
+      p.stats[(slot0 + row) * 2 + 1] = total;
     }
   }
   __syncthreads();
@@ -440,7 +453,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         for (int c = 0; c < 4; ++c) sum[c] += v[c] * f;
       }
     }
-    if (p.splits == 1) {
+    if (whole) {
       uint16_t* to = (uint16_t*)p.y + (size_t)(w.start + row / p.group) * p.y_stride +
                      (size_t)(kvh * p.group + row % p.group) * D + d;
       const u32x2 y = {pack2(p.q_type, sum[0], sum[1]), pack2(p.q_type, sum[2], sum[3])};
@@ -451,8 +464,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         for (int c = 0; c < 4; ++c) to[c] = (uint16_t)(y[c / 2] >> (16 * (c & 1)));
       }
     } else {
-      const size_t slot = ((size_t)(seq * p.cache.kv_heads + kvh) * p.splits + split) * (16 * RT) + row;
-      *(float4v*)(p.part + slot * D + d) = float4v{sum[0], sum[1], sum[2], sum[3]};
+      *(float4v*)(p.part + (slot0 + row) * D + d) = float4v{sum[0], sum[1], sum[2], sum[3]};
     }
   }
 }

@@ -32,6 +32,7 @@ struct Many {
   static constexpr int kLoads = kMine > kRows ? kMine / kRows : 1;
   static constexpr int kTile = kTokens * D * 2;                         // bytes in LDS
   static constexpr int kLds = 4 * kTile;                                // keys and values, twice
+  static constexpr int kGroups = D == 64 ? 3 : 256 / D;                 // workgroups that share a CU
 
   struct Loads {  // of coded caches
     u32x4 k[kLoads], v[kLoads];
@@ -136,7 +137,9 @@ struct Many {
 // One-dimensional grid of tiles x splits x kv heads, the heads fastest (blocks go to the
 // XCDs in turn, so a head's tiles share few L2s), a sequence's last and longest tiles first.
 template <int FMT, typename T, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(256 / D > 3 ? 3 : 256 / D, 256 / D > 3 ? 3 : 256 / D))) void attn_many_kernel(AttnParams p, int tiles) {
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(Many<FMT, T, D>::kGroups, Many<FMT, T, D>::kGroups)))
+void attn_many_kernel(AttnParams p, int tiles) {
   typedef Many<FMT, T, D> F;
   typedef typename T::V8 V8;
   constexpr int TK = F::kTokens, NT = TK / 32;
@@ -150,9 +153,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(256 / D > 3
   const int rows = min(w.rows - row0, kManyRows);
   if (rows <= 0) return;
   const Seen top = row_sees(p, w.first, w.len, row0), end = row_sees(p, w.first, w.len, row0 + rows - 1);
-  int t0, t1;
-  split_range(p, top.lo, end.hi, split, t0, t1);
-  const size_t slot0 = ((size_t)(tile * p.cache.kv_heads + kvh) * p.splits + split) * kManyRows;
+  const int lo = top.lo & ~15, seen = max(end.hi - lo, 0), size = split_tokens(p, seen);
+  const int t0 = (int)min((int64_t)lo + (int64_t)split * size, (int64_t)INT32_MAX - 4095);
+  const int t1 = (int)min((int64_t)t0 + size, (int64_t)end.hi);
+  const size_t slot0 = ((size_t)(tile * p.splits + split) * p.cache.kv_heads + kvh) * kManyRows;
   if (p.splits > 1 && t0 >= t1) {
     for (int e = threadIdx.x; e < 2 * rows; e += 256)
       p.stats[slot0 * 2 + e] = e & 1 ? 0.0f : -__builtin_inff();
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(256 / D > 3
     if (busy && t < wend.hi && t + TK > wtop.lo) {
       // The compiler orders these reads and products for few registers, each product right
       // behind its read; pin() keeps kDepth reads ahead of the products.
-            constexpr int QK = NT * (D / 16), kDepth = 4;
+      constexpr int QK = NT * (D / 16), kDepth = 4;
       float16v s[NT];
       auto key = [&](int i) __attribute__((always_inline)) {
         return *(const V8*)(keys + F::key_place(32 * (i % NT) + n, 2 * (i / NT) + h));

@@ -443,6 +443,31 @@ def test_many_sequences(most):
     check(pool, new, q, mlxl3_amd.attention(q.cuda(), cache, loose))
 
 
+@pytest.mark.parametrize("bits, cdtype, dtype", FORMATS)
+@pytest.mark.parametrize("dim, kv_heads, group, new, old", [
+    (128, 8, 4, [1, 1, 1, 0, 1], [5000, 0, 300, 77, 1290]),
+    (64, 2, 7, [2, 1, 4, 1], [2, 6000, 40, 700]),
+    (256, 4, 2, [1, 3], [200, 3333]),
+])
+@pytest.mark.parametrize("window", [0, 50000, 700])
+def test_ragged_batches_told_long_ones(bits, cdtype, dtype, dim, kv_heads, group, new, old, window):
+    """Bounds of 100000 tokens: the ranges go by the tokens that there are."""
+    lens = [n + o for n, o in zip(new, old)]
+    pool = Pool(68, lens, kv_heads, dim, 64, bits, cdtype, table_pages=1600)
+    q, _, _, y = run(pool, new, kv_heads * group, dtype, window=window)
+    check(pool, new, q, y, window=window)
+
+
+def test_many_ragged_sequences_told_long_ones():
+    g = torch.Generator().manual_seed(69)
+    lens = torch.randint(1, 500, (150,), generator=g).tolist()
+    lens[77] = 9000
+    pool = Pool(70, lens, 1, 64, 64, 16, F16, table_pages=2000)
+    new = [min(1 + i % 3, n) for i, n in enumerate(lens)]
+    q, _, _, y = run(pool, new, 4, F16)
+    check(pool, new, q, y)
+
+
 @pytest.mark.parametrize("group, new", [(33, [1, 2]), (200, [1, 3]), (129, [2])])
 def test_groups_larger_than_a_tile(group, new):
     """The rows of one token fall into several tiles."""
