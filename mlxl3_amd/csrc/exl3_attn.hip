@@ -172,8 +172,8 @@ Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int h
 
 template <int FMT, typename T, int PARTS, int D, int RT>
 void launch_few(const AttnParams& p, hipStream_t s) {
-  const int ranges = p.budget ? p.budget + p.batch.seqs + 1 : p.batch.seqs * p.splits;
-  const dim3 grid((unsigned)p.cache.kv_heads, (unsigned)ranges);
+  const dim3 grid = p.budget ? dim3((unsigned)p.cache.kv_heads, (unsigned)(p.budget + p.batch.seqs + 1))
+                             : dim3((unsigned)p.cache.kv_heads, (unsigned)p.splits, (unsigned)p.batch.seqs);
   constexpr size_t lds = 4 * (Few<FMT, T, D, RT, PARTS>::kWaveLds);
   hipLaunchKernelGGL((attn_few_kernel<FMT, T, D, RT, PARTS>), grid, dim3(256), lds, s, p);
 }

@@ -201,8 +201,8 @@ struct Few {
   }
 };
 
-// grid (kv heads, sequences x splits, or ranges by the batch's sum): ranges that there are come
-// before those left over, which would take the place of others on a CU
+// grid (kv heads, splits, sequences) or (kv heads, ranges by the batch's sum): ranges that there
+// are come before those left over, which would take the place of others on a CU
 template <int FMT, typename T, int D, int RT, int PARTS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_kernel(AttnParams p) {
   typedef Few<FMT, T, D, RT, PARTS> F;
@@ -212,16 +212,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   __shared__ int retry;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x;
-  int part, size = INT32_MAX & ~127;
+  int part = blockIdx.y, size = INT32_MAX & ~127;
   Work w;
   if (p.budget) {
-    part = blockIdx.y;
     size = range_tokens(p);
     w = work_of(p, part, [&](const Work& x) { return range_count(size, seen_tokens(p, x)); });
   } else {
-    const int seq = p.splits > 1 ? blockIdx.y / p.splits : blockIdx.y;
-    part = blockIdx.y - seq * p.splits;
-    w = sequence_work(p, seq);
+    w = sequence_work(p, blockIdx.z);
   }
   if (w.rows == 0) return;
   const Seen top = row_sees(p, w.first, w.len, 0), end = row_sees(p, w.first, w.len, w.rows - 1);
@@ -230,7 +227,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   const int seen = seen_tokens(p, w);
   size = p.budget ? range_tokens(size, seen) : p.splits > 1 ? split_tokens(p, seen) : size;
   const bool whole = p.budget ? seen <= size : p.splits == 1;  // the result is final
-  const size_t slot0 = ((size_t)blockIdx.y * p.cache.kv_heads + kvh) * (16 * RT);
+  const size_t slot0 = ((size_t)(blockIdx.z * gridDim.y + blockIdx.y) * p.cache.kv_heads + kvh) * (16 * RT);
   if ((int64_t)part * size >= seen) {  // a split that a short sequence has no tokens for
     for (int e = threadIdx.x; e < 2 * w.rows; e += 256)
       p.stats[slot0 * 2 + e] = e & 1 ? 0.0f : -__builtin_inff();
