@@ -285,7 +285,8 @@ typedef enum {
  * A stored value is code * scale, scale = f16(max|x| / 127) of its group
  * (4 bits: / 7; at most 65504), code = x / scale rounded to nearest even and
  * clipped to +-127 (+-7).  A group that holds a NaN or an infinity reads back
- * as NaN. */
+ * as NaN.  exl3_attention forms stored values in f16: beyond 65504 they need
+ * not stay finite there. */
 typedef struct exl3_kv_cache exl3_kv_cache;
 int exl3_kv_cache_create(void* k, void* v, uint16_t* k_scales, uint16_t* v_scales,
                          int32_t format, int64_t pages, int32_t page_tokens, int32_t kv_heads,
@@ -374,7 +375,7 @@ int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const
  * it with o, in exl3_linear_output_dtype(o, x_type).  x_type is f16 or bf16
  * (the cache's type where that is 16-bit).  q.out = o.in = heads * head_dim,
  * k.out = v.out = kv_heads * head_dim.  Bit-identical to the calls it stands
- * for.  Rows outside every sequence get unspecified values.  Biased
+ * for.  Rows outside every sequence and past max_q get unspecified values.  Biased
  * projections under bf16 give f32 queries, which are rounded to bf16 by the
  * rotation: without one they are refused.  Workspace:
  * exl3_attn_block_workspace_bytes, zero-filled once like the others. */

@@ -22,10 +22,12 @@
 namespace exl3 {
 
 // The splits or ranges of a row joined: grid (rows / rows per workgroup, kv heads, tiles or
-// sequences).  D / 4 lanes hold a row's sums, four channels each; 2^shift such groups share the splits of
-// one row, so that a row's loads are in flight together, and meet in LDS in a fixed order.
+// sequences).  D / 4 lanes hold a row's sums, four channels each; 2^shift such groups share
+// the splits of one row, so that a row's loads are in flight together, and meet in LDS in a
+// fixed order.
 // A split that saw nothing has a maximum of -inf and a sum of 0, and its sums, which are
-// not written, are not read.
+// not written, are not used.  Its latency bounds it: 5 us for 32 splits of 32 rows (a launch
+// alone takes 2 to 3), 53 before the loads went out together.
 template <int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows, int shift) {
   constexpr int L = D / 4, kGroups = 256 / L, kBatch = 8;
@@ -144,6 +146,21 @@ struct Shape {
   int64_t slots;  // of partial results to join, `rows` rows each
 };
 
+// Few rows (decode, drafts) go to attn_few_kernel, up to 16 or 32 of them -- 32 of 256 channels
+// do not fit its registers -- others to attn_many_kernel.  Rows 17 to 32, us: 20 rows over
+// 6001 4-bit tokens 24.5 (many 26.5), 32 rows of 8 sequences over 4096 16-bit ones 36.3 (34.5).
+//
+// Where the tiles leave the chip idle their tokens are split, evenly or by the batch's sum, into
+// as many workgroups as run at once: three a CU with 16 rows, two with 32 or 128, one of 256
+// channels.  (Half as many: 32 8-bit decodes 122 us instead of 95, 512 rows over 8192 107 for
+// 103; twice as many: drafts 33 for 24, 512 rows 127.)  No more than 32 of a sequence, which
+// one launch has to join (16: one token over 131071 120 us for 105; 64: 110, of 64 channels 24
+// for 21, of 256 40 for 45), and none shorter than 128 tokens for few rows (256: one token over
+// 1000 12.2 us for 11.2) or 512 for many (256: 256 rows over 8192 36 us for 30).
+//
+// Ranges by the sum cost every workgroup a look at all lengths, some 3 us a call (drafts 28.0
+// for 24.5), and save the wait for the longest sequence (8192 + 31 x 200 tokens 39 us to 24, 32
+// decodes of 1000 to 8192 99 to 95): from 1024 tokens a split on.
 Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int heads, int window) {
   const int group = heads / c.kv_heads;
   const int64_t rows = (int64_t)b.max_q * group;
@@ -154,17 +171,16 @@ Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int h
   s.tiles = s.one_tile ? b.seqs
                        : std::min((rows + s.rows - 1) / s.rows * b.seqs, tokens * group / s.rows + b.seqs);
   const int64_t room = (int64_t)b.table_pages << c.page_shift;
-  int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;
+  int64_t most = b.max_kv > 0 ? std::min<int64_t>(b.max_kv, room) : room;  // tokens a row sees
   if (window > 0) most = std::min<int64_t>(most, (int64_t)window + b.max_q);
   const int64_t resident = c.head_dim == 256 ? 256 : s.rows == 16 ? 768 : 512;
-  s.budget = 0;
-  s.slots = 0;
   const int64_t groups = s.tiles * c.kv_heads, want = (resident + groups - 1) / groups;
-  const int64_t least = s.few ? 128 : 256;
-  s.splits = (int)std::max<int64_t>(1, std::min(std::min<int64_t>(want, 32), (most + least / 2) / least));
-  if (s.splits > 1) s.slots = groups * s.splits;
+  const int64_t least = s.few ? 128 : 512;
+  s.splits = (int)std::max<int64_t>(1, std::min(std::min<int64_t>(want, kMostRanges), (most + least / 2) / least));
+  s.slots = s.splits > 1 ? groups * s.splits : 0;
+  s.budget = 0;
   if (s.few && b.seqs > 1 && s.splits > 1 && most / s.splits >= 1024) {
-    s.budget = (int)(resident / c.kv_heads - b.seqs / 2);
+    s.budget = (int)(resident / c.kv_heads - b.seqs / 2);  // seqs * kv_heads < resident: at least 1
     s.slots = std::max(s.slots, (s.budget + b.seqs + 1) * (int64_t)c.kv_heads);  // a window may ask for either
   }
   return s;

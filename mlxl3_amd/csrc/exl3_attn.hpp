@@ -80,7 +80,9 @@ __device__ __forceinline__ bool not_finite(const u32x4& v) {
 __device__ __forceinline__ constexpr int place4(int e) { return e < 4 ? 2 * e : 2 * e - 7; }
 __device__ __forceinline__ constexpr int channel4(int e) { return (e >> 1) | ((e & 1) << 2); }
 
-// f16 of a query of a coded cache; a bf16 beyond f16's range takes its largest value.
+// f16 of a query of a coded cache, whose products are f16: a bf16 has fewer bits than that, so
+// it stays exact down to 2^-14 (below, off by at most 2^-25); beyond f16's range it takes its
+// largest value.
 __device__ __forceinline__ uint16_t f2h_sat(float v) {
   const float a = fabsf(v);
   return f2h(a > 65504.0f && a <= 3.402823466e38f ? copysignf(65504.0f, v) : v);
@@ -244,6 +246,7 @@ __device__ __forceinline__ int range_count(int each, int n) {
 
 // A score above the running maximum by no more than this (in factors of two) does not
 // move it: weights stay below 256 and far inside 16 bits' range, their sums inside f32's.
+// So most steps rescale nothing and exchange nothing between lanes.
 constexpr float kSlack = 8.0f;
 
 // One row over the tokens [lo, hi) by one wave, its channels spread over the lanes (lane

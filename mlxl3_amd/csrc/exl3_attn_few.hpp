@@ -17,6 +17,18 @@
 // at all; the sum l is kept per lane and reduced once at the end.
 // The waves' results meet in LDS; with more than one range per sequence they are joined
 // by attn_join_kernel.
+//
+// P rounded to 16 bits is the product's operand type; its sum l is of the unrounded ones.
+// The loop's only waits are for its own loads: the next step's keys and values are on the
+// way while this one's are used.
+//
+// Measured, heads of 128 channels, 4 query heads a cache head, the join included: one bf16
+// token over 131071 16-bit tokens 105 us, 5.1 TB/s; 32 f16 tokens (5 heads) over 32 sequences
+// of up to 8192 8-bit tokens 95 us, 4.0 TB/s (equally long ones 4.75, 16 bits 5.5: there
+// decoding and its two parts are 1.7e7 vector instructions, a third of the time, with no unit
+// at its limit -- 12 waves a CU and 42 % of their time waiting); drafts of 5, 4, 3 and 2
+// tokens over 6001 to 2988 4-bit tokens 24.4 us; one token over 1000 11 us, two launches and
+// a few dependent loads.
 #pragma once
 
 #include "exl3_attn.hpp"
@@ -34,7 +46,8 @@ struct Few {
   static constexpr int kKeyWords = kVec * kRow / D / 4;
   static constexpr int kParts = PARTS;  // f16 that a coded value is made of (below)
   // Values go through LDS kSpan channels at a time: with two parts half a head, so that
-  // three workgroups still fit a CU (32 rows: the results at the end need as much).  16-byte loads: lanes per row, rows per load, loads.
+  // three workgroups still fit a CU (32 rows: the results at the end need as much).  Of their
+  // 16-byte loads: lanes per row, rows per load, loads.
   static constexpr int kSpans = PARTS == 1 || D == 64 || RT == 2 ? 1 : 2, kSpan = D / kSpans;
   static constexpr int kLanes = kRow / kSpans / 16, kRows = 64 / kLanes, kSpanLoads = 32 / kRows;
   static constexpr int kValueLoads = kSpans * kSpanLoads;

@@ -7,12 +7,26 @@
 //   S^T = K Q^T   32x32x16 MFMAs, K from LDS as the A operand, the wave's queries in
 //                 registers as the B operand.  Lane l holds scores of query l % 32 only, so
 //                 a row's maximum and sum stay in the lane (its other half in lane l ^ 32);
-//   P             as in the kernel for few rows: already the next product's B operand;
+//   P             rounded to 16 bits, already the next product's B operand, its sum f32 of the
+//                 unrounded ones, the maximum with kSlack, as in attn_few_kernel;
 //   O^T += V^T P^T  V read from LDS transposed.
 // The next tile's loads are in flight meanwhile, straight into the other half of LDS or,
 // coded ones, into registers and from there decoded behind the products: one barrier per
-// tile.  Two workgroups share a CU, so that
-// one's exponentials run beside the other's products.
+// tile.  Two workgroups share a CU (D = 64: three), so that one's exponentials run beside the
+// other's products.
+//
+// A coded value is one f16, code * scale rounded (2^-11 of it): two as in attn_few_kernel
+// would double the products, which bound this kernel.  With f16 queries over 8 bits the
+// result is off by 4e-4 to 6e-4 in the 2-norm so, where the output's own rounding is 2.1e-4;
+// the codes themselves are off by 4e-3.
+//
+// Measured (us, TFLOP/s of the products that the mask leaves): 2048 tokens over 16384 bf16
+// ones, 32 heads of 128 on 8: 506, 1020 -- a large product of the library's runs at 1238 --
+// with the matrix units busy half of the cycles and the exponentials beside them; 2048 over
+// 8192 921 TFLOP/s, 8 bits 788, 4 bits 799; heads of 64 701 / 625 / 521 (half the products per
+// exponential); of 256 627 / 493 / 494 (one workgroup a CU: its registers).  Six prompts of
+// 496 to 1500 tokens, heads of 64, window 512: 47 us, 425 TFLOP/s, masked tiles and two
+// rounds of short workgroups.
 #pragma once
 
 #include "exl3_attn.hpp"

@@ -416,7 +416,7 @@ class Exl3Attention:
             raise Exl3Error(-1, "attention block widths differ")
         self.q, self.k, self.v, self.o = q, k, v, o
         self.rope, self.scale, self.window = rope, scale, _window(window)
-        self._ws = _Workspace()
+        self._ws: dict = {}  # by stream
 
     def workspace_bytes(self, cache: KvCache, batch: KvBatch, rows: int, dtype) -> int:
         return int(load_library().exl3_attn_block_workspace_bytes(
@@ -426,8 +426,9 @@ class Exl3Attention:
     def forward(self, x, cache: KvCache, batch: KvBatch, workspace=None):
         """x [rows, in] (f16 or bf16) -> [rows, out] in the o projection's result dtype;
         the cache's pages get the rows' keys and values.  `workspace`: a zero-filled uint8
-        tensor of :meth:`workspace_bytes`; by default one that the block keeps, so that two
-        calls must not run concurrently (two captured graphs: give each its own)."""
+        tensor of :meth:`workspace_bytes`, of which two calls that run at once need one each;
+        by default one that the block keeps for the stream, and in a captured graph one of
+        the graph's."""
         torch = _torch()
         _floats()
         x = _device_tensor(x, "x", _HALVES, 2).contiguous()
@@ -442,7 +443,11 @@ class Exl3Attention:
         y = torch.empty(rows, self.o.out_features, device=device,
                         dtype=_code_dtype(lib.exl3_linear_output_dtype(self.o.handle, code)))
         if workspace is None:
-            workspace = self._ws.get(self.workspace_bytes(cache, batch, rows, x.dtype), device)
+            need = self.workspace_bytes(cache, batch, rows, x.dtype)
+            if torch.cuda.is_current_stream_capturing():  # a kept one could be replaced before a replay
+                workspace = torch.zeros(max(need, 256), dtype=torch.uint8, device=device)
+            else:
+                workspace = self._ws.setdefault((device, _stream_ptr(device)), _Workspace()).get(need, device)
         else:
             _plain(workspace, "workspace", (torch.uint8,), 1)
             _same(device, workspace, "workspace")

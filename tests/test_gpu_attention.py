@@ -720,6 +720,43 @@ def test_attention_block_in_graphs():
             assert torch.equal(s.cache.v, eager.cache.v)
 
 
+def test_attention_block_keeps_workspaces_apart():
+    """The block's own workspaces: calls on two streams at once, and a captured step whose
+    graph is replayed after an eager call that needed a larger one."""
+    hidden, heads, kv_heads, dim = 256, 4, 2, 64
+    block = mlxl3_amd.Exl3Attention(*projections(7, hidden, heads, kv_heads, dim, 4, 0, False))
+    gen = torch.Generator().manual_seed(12)
+    pool = Pool(80, [64, 64], kv_heads, dim, 16, 16, F16, poison=False, loud=1.0)
+
+    def side(rows):
+        b = kv_ref.batch(mlxl3_amd, [rows], [40 + rows - 1], pool.table[:1], max_kv=64)
+        return pool.cuda(mlxl3_amd), b, torch.randn(rows, hidden, generator=gen).half().cuda()
+
+    sides = [side(1), side(20)]
+    want = [block(x, c, b) for c, b, x in sides]  # a kept one grows from 1 row's to 20's
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(20):
+        for s, (c, b, x), w in zip(streams, sides, want):
+            with torch.cuda.stream(s):
+                outs.append((block(x, c, b), w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for y, w in outs)
+
+    c, b, x = sides[0]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = block(x, c, b)
+    for rows in (24, 30):
+        c2, b2, x2 = side(rows)
+        block(x2, c2, b2)
+        fill = torch.full((1 << 22,), 255, dtype=torch.uint8, device="cuda")  # takes what a replaced workspace left
+        y.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and bool((fill == 255).all())
+
+
 def test_attention_in_place():
     for new in ([1, 2], [40, 33]):
         pool = Pool(83, [900, 55], 2, 128, 16, 16, F16)
