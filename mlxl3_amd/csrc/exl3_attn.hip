@@ -120,10 +120,12 @@ template __global__ void attn_join_kernel<256>(AttnParams, int, int);
   template __global__ void attn_few_kernel<FMT, T, D, RT, PARTS>(AttnParams);
 EXL3_FEW(EXL3_FEW_INST)
 
-#define EXL3_MANY_D(M, FMT, T) M(FMT, T, 64) M(FMT, T, 128) M(FMT, T, 256)
-#define EXL3_MANY(M) \
-  EXL3_MANY_D(M, KV_F16, F16) EXL3_MANY_D(M, KV_BF16, BF16) EXL3_MANY_D(M, KV_Q8, F16) EXL3_MANY_D(M, KV_Q4, F16)
-#define EXL3_MANY_INST(FMT, T, D) template __global__ void attn_many_kernel<FMT, T, D>(AttnParams, int);
+#define EXL3_MANY_D(M, FMT, T, PARTS) M(FMT, T, 64, PARTS) M(FMT, T, 128, PARTS) M(FMT, T, 256, PARTS)
+#define EXL3_MANY(M)                                                                      \
+  EXL3_MANY_D(M, KV_F16, F16, 1) EXL3_MANY_D(M, KV_BF16, BF16, 1) EXL3_MANY_D(M, KV_Q8, F16, 1) \
+  EXL3_MANY_D(M, KV_Q8, F16, 2) EXL3_MANY_D(M, KV_Q4, F16, 1) EXL3_MANY_D(M, KV_Q4, F16, 2)
+#define EXL3_MANY_INST(FMT, T, D, PARTS) \
+  template __global__ void attn_many_kernel<FMT, T, D, PARTS>(AttnParams, int);
 EXL3_MANY(EXL3_MANY_INST)
 
 }  // namespace exl3
@@ -204,22 +206,20 @@ void launch_few(const AttnParams& p, int rows, hipStream_t s) {
   }
 }
 
-template <int FMT, typename T, int D>
+template <int FMT, typename T, int PARTS, int D>
 void launch_many(const AttnParams& p, int tiles, hipStream_t s) {
-  constexpr size_t lds = Many<FMT, T, D>::kLds;
+  constexpr size_t lds = Many<FMT, T, D, PARTS>::kLds;
   const dim3 grid((unsigned)tiles * p.splits * p.cache.kv_heads);
-  hipLaunchKernelGGL((attn_many_kernel<FMT, T, D>), grid, dim3(256), lds, s, p, tiles);
+  hipLaunchKernelGGL((attn_many_kernel<FMT, T, D, PARTS>), grid, dim3(256), lds, s, p, tiles);
 }
-template <int FMT, typename T>
+template <int FMT, typename T, int PARTS>
 void launch(const AttnParams& p, const Shape& sh, hipStream_t s) {
   const int d = p.cache.head_dim, tiles = (int)sh.tiles;
-  if (sh.few && FMT < 9 && p.q_type == DT_F16)
-    launch_few<FMT, T, FMT < 9 ? 2 : 1>(p, sh.rows, s);
-  else if (sh.few)
-    launch_few<FMT, T, 1>(p, sh.rows, s);
+  if (sh.few)
+    launch_few<FMT, T, PARTS>(p, sh.rows, s);
   else
-    d == 64 ? launch_many<FMT, T, 64>(p, tiles, s) : d == 128 ? launch_many<FMT, T, 128>(p, tiles, s)
-                                                              : launch_many<FMT, T, 256>(p, tiles, s);
+    d == 64 ? launch_many<FMT, T, PARTS, 64>(p, tiles, s) : d == 128 ? launch_many<FMT, T, PARTS, 128>(p, tiles, s)
+                                                                     : launch_many<FMT, T, PARTS, 256>(p, tiles, s);
 }
 
 }  // namespace
@@ -297,11 +297,12 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   const int D = p.cache.head_dim;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = launch_gate("attention")) return rc;
+  const bool fine = q_type == EXL3_F16;  // coded values in two parts
   switch (p.cache.format) {
-    case EXL3_KV_F16: launch<KV_F16, F16>(p, sh, s); break;
-    case EXL3_KV_BF16: launch<KV_BF16, BF16>(p, sh, s); break;
-    case EXL3_KV_Q8: launch<KV_Q8, F16>(p, sh, s); break;
-    default: launch<KV_Q4, F16>(p, sh, s);
+    case EXL3_KV_F16: launch<KV_F16, F16, 1>(p, sh, s); break;
+    case EXL3_KV_BF16: launch<KV_BF16, BF16, 1>(p, sh, s); break;
+    case EXL3_KV_Q8: fine ? launch<KV_Q8, F16, 2>(p, sh, s) : launch<KV_Q8, F16, 1>(p, sh, s); break;
+    default: fine ? launch<KV_Q4, F16, 2>(p, sh, s) : launch<KV_Q4, F16, 1>(p, sh, s);
   }
   if (int rc = check_launch("attention")) return rc;
   if (!sh.slots) return EXL3_OK;

@@ -54,20 +54,6 @@ struct Few {
   static constexpr int kPart = 32 * kSpan * 2;
   static constexpr int kWaveLds = kParts * kPart > 16 * RT * D * 4 ? kParts * kPart : 16 * RT * D * 4;
 
-  // code * scale needs up to 18 bits, an f16 has 11.  Rounded to those it is off by half as
-  // much as an f16 query or output is, and a large score by many times that: with f16
-  // queries a value is two f16 -- the scale's leading bits times the code, exact, and the
-  // rest (8 bits: to 2^-15) -- each with its own product.  bf16 queries' outputs are 8 times
-  // coarser, so one rounded f16 is enough there.  Same box, us: 32 decodes over 8192 8-bit
-  // tokens, f16, one part 86.4 (2-norm error 8.3e-4, 2.1e-4 of it the output's own
-  // rounding), two 94.5 (2.9e-4); four drafts of 5 over 6001 4-bit tokens, bf16, 24.3 (1.8e-3
-  // against 1.6e-3) and 27.6 (1.6e-3).
-  static __device__ __forceinline__ void scale_parts(uint32_t scale, _Float16& hi, _Float16& lo) {
-    const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)scale);
-    hi = PARTS == 1 ? s : __builtin_bit_cast(_Float16, (uint16_t)(scale & (FMT == KV_Q8 ? 0xff80u : 0xfff8u)));
-    lo = s - hi;
-  }
-
   // First channel of lane group g's operand in MFMA step s.
   static __device__ __forceinline__ int channel(int s, int g) {
     constexpr int n = kVec / 8;
@@ -131,7 +117,7 @@ struct Few {
       part[0] = __builtin_bit_cast(typename T::V8, r);
     } else {
       _Float16 hi, lo;
-      scale_parts(k.s[a][u], hi, lo);
+      scale_parts<FMT, PARTS>(k.s[a][u], hi, lo);
       u32x4 c;
       if constexpr (FMT == KV_Q8)
         c = codes8(k.w[a][u][2 * i], k.w[a][u][2 * i + 1]);
@@ -188,7 +174,7 @@ struct Few {
           *(u32x4*)(lds + at) = live ? v.w[u] : u32x4{0, 0, 0, 0};
         } else {
           _Float16 hi, lo;
-          scale_parts(v.s[u], hi, lo);
+          scale_parts<FMT, PARTS>(v.s[u], hi, lo);
           u32x4 c;
           if constexpr (FMT == KV_Q8) {
             const uint32_t w0 = v.w[u][2 * i], w1 = v.w[u][2 * i + 1];

@@ -15,16 +15,17 @@
 // tile.  Two workgroups share a CU (D = 64: three), so that one's exponentials run beside the
 // other's products.
 //
-// A coded value is one f16, code * scale rounded (2^-11 of it): two as in attn_few_kernel
-// would double the products, which bound this kernel.  With f16 queries over 8 bits the
-// result is off by 4e-4 to 6e-4 in the 2-norm so, where the output's own rounding is 2.1e-4;
-// the codes themselves are off by 4e-3.
+// Coded values are one or two f16 by the queries' type (scale_parts): two double the products,
+// in tiles half as long where the others' would leave one workgroup a CU.  With one, f16
+// results are off by 5.3e-4 to 8.1e-4 in the 2-norm, with two by 2.9e-4, where rounding the
+// exact ones takes 2.1e-4.
 //
 // Measured (us, TFLOP/s of the products that the mask leaves): 2048 tokens over 16384 bf16
 // ones, 32 heads of 128 on 8: 506, 1020 -- a large product of the library's runs at 1238 --
 // with the matrix units busy half of the cycles and the exponentials beside them; 2048 over
-// 8192 921 TFLOP/s, 8 bits 788, 4 bits 799; heads of 64 701 / 625 / 521 (half the products per
-// exponential); of 256 627 / 493 / 494 (one workgroup a CU: its registers).  Six prompts of
+// 8192 921 TFLOP/s, 8 bits 788 in one part and 463 in two, 4 bits 799 and 402; heads of 64 701,
+// 625 / 415, 521 / 357 (half the products per exponential); of 256 627, 493 / 349, 494 / 330
+// (one workgroup a CU: its registers).  Six prompts of
 // 496 to 1500 tokens, heads of 64, window 512: 47 us, 425 TFLOP/s, masked tiles and two
 // rounds of short workgroups.
 #pragma once
@@ -35,18 +36,19 @@ namespace exl3 {
 
 constexpr int kManyRows = 128;
 
-template <int FMT, typename T, int D>
+template <int FMT, typename T, int D, int PARTS>
 struct Many {
   static constexpr bool kRaw = FMT >= 9;
-  static constexpr int kTokens = D == 256 ? 32 : 64;                    // of a tile
+  static constexpr int kTokens = D * PARTS >= 256 ? 32 : 64;// of a tile
   static constexpr int kRow = kRaw ? 2 * D : FMT == KV_Q8 ? D : D / 2;  // bytes of a cached head
   static constexpr int kLanes = kRow / 16;                              // lanes that load a row
   static constexpr int kRows = 64 / kLanes;                             // rows of a wave's load
   static constexpr int kMine = kTokens / 4;                             // a wave's rows of a tile
   static constexpr int kLoads = kMine > kRows ? kMine / kRows : 1;
   static constexpr int kTile = kTokens * D * 2;                         // bytes in LDS
-  static constexpr int kLds = 4 * kTile;                                // keys and values, twice
-  static constexpr int kGroups = D == 64 ? 3 : 256 / D;                 // workgroups that share a CU
+  static constexpr int kHalf = 2 * PARTS * kTile;                       // keys' parts, values' parts
+  static constexpr int kLds = 2 * kHalf;
+  static constexpr int kGroups = D == 64 ? (PARTS == 2 ? 2 : 3) : 256 / D;                 // workgroups that share a CU
 
   struct Loads {  // of coded caches
     u32x4 k[kLoads], v[kLoads];
@@ -115,8 +117,8 @@ struct Many {
       x.vs[u] = (c.vs + s)[g];
     }
   }
-  static __device__ __forceinline__ u32x4 decoded(const u32x4& w, uint32_t scale, int i) {
-    const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)scale);
+  // Eight channels of a lane's load, times a scale.
+  static __device__ __forceinline__ u32x4 decoded(const u32x4& w, _Float16 s, int i) {
     if constexpr (FMT == KV_Q8) {
       const uint32_t a = w[2 * i], b = w[2 * i + 1];
       return decode8(a, b, s);
@@ -138,10 +140,15 @@ struct Many {
       if (edge && live) bad = bad || (x.vs[u] & 0x7c00) == 0x7c00;
 #pragma unroll
       for (int i = 0; i < n; ++i) {
-        *(u32x4*)(keys + key_place(t, ch * n + i)) = decoded(x.k[u], x.ks[u], i);
-        u32x4 v = decoded(x.v[u], x.vs[u], i);
-        if (!live) v = u32x4{0, 0, 0, 0};
-        *(u32x4*)(values + value_place(t, ch * n + i)) = v;
+        const int kat = key_place(t, ch * n + i), vat = value_place(t, ch * n + i);
+        _Float16 hi, lo;
+        scale_parts<FMT, PARTS>(x.ks[u], hi, lo);
+        *(u32x4*)(keys + kat) = decoded(x.k[u], hi, i);
+        if constexpr (PARTS == 2) *(u32x4*)(keys + kTile + kat) = decoded(x.k[u], lo, i);
+        scale_parts<FMT, PARTS>(x.vs[u], hi, lo);
+        const u32x4 none = {0, 0, 0, 0};
+        *(u32x4*)(values + vat) = live ? decoded(x.v[u], hi, i) : none;
+        if constexpr (PARTS == 2) *(u32x4*)(values + kTile + vat) = live ? decoded(x.v[u], lo, i) : none;
       }
     }
     return bad;
@@ -150,11 +157,11 @@ struct Many {
 
 // One-dimensional grid of tiles x splits x kv heads, the heads fastest (blocks go to the
 // XCDs in turn, so a head's tiles share few L2s), a sequence's last and longest tiles first.
-template <int FMT, typename T, int D>
+template <int FMT, typename T, int D, int PARTS>
 __global__ __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(Many<FMT, T, D>::kGroups, Many<FMT, T, D>::kGroups)))
+__attribute__((amdgpu_waves_per_eu(Many<FMT, T, D, PARTS>::kGroups, Many<FMT, T, D, PARTS>::kGroups)))
 void attn_many_kernel(AttnParams p, int tiles) {
-  typedef Many<FMT, T, D> F;
+  typedef Many<FMT, T, D, PARTS> F;
   typedef typename T::V8 V8;
   constexpr int TK = F::kTokens, NT = TK / 32;
   extern __shared__ __align__(16) uint8_t lds[];
@@ -205,23 +212,23 @@ void attn_many_kernel(AttnParams p, int tiles) {
   auto page_at = [&](int entry, int t) { return page_ok(p, entry, (t + off) & ~15, t1); };
   // starts the loads of the tile at t, and ends them in half `half` of LDS
   auto fetch = [&](int t, int page, int half) __attribute__((always_inline)) {
-    uint8_t* buf = lds + half * 2 * F::kTile;
+    uint8_t* buf = lds + half * F::kHalf;
     if constexpr (F::kRaw)
-      F::copy(p, kvh, page, t + off, off, lane, buf, buf + F::kTile);
+      F::copy(p, kvh, page, t + off, off, lane, buf, buf + PARTS * F::kTile);
     else
       F::load(p, kvh, page, t + off, lane, x);
   };
   auto stage = [&](int t, int page, int half) __attribute__((always_inline)) {
-    uint8_t* buf = lds + half * 2 * F::kTile;
+    uint8_t* buf = lds + half * F::kHalf;
     // an edge: some row of the workgroup does not see some token of the tile
     const bool edge = t < end.lo || t + TK > min(top.hi, t1) || page < 0;
     const int lo = top.lo - t, hi = page < 0 ? 0 : min(end.hi, t1) - t;
     bool bad = false;
     if constexpr (F::kRaw) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (edge) bad = F::clear(buf + F::kTile, off, lane, lo, hi);
+      if (edge) bad = F::clear(buf + PARTS * F::kTile, off, lane, lo, hi);
     } else {
-      bad = F::put(x, buf, buf + F::kTile, off, lane, edge, lo, hi);
+      bad = F::put(x, buf, buf + PARTS * F::kTile, off, lane, edge, lo, hi);
     }
     again = again || (bad && (top.lo < end.lo || top.hi < end.hi));
     if (lane == 0) page_on[half][wave] = page >= 0;
@@ -241,8 +248,8 @@ void attn_many_kernel(AttnParams p, int tiles) {
   int cur = 0;
   for (int t = t0; t < t1; t += TK, cur ^= 1) {
     __syncthreads();
-    const uint8_t* keys = lds + cur * 2 * F::kTile;
-    const uint8_t* values = keys + F::kTile;
+    const uint8_t* keys = lds + cur * F::kHalf;
+    const uint8_t* values = keys + PARTS * F::kTile;
     // always, so that no later wait has to count both ways (behind the end: the pool's first
     // page, and nobody uses it)
     page = page_at(next, t + TK);
@@ -250,10 +257,11 @@ void attn_many_kernel(AttnParams p, int tiles) {
     if (busy && t < wend.hi && t + TK > wtop.lo) {
       // The compiler orders these reads and products for few registers, each product right
       // behind its read; pin() keeps kDepth reads ahead of the products.
-      constexpr int QK = NT * (D / 16), kDepth = 4;
-      float16v s[NT];
+      constexpr int N = NT * PARTS, QK = N * (D / 16), kDepth = 4;
+      float16v s[N];  // of part c of block a: s[a + NT c]
       auto key = [&](int i) __attribute__((always_inline)) {
-        return *(const V8*)(keys + F::key_place(32 * (i % NT) + n, 2 * (i / NT) + h));
+        const int a = i % NT, c = i / NT % PARTS, st = i / N;
+        return *(const V8*)(keys + c * F::kTile + F::key_place(32 * a + n, 2 * st + h));
       };
       V8 kf[kDepth];
 #pragma unroll
@@ -262,23 +270,29 @@ void attn_many_kernel(AttnParams p, int tiles) {
 #pragma unroll
       for (int i = 0; i < QK; ++i) {
         pin();
-        const int a = i % NT, st = i / NT;
-        if (st == 0) s[a] = float16v{};
-        s[a] = T::mfma32(kf[i % kDepth], q[st], s[a]);
+        if (i < N) s[i] = float16v{};
+        s[i % N] = T::mfma32(kf[i % kDepth], q[i / N], s[i % N]);
         if (i + kDepth < QK) kf[i % kDepth] = key(i + kDepth);
       }
-      constexpr int KS = TK / 16, DT = D / 32;
-      auto value = [&](int ks, int dt) __attribute__((always_inline)) {
+      if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int a = 0; a < NT; ++a) s[a] += s[a + NT];
+      }
+      // product i of the second kind: 16 tokens, part of their values, 32 channels
+      constexpr int DT = D / 32, PV = TK / 16 * PARTS * DT;
+      auto value = [&](int i) __attribute__((always_inline)) {
+        const int ks = i / (PARTS * DT), c = i / DT % PARTS, dt = i % DT;
         const int tok = 16 * ks + 4 * h + ((lane >> 2) & 3);
         const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), half = (lane & 1) * 8;
-        const u32x2 lo = lds_transpose4(values + F::value_place(tok, chunk) + half);
-        const u32x2 hi = lds_transpose4(values + F::value_place(tok + 8, chunk) + half);
+        const uint8_t* from = values + c * F::kTile + half;
+        const u32x2 lo = lds_transpose4(from + F::value_place(tok, chunk));
+        const u32x2 hi = lds_transpose4(from + F::value_place(tok + 8, chunk));
         const u32x4 r = {lo[0], lo[1], hi[0], hi[1]};
         return __builtin_bit_cast(V8, r);
       };
       V8 vf[DT];
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) vf[dt] = value(0, dt);
+      for (int i = 0; i < DT; ++i) vf[i] = value(i);
       pin();
       __builtin_amdgcn_s_setprio(0);
       if (t < wend.lo || t + TK > min(wtop.hi, t1)) {
@@ -327,17 +341,15 @@ void attn_many_kernel(AttnParams p, int tiles) {
       for (int i = 0; i < 8; ++i) following[i] = weight(0, i);
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        w8 = following;
+      for (int i = 0; i < PV; ++i) {
+        const int ks = i / (PARTS * DT), dt = i % DT;
+        if (i % (PARTS * DT) == 0) w8 = following;
+        pin();
+        o[dt] = T::mfma32(vf[dt], w8, o[dt]);
+        if (i + DT < PV) vf[dt] = value(i + DT);
+        if (i % (PARTS * DT) < DT && ks + 1 < TK / 16) {  // beside it the next 16 tokens' weights
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          pin();
-          o[dt] = T::mfma32(vf[dt], w8, o[dt]);
-          if (ks + 1 < KS) {  // beside it the next 16 tokens' values and weights
-            vf[dt] = value(ks + 1, dt);
-#pragma unroll
-            for (int i = 0; i < 8 / DT; ++i) following[dt * (8 / DT) + i] = weight(ks + 1, dt * (8 / DT) + i);
-          }
+          for (int e = 0; e < 8 / DT; ++e) following[dt * (8 / DT) + e] = weight(ks + 1, dt * (8 / DT) + e);
         }
       }
       pin();

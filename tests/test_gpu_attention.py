@@ -266,6 +266,23 @@ def test_windows_and_no_causal_mask(bits, cdtype, dtype, causal, window, new, ol
     check(pool, new, q, y, causal, window)
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new, old", [([1, 2], [333, 40]), ([150, 60], [0, 500])])
+def test_f16_queries_see_codes_to_15_bits(bits, dim, new, old):
+    """The bound's terms for coded values (2^-11 each) shrink to 2^-15."""
+    lens = [n + o for n, o in zip(new, old)]
+    pool = Pool(72, lens, 2, dim, 16, bits, None)
+    q, _, _, y = run(pool, new, 8, F16, gain=3.0)
+    at = 0
+    for s, n in enumerate(new):
+        args = (q[at : at + n].double(), pool.values("k", s), pool.values("v", s), pool.lens[s] - n, dim**-0.5, True, 0)
+        want, exact = kv_ref.attend(*args, dtype=F16)
+        rounded = kv_ref.attend(*args, coded=True, dtype=F16)[1]
+        within(y[at : at + n], want, exact + (rounded - exact) / 16, f"sequence {s}")
+        at += n
+
+
 @pytest.mark.parametrize("new, old", [([1], [40000]), ([3, 1], [9000, 5]), ([64], [12000])])
 @pytest.mark.parametrize("bits, cdtype, dtype", [FORMATS[1], FORMATS[2], FORMATS[4]])
 def test_long_contexts(bits, cdtype, dtype, new, old):
