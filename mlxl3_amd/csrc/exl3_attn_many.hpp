@@ -12,8 +12,8 @@
 //   O^T += V^T P^T  V read from LDS transposed.
 // The next tile's loads are in flight meanwhile, straight into the other half of LDS or,
 // coded ones, into registers and from there decoded behind the products: one barrier per
-// tile.  Two workgroups share a CU (D = 64: three), so that one's exponentials run beside the
-// other's products.
+// tile.  Two workgroups share a CU (heads of 64: three), so that one's exponentials run beside
+// the other's products.
 //
 // Coded values are one or two f16 by the queries' type (scale_parts): two double the products,
 // in tiles half as long where the others' would leave one workgroup a CU.  With one, f16
@@ -25,9 +25,8 @@
 // with the matrix units busy half of the cycles and the exponentials beside them; 2048 over
 // 8192 921 TFLOP/s, 8 bits 788 in one part and 463 in two, 4 bits 799 and 402; heads of 64 701,
 // 625 / 415, 521 / 357 (half the products per exponential); of 256 627, 493 / 349, 494 / 330
-// (one workgroup a CU: its registers).  Six prompts of
-// 496 to 1500 tokens, heads of 64, window 512: 47 us, 425 TFLOP/s, masked tiles and two
-// rounds of short workgroups.
+// (one workgroup a CU: its registers).  Six prompts of 496 to 1500 tokens, heads of 64, window
+// 512: 47 us, 425 TFLOP/s, masked tiles and two rounds of short workgroups.
 #pragma once
 
 #include "exl3_attn.hpp"
@@ -39,7 +38,7 @@ constexpr int kManyRows = 128;
 template <int FMT, typename T, int D, int PARTS>
 struct Many {
   static constexpr bool kRaw = FMT >= 9;
-  static constexpr int kTokens = D * PARTS >= 256 ? 32 : 64;// of a tile
+  static constexpr int kTokens = D * PARTS >= 256 ? 32 : 64;            // of a tile
   static constexpr int kRow = kRaw ? 2 * D : FMT == KV_Q8 ? D : D / 2;  // bytes of a cached head
   static constexpr int kLanes = kRow / 16;                              // lanes that load a row
   static constexpr int kRows = 64 / kLanes;                             // rows of a wave's load
@@ -48,7 +47,7 @@ struct Many {
   static constexpr int kTile = kTokens * D * 2;                         // bytes in LDS
   static constexpr int kHalf = 2 * PARTS * kTile;                       // keys' parts, values' parts
   static constexpr int kLds = 2 * kHalf;
-  static constexpr int kGroups = D == 64 ? (PARTS == 2 ? 2 : 3) : 256 / D;                 // workgroups that share a CU
+  static constexpr int kGroups = D == 256 ? 1 : D == 64 && PARTS == 1 ? 3 : 2;  // workgroups that share a CU
 
   struct Loads {  // of coded caches
     u32x4 k[kLoads], v[kLoads];

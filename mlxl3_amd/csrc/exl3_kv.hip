@@ -17,10 +17,12 @@
 // NaN.  Everything is f32 with one rounding per operation, the quotient correctly
 // rounded, so the codes do not depend on how the work is laid out.
 //
-// Writing 4096 tokens of 8 heads of 128, keys rotated, to 8 bits takes 20 us (51 MB, 2.6 TB/s;
-// 16 bits 18 us, 3.7 TB/s): the memory, and one short-lived workgroup's chain of dependent
-// steps -- where its tokens belong, their turns, their page, the scale -- which four
-// workgroups a CU do not hide.  64 decoded tokens take 7.9, one 6.5: that chain.
+// Writing 4096 tokens of 8 heads of 128, keys rotated, takes 11 us (values in the caches) to
+// 12.5: to 16 bits 3.1 TB/s, to 8 bits 2.3.  What bounds it is one short-lived workgroup's
+// chain of dependent steps -- where its tokens belong, their turns, their page, the scale --
+// which four workgroups a CU do not hide, and a thousand vector instructions a wave beside it.
+// Written and read back, 4096 tokens take 19.3 us, 64 sequences' tokens 7.7, one token 6.3:
+// two launches with that chain each.
 // Reading 60059 tokens of two sequences back from 4 bits as f16 takes 56 us, 5.6 TB/s; the
 // writes alone (246 MB) take 37 in a plain fill.  Stores that bypass the caches take
 // 5 us off it and put as many on whoever reads the values next: not used.
@@ -215,14 +217,20 @@ __device__ __forceinline__ uint16_t group_scale(float most, float levels) {
   return f2h(fminf(most / levels, 65504.0f));
 }
 
-// rint(x / s) clipped to +-levels: the quotient from the rounded reciprocal and one
-// residual step, which rounds it correctly (s is an f16 value, so neither the reciprocal
-// nor the residual under- or overflows where the clip does not decide).
-__device__ __forceinline__ int group_code(float x, float s, float inv, float levels) {
+// rint(x / s) clipped to +-levels, plus levels + 1, in the low byte: the quotient from the
+// rounded reciprocal and one residual step, which rounds it correctly (s is an f16 value, so
+// neither the reciprocal nor the residual under- or overflows where the clip does not
+// decide); a sum of that size rounds to whole numbers, ties to even.
+__device__ __forceinline__ uint32_t group_code(float x, float s, float inv, float levels) {
   float q = x * inv;
   q = fmaf(fmaf(-q, s, x), inv, q);
-  q = fabsf(q) <= levels ? q : copysignf(levels, x);
-  return (int)rintf(q);
+  q = __builtin_amdgcn_fmed3f(q, -levels, levels) + (12582912.0f + levels + 1.0f);
+  return __builtin_bit_cast(uint32_t, q);
+}
+// Four low bytes as one word.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+  return lo | hi;
 }
 
 struct AppendParams {
@@ -359,19 +367,19 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
         const float s = h2f(sh);
         const bool on = s > 0.0f;
         const float inv = on ? 1.0f / s : 0.0f;
-        int code[8];
+        uint32_t code[8];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) code[n] = on ? group_code(v[n], s, inv, levels) : 0;
+        for (int n = 0; n < 8; ++n) code[n] = group_code(v[n], s, inv, levels);
         if constexpr (FMT == KV_Q8) {
-          u32x2 o = {0, 0};
-#pragma unroll
-          for (int n = 0; n < 8; ++n) o[n / 4] |= (uint32_t)(code[n] + 128) << (8 * (n & 3));
+          const uint32_t zero = 0x80808080u;
+          const u32x2 o = {on ? low_bytes(code[0], code[1], code[2], code[3]) : zero,
+                           on ? low_bytes(code[4], code[5], code[6], code[7]) : zero};
           *(u32x2*)(base + token * D + w.d0) = o;
         } else {
-          uint32_t o = 0;
-#pragma unroll
-          for (int n = 0; n < 8; ++n) o |= (uint32_t)(code[n] + 8) << (4 * n);
-          *(uint32_t*)(base + (token * D + w.d0) / 2) = o;
+          // a byte each: the even channel's nibble, and the odd one's above it
+          const uint32_t even = low_bytes(code[0], code[2], code[4], code[6]) & 0x0f0f0f0fu;
+          const uint32_t odd = low_bytes(code[1], code[3], code[5], code[7]) & 0x0f0f0f0fu;
+          *(uint32_t*)(base + (token * D + w.d0) / 2) = on ? even | odd << 4 : 0x88888888u;
         }
         if ((w.d0 & 31) == 0) {
           uint16_t* sc = w.value ? c.vs : c.ks;
@@ -561,8 +569,8 @@ static int check_rope(const exl3_rope_spec* rope, int head_dim, RopeView* view) 
 }
 
 // Heads per workgroup of an append or a read: a batch of loads each while that leaves
-// four workgroups per CU.  Appending 4096 tokens of 8 heads to 8 bits: 4 heads each 20.2 us;
-// 2 heads 22.8 and 1 head 30.1 (the turns are computed for each), 8 heads 22.2.
+// four workgroups per CU.  4096 tokens of 8 heads, 8 bits, written and read back: 4 heads each
+// 20.2 us; 2 heads 22.8 and 1 head 30.1 (the turns are computed for each), 8 heads 22.2.
 static int head_parts(int64_t tokens, const KvCacheView& c, dim3* grid, int* heads, int* parts) {
   const int64_t n = (tokens + 2048 / c.head_dim - 1) / (2048 / c.head_dim);
   if (n > kMostBlocks) return fail(EXL3_EUNSUPPORTED, "too many tokens: %lld", (long long)tokens);
