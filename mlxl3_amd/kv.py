@@ -255,6 +255,8 @@ class Rope:
         if batch is not None:
             _same(device, batch.kv_lens, "batch")
         _same(device, self.inv_freq, "inv_freq")
+        if n == 0 and (where is not None) != (batch is not None):
+            return out  # no tokens: an empty tensor's address is null
         _launch(device, load_library().exl3_rope, self._ref, src.data_ptr(), _FLOATS[src.dtype], n, heads, dim,
                 src.stride(0), where, None if batch is None else batch._ref, out.data_ptr(), _FLOATS[out.dtype],
                 out.stride(0))

@@ -581,6 +581,52 @@ def test_same_call_same_bits_and_longer_bounds_of_the_launch():
             check(pool, new, q, mlxl3_amd.attention(q.cuda(), cache, b2))
 
 
+def test_no_tokens():
+    pool = Pool(73, [20], 2, 64, 16, 8, None)
+    cache = pool.cuda(mlxl3_amd)
+    b = kv_ref.batch(mlxl3_amd, [0], [20], pool.table)
+    rope = mlxl3_amd.Rope(mlxl3_amd.rope_frequencies(64)[0].cuda())
+    none = torch.empty(0, 2, 64, dtype=F16, device="cuda")
+    before = cache.k.clone()
+    cache.append(b, none, none, rope=rope)
+    assert torch.equal(cache.k, before)
+    assert [t.shape[0] for t in cache.read(b, 0)] == [0, 0]
+    assert rope.apply(none, batch=b).shape == none.shape
+    assert rope.apply(none, torch.empty(0, dtype=torch.int32, device="cuda")).shape == none.shape
+    assert mlxl3_amd.attention(none, cache, b).shape == none.shape
+    with pytest.raises(mlxl3_amd.Exl3Error, match="from an array or from a KV batch"):
+        rope.apply(none)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_graph_told_long_lengths_follows_short_ones(new):
+    """Captured once with bounds of 100000 tokens, replayed for lengths that change between
+    the replays, eager work beside it; every replay against the eager call."""
+    lens = [3000, 90, 700]
+    pool = Pool(74, lens, 8, 64, 64, 16, F16, table_pages=1600, poison=False)
+    cache = pool.cuda(mlxl3_amd)
+    b = kv_ref.batch(mlxl3_amd, [new] * 3, lens, pool.table)
+    q = torch.randn(3 * new, 16, 64, generator=torch.Generator().manual_seed(75)).half().cuda()
+    mlxl3_amd.attention(q, cache, b)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = mlxl3_amd.attention(q, cache, b)
+    for now in ([3000, 90, 700], [2999, 40, 641], [1500, 60, 40], [40, 40, 699], [2048, 64, 128]):
+        b.kv_lens.copy_(torch.tensor(now, dtype=torch.int32))
+        want = mlxl3_amd.attention(q, cache, b)
+        y.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), now
+        at = 0
+        for s, length in enumerate(now):
+            w, bound = kv_ref.attend(q[at : at + new].cpu().double(), pool.values("k", s)[:length], pool.values("v", s)[:length],
+                                     length - new, 64**-0.5, True, 0, dtype=F16)
+            within(y[at : at + new], w, bound, f"{now} sequence {s}")
+            at += new
+
+
 def test_other_streams():
     pool = Pool(61, [2000], 2, 128, 16, 16, BF16)
     q, cache, b, y = run(pool, [1], 8, BF16)
