@@ -246,10 +246,8 @@ def scores_result_dtype(scores_dtype):
 def _stream_ptr(device) -> int:
     torch = _torch()
     # the handle alone: torch.cuda.current_stream makes an object around it, 2 us a call
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if raw is not None and device.index is not None:
-        return raw(device.index)
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return torch.cuda.current_stream(device).cuda_stream if index is None else torch._C._cuda_getCurrentRawStream(index)
 
 
 def _ptr(t) -> Optional[int]:
