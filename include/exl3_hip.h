@@ -299,7 +299,8 @@ void exl3_kv_cache_destroy(exl3_kv_cache* handle);
  * position t lies in page block_table[b][t / page_tokens].  The arrays are
  * device memory that the host does not read, so a captured graph can be
  * replayed for other lengths.  What they say is checked on the device: rows
- * outside every sequence are left as they were; a token whose position or page
+ * outside every sequence are left as they were, rows that the call's tensors do
+ * not have are not touched; a token whose position or page
  * lies outside the table or the pool is not written, reads as zeros and is
  * not attended to.  max_q and max_kv bound the new tokens of a sequence and
  * its length (max_kv <= 0: the table's room): rows past max_q are left as they
