@@ -286,7 +286,7 @@ typedef enum {
  * (4 bits: / 7; at most 65504), code = x / scale rounded to nearest even and
  * clipped to +-127 (+-7).  A group that holds a NaN or an infinity reads back
  * as NaN.  exl3_attention forms stored values in f16: beyond 65504 they need
- * not stay finite there. */
+ * not stay finite there, for the rows that see them. */
 typedef struct exl3_kv_cache exl3_kv_cache;
 int exl3_kv_cache_create(void* k, void* v, uint16_t* k_scales, uint16_t* v_scales,
                          int32_t format, int64_t pages, int32_t page_tokens, int32_t kv_heads,

@@ -76,6 +76,14 @@ __device__ __forceinline__ bool not_finite(const u32x4& v) {
   return bad;
 }
 
+// Whether a coded group may hold a value that is no finite f16: its scale's magnitude against the
+// least one that a code takes past 65504 -- 512 = 65536 / 128 for 8 bits, 8192 = 65536 / 8 for
+// 4 -- NaN and infinity lie above both.
+template <int FMT>
+__device__ __forceinline__ bool past_f16(uint32_t scale) {
+  return (scale & 0x7fff) >= (FMT == KV_Q8 ? 0x6000u : 0x7000u);
+}
+
 // Where channel e of eight lies in codes4's order, and which channel lies at place e.
 __device__ __forceinline__ constexpr int place4(int e) { return e < 4 ? 2 * e : 2 * e - 7; }
 __device__ __forceinline__ constexpr int channel4(int e) { return (e >> 1) | ((e & 1) << 2); }

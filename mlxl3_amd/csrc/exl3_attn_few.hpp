@@ -155,7 +155,7 @@ struct Few {
   }
   // A span's values to LDS as 16-bit rows (4 bits: channels in codes4's order); rows outside
   // [live_lo, live_hi) or of a block without a page become zeros.  Returns whether an
-  // edge's other rows hold a value that is not finite.
+  // edge's other rows may hold a value that is not finite.
   template <bool EDGE>
   static __device__ __forceinline__ bool put_values(const Values& v, int span, uint8_t* lds, int lane, int live_lo,
                                                     int live_hi, bool on0, bool on1) {
@@ -165,7 +165,7 @@ struct Few {
     for (int u0 = 0; u0 < kSpanLoads; ++u0) {
       const int u = span * kSpanLoads + u0, t = u0 * kRows + r;
       const bool live = !EDGE || (t >= live_lo && t < live_hi && (t < 16 ? on0 : on1));
-      if (EDGE && live) bad = bad || (kRaw ? not_finite<T>(v.w[u]) : (v.s[kRaw ? 0 : u] & 0x7c00) == 0x7c00);
+      if (EDGE && live) bad = bad || (kRaw ? not_finite<T>(v.w[u]) : past_f16<FMT>(v.s[kRaw ? 0 : u]));
       constexpr int n = kRaw ? 1 : FMT == KV_Q8 ? 2 : 4;  // 16-byte chunks of the decoded row
 #pragma unroll
       for (int i = 0; i < n; ++i) {

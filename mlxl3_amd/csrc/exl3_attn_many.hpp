@@ -136,7 +136,7 @@ struct Many {
       const int t = first + row_of(u, lane);
       if (kRows > kMine && row_of(u, lane) >= kMine) continue;
       const bool live = !edge || (t >= lo && t < hi);
-      if (edge && live) bad = bad || (x.vs[u] & 0x7c00) == 0x7c00;
+      if (edge && live) bad = bad || past_f16<FMT>(x.vs[u]);
 #pragma unroll
       for (int i = 0; i < n; ++i) {
         const int kat = key_place(t, ch * n + i), vat = value_place(t, ch * n + i);

@@ -1,0 +1,70 @@
+"""Attention where 16 bits end: coded values beyond f16's range, values that a row does not see
+over coded caches.  Against the 64-bit forms of kv_ref.py."""
+
+import math
+
+import pytest
+import torch
+
+import kv_ref
+from kv_ref import Pool
+from test_gpu_attention import BF16, F16, check, run, within
+
+pytestmark = pytest.mark.gpu
+
+CODED = [(8, F16), (8, BF16), (4, F16), (4, BF16)]
+
+
+def put_value(pool, seq, t, value):
+    """Token t's values in every head: `value` in channel 7 (and its group's scale with it)."""
+    row = torch.zeros(pool.kv_heads, pool.dim)
+    row[:, 7] = value
+    c, s = kv_ref.quantise(row, pool.bits)
+    at = int(pool.table[seq, t // pool.page]), slice(None), t % pool.page
+    pool.v[at] = kv_ref.pack(c, pool.bits)
+    pool.vs.transpose(2, 3)[at] = s
+    return s[:, 0].float()
+
+
+@pytest.mark.parametrize("bits, dtype", CODED)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("value", [math.nan, math.inf, 6.0e4, 6.7e4, -1.0e5, 5.0e5, -8.0e6])
+@pytest.mark.parametrize("new", [[1, 3], [40, 33]])
+def test_coded_values_that_a_row_does_not_see_do_not_reach_it(bits, dtype, dim, value, new):
+    """Groups that are not finite and groups whose largest values f16 does not hold, behind a
+    row's position or before its window.  The rows that do not see them are as exact as with
+    zeros there."""
+    window = 8
+    lens = [new[0] + 100, new[1] + 20]
+    pool = Pool(44, lens, 2, dim, 16, bits, None)
+    for s in range(2):
+        for t in (lens[s] - new[s] - window + 1, lens[s] - 1):  # in the first row's window alone; the newest token
+            put_value(pool, s, t, value)
+    q, _, _, y = run(pool, new, 4, dtype, window=window)
+    at = 0
+    for s, n in enumerate(new):
+        args = q[at : at + n].double(), pool.values("k", s), pool.values("v", s)
+        old = lens[s] - n
+        for i in range(n):
+            sees = [t for t in (old - window + 1, lens[s] - 1) if old + i - window < t <= old + i]
+            if not sees:
+                lo, hi = old + i - window + 1, old + i + 1
+                want, bound = kv_ref.attend(args[0][i : i + 1], args[1][lo:hi], args[2][lo:hi], 0, dim**-0.5, False, 0,
+                                            coded=True, dtype=dtype)
+                within(y[at + i : at + i + 1], want, bound, f"sequence {s} row {i}")
+            elif not math.isfinite(value):
+                assert bool(y[at + i, :, :32].isnan().any()), f"sequence {s} row {i} sees it"
+        at += n
+
+
+@pytest.mark.parametrize("bits, dtype", CODED)
+@pytest.mark.parametrize("new", [[2], [40]])
+def test_the_largest_values_that_f16_holds_are_attended_to(bits, dtype, new):
+    """Groups just below the border, seen by some rows: every row within the bound."""
+    levels = kv_ref.LEVELS[bits]
+    pool = Pool(45, [new[0] + 30], 2, 128, 16, bits, None)
+    scales = put_value(pool, 0, pool.lens[0] - 1, 6.4e4)
+    assert bool((scales * levels < 65504).all())
+    q, _, _, y = run(pool, new, 4, dtype)
+    assert bool(y[:-1].isfinite().all())
+    check(pool, new, q, y)
