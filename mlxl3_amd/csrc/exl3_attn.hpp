@@ -272,6 +272,16 @@ __device__ __forceinline__ int range_count(int each, int n) {
 // So most steps rescale nothing and exchange nothing between lanes.
 constexpr float kSlack = 8.0f;
 
+// Weights are exp2(fma(score, scale2, -m)), m the rounded product for some score: the others'
+// unrounded ones pass it by up to half a step of m, nothing until m is large, and at 2^27 a
+// factor of 2^8, at 2^34 of 2^512.  Once a maximum of a wave is beyond this, products are
+// rounded before m is taken off, exactly: none passes the largest.  (Then every step goes the
+// way of a moving maximum, so that others have no further branch.)
+constexpr float kFar = 65536.0f;
+__device__ __forceinline__ bool is_far(float m) {
+  return fabsf(m) > kFar && m != -__builtin_inff();
+}
+
 // One row over the tokens [lo, hi) by one wave, its channels spread over the lanes (lane
 // l holds channels E l ..): running maximum m, sum l and weighted values acc.  Touches
 // only tokens that the row sees.

@@ -252,15 +252,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     for (int s = 0; s < F::kSteps; ++s) q[rt][s] = load_q8<FMT, T>(p, qi + F::channel(s, g));
   }
   float4v o[RT][D / 16];
-  float m[RT], l[RT];
+  float m[RT], l[RT], less[RT];  // less: what weights are taken against, -m or 0
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -__builtin_inff();
-    l[rt] = 0.0f;
+    l[rt] = less[rt] = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = float4v{0, 0, 0, 0};
   }
   bool again = false;
+  float slack = kSlack, unit = p.scale2;  // of the wave; far (kFar): slack < 0, unit 1
 
   typename F::Keys k;
   typename F::Values v;
@@ -333,20 +334,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         most = fmaxf(most, x[i]);
       }
       most *= p.scale2;
-      if (__any(most > m[rt] + kSlack)) {
+      if (__any(most - m[rt] > slack)) {
         most = fmaxf(most, xor_lanes<16>(most));
         most = fmaxf(most, xor_lanes<32>(most));
         const float up = fmaxf(m[rt], most);
         const float f = up == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - up);
         m[rt] = up;
+        less[rt] = up == -__builtin_inff() ? 0.0f : -up;
         l[rt] *= f;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
+        if (__any(is_far(up))) slack = -__builtin_inff();
+        if (slack < 0.0f) {
+          unit = 1.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= p.scale2;
+        }
       }
-      const float base = m[rt] == -__builtin_inff() ? 0.0f : m[rt];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], p.scale2, -base));
+        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], unit, less[rt]));
         l[rt] += x[i];
         w8[rt][i] = (typename T::E)x[i];
       }

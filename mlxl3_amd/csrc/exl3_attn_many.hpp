@@ -202,8 +202,9 @@ void attn_many_kernel(AttnParams p, int tiles) {
   float16v o[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
-  float m = -__builtin_inff(), l = 0.0f;
+  float m = -__builtin_inff(), l = 0.0f, less = 0.0f;  // less: what weights are taken against, -m or 0
   bool again = false;
+  float slack = kSlack, unit = p.scale2;  // of the wave; far (kFar): slack < 0, unit 1
 
   typename F::Loads x;
   const int off = F::kMine * wave;  // of this wave's rows in a tile
@@ -320,19 +321,27 @@ void attn_many_kernel(AttnParams p, int tiles) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, s[a][i]);
       most *= p.scale2;
-      if (__any(most > m + kSlack)) {
+      if (__any(most - m > slack)) {
         most = fmaxf(most, xor_lanes<32>(most));
         const float up = fmaxf(m, most);
         const float f = up == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - up);
         m = up;
+        less = up == -__builtin_inff() ? 0.0f : -up;
         l *= f;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) o[dt] *= f;
+        if (__any(is_far(up))) slack = -__builtin_inff();
+        if (slack < 0.0f) {
+          unit = 1.0f;
+#pragma unroll
+          for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[a][i] *= p.scale2;
+        }
       }
-      const float base = m == -__builtin_inff() ? 0.0f : m;
       V8 w8, following;
       auto weight = [&](int ks, int i) __attribute__((always_inline)) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[ks / 2][8 * (ks & 1) + i], p.scale2, -base));
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[ks / 2][8 * (ks & 1) + i], unit, less));
         l += e;
         return (typename T::E)e;
       };

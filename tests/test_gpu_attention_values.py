@@ -1,5 +1,5 @@
-"""Attention where 16 bits end: coded values beyond f16's range, values that a row does not see
-over coded caches.  Against the 64-bit forms of kv_ref.py."""
+"""Attention where 16 and 32 bits end: coded values beyond f16's range, values that a row does not
+see over coded caches, scores of any size.  Against the 64-bit forms of kv_ref.py."""
 
 import math
 
@@ -9,6 +9,8 @@ import torch
 import kv_ref
 from kv_ref import Pool
 from test_gpu_attention import BF16, F16, check, run, within
+
+import mlxl3_amd
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +70,44 @@ def test_the_largest_values_that_f16_holds_are_attended_to(bits, dtype, new):
     q, _, _, y = run(pool, new, 4, dtype)
     assert bool(y[:-1].isfinite().all())
     check(pool, new, q, y)
+
+
+def set_keys(pool, seq, x):
+    """A sequence's keys: x [tokens] times ones, in every head."""
+    for t in range(pool.lens[seq]):
+        row = x[t].expand(pool.kv_heads, pool.dim)
+        at = int(pool.table[seq, t // pool.page]), slice(None), t % pool.page
+        if pool.bits == 16:
+            pool.k[at] = row.to(pool.dtype)
+        else:
+            c, s = kv_ref.quantise(row, pool.bits)
+            pool.k[at] = kv_ref.pack(c, pool.bits)
+            pool.ks.transpose(2, 3)[at] = s
+
+
+ALL = [(16, F16, F16), (16, BF16, BF16)] + [(b, None, t) for b, t in CODED]
+
+
+@pytest.mark.parametrize("bits, cdtype, dtype", ALL)
+@pytest.mark.parametrize("size", [1.0e3, 8.0e3, 3.0e4])
+@pytest.mark.parametrize("new, old", [([2], [100]), ([40], [90]), ([3], [2500]), ([70], [2600])])
+def test_scores_so_large_that_f32_does_not_resolve_their_neighbours(bits, cdtype, dtype, size, new, old):
+    """Scores up to 2^34 (in powers of two), where a rounding is worth 2^10: the tokens of the
+    largest score share the whole weight.  Keys of nine levels 9 % apart, so that no
+    rounding joins two of them; queries of both signs."""
+    lens = [new[0] + old[0]]
+    pool = Pool(46, lens, 1, 128, 16, bits, cdtype)
+    set_keys(pool, 0, size * (0.2 + 0.09 * (torch.arange(lens[0]) * 7 % 9).float()))
+    q = torch.full((new[0], 4, 128), size)
+    q[:, 1::2] *= -1
+    q = q.to(dtype)
+    b = kv_ref.batch(mlxl3_amd, new, lens, pool.table)
+    y = mlxl3_amd.attention(q.cuda(), pool.cuda(mlxl3_amd), b)
+    k, v = pool.values("k", 0), pool.values("v", 0)
+    want, _ = kv_ref.attend(q.double(), k, v, old[0], 128**-0.5, True, 0, coded=bits != 16, dtype=dtype)
+    mean, _ = kv_ref.attend(q.double(), k, v.abs(), old[0], 128**-0.5, True, 0, coded=bits != 16, dtype=dtype)
+    # equal scores are equal bit for bit, so no error of theirs moves the shares: of attend's terms
+    # those of the weights (half a step of 16 bits), coded values, sums and the result are left
+    half = kv_ref.EPS[dtype] / 2
+    rounded = half + (2.0**-11 if bits != 16 else 0.0) + 64 * 2.0**-24
+    within(y, want, half * want.abs() + mean * rounded + 2.0**-24, "huge")
