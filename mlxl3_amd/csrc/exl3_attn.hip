@@ -3,7 +3,7 @@
 //   y_row = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q_row . k_t - m),
 //
 // over the tokens t that the row sees: t < kv_len, causal t <= its position, window
-// t > its position - window.  m is the largest score so far, or at most kSlack below: one pass
+// t > its position - window.  m lies near the largest score so far (kSlack, kRoom): one pass
 // over the cache with a running maximum and sum, both f32.  A row that sees nothing gives zeros.
 //
 // The rows of a launch are (token, query head of a group) pairs: all heads that read one

@@ -30,6 +30,7 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 struct F16 {
   typedef half8 V8;
   typedef _Float16 E;
+  static constexpr float kRoom = 7.0f;  // below
   static __device__ __forceinline__ float4v mfma16(V8 a, V8 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -41,6 +42,7 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 struct BF16 {
   typedef bf8 V8;
   typedef __bf16 E;
+  static constexpr float kRoom = 0.0f;
   static __device__ __forceinline__ float4v mfma16(V8 a, V8 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -267,13 +269,17 @@ __device__ __forceinline__ int range_count(int each, int n) {
   return (int)(((uint32_t)n + size - 1) / size);
 }
 
-// A score above the running maximum by no more than this (in factors of two) does not
-// move it: weights stay below 256 and far inside 16 bits' range, their sums inside f32's.
-// So most steps rescale nothing and exchange nothing between lanes.
+// Weights are taken against m, at first the largest score less T::kRoom (in factors of two).  A
+// score above it by no more than T::kRoom and this does not move m: so most steps rescale
+// nothing and exchange nothing between lanes.  The largest weight is then one of 2^kRoom to
+// 2^(kRoom + kSlack): 256 for bf16, 2^15 for f16, and their sums stay far inside f32's range.
+// f16 needs the room below: what it cannot hold, weights under 2^-25, is 2^-32 of the largest
+// then and was 2^-25 of it without, so that thousands of tokens 15 to 17 nats below one whose
+// values are small lost 6 to 100 % of their part.
 constexpr float kSlack = 8.0f;
 
-// Weights are exp2(fma(score, scale2, -m)), m the rounded product for some score: the others'
-// unrounded ones pass it by up to half a step of m, nothing until m is large, and at 2^27 a
+// They are exp2(fma(score, scale2, -m)), m from the rounded product for some score: the others'
+// unrounded ones pass that by up to half a step of it, nothing until m is large, and at 2^27 a
 // factor of 2^8, at 2^34 of 2^512.  Once a maximum of a wave is beyond this, products are
 // rounded before m is taken off, exactly: none passes the largest.  (Then every step goes the
 // way of a moving maximum, so that others have no further branch.)

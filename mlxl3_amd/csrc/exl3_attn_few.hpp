@@ -12,8 +12,8 @@
 //   O^T += V^T P^T  with V^T read from LDS transposed (four tokens of a channel a read),
 //                 in the token order that P has.  V goes through the wave's own LDS, so
 //                 there is no barrier in the loop.
-// m moves only when some score passes it by kSlack (a factor of 256: P and its sums stay
-// far inside 16 bits' and f32's range), so a step usually has no exchange between lanes
+// m moves only when some score passes it by kSlack and the type's room (P and its sums stay
+// inside 16 bits' and f32's range), so a step usually has no exchange between lanes
 // at all; the sum l is kept per lane and reduced once at the end.
 // The waves' results meet in LDS; with more than one range per sequence they are joined
 // by attn_join_kernel.
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = float4v{0, 0, 0, 0};
   }
   bool again = false;
-  float slack = kSlack, unit = p.scale2;  // of the wave; far (kFar): slack < 0, unit 1
+  float slack = kSlack + T::kRoom, unit = p.scale2;  // of the wave; far (kFar): slack < 0, unit 1
 
   typename F::Keys k;
   typename F::Values v;
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
       if (__any(most - m[rt] > slack)) {
         most = fmaxf(most, xor_lanes<16>(most));
         most = fmaxf(most, xor_lanes<32>(most));
-        const float up = fmaxf(m[rt], most);
+        const float up = fmaxf(m[rt], most - T::kRoom);
         const float f = up == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - up);
         m[rt] = up;
         less[rt] = up == -__builtin_inff() ? 0.0f : -up;

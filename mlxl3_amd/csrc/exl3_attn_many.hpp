@@ -204,7 +204,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
   float m = -__builtin_inff(), l = 0.0f, less = 0.0f;  // less: what weights are taken against, -m or 0
   bool again = false;
-  float slack = kSlack, unit = p.scale2;  // of the wave; far (kFar): slack < 0, unit 1
+  float slack = kSlack + T::kRoom, unit = p.scale2;  // of the wave; far (kFar): slack < 0, unit 1
 
   typename F::Loads x;
   const int off = F::kMine * wave;  // of this wave's rows in a tile
@@ -323,7 +323,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
       most *= p.scale2;
       if (__any(most - m > slack)) {
         most = fmaxf(most, xor_lanes<32>(most));
-        const float up = fmaxf(m, most);
+        const float up = fmaxf(m, most - T::kRoom);
         const float f = up == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - up);
         m = up;
         less = up == -__builtin_inff() ? 0.0f : -up;

@@ -1,5 +1,6 @@
 """Attention where 16 and 32 bits end: coded values beyond f16's range, values that a row does not
-see over coded caches, scores of any size.  Against the 64-bit forms of kv_ref.py."""
+see over coded caches, scores of any size, weights far below the largest.  Against the 64-bit
+forms of kv_ref.py."""
 
 import math
 
@@ -111,3 +112,38 @@ def test_scores_so_large_that_f32_does_not_resolve_their_neighbours(bits, cdtype
     half = kv_ref.EPS[dtype] / 2
     rounded = half + (2.0**-11 if bits != 16 else 0.0) + 64 * 2.0**-24
     within(y, want, half * want.abs() + mean * rounded + 2.0**-24, "huge")
+
+
+@pytest.mark.parametrize("bits, cdtype, dtype", ALL)
+@pytest.mark.parametrize("nats", [12.0, 15.0, 16.0, 17.4])
+@pytest.mark.parametrize("new, old", [([1], [4000]), ([2], [4000]), ([40], [4000]), ([300], [3700])])
+def test_a_long_tail_far_below_one_token(bits, cdtype, dtype, nats, new, old):
+    """One key `nats` above thousands of equal ones, with values of zero: the small weights are
+    all of the result.  An f16 weight below the normal range is off by up to 2^-25, against a
+    largest one of 2^7 or more: 2^-32 of it, not the 2^-25 of weights up to 1."""
+    lens = [new[0] + old[0]]
+    pool = Pool(47, lens, 1, 128, 64, bits, cdtype)
+    x = torch.zeros(lens[0])
+    x[0] = nats / 128**0.5
+    set_keys(pool, 0, x)
+    g = torch.Generator().manual_seed(48)
+    for t in range(lens[0]):
+        row = torch.rand(1, 128, generator=g) + 0.5 if t else torch.zeros(1, 128)
+        at = int(pool.table[0, t // 64]), slice(None), t % 64
+        if bits == 16:
+            pool.v[at] = row.to(cdtype)
+        else:
+            c, s = kv_ref.quantise(row, bits)
+            pool.v[at] = kv_ref.pack(c, bits)
+            pool.vs.transpose(2, 3)[at] = s
+    q = torch.ones(new[0], 4, 128).to(dtype)
+    b = kv_ref.batch(mlxl3_amd, new, lens, pool.table)
+    y = mlxl3_amd.attention(q.cuda(), pool.cuda(mlxl3_amd), b)
+    k, v = pool.values("k", 0), pool.values("v", 0)
+    want, bound = kv_ref.attend(q.double(), k, v, old[0], 128**-0.5, True, 0, coded=bits != 16, dtype=dtype)
+    if bits != 16 or dtype == F16:
+        for i in range(new[0]):
+            seen = slice(0, old[0] + i + 1)
+            s = (k[seen, 0] @ q[i, 0].double()) * 128**-0.5
+            bound[i] -= 2.0**-25 * (1 - 2.0**-7) * v[seen, 0].abs().sum(0) / torch.exp(s - s.max()).sum()
+    within(y, want, bound, f"tail {nats} nats below")
