@@ -105,31 +105,50 @@ __device__ __forceinline__ void scale_parts(uint32_t scale, _Float16& hi, _Float
   lo = s - hi;
 }
 
-// f16 of a query of a coded cache, whose products are f16: a bf16 has fewer bits than that, so
-// it stays exact down to 2^-14 (below, off by at most 2^-25); beyond f16's range it takes its
-// largest value.
-__device__ __forceinline__ uint16_t f2h_sat(float v) {
-  const float a = fabsf(v);
-  return f2h(a > 65504.0f && a <= 3.402823466e38f ? copysignf(65504.0f, v) : v);
+// Eight query channels from element i on, as they lie.
+__device__ __forceinline__ u32x4 load_q8(const AttnParams& p, size_t i) {
+  const uint16_t* q = (const uint16_t*)p.q + i;
+  if (p.q_vec) return *(const u32x4*)q;
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = (uint32_t)q[2 * e] | (uint32_t)q[2 * e + 1] << 16;
+  return r;
 }
 
-// Eight query channels from element i on, as T: T is the queries' own type for 16-bit
-// caches, f16 for coded ones (4 bits: in codes4's order).
-template <int FMT, typename T>
-__device__ __forceinline__ typename T::V8 load_q8(const AttnParams& p, size_t i) {
-  const uint16_t* q = (const uint16_t*)p.q + i;
-  uint16_t h[8];
-  if (p.q_vec) {
-    const u32x4 w = *(const u32x4*)q;
+// The products of coded caches are f16.  A bf16 has fewer bits than that and a wider range, so
+// bf16 queries are multiplied by the power of two that takes a row's largest magnitude to
+// 2^15 .. 2^16: exact but for channels below 2^-29 of it, which are off by up to 2^-40 of it.
+// Their scores are multiplied by its inverse, with the scale.  (From 2^-111 down the factor stays
+// 2^126, so that the inverse is a normal f32.)
+__device__ __forceinline__ float largest_bf16(const u32x4& w, float most) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = q[e];
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t v = w[e];
+    most = fmaxf(most, fmaxf(fabsf(bf2f((uint16_t)v)), fabsf(bf2f((uint16_t)(v >> 16)))));
   }
-  if (FMT < 9 && p.q_type == DT_BF16) {
+  return most;
+}
+__device__ __forceinline__ uint32_t fit_exponent(float most) {
+  return max(__builtin_bit_cast(uint32_t, most) >> 23, 16u);
+}
+__device__ __forceinline__ float fit_factor(uint32_t e) { return __builtin_bit_cast(float, (269 - e) << 23); }
+// The scale times the inverse, a normal f32 too: a masked score, -inf, times zero would be NaN,
+// as would a score of zero times infinity (at the lower border all scores round to weights of 1).
+__device__ __forceinline__ float fit_scale(float scale2, uint32_t e) {
+  const float inverse = __builtin_bit_cast(float, (e - 15) << 23);
+  return fminf(fmaxf(scale2 * inverse, 1.17549435e-38f), 3.402823466e38f);
+}
+
+// Eight query channels as T: T is the queries' own type for 16-bit caches, f16 for coded ones
+// (bf16 queries times `factor`; 4 bits: in codes4's order).
+template <int FMT, typename T, bool SCALED>
+__device__ __forceinline__ typename T::V8 query_operand(const u32x4& w, float factor) {
+  uint16_t h[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = f2h_sat(bf2f(h[e]));
+  for (int e = 0; e < 8; ++e) h[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+  if constexpr (SCALED) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = f2h(bf2f(h[e]) * factor);
   }
   u32x4 r;
 #pragma unroll

@@ -45,6 +45,7 @@ struct Few {
   static constexpr int kKeyLoads = D / 4 / kVec;
   static constexpr int kKeyWords = kVec * kRow / D / 4;
   static constexpr int kParts = PARTS;  // f16 that a coded value is made of (below)
+  static constexpr bool kScaled = !kRaw && PARTS == 1;  // bf16 queries, to fit f16
   // Values go through LDS kSpan channels at a time: with two parts half a head, so that
   // three workgroups still fit a CU (32 rows: the results at the end need as much).  Of their
   // 16-byte loads: lanes per row, rows per load, loads.
@@ -240,6 +241,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   const int n = lane & 15, g = lane >> 4;
   uint8_t* my = lds + wave * F::kWaveLds;
   V8 q[RT][F::kSteps];
+  float scale2[RT];  // the call's, of rows that were scaled times the inverse
   Seen see[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -248,8 +250,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     see[rt] = row_sees(p, w.first, w.len, r);
     const size_t qi =
         (size_t)(w.start + r / p.group) * p.q_stride + (size_t)(kvh * p.group + r % p.group) * D;
+    u32x4 raw[F::kSteps];
+    float factor = 1.0f, most = 0.0f;
+    scale2[rt] = p.scale2;
 #pragma unroll
-    for (int s = 0; s < F::kSteps; ++s) q[rt][s] = load_q8<FMT, T>(p, qi + F::channel(s, g));
+    for (int s = 0; s < F::kSteps; ++s) raw[s] = load_q8(p, qi + F::channel(s, g));
+    if constexpr (F::kScaled) {
+#pragma unroll
+      for (int s = 0; s < F::kSteps; ++s) most = largest_bf16(raw[s], most);
+      most = fmaxf(most, xor_lanes<16>(most));
+      most = fmaxf(most, xor_lanes<32>(most));
+      const uint32_t e = fit_exponent(most);
+      factor = fit_factor(e);
+      scale2[rt] = fit_scale(p.scale2, e);
+    }
+#pragma unroll
+    for (int s = 0; s < F::kSteps; ++s) q[rt][s] = query_operand<FMT, T, F::kScaled>(raw[s], factor);
   }
   float4v o[RT][D / 16];
   float m[RT], l[RT], less[RT];  // less: what weights are taken against, -m or 0
@@ -261,7 +277,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = float4v{0, 0, 0, 0};
   }
   bool again = false;
-  float slack = kSlack + T::kRoom, unit = p.scale2;  // of the wave; far (kFar): slack < 0, unit 1
+  // of the wave, and what scores are multiplied by as weights; far (kFar): less than 0 and 1
+  float slack = kSlack + T::kRoom, unit[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) unit[rt] = scale2[rt];
 
   typename F::Keys k;
   typename F::Values v;
@@ -333,7 +352,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         }
         most = fmaxf(most, x[i]);
       }
-      most *= p.scale2;
+      most *= scale2[rt];
       if (__any(most - m[rt] > slack)) {
         most = fmaxf(most, xor_lanes<16>(most));
         most = fmaxf(most, xor_lanes<32>(most));
@@ -346,14 +365,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
         if (__any(is_far(up))) slack = -__builtin_inff();
         if (slack < 0.0f) {
-          unit = 1.0f;
+          unit[rt] = 1.0f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= p.scale2;
+          for (int i = 0; i < 8; ++i) x[i] *= scale2[rt];
         }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], unit, less[rt]));
+        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], unit[rt], less[rt]));
         l[rt] += x[i];
         w8[rt][i] = (typename T::E)x[i];
       }

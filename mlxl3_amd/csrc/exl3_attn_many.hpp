@@ -193,18 +193,33 @@ void attn_many_kernel(AttnParams p, int tiles) {
   const Seen wtop = row_sees(p, w.first, w.len, min(wrow, row0 + rows - 1));
   const Seen wend = row_sees(p, w.first, w.len, min(wrow + 31, row0 + rows - 1));
   V8 q[D / 16];
+  float scale2 = p.scale2;  // of rows that were scaled times the inverse
   {
+    constexpr bool kScaled = !F::kRaw && PARTS == 1;  // bf16 queries, to fit f16
     const size_t qi = (size_t)(w.start + mine / p.group) * p.q_stride +
                       (size_t)(kvh * p.group + mine % p.group) * D;
+    u32x4 raw[D / 16];
+    float factor = 1.0f, most = 0.0f;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) q[s] = load_q8<FMT == KV_Q4 ? KV_Q8 : FMT, T>(p, qi + 16 * s + 8 * h);
+    for (int s = 0; s < D / 16; ++s) raw[s] = load_q8(p, qi + 16 * s + 8 * h);
+    if constexpr (kScaled) {
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) most = largest_bf16(raw[s], most);
+      most = fmaxf(most, xor_lanes<32>(most));
+      const uint32_t e = fit_exponent(most);
+      factor = fit_factor(e);
+      scale2 = fit_scale(p.scale2, e);
+    }
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) q[s] = query_operand<FMT == KV_Q4 ? KV_Q8 : FMT, T, kScaled>(raw[s], factor);
   }
   float16v o[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
   float m = -__builtin_inff(), l = 0.0f, less = 0.0f;  // less: what weights are taken against, -m or 0
   bool again = false;
-  float slack = kSlack + T::kRoom, unit = p.scale2;  // of the wave; far (kFar): slack < 0, unit 1
+  // of the wave, and what scores are multiplied by as weights; far (kFar): less than 0 and 1
+  float slack = kSlack + T::kRoom, unit = scale2;
 
   typename F::Loads x;
   const int off = F::kMine * wave;  // of this wave's rows in a tile
@@ -320,7 +335,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
       for (int a = 0; a < NT; ++a)
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, s[a][i]);
-      most *= p.scale2;
+      most *= scale2;
       if (__any(most - m > slack)) {
         most = fmaxf(most, xor_lanes<32>(most));
         const float up = fmaxf(m, most - T::kRoom);
@@ -336,7 +351,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
 #pragma unroll
           for (int a = 0; a < NT; ++a)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[a][i] *= p.scale2;
+            for (int i = 0; i < 16; ++i) s[a][i] *= scale2;
         }
       }
       V8 w8, following;

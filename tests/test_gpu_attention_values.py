@@ -1,6 +1,6 @@
 """Attention where 16 and 32 bits end: coded values beyond f16's range, values that a row does not
-see over coded caches, scores of any size, weights far below the largest.  Against the 64-bit
-forms of kv_ref.py."""
+see over coded caches, scores of any size, weights far below the largest, bf16 queries that f16
+does not hold.  Against the 64-bit forms of kv_ref.py."""
 
 import math
 
@@ -147,3 +147,33 @@ def test_a_long_tail_far_below_one_token(bits, cdtype, dtype, nats, new, old):
             s = (k[seen, 0] @ q[i, 0].double()) * 128**-0.5
             bound[i] -= 2.0**-25 * (1 - 2.0**-7) * v[seen, 0].abs().sum(0) / torch.exp(s - s.max()).sum()
     within(y, want, bound, f"tail {nats} nats below")
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("shift", [17, 100, -20, -100])
+@pytest.mark.parametrize("new", [[2, 1], [40, 33]])
+def test_bf16_queries_beyond_f16_over_codes(bits, dim, shift, new):
+    """Queries around 2^shift, which f16 does not hold or only in part, with a scale that gives
+    ordinary scores.  One row is zeros."""
+    lens = [new[0] + 150, new[1] + 9]
+    pool = Pool(49, lens, 2, dim, 16, bits, None)
+    scale = 2.0**-shift / dim**0.5
+    g = torch.Generator().manual_seed(50)
+    q = (torch.randn(sum(new), 6, dim, generator=g) * 2.0**shift).to(BF16)
+    q[0, 1] = 0
+    b = kv_ref.batch(mlxl3_amd, new, lens, pool.table)
+    y = mlxl3_amd.attention(q.cuda(), pool.cuda(mlxl3_amd), b, scale=scale)
+    check(pool, new, q, y, scale=scale)
+
+
+def test_a_bf16_query_with_channels_far_apart():
+    """One channel of 2^20, whose key's channel is zero: the others count as ever."""
+    pool = Pool(51, [300], 1, 128, 16, 8, None)
+    codes = pool.k.view(-1, 128)
+    codes[:, 64] = 128  # code 0
+    q = torch.randn(2, 4, 128, generator=torch.Generator().manual_seed(52))
+    q[..., 64] = 2.0**20
+    q = q.to(BF16)
+    y = mlxl3_amd.attention(q.cuda(), pool.cuda(mlxl3_amd), kv_ref.batch(mlxl3_amd, [2], [300], pool.table))
+    check(pool, [2], q, y)
