@@ -12,8 +12,10 @@ positions, the paged key/value cache and attention over it (``exl3_rope``,
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
+import threading
 from typing import Optional
 
 from . import (
@@ -426,19 +428,25 @@ class Exl3Attention:
             raise Exl3Error(-1, "attention block widths differ")
         self.q, self.k, self.v, self.o = q, k, v, o
         self.rope, self.scale, self.window = rope, scale, _window(window)
-        self._ws: dict = {}  # by stream
+        self._ws: dict = {}  # (lock, workspace) by stream
 
     def workspace_bytes(self, cache: KvCache, batch: KvBatch, rows: int, dtype) -> int:
         return int(load_library().exl3_attn_block_workspace_bytes(
             self.q.handle, self.k.handle, self.v.handle, self.o.handle, cache.handle, batch._ref, _dtype_code(dtype),
             int(rows)))
 
+    def _kept(self, device):
+        """The lock and the workspace of the current stream.  A call is several launches, which
+        leave their results to each other in the workspace: the lock keeps those of one call
+        together in the stream."""
+        return self._ws.setdefault((device, _stream_ptr(device)), (threading.Lock(), _Workspace()))
+
     def forward(self, x, cache: KvCache, batch: KvBatch, workspace=None):
         """x [rows, in] (f16 or bf16) -> [rows, out] in the o projection's result dtype;
         the cache's pages get the rows' keys and values.  `workspace`: a zero-filled uint8
         tensor of :meth:`workspace_bytes`, of which two calls that run at once need one each;
-        by default one that the block keeps for the stream, and in a captured graph one of
-        the graph's."""
+        by default one that the block keeps for the stream (threads on one stream take turns), and
+        in a captured graph one of the graph's."""
         torch = _torch()
         _floats()
         x = _device_tensor(x, "x", _HALVES, 2).contiguous()
@@ -452,19 +460,23 @@ class Exl3Attention:
         lib, code = load_library(), _HALVES[x.dtype]
         y = torch.empty(rows, self.o.out_features, device=device,
                         dtype=_code_dtype(lib.exl3_linear_output_dtype(self.o.handle, code)))
+        turn = contextlib.nullcontext()
         if workspace is None:
             need = self.workspace_bytes(cache, batch, rows, x.dtype)
             if torch.cuda.is_current_stream_capturing():  # a kept one could be replaced before a replay
                 workspace = torch.zeros(max(need, 256), dtype=torch.uint8, device=device)
             else:
-                workspace = self._ws.setdefault((device, _stream_ptr(device)), _Workspace()).get(need, device)
+                turn, kept = self._kept(device)
         else:
             _plain(workspace, "workspace", (torch.uint8,), 1)
             _same(device, workspace, "workspace")
         scale = cache.head_dim**-0.5 if self.scale is None else float(self.scale)
-        _launch(device, lib.exl3_attn_block_forward, self.q.handle, self.k.handle, self.v.handle, self.o.handle,
-                cache.handle, batch._ref, None if self.rope is None else self.rope._ref, scale, self.window,
-                x.data_ptr(), code, rows, y.data_ptr(), workspace.data_ptr(), workspace.numel())
+        with turn:
+            if workspace is None:
+                workspace = kept.get(need, device)
+            _launch(device, lib.exl3_attn_block_forward, self.q.handle, self.k.handle, self.v.handle, self.o.handle,
+                    cache.handle, batch._ref, None if self.rope is None else self.rope._ref, scale, self.window,
+                    x.data_ptr(), code, rows, y.data_ptr(), workspace.data_ptr(), workspace.numel())
         return y
 
     __call__ = forward
