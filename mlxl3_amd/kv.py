@@ -415,6 +415,9 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     return out
 
 
+_MOST_STREAMS = 40  # that a block keeps a workspace for; PyTorch's own pool has 32 of a device
+
+
 class Exl3Attention:
     """The attention block of a decoder layer (``exl3_attn_block_forward``): the q/k/v
     projections of x as a group, keys rotated and appended with the values, queries rotated,
@@ -428,7 +431,8 @@ class Exl3Attention:
             raise Exl3Error(-1, "attention block widths differ")
         self.q, self.k, self.v, self.o = q, k, v, o
         self.rope, self.scale, self.window = rope, scale, _window(window)
-        self._ws: dict = {}  # (lock, workspace) by stream
+        self._ws: dict = {}  # (lock, workspace) by stream, the last used one last
+        self._ws_lock = threading.Lock()
 
     def workspace_bytes(self, cache: KvCache, batch: KvBatch, rows: int, dtype) -> int:
         return int(load_library().exl3_attn_block_workspace_bytes(
@@ -438,8 +442,15 @@ class Exl3Attention:
     def _kept(self, device):
         """The lock and the workspace of the current stream.  A call is several launches, which
         leave their results to each other in the workspace: the lock keeps those of one call
-        together in the stream."""
-        return self._ws.setdefault((device, _stream_ptr(device)), (threading.Lock(), _Workspace()))
+        together in the stream.  Those of the streams used longest ago are dropped (their memory
+        goes back to the allocator, which reuses it in the same stream's order)."""
+        key = device, _stream_ptr(device)
+        with self._ws_lock:
+            kept = self._ws.pop(key, None) or (threading.Lock(), _Workspace())
+            self._ws[key] = kept
+            while len(self._ws) > _MOST_STREAMS:
+                del self._ws[next(iter(self._ws))]
+        return kept
 
     def forward(self, x, cache: KvCache, batch: KvBatch, workspace=None):
         """x [rows, in] (f16 or bf16) -> [rows, out] in the o projection's result dtype;

@@ -73,3 +73,12 @@ def test_two_threads_on_two_streams_do_not_wait(block):
     together(lambda: call(7), lambda: call(8))
     assert launches[0][0] != launches[1][0]
     assert [n for _, n, _ in launches] == [1, 1] and all(met for *_, met in launches)
+
+
+def test_kept_workspaces_are_bounded(block, monkeypatch):
+    """A program that makes streams for ever does not keep a workspace for each."""
+    made, call, launches = block
+    monkeypatch.setattr(kv, "_launch", lambda *a: None)
+    for at in range(500):
+        call(at)
+    assert len(made._ws) <= 64
