@@ -590,6 +590,12 @@ static int check_rows(const Group& g, int64_t rows) {
   return EXL3_OK;
 }
 
+int exl3::check_linear_rows(const exl3_linear* h, int64_t rows) {
+  Group g;
+  if (int rc = make_group(&h, 1, g)) return rc;
+  return check_rows(g, rows);
+}
+
 static Member member_of(const exl3_linear* h, void* y, int cblk0, int x_type) {
   Member m;
   m.trellis = (const uint32_t*)h->trellis;

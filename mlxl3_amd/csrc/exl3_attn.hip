@@ -235,11 +235,11 @@ extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
   return align256(rows * cache->view.head_dim * 4) + align256(rows * 8);
 }
 
-extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
-                              const void* q, int32_t q_type, int64_t tokens, int32_t heads,
-                              int64_t q_stride, float scale, int32_t causal, int32_t window,
-                              void* y, int64_t y_stride, void* workspace, size_t workspace_bytes,
-                              void* stream) {
+// exl3_attention; without `run` its checks alone.
+static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const void* q,
+                          int32_t q_type, int64_t tokens, int32_t heads, int64_t q_stride,
+                          float scale, int32_t causal, int32_t window, void* y, int64_t y_stride,
+                          void* workspace, size_t workspace_bytes, void* stream, bool run) {
   if (!cache) return fail(EXL3_EINVAL, "null KV cache");
   AttnParams p{};
   p.cache = cache->view;
@@ -275,12 +275,12 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   const Shape sh = choose(p.cache, *batch, tokens, heads, window);
   if (sh.tiles * sh.splits * p.cache.kv_heads > kMostBlocks)
     return fail(EXL3_EUNSUPPORTED, "attention of %lld tokens needs too many workgroups", (long long)tokens);
+  if (!run) return EXL3_OK;
   p.q = q;
   p.y = y;
   p.q_stride = q_stride;
   p.y_stride = y_stride;
   p.tokens = (int)tokens;
-  p.heads = heads;
   p.group = heads / p.cache.kv_heads;
   p.q_type = q_type;
   p.causal = causal != 0;
@@ -322,6 +322,15 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
   else
     hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(256), 0, s, p, sh.rows, shift);
   return check_launch("attention join");
+}
+
+extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                              const void* q, int32_t q_type, int64_t tokens, int32_t heads,
+                              int64_t q_stride, float scale, int32_t causal, int32_t window,
+                              void* y, int64_t y_stride, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  return attention_call(cache, batch, q, q_type, tokens, heads, q_stride, scale, causal, window, y, y_stride,
+                        workspace, workspace_bytes, stream, true);
 }
 
 namespace {
@@ -399,22 +408,28 @@ extern "C" int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* 
   void* query = b.types[0] == x_type ? qkv[0] : ws + b.rounded;
   const int D = cache->view.head_dim;
   const int64_t wide = (int64_t)b.heads * D, narrow = (int64_t)cache->view.kv_heads * D;
-  // what a later call would refuse is refused before the first launch
-  if (int rc = exl3_kv_append(cache, batch, nullptr, narrow, nullptr, narrow, b.types[1], 0, rope, stream))
-    return rc;
-  if (int rc = exl3_attention(cache, batch, nullptr, x_type, 0, b.heads, wide, scale, 1, window, nullptr, wide,
-                              nullptr, 0, stream))
-    return rc;
+  auto turn = [&](bool run) {
+    return rope ? rope_call(rope, qkv[0], b.types[0], rows, b.heads, D, wide, nullptr, batch, query, x_type, wide,
+                            stream, run)
+                : (int)EXL3_OK;
+  };
+  auto append = [&](bool run) {
+    return append_call(cache, batch, qkv[1], narrow, qkv[2], narrow, b.types[1], rows, rope, stream, run);
+  };
+  auto attend = [&](bool run) {
+    return attention_call(cache, batch, query, x_type, rows, b.heads, wide, scale, 1, window, query, wide,
+                          ws + b.attention, b.total - b.attention, stream, run);
+  };
+  // what a later part would refuse is refused before the first one's launch (the group's own
+  // checks come before that)
+  if (int rc = turn(false)) return rc;
+  if (int rc = append(false)) return rc;
+  if (int rc = attend(false)) return rc;
+  if (int rc = check_linear_rows(o, rows)) return rc;
   if (int rc = exl3_group_forward(parts, 3, x, x_type, rows, qkv, ws, b.linear, stream)) return rc;
-  if (rope)
-    if (int rc = exl3_rope(rope, qkv[0], b.types[0], rows, b.heads, D, wide, nullptr, batch, query, x_type, wide,
-                           stream))
-      return rc;
-  if (int rc = exl3_kv_append(cache, batch, qkv[1], narrow, qkv[2], narrow, b.types[1], rows, rope, stream))
-    return rc;
-  if (int rc = exl3_attention(cache, batch, query, x_type, rows, b.heads, wide, scale, 1, window, query, wide,
-                              ws + b.attention, b.total - b.attention, stream))
-    return rc;
+  if (int rc = turn(true)) return rc;
+  if (int rc = append(true)) return rc;
+  if (int rc = attend(true)) return rc;
   return exl3_linear_forward(o, query, x_type, rows, y, exl3_linear_output_dtype(o, x_type), ws, b.linear,
                              stream);
 }

@@ -15,7 +15,7 @@ struct AttnParams {
   float* stats;   // [slots][rows][2] their maximum and sum of weights
   int64_t q_stride, y_stride;
   int tokens;     // rows of q and y
-  int heads, group, q_type, causal, window;
+  int group, q_type, causal, window;
   int max_q;
   int splits;     // even ranges of the tokens that a tile sees
   int budget;     // else ranges by the batch's sum (few rows), about; 0: even ones

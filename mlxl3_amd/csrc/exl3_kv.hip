@@ -601,10 +601,10 @@ static void by_format(const KvCacheView& c, F&& f) {
   }
 }
 
-extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_type, int64_t tokens,
-                         int32_t heads, int32_t head_dim, int64_t x_stride,
-                         const int32_t* positions, const exl3_kv_batch* batch, void* y,
-                         int32_t y_type, int64_t y_stride, void* stream) {
+int exl3::rope_call(const exl3_rope_spec* rope, const void* x, int32_t x_type, int64_t tokens,
+                    int32_t heads, int32_t head_dim, int64_t x_stride, const int32_t* positions,
+                    const exl3_kv_batch* batch, void* y, int32_t y_type, int64_t y_stride,
+                    void* stream, bool launch) {
   if (!rope) return fail(EXL3_EINVAL, "null rotary spec");
   if (tokens < 0) return fail(EXL3_EINVAL, "negative token count");
   if (!known_type(x_type) || !known_type(y_type))
@@ -649,6 +649,7 @@ extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_ty
   p.per = 2 * kBatch;
   while (p.per > 1 && blocks * ((heads + p.per - 1) / p.per) < 512) p.per /= 2;
   const dim3 grid((unsigned)blocks, (unsigned)((heads + p.per - 1) / p.per));
+  if (!launch) return EXL3_OK;
   if (int rc = launch_gate("rotary launch")) return rc;
   hipStream_t s = (hipStream_t)stream;
   if (vec && x_type == EXL3_F32)
@@ -660,10 +661,17 @@ extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_ty
   return check_launch("rotary launch");
 }
 
-extern "C" int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
-                              const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                              int32_t type, int64_t tokens, const exl3_rope_spec* rope,
-                              void* stream) {
+extern "C" int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_type, int64_t tokens,
+                         int32_t heads, int32_t head_dim, int64_t x_stride,
+                         const int32_t* positions, const exl3_kv_batch* batch, void* y,
+                         int32_t y_type, int64_t y_stride, void* stream) {
+  return rope_call(rope, x, x_type, tokens, heads, head_dim, x_stride, positions, batch, y, y_type, y_stride,
+                   stream, true);
+}
+
+int exl3::append_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const void* k,
+                      int64_t k_stride, const void* v, int64_t v_stride, int32_t type,
+                      int64_t tokens, const exl3_rope_spec* rope, void* stream, bool launch) {
   if (!cache) return fail(EXL3_EINVAL, "null KV cache");
   AppendParams p{};
   p.cache = cache->view;
@@ -686,6 +694,7 @@ extern "C" int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* b
   p.type = type;
   p.vec = rows_aligned(k, tokens > 1 ? k_stride : 0, type) &&
           rows_aligned(v, tokens > 1 ? v_stride : 0, type);
+  if (!launch) return EXL3_OK;
   if (int rc = launch_gate("KV append")) return rc;
   by_format(p.cache, [&](auto fmt, auto dim) {
     if (type == EXL3_F32)
@@ -694,6 +703,13 @@ extern "C" int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* b
       hipLaunchKernelGGL((kv_append_kernel<fmt(), dim(), 2>), grid, dim3(256), 0, (hipStream_t)stream, p);
   });
   return check_launch("KV append");
+}
+
+extern "C" int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                              const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                              int32_t type, int64_t tokens, const exl3_rope_spec* rope,
+                              void* stream) {
+  return append_call(cache, batch, k, k_stride, v, v_stride, type, tokens, rope, stream, true);
 }
 
 extern "C" int exl3_kv_read(const exl3_kv_cache* cache, const exl3_kv_batch* batch, void* k,

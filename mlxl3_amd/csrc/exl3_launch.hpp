@@ -78,6 +78,8 @@ int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int check_launch(const char* what);
 // The fault hook before a launch: EXL3_EDEVICE when `what` is armed.
 int launch_gate(const char* what);
+// The sizes that exl3_linear_forward refuses for this projection.
+int check_linear_rows(const exl3_linear* h, int64_t rows);
 
 // Hands a device allocation (hipMalloc) to a handle, which frees it when it is
 // destroyed: the checkpoint loaders own the weights they upload.
