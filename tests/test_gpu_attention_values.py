@@ -73,17 +73,21 @@ def test_the_largest_values_that_f16_holds_are_attended_to(bits, dtype, new):
     check(pool, new, q, y)
 
 
+def set_side(pool, name, seq, x):
+    """A sequence's keys or values: x [tokens, kv_heads, dim]."""
+    t = torch.arange(pool.lens[seq])
+    at = pool.table[seq, t // pool.page].long(), slice(None), t % pool.page
+    if pool.bits == 16:
+        getattr(pool, name)[at] = x.to(pool.dtype)
+    else:
+        c, s = kv_ref.quantise(x, pool.bits)
+        getattr(pool, name)[at] = kv_ref.pack(c, pool.bits)
+        getattr(pool, name + "s").transpose(2, 3)[at] = s
+
+
 def set_keys(pool, seq, x):
     """A sequence's keys: x [tokens] times ones, in every head."""
-    for t in range(pool.lens[seq]):
-        row = x[t].expand(pool.kv_heads, pool.dim)
-        at = int(pool.table[seq, t // pool.page]), slice(None), t % pool.page
-        if pool.bits == 16:
-            pool.k[at] = row.to(pool.dtype)
-        else:
-            c, s = kv_ref.quantise(row, pool.bits)
-            pool.k[at] = kv_ref.pack(c, pool.bits)
-            pool.ks.transpose(2, 3)[at] = s
+    set_side(pool, "k", seq, x[:, None, None].expand(-1, pool.kv_heads, pool.dim))
 
 
 ALL = [(16, F16, F16), (16, BF16, BF16)] + [(b, None, t) for b, t in CODED]
@@ -127,15 +131,9 @@ def test_a_long_tail_far_below_one_token(bits, cdtype, dtype, nats, new, old):
     x[0] = nats / 128**0.5
     set_keys(pool, 0, x)
     g = torch.Generator().manual_seed(48)
-    for t in range(lens[0]):
-        row = torch.rand(1, 128, generator=g) + 0.5 if t else torch.zeros(1, 128)
-        at = int(pool.table[0, t // 64]), slice(None), t % 64
-        if bits == 16:
-            pool.v[at] = row.to(cdtype)
-        else:
-            c, s = kv_ref.quantise(row, bits)
-            pool.v[at] = kv_ref.pack(c, bits)
-            pool.vs.transpose(2, 3)[at] = s
+    v = torch.rand(lens[0], 1, 128, generator=g) + 0.5
+    v[0] = 0
+    set_side(pool, "v", 0, v)
     q = torch.ones(new[0], 4, 128).to(dtype)
     b = kv_ref.batch(mlxl3_amd, new, lens, pool.table)
     y = mlxl3_amd.attention(q.cuda(), pool.cuda(mlxl3_amd), b)
