@@ -124,10 +124,13 @@ class KvBatch:
     block_table int32 [seqs, pages]: the page of every page_tokens positions.  The
     tensors are read on the device at every call (a captured graph can be replayed after
     they were changed in place).  max_q and max_kv bound a sequence's new tokens and its
-    length (max_kv None: what the table has room for).
+    length (None: all tokens of a call, and what the table has room for).  Attention is
+    launched for max_q tokens of every sequence, and rows past it are not computed: a batch
+    of decoded tokens says max_q=1, or pays for rows that it may have.
     """
 
-    def __init__(self, q_starts, kv_lens, block_table=None, max_q: int = 1, max_kv: Optional[int] = None):
+    def __init__(self, q_starts, kv_lens, block_table=None, max_q: Optional[int] = None,
+                 max_kv: Optional[int] = None):
         i32 = (_torch().int32,)
         self.q_starts = _plain(q_starts, "q_starts", i32, 1)
         self.kv_lens = _plain(kv_lens, "kv_lens", i32, 1)
@@ -137,7 +140,7 @@ class KvBatch:
             raise Exl3Error(-1, "q_starts has one entry more than kv_lens, which has at least one")
         if block_table is not None and self.block_table.shape[0] != self.seqs:
             raise Exl3Error(-1, "block_table has one row per sequence")
-        if not 1 <= int(max_q) < 2**31 or not 0 <= int(max_kv or 0) < 2**31:
+        if not 1 <= int(1 if max_q is None else max_q) < 2**31 or not 0 <= int(max_kv or 0) < 2**31:
             raise Exl3Error(-1, "max_q must be positive, max_kv not negative, both 32 bits")
         self.device = self.kv_lens.device
         _same(self.device, self.q_starts, "q_starts")
@@ -145,15 +148,28 @@ class KvBatch:
             _same(self.device, self.block_table, "block_table")
         pages = 0 if block_table is None else int(self.block_table.shape[1])
         self._c = _KvBatchC(_ptr(self.q_starts), _ptr(self.kv_lens), _ptr(self.block_table), self.seqs, pages,
-                            int(max_q), 0 if max_kv is None else int(max_kv))
+                            int(max_q or 1), 0 if max_kv is None else int(max_kv))
         self._ref = ctypes.byref(self._c)
+        self._given = max_q is not None
+        self._bounded = (0, None, None)  # without max_q: the last attention's tokens, with them as max_q
         self._sized = (None, 0)  # the last attention's sizes and workspace
+
+    def _attended(self, tokens: int):
+        """The batch of an attention call of so many tokens."""
+        if self._given:
+            return self._ref
+        bounded = self._bounded  # read once: another thread may replace it
+        if bounded[0] != tokens:
+            c = _KvBatchC.from_buffer_copy(self._c)
+            c.max_q = max(1, tokens)
+            self._bounded = bounded = (tokens, c, ctypes.byref(c))
+        return bounded[2]
 
     def _workspace_bytes(self, cache: "KvCache", tokens: int, heads: int) -> int:
         key = (cache.kv_heads, cache.head_dim, cache.page_tokens, tokens, heads)
         sized = self._sized  # read once: another thread may replace it
         if sized[0] != key:
-            need = load_library().exl3_attention_workspace_bytes(cache.handle, self._ref, tokens, heads)
+            need = load_library().exl3_attention_workspace_bytes(cache.handle, self._attended(tokens), tokens, heads)
             self._sized = sized = (key, int(need))
         return sized[1]
 
@@ -381,7 +397,7 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     [tokens, heads, head_dim] (f16 or bf16, the cache's type where it is 16-bit) -> the
     same shape and type.  scale defaults to 1 / sqrt(head_dim); causal: a token sees the
     positions up to its own; window > 0: only the last `window` of them.  Rows outside
-    every sequence are not written."""
+    every sequence and past the batch's max_q are not written (in a new tensor they hold anything)."""
     torch = _torch()
     _floats()
     q = _heads(q, "q", _HALVES)
@@ -409,7 +425,7 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
         room = workspace.numel()
     if workspace is not None:
         space = workspace.data_ptr()
-    _launch(device, load_library().exl3_attention, cache._handle, batch._ref, q.data_ptr(), _HALVES[q.dtype], n, heads,
+    _launch(device, load_library().exl3_attention, cache._handle, batch._attended(n), q.data_ptr(), _HALVES[q.dtype], n, heads,
             q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, window,
             out.data_ptr(), out.stride(0), space, room)
     return out
@@ -436,8 +452,8 @@ class Exl3Attention:
 
     def workspace_bytes(self, cache: KvCache, batch: KvBatch, rows: int, dtype) -> int:
         return int(load_library().exl3_attn_block_workspace_bytes(
-            self.q.handle, self.k.handle, self.v.handle, self.o.handle, cache.handle, batch._ref, _dtype_code(dtype),
-            int(rows)))
+            self.q.handle, self.k.handle, self.v.handle, self.o.handle, cache.handle, batch._attended(int(rows)),
+            _dtype_code(dtype), int(rows)))
 
     def _kept(self, device):
         """The lock and the workspace of the current stream.  A call is several launches, which
@@ -486,7 +502,7 @@ class Exl3Attention:
             if workspace is None:
                 workspace = kept.get(need, device)
             _launch(device, lib.exl3_attn_block_forward, self.q.handle, self.k.handle, self.v.handle, self.o.handle,
-                    cache.handle, batch._ref, None if self.rope is None else self.rope._ref, scale, self.window,
+                    cache.handle, batch._attended(rows), None if self.rope is None else self.rope._ref, scale, self.window,
                     x.data_ptr(), code, rows, y.data_ptr(), workspace.data_ptr(), workspace.numel())
         return y
 

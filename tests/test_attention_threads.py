@@ -42,7 +42,7 @@ def block(monkeypatch):
     linear = lambda n: types.SimpleNamespace(in_features=64, out_features=n, k=4, cb=0, handle=None)
     made = mlxl3_amd.Exl3Attention(linear(64), linear(64), linear(64), linear(64))
     cache = types.SimpleNamespace(device=torch.device("cpu"), head_dim=64, handle=None)
-    batch = types.SimpleNamespace(kv_lens=torch.zeros(1), _ref=None)
+    batch = types.SimpleNamespace(kv_lens=torch.zeros(1), _attended=lambda rows: None)
 
     def call(at):
         stream.at = at

@@ -1,0 +1,41 @@
+"""Calls of the attention operators that say less than they could."""
+
+import pytest
+import torch
+
+import kv_ref
+from kv_ref import Pool
+from test_gpu_attention import BF16, F16, check, projections
+
+import mlxl3_amd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("new, old", [([1], [40]), ([1, 1, 1], [40, 900, 3]), ([5, 1, 0, 2], [40, 900, 3, 7]), ([2, 0], [9, 30]),
+                                      ([70, 33], [0, 500])])
+def test_without_max_q_every_row_is_computed(new, old):
+    lens = [n + m for n, m in zip(new, old)]
+    pool = Pool(90, lens, 2, 64, 16, 8, None)
+    cache = pool.cuda(mlxl3_amd)
+    told = kv_ref.batch(mlxl3_amd, new, lens, pool.table)
+    b = mlxl3_amd.KvBatch(told.q_starts, told.kv_lens, told.block_table)
+    for rows in (sum(new), sum(new) + 5, sum(new)):  # the same object, with rows behind the last sequence too
+        q = torch.randn(rows, 6, 64, generator=torch.Generator().manual_seed(rows)).to(BF16)
+        out = torch.full((rows, 6, 64), 7.0, dtype=BF16, device="cuda")
+        mlxl3_amd.attention(q.cuda(), cache, b, out=out)
+        check(pool, new, q[: sum(new)], out[: sum(new)])
+        assert bool((out[sum(new) :] == 7.0).all())
+
+
+def test_attention_block_without_max_q():
+    new, lens, dim, heads, kv_heads = [9, 1, 30], [50, 8, 30], 64, 4, 2
+    pool = Pool(91, lens, kv_heads, dim, 16, 16, F16, loud=1.0)
+    block = mlxl3_amd.Exl3Attention(*projections(9, 256, heads, kv_heads, dim, 4, 0, False))
+    x = torch.randn(sum(new), 256, generator=torch.Generator().manual_seed(3)).half().cuda()
+    told = kv_ref.batch(mlxl3_amd, new, lens, pool.table, max_q=sum(new))
+    b = mlxl3_amd.KvBatch(told.q_starts, told.kv_lens, told.block_table)
+    one, two = pool.cuda(mlxl3_amd), pool.cuda(mlxl3_amd)
+    assert torch.equal(block(x, one, b), block(x, two, told))
+    for name in "kv":  # bit for bit: slots never written hold NaN
+        assert torch.equal(*(getattr(c, name).view(torch.int16) for c in (one, two)))
