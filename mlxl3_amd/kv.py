@@ -446,6 +446,13 @@ class Exl3Attention:
         if o.in_features != q.out_features or k.out_features != v.out_features:
             raise Exl3Error(-1, "attention block widths differ")
         self.q, self.k, self.v, self.o = q, k, v, o
+        self.device = None  # of the projections; not known of those loaded to "cuda"
+        for name, m in zip("qkvo", (q, k, v, o)):
+            at = m.device if m.trellis is None else m.trellis.device
+            if at.index is not None:
+                if self.device not in (None, at):
+                    raise Exl3Error(-1, f"projection {name} is on {at}, others on {self.device}")
+                self.device = at
         self.rope, self.scale, self.window = rope, scale, _window(window)
         self._ws: dict = {}  # (lock, workspace) by stream, the last used one last
         self._ws_lock = threading.Lock()
@@ -482,6 +489,8 @@ class Exl3Attention:
             raise Exl3Error(-1, f"invalid attention block input for {self.q.in_features} inputs")
         _same(device, x, "x")
         _same(device, batch.kv_lens, "batch")
+        if self.device is not None:
+            _same(device, self, "projections")
         if self.rope is not None:
             _same(device, self.rope.inv_freq, "rope")
         lib, code = load_library(), _HALVES[x.dtype]

@@ -39,7 +39,7 @@ def block(monkeypatch):
     monkeypatch.setattr(kv, "_stream_ptr", lambda device: stream.at)
     monkeypatch.setattr(kv, "_launch", launch)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
-    linear = lambda n: types.SimpleNamespace(in_features=64, out_features=n, k=4, cb=0, handle=None)
+    linear = lambda n: types.SimpleNamespace(in_features=64, out_features=n, k=4, cb=0, handle=None, trellis=torch.zeros(1))
     made = mlxl3_amd.Exl3Attention(linear(64), linear(64), linear(64), linear(64))
     cache = types.SimpleNamespace(device=torch.device("cpu"), head_dim=64, handle=None)
     batch = types.SimpleNamespace(kv_lens=torch.zeros(1), _attended=lambda rows: None)
