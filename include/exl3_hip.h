@@ -332,7 +332,8 @@ typedef struct {
 /* y[tokens][heads][head_dim] = x rotated; x_type and y_type f16, bf16 or f32
  * (rounded once), token strides in elements, heads contiguous (head_dim at
  * most 256).  Positions come from `positions` [tokens] or, where that is NULL,
- * from `batch` (whose block table is not used).  y may be x. */
+ * from `batch` (whose block table is not used).  y may be x (with its type and
+ * stride); else the two do not overlap. */
 int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_type, int64_t tokens,
               int32_t heads, int32_t head_dim, int64_t x_stride, const int32_t* positions,
               const exl3_kv_batch* batch, void* y, int32_t y_type, int64_t y_stride,
@@ -358,9 +359,9 @@ int exl3_kv_read(const exl3_kv_cache* cache, const exl3_kv_batch* batch, void* k
  * tokens t < kv_lens[b], with causal != 0 only t <= the token's position, with
  * window > 0 only t > its position - window.  A token that sees none gives
  * zeros.  q_type is f16 or bf16 and the cache's where that is 16-bit; y has
- * q_type; token strides in elements; y may be q (with its stride).  Rows are
- * equal bit for bit in repeated calls; the same row in a call of other sizes
- * may differ in the order of its f32 sums.  Workspace:
+ * q_type; token strides in elements; y may be q (with its stride), else the two
+ * do not overlap.  Rows are equal bit for bit in repeated calls; the same row in
+ * a call of other sizes may differ in the order of its f32 sums.  Workspace:
  * exl3_attention_workspace_bytes, 16-byte aligned, not initialised and not
  * shared between calls that run concurrently. */
 size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache, const exl3_kv_batch* batch,

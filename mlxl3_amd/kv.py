@@ -257,11 +257,14 @@ class Rope:
 
     def apply(self, x, positions=None, batch: Optional[KvBatch] = None, out=None, dtype=None):
         """x [tokens, heads, channels] (f16, bf16 or f32) rotated by its tokens' positions
-        (int32 [tokens], or the batch's) into `out` (x itself: in place) or a new tensor
-        of `dtype` (default x's)."""
+        (int32 [tokens], or the batch's) into `out` (x itself: in place; else apart from it) or a
+        new tensor of `dtype` (default x's).  Rows outside every sequence of a batch are not
+        written."""
         if out is x and not _rows_ok(x):
             raise Exl3Error(-1, "rotation in place needs contiguous heads")
         src = _heads(x, "x", _floats())
+        if dtype is not None and dtype not in _FLOATS:
+            raise Exl3Error(-1, f"unsupported rotary output dtype {dtype}")
         n, heads, dim = src.shape
         device = src.device
         if out is None:
@@ -377,6 +380,8 @@ class KvCache:
         if dtype not in _floats():
             raise Exl3Error(-1, f"unsupported KV output dtype {dtype}")
         device, tokens = self.device, int(tokens)
+        if tokens < 0:
+            raise Exl3Error(-1, "negative token count")
         _same(device, batch.kv_lens, "batch")
         shape = (tokens, self.kv_heads, self.head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
@@ -396,8 +401,8 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     """Attention of the batch's new tokens over the cache (``exl3_attention``): q
     [tokens, heads, head_dim] (f16 or bf16, the cache's type where it is 16-bit) -> the
     same shape and type.  scale defaults to 1 / sqrt(head_dim); causal: a token sees the
-    positions up to its own; window > 0: only the last `window` of them.  Rows outside
-    every sequence and past the batch's max_q are not written (in a new tensor they hold anything)."""
+    positions up to its own; window > 0: only the last `window` of them.  `out` may be q and is
+    apart from it else.  Rows outside every sequence and past the batch's max_q are not written (in a new tensor they hold anything)."""
     torch = _torch()
     _floats()
     q = _heads(q, "q", _HALVES)
@@ -410,7 +415,7 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     window = _window(window)
     if out is None:
         out = _new(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda or not _rows_ok(out):
+    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda or not _rows_ok(out):
         raise Exl3Error(-1, "out must have q's shape and type and contiguous heads")
     else:
         _same(device, out, "out")
@@ -458,9 +463,12 @@ class Exl3Attention:
         self._ws_lock = threading.Lock()
 
     def workspace_bytes(self, cache: KvCache, batch: KvBatch, rows: int, dtype) -> int:
+        _floats()
+        if dtype not in _HALVES:
+            raise Exl3Error(-1, f"attention blocks take f16 or bf16 activations, got {dtype}")
         return int(load_library().exl3_attn_block_workspace_bytes(
             self.q.handle, self.k.handle, self.v.handle, self.o.handle, cache.handle, batch._attended(int(rows)),
-            _dtype_code(dtype), int(rows)))
+            _HALVES[dtype], int(rows)))
 
     def _kept(self, device):
         """The lock and the workspace of the current stream.  A call is several launches, which
@@ -480,7 +488,8 @@ class Exl3Attention:
         the cache's pages get the rows' keys and values.  `workspace`: a zero-filled uint8
         tensor of :meth:`workspace_bytes`, of which two calls that run at once need one each;
         by default one that the block keeps for the stream (threads on one stream take turns), and
-        in a captured graph one of the graph's."""
+        in a captured graph one of the graph's, all of which every replay clears first (a given
+        one saves that)."""
         torch = _torch()
         _floats()
         x = _device_tensor(x, "x", _HALVES, 2).contiguous()

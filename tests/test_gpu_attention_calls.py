@@ -39,3 +39,20 @@ def test_attention_block_without_max_q():
     assert torch.equal(block(x, one, b), block(x, two, told))
     for name in "kv":  # bit for bit: slots never written hold NaN
         assert torch.equal(*(getattr(c, name).view(torch.int16) for c in (one, two)))
+
+
+def test_arguments_of_the_wrong_kind_are_refused_as_such():
+    pool = Pool(92, [20], 2, 64, 16, 16, F16)
+    cache, b = pool.cuda(mlxl3_amd), kv_ref.batch(mlxl3_amd, [1], [20], pool.table)
+    q = torch.zeros(1, 4, 64, dtype=F16, device="cuda")
+    rope = mlxl3_amd.Rope(torch.ones(32, device="cuda"))
+    for dtype in (torch.int32, torch.float64):
+        with pytest.raises(mlxl3_amd.Exl3Error, match="unsupported rotary output dtype"):
+            rope.apply(q, batch=b, dtype=dtype)
+    with pytest.raises(mlxl3_amd.Exl3Error, match="out must have q's shape"):
+        mlxl3_amd.attention(q, cache, b, out=[1.0])
+    with pytest.raises(mlxl3_amd.Exl3Error, match="negative token count"):
+        cache.read(b, -1)
+    with pytest.raises(mlxl3_amd.Exl3Error, match="attention blocks take f16 or bf16"):
+        block = mlxl3_amd.Exl3Attention(*projections(9, 256, 4, 2, 64, 4, 0, False))
+        block.workspace_bytes(cache, b, 1, torch.float32)
