@@ -41,6 +41,37 @@ def test_attention_block_without_max_q():
         assert torch.equal(*(getattr(c, name).view(torch.int16) for c in (one, two)))
 
 
+def test_threads_on_one_stream_share_a_block():
+    """Two threads on the default stream, each with its cache: results as one after the other."""
+    import threading
+
+    block = mlxl3_amd.Exl3Attention(*projections(10, 256, 4, 2, 64, 4, 0, False))
+    sides = []
+    for rows in (1, 24):
+        pool = Pool(93, [64], 2, 64, 16, 16, F16, poison=False, loud=1.0)
+        b = kv_ref.batch(mlxl3_amd, [rows], [64], pool.table)
+        x = torch.randn(rows, 256, generator=torch.Generator().manual_seed(rows)).half().cuda()
+        sides.append((x, pool.cuda(mlxl3_amd), b))
+    want = [block(*s) for s in sides]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            outs = [block(*sides[i]) for _ in range(100)]
+            torch.cuda.synchronize()
+            failed.extend(f"thread {i}: another result" for y in outs if not torch.equal(y, want[i]))
+        except Exception as e:  # told to the main thread
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
 def test_arguments_of_the_wrong_kind_are_refused_as_such():
     pool = Pool(92, [20], 2, 64, 16, 16, F16)
     cache, b = pool.cuda(mlxl3_amd), kv_ref.batch(mlxl3_amd, [1], [20], pool.table)

@@ -61,6 +61,32 @@ def test_coded_values_that_a_row_does_not_see_do_not_reach_it(bits, dtype, dim, 
 
 
 @pytest.mark.parametrize("bits, dtype", CODED)
+@pytest.mark.parametrize("value", [math.nan, 1.0e6])
+@pytest.mark.parametrize("new", [[1, 3], [40, 33]])
+def test_coded_keys_that_a_row_does_not_see_do_not_reach_it(bits, dtype, value, new):
+    """Keys that are not finite, or not as f16, in the newest token: the rows before it are as exact
+    as without it."""
+    lens = [new[0] + 100, new[1] + 20]
+    pool = Pool(53, lens, 2, 128, 16, bits, None)
+    clean = Pool(53, lens, 2, 128, 16, bits, None)
+    for s in range(2):
+        row = torch.zeros(2, 128)
+        row[:, 7] = value
+        c, scales = kv_ref.quantise(row, bits)
+        t = lens[s] - 1
+        at = int(pool.table[s, t // 16]), slice(None), t % 16
+        pool.k[at] = kv_ref.pack(c, bits)
+        pool.ks.transpose(2, 3)[at] = scales
+    q, _, _, y = run(pool, new, 4, dtype)
+    at = 0
+    for s, n in enumerate(new):
+        want, bound = kv_ref.attend(q[at : at + n].double(), clean.values("k", s), clean.values("v", s), lens[s] - n, 128**-0.5,
+                                    True, 0, coded=True, dtype=dtype)
+        within(y[at : at + n - 1], want[:-1], bound[:-1], f"sequence {s}")
+        at += n
+
+
+@pytest.mark.parametrize("bits, dtype", CODED)
 @pytest.mark.parametrize("new", [[2], [40]])
 def test_the_largest_values_that_f16_holds_are_attended_to(bits, dtype, new):
     """Groups just below the border, seen by some rows: every row within the bound."""
