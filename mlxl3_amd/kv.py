@@ -151,7 +151,7 @@ class KvBatch:
                             int(max_q or 1), 0 if max_kv is None else int(max_kv))
         self._ref = ctypes.byref(self._c)
         self._given = max_q is not None
-        self._bounded = (0, None, None)  # without max_q: the last attention's tokens, with them as max_q
+        self._bounded = (None, None, None)  # without max_q: the last attention's tokens, with them as max_q
         self._sized = (None, 0)  # the last attention's sizes and workspace
 
     def _attended(self, tokens: int):
@@ -161,7 +161,7 @@ class KvBatch:
         bounded = self._bounded  # read once: another thread may replace it
         if bounded[0] != tokens:
             c = _KvBatchC.from_buffer_copy(self._c)
-            c.max_q = max(1, tokens)
+            c.max_q = min(max(1, tokens), 2**31 - 1)
             self._bounded = bounded = (tokens, c, ctypes.byref(c))
         return bounded[2]
 
@@ -402,7 +402,8 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     [tokens, heads, head_dim] (f16 or bf16, the cache's type where it is 16-bit) -> the
     same shape and type.  scale defaults to 1 / sqrt(head_dim); causal: a token sees the
     positions up to its own; window > 0: only the last `window` of them.  `out` may be q and is
-    apart from it else.  Rows outside every sequence and past the batch's max_q are not written (in a new tensor they hold anything)."""
+    apart from it else.  Rows outside every sequence and past the batch's max_q are not
+    written (in a new tensor they hold anything)."""
     torch = _torch()
     _floats()
     q = _heads(q, "q", _HALVES)
@@ -415,7 +416,8 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     window = _window(window)
     if out is None:
         out = _new(q)
-    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda or not _rows_ok(out):
+    elif (not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda
+          or not _rows_ok(out)):
         raise Exl3Error(-1, "out must have q's shape and type and contiguous heads")
     else:
         _same(device, out, "out")
@@ -430,8 +432,8 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
         room = workspace.numel()
     if workspace is not None:
         space = workspace.data_ptr()
-    _launch(device, load_library().exl3_attention, cache._handle, batch._attended(n), q.data_ptr(), _HALVES[q.dtype], n, heads,
-            q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, window,
+    _launch(device, load_library().exl3_attention, cache._handle, batch._attended(n), q.data_ptr(), _HALVES[q.dtype],
+            n, heads, q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, window,
             out.data_ptr(), out.stride(0), space, room)
     return out
 
@@ -520,8 +522,8 @@ class Exl3Attention:
             if workspace is None:
                 workspace = kept.get(need, device)
             _launch(device, lib.exl3_attn_block_forward, self.q.handle, self.k.handle, self.v.handle, self.o.handle,
-                    cache.handle, batch._attended(rows), None if self.rope is None else self.rope._ref, scale, self.window,
-                    x.data_ptr(), code, rows, y.data_ptr(), workspace.data_ptr(), workspace.numel())
+                    cache.handle, batch._attended(rows), None if self.rope is None else self.rope._ref, scale,
+                    self.window, x.data_ptr(), code, rows, y.data_ptr(), workspace.data_ptr(), workspace.numel())
         return y
 
     __call__ = forward

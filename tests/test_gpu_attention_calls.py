@@ -28,6 +28,14 @@ def test_without_max_q_every_row_is_computed(new, old):
         assert bool((out[sum(new) :] == 7.0).all())
 
 
+def test_no_tokens_without_max_q():
+    pool = Pool(94, [20], 2, 64, 16, 16, F16)
+    told = kv_ref.batch(mlxl3_amd, [0], [20], pool.table)
+    b = mlxl3_amd.KvBatch(told.q_starts, told.kv_lens, told.block_table)
+    none = torch.empty(0, 4, 64, dtype=F16, device="cuda")
+    assert mlxl3_amd.attention(none, pool.cuda(mlxl3_amd), b).shape == none.shape
+
+
 def test_attention_block_without_max_q():
     new, lens, dim, heads, kv_heads = [9, 1, 30], [50, 8, 30], 64, 4, 2
     pool = Pool(91, lens, kv_heads, dim, 16, 16, F16, loud=1.0)
