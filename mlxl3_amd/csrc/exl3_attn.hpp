@@ -303,8 +303,14 @@ constexpr float kSlack = 8.0f;
 // rounded before m is taken off, exactly: none passes the largest.  (Then every step goes the
 // way of a moving maximum, so that others have no further branch.)
 constexpr float kFar = 65536.0f;
-__device__ __forceinline__ bool is_far(float m) {
-  return fabsf(m) > kFar && m != -__builtin_inff();
+// m of a row that has seen nothing yet: finite, so that neither m less m nor a masked score
+// (-inf) less m is NaN.  Kept as -inf outside the loops.
+constexpr float kNothing = -3.402823466e38f;
+__device__ __forceinline__ float seen_max(float m) { return m == kNothing ? -__builtin_inff() : m; }
+// The slack of a wave whose lanes' maxima are now m: kept as it is or, far, below every difference.
+__device__ __forceinline__ float slack_at(float m, float slack) {
+  const float s = __any(fabsf(m) > kFar && m != kNothing) ? kNothing : slack;
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s)));
 }
 
 // One row over the tokens [lo, hi) by one wave, its channels spread over the lanes (lane

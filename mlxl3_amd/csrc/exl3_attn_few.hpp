@@ -268,11 +268,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     for (int s = 0; s < F::kSteps; ++s) q[rt][s] = query_operand<FMT, T, F::kScaled>(raw[s], factor);
   }
   float4v o[RT][D / 16];
-  float m[RT], l[RT], less[RT];  // less: what weights are taken against, -m or 0
+  float m[RT], l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -__builtin_inff();
-    l[rt] = less[rt] = 0.0f;
+    m[rt] = kNothing;
+    l[rt] = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] = float4v{0, 0, 0, 0};
   }
@@ -357,13 +357,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         most = fmaxf(most, xor_lanes<16>(most));
         most = fmaxf(most, xor_lanes<32>(most));
         const float up = fmaxf(m[rt], most - T::kRoom);
-        const float f = up == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - up);
+        const float f = __builtin_amdgcn_exp2f(m[rt] - up);
         m[rt] = up;
-        less[rt] = up == -__builtin_inff() ? 0.0f : -up;
         l[rt] *= f;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
-        if (__any(is_far(up))) slack = -__builtin_inff();
+        slack = slack_at(up, slack);
         if (slack < 0.0f) {
           unit[rt] = 1.0f;
 #pragma unroll
@@ -372,7 +371,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], unit[rt], less[rt]));
+        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], unit[rt], -m[rt]));
         l[rt] += x[i];
         w8[rt][i] = (typename T::E)x[i];
       }
@@ -405,7 +404,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     l[rt] += xor_lanes<16>(l[rt]);
     l[rt] += xor_lanes<32>(l[rt]);
     if (g == 0) {
-      wave_m[wave][rt * 16 + n] = m[rt];
+      wave_m[wave][rt * 16 + n] = seen_max(m[rt]);
       wave_l[wave][rt * 16 + n] = l[rt];
     }
     float* out = (float*)my + (rt * 16 + n) * D;

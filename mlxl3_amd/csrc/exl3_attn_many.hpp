@@ -216,7 +216,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
   float16v o[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
-  float m = -__builtin_inff(), l = 0.0f, less = 0.0f;  // less: what weights are taken against, -m or 0
+  float m = kNothing, l = 0.0f;
   bool again = false;
   // of the wave, and what scores are multiplied by as weights; far (kFar): less than 0 and 1
   float slack = kSlack + T::kRoom, unit = scale2;
@@ -339,13 +339,12 @@ void attn_many_kernel(AttnParams p, int tiles) {
       if (__any(most - m > slack)) {
         most = fmaxf(most, xor_lanes<32>(most));
         const float up = fmaxf(m, most - T::kRoom);
-        const float f = up == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+        const float f = __builtin_amdgcn_exp2f(m - up);
         m = up;
-        less = up == -__builtin_inff() ? 0.0f : -up;
         l *= f;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) o[dt] *= f;
-        if (__any(is_far(up))) slack = -__builtin_inff();
+        slack = slack_at(up, slack);
         if (slack < 0.0f) {
           unit = 1.0f;
 #pragma unroll
@@ -356,7 +355,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
       }
       V8 w8, following;
       auto weight = [&](int ks, int i) __attribute__((always_inline)) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[ks / 2][8 * (ks & 1) + i], unit, less));
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[ks / 2][8 * (ks & 1) + i], unit, -m));
         l += e;
         return (typename T::E)e;
       };
@@ -421,7 +420,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
         *(float4v*)(out + 32 * dt + 8 * i + 4 * h) =
             float4v{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
     if (h == 0) {
-      p.stats[(slot0 + 32 * wave + n) * 2] = m;
+      p.stats[(slot0 + 32 * wave + n) * 2] = seen_max(m);
       p.stats[(slot0 + 32 * wave + n) * 2 + 1] = l;
     }
     return;
