@@ -150,12 +150,14 @@ struct Shape {
 
 // Few rows (decode, drafts) go to attn_few_kernel, up to 16 or 32 of them -- 32 of 256 channels
 // do not fit its registers -- others to attn_many_kernel.  Rows 17 to 32, us: 20 rows over
-// 6001 4-bit tokens 24.5 (many 26.5), 32 rows of 8 sequences over 4096 16-bit ones 36.3 (34.5).
+// 6001 4-bit tokens 24.5 (many 26.5), 32 rows of 8 sequences over 4096 16-bit ones 36.3 (34.5):
+// the border could lie between the two for 16 bits, by 5 %.
 //
 // Where the tiles leave the chip idle their tokens are split, evenly or by the batch's sum, into
 // as many workgroups as run at once: three a CU with 16 rows, two with 32 or 128, one of 256
 // channels.  (Half as many: 32 8-bit decodes 122 us instead of 95, 512 rows over 8192 107 for
-// 103; twice as many: drafts 33 for 24, 512 rows 127.)  No more than 32 of a sequence, which
+// 103, but a sequence of 4000 with fifteen of 200 17.7 for 21.3 and 64 rows over 8192 30.4 for
+// 35.8; twice as many: drafts 33 for 24, 512 rows 127.)  No more than 32 of a sequence, which
 // one launch has to join (16: one token over 131071 120 us for 105; 64: 110, of 64 channels 24
 // for 21, of 256 40 for 45), and none shorter than 128 tokens for few rows (256: one token over
 // 1000 12.2 us for 11.2) or 512 for many (256: 256 rows over 8192 36 us for 30).

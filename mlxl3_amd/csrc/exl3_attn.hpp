@@ -93,8 +93,10 @@ __device__ __forceinline__ constexpr int channel4(int e) { return (e >> 1) | ((e
 // code * scale needs up to 18 bits, an f16 has 11.  Rounded to those it is off by half as much
 // as an f16 query or output is, and a large score by many times that: with f16 queries a
 // value is two f16 -- the scale's leading bits times the code, exact, and the rest (8 bits:
-// to 2^-15) -- each with its own product.  bf16 queries' outputs are 8 times coarser, so
-// one rounded f16 is enough there.  Same box, us: 32 decodes over 8192 8-bit tokens, f16, one
+// to 2^-15) -- each with its own product.  With bf16 queries one rounded f16 is enough: the
+// outputs are 8 times coarser than its 2^-11, and so were the queries when they were rounded to
+// bf16, so that a key's part in a score's error (2^-11 of the sum of magnitudes at most) is an
+// eighth of what the query's is already.  Same box, us: 32 decodes over 8192 8-bit tokens, f16, one
 // part 86.4 (2-norm error 8.3e-4, 2.1e-4 of it the output's own rounding), two 94.5 (2.9e-4);
 // four drafts of 5 over 6001 4-bit tokens, bf16, 24.3 (1.8e-3 against 1.6e-3) and 27.6 (1.6e-3);
 // 2048 f16 rows over 8192 8-bit tokens 307 (6.7e-4) and 520 (2.9e-4).

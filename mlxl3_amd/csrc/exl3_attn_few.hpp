@@ -26,9 +26,9 @@
 // token over 131071 16-bit tokens 105 us, 5.1 TB/s; 32 f16 tokens (5 heads) over 32 sequences
 // of up to 8192 8-bit tokens 95 us, 4.0 TB/s (equally long ones 4.75, 16 bits 5.5: there
 // decoding and its two parts are 1.7e7 vector instructions, a third of the time, with no unit
-// at its limit -- 12 waves a CU and 42 % of their time waiting); drafts of 5, 4, 3 and 2
-// tokens over 6001 to 2988 4-bit tokens 24.4 us; one token over 1000 11 us, two launches and
-// a few dependent loads.
+// at its limit -- 12 waves a CU and 41 % of their time waiting), over 4 bits 75, with bf16 queries
+// 61; drafts of 5, 4, 3 and 2 tokens over 6001 to 2988 4-bit tokens 23.5 us; one token over 1000
+// 11 us, two launches and a few dependent loads.
 #pragma once
 
 #include "exl3_attn.hpp"

@@ -20,13 +20,16 @@
 // results are off by 5.3e-4 to 8.1e-4 in the 2-norm, with two by 2.9e-4, where rounding the
 // exact ones takes 2.1e-4.
 //
-// Measured (us, TFLOP/s of the products that the mask leaves): 2048 tokens over 16384 bf16
-// ones, 32 heads of 128 on 8: 506, 1020 -- a large product of the library's runs at 1238 --
+// Measured (us, TFLOP/s of the products that the mask leaves; one box): 2048 tokens over 16384
+// bf16 ones, 32 heads of 128 on 8: 496, 1040 -- a large product of the library's runs at 1238 --
 // with the matrix units busy half of the cycles and the exponentials beside them; 2048 over
-// 8192 921 TFLOP/s, 8 bits 788 in one part and 463 in two, 4 bits 799 and 402; heads of 64 701,
-// 625 / 415, 521 / 357 (half the products per exponential); of 256 627, 493 / 349, 494 / 330
-// (one workgroup a CU: its registers).  Six prompts of 496 to 1500 tokens, heads of 64, window
-// 512: 47 us, 425 TFLOP/s, masked tiles and two rounds of short workgroups.
+// 8192 bf16 998 TFLOP/s, f16 952, 8 bits 815 in one part and 477 in two, 4 bits 820 and 410; heads
+// of 64 733 to 757, 610 / 431, 514 / 370 (half the products per exponential); of 256 630, 475 / 348,
+// 486 / 337 (one workgroup a CU: its registers).  Six prompts of 496 to 1500 tokens, heads of 64,
+// window 512: 46 us, 432 TFLOP/s, masked tiles and two rounds of short workgroups.
+// Where rows are done one by one (below, values that are not finite and some rows do not see) a
+// workgroup takes its rows times its tokens: one NaN in the newest of 8192 tokens makes 2048 rows'
+// 0.29 ms 268 ms.
 #pragma once
 
 #include "exl3_attn.hpp"
