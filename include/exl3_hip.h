@@ -391,6 +391,19 @@ int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* k, const ex
                             int32_t window, const void* x, int32_t x_type, int64_t rows, void* y,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* Root-mean-square norm of the rows x[tokens][heads][width], in front of an attention block or a
+ * feed-forward, or of query and key heads: y = s / sqrt(mean(s^2) + eps) * weight with s = x or,
+ * where residual is not NULL, x + residual, which goes to total (may be NULL) rounded to
+ * residual_type; the norm is taken of the sum before it is rounded.  Types f16, bf16 or f32, each
+ * of its own; token strides in elements, heads contiguous, width at most 131072; weight [width] may
+ * be NULL (ones); eps a positive normal number.  y and total may each be x or residual (with its
+ * type and stride); else outputs do not overlap inputs or each other.  Sums are f32. */
+int exl3_rms_norm(const void* x, int32_t x_type, int64_t tokens, int32_t heads, int32_t width,
+                  int64_t x_stride, const void* weight, int32_t weight_type, float eps,
+                  const void* residual, int32_t residual_type, int64_t residual_stride,
+                  void* total, int64_t total_stride, void* y, int32_t y_type, int64_t y_stride,
+                  void* stream);
+
 /* Decode hook, the reference's `metal-decode` codec op (exl3.metal:102-109,
  * main.rs:945-967): for every tile, states[t*256 + i] (nullable) and the f16
  * bits values[t*256 + i] of state index i, in the tile's stored order. */

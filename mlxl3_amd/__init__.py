@@ -14,6 +14,7 @@ behaviour:
 * :class:`Rope`, :class:`KvCache`, :class:`KvBatch`, :func:`attention` (``kv.py``) -- rotary
   positions, the paged key/value cache and attention over it; :class:`Exl3Attention` -- the
   attention block of a decoder layer around them
+* :func:`rms_norm` (``norm.py``) -- with the residual's addition
 * :class:`Checkpoint`   -- ``checkpoint::inspect`` / ``TensorInfo`` (native/src/checkpoint.rs),
   with ``Exl3Linear.from_checkpoint`` and ``Exl3SwitchGlu.from_checkpoint``
 
@@ -50,6 +51,7 @@ __all__ = [
     "KvCache",
     "Rope",
     "attention",
+    "rms_norm",
     "rope_frequencies",
     "decode_tiles",
     "load_library",
@@ -132,6 +134,11 @@ _SIGNATURES = {
         _i32, [_vp, _vp, _i32, _i64, _i32, _i32, _i64, _vp, _vp, _vp, _i32, _i64, _vp],
     ),
     "exl3_kv_append": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _i64, _vp, _vp]),
+    "exl3_rms_norm": (
+        _i32,
+        [_vp, _i32, _i64, _i32, _i32, _i64, _vp, _i32, ctypes.c_float, _vp, _i32, _i64, _vp, _i64, _vp, _i32, _i64,
+         _vp],
+    ),
     "exl3_kv_read": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _vp]),
     "exl3_attention_workspace_bytes": (_sz, [_vp, _vp, _i64, _i32]),
     "exl3_attention": (
@@ -938,3 +945,4 @@ def decode_tiles(packed, k: int, cb: int, with_states: bool = True):
 
 
 from .kv import Exl3Attention, KvBatch, KvCache, Rope, attention, rope_frequencies  # noqa: E402
+from .norm import rms_norm  # noqa: E402
