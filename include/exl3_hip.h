@@ -353,6 +353,15 @@ int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const
 int exl3_kv_read(const exl3_kv_cache* cache, const exl3_kv_batch* batch, void* k, void* v,
                  int32_t type, int64_t tokens, void* stream);
 
+/* Copies page src[i] to page dst[i] in each of `count` caches (a model's layers), keys, values
+ * and scales, i < pairs: its first slots[i] tokens, or the whole page where slots is NULL.  The
+ * caches have as many pages of as many tokens each; heads, widths and formats may differ.  The
+ * lists are host memory, read before the call returns (in a captured graph they are those of the
+ * capture).  A page may be copied to several; one that is copied to twice, or copied and copied
+ * to, is refused. */
+int exl3_kv_copy_pages(const exl3_kv_cache* const* caches, int32_t count, const int32_t* src,
+                       const int32_t* dst, const int32_t* slots, int64_t pairs, void* stream);
+
 /* y[tokens][heads][head_dim]: every new token's query heads (head h reads
  * cache head h / (heads / kv_heads)) over its sequence's cache, which holds
  * the new tokens' keys and values already: softmax(scale q.k) v over the

@@ -14,7 +14,8 @@ behaviour:
 * :class:`Rope`, :class:`KvCache`, :class:`KvBatch`, :func:`attention` (``kv.py``) -- rotary
   positions, the paged key/value cache and attention over it; :class:`Exl3Attention` -- the
   attention block of a decoder layer around them
-* :func:`rms_norm` (``norm.py``) -- with the residual's addition
+* :class:`KvPages` (``pages.py``) -- which pages belong to which sequence: sequences forked, cut and
+  freed, pools compacted; :func:`rms_norm` (``norm.py``) -- with the residual's addition
 * :class:`Checkpoint`   -- ``checkpoint::inspect`` / ``TensorInfo`` (native/src/checkpoint.rs),
   with ``Exl3Linear.from_checkpoint`` and ``Exl3SwitchGlu.from_checkpoint``
 
@@ -49,6 +50,7 @@ __all__ = [
     "Exl3Attention",
     "KvBatch",
     "KvCache",
+    "KvPages",
     "Rope",
     "attention",
     "rms_norm",
@@ -134,6 +136,7 @@ _SIGNATURES = {
         _i32, [_vp, _vp, _i32, _i64, _i32, _i32, _i64, _vp, _vp, _vp, _i32, _i64, _vp],
     ),
     "exl3_kv_append": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _i64, _vp, _vp]),
+    "exl3_kv_copy_pages": (_i32, [_vp, _i32, _vp, _vp, _vp, _i64, _vp]),
     "exl3_rms_norm": (
         _i32,
         [_vp, _i32, _i64, _i32, _i32, _i64, _vp, _i32, ctypes.c_float, _vp, _i32, _i64, _vp, _i64, _vp, _i32, _i64,
@@ -946,3 +949,4 @@ def decode_tiles(packed, k: int, cb: int, with_states: bool = True):
 
 from .kv import Exl3Attention, KvBatch, KvCache, Rope, attention, rope_frequencies  # noqa: E402
 from .norm import rms_norm  # noqa: E402
+from .pages import KvPages  # noqa: E402
