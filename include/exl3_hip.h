@@ -380,6 +380,24 @@ int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const
                    int32_t causal, int32_t window, void* y, int64_t y_stride, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/* exl3_attention with shaped scores.  A score z = scale q.k becomes softcap tanh(z / softcap)
+ * where softcap is not 0 (2^-64 to 2^64), then slopes[head] times the distance of the
+ * row's position and the token's is taken off it (slopes finite, the sum of a score and a bias
+ * too); and with causal != 0 every row sees the first prefix[b] tokens of its sequence beside
+ * those up to its own position (t < kv_lens[b] and the window hold for them as for others).
+ * slopes (f32 [heads]) and prefix (int32 [seqs]) are device memory, read at every call, and may
+ * be NULL; so may `scores`. */
+typedef struct {
+  float softcap;
+  const float* slopes;
+  const int32_t* prefix;
+} exl3_attn_scores;
+int exl3_attention_scores(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const void* q,
+                          int32_t q_type, int64_t tokens, int32_t heads, int64_t q_stride,
+                          float scale, int32_t causal, int32_t window,
+                          const exl3_attn_scores* scores, void* y, int64_t y_stride,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 /* The attention block of a decoder layer, next to exl3_mlp_forward: q, k, v =
  * exl3_group_forward of x; k and v appended and q rotated (rope may be NULL);
  * exl3_attention with causal masking; y[rows][o.out] = exl3_linear_forward of
@@ -399,6 +417,14 @@ int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* k, const ex
                             const exl3_kv_batch* batch, const exl3_rope_spec* rope, float scale,
                             int32_t window, const void* x, int32_t x_type, int64_t rows, void* y,
                             void* workspace, size_t workspace_bytes, void* stream);
+/* The same with exl3_attention_scores in it. */
+int exl3_attn_block_forward_scores(const exl3_linear* q, const exl3_linear* k,
+                                   const exl3_linear* v, const exl3_linear* o,
+                                   const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                                   const exl3_rope_spec* rope, float scale, int32_t window,
+                                   const exl3_attn_scores* scores, const void* x, int32_t x_type,
+                                   int64_t rows, void* y, void* workspace, size_t workspace_bytes,
+                                   void* stream);
 
 /* Root-mean-square norm of the rows x[tokens][heads][width], in front of an attention block or a
  * feed-forward, or of query and key heads: y = s / sqrt(mean(s^2) + eps) * weight with s = x or,

@@ -149,6 +149,16 @@ _SIGNATURES = {
         [_vp, _vp, _vp, _i32, _i64, _i32, _i64, ctypes.c_float, _i32, _i32, _vp, _i64, _vp, _sz,
          _vp],
     ),
+    "exl3_attention_scores": (
+        _i32,
+        [_vp, _vp, _vp, _i32, _i64, _i32, _i64, ctypes.c_float, _i32, _i32, _vp, _vp, _i64, _vp, _sz,
+         _vp],
+    ),
+    "exl3_attn_block_forward_scores": (
+        _i32,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _i32, _vp, _vp, _i32, _i64, _vp, _vp, _sz,
+         _vp],
+    ),
     "exl3_attn_block_workspace_bytes": (_sz, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64]),
     "exl3_attn_block_forward": (
         _i32,

@@ -3,7 +3,8 @@
 //   y_row = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q_row . k_t - m),
 //
 // over the tokens t that the row sees: t < kv_len, causal t <= its position, window
-// t > its position - window.  m lies near the largest score so far (kSlack, kRoom): one pass
+// t > its position - window; with a prefix t < prefix too, whatever its position.  Shaped scores
+// are capped and biased first (exl3_attn.hpp).  m lies near the largest score so far (kSlack, kRoom): one pass
 // over the cache with a running maximum and sum, both f32.  A row that sees nothing gives zeros.
 //
 // The rows of a launch are (token, query head of a group) pairs: all heads that read one
@@ -14,8 +15,7 @@
 #include <cmath>
 
 #include "../../include/exl3_hip.h"
-#include "exl3_attn_few.hpp"
-#include "exl3_attn_many.hpp"
+#include "exl3_attn_launch.hpp"
 #include "exl3_kv_host.hpp"
 #include "exl3_launch.hpp"
 
@@ -28,7 +28,7 @@ namespace exl3 {
 // A split that saw nothing has a maximum of -inf and a sum of 0, and its sums, which are
 // not written, are not used.  Its latency bounds it: 5 us for 32 splits of 32 rows (a launch
 // alone takes 2 to 3), 53 before the loads went out together.
-template <int D>
+template <int D, bool S>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows, int shift) {
   constexpr int L = D / 4, kGroups = 256 / L, kBatch = 8;
   __shared__ float4v sums[kGroups][L];
@@ -38,19 +38,19 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows, 
   const int in_tile = blockIdx.x * (kGroups >> shift) + (group >> shift);
   const int kvh = blockIdx.y, tile = blockIdx.z;
   int row0;
-  const Work w = tile_work(p, tile, rows, row0);
+  const Work w = tile_work<S>(p, tile, rows, row0);
   const int row = row0 + in_tile;
   const bool live = in_tile < rows && row < w.rows;
   int count = p.splits;
   const size_t step = (size_t)p.cache.kv_heads * rows;
   size_t first = (size_t)tile * p.splits;
   if (p.budget) {  // this sequence's ranges lie behind those of the ones before
-    const int size = range_tokens(p);
-    count = range_count(size, seen_tokens(p, w));
+    const int size = range_tokens<S>(p);
+    count = range_count(size, seen_tokens<S>(p, w));
     if (count < 2) return;
     float before = 0.0f;
     for (int seq = threadIdx.x & 63; seq < tile; seq += 64)
-      before += (float)range_count(size, seen_tokens(p, sequence_work(p, seq)));
+      before += (float)range_count(size, seen_tokens<S>(p, sequence_work<S>(p, seq)));
     first = (size_t)wave_sum(before);
   }
   const size_t slot = first * step + (size_t)kvh * rows + in_tile;
@@ -106,27 +106,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows, 
 #pragma unroll
   for (int e = 0; e < 4; ++e) store1(p.y, p.q_type, yi + e, total != 0.0f ? acc[e] / total : 0.0f);
 }
-template __global__ void attn_join_kernel<64>(AttnParams, int, int);
-template __global__ void attn_join_kernel<128>(AttnParams, int, int);
-template __global__ void attn_join_kernel<256>(AttnParams, int, int);
+#define EXL3_JOIN_INST(D) \
+  template __global__ void attn_join_kernel<D, false>(AttnParams, int, int); \
+  template __global__ void attn_join_kernel<D, true>(AttnParams, int, int);
+EXL3_JOIN_INST(64) EXL3_JOIN_INST(128) EXL3_JOIN_INST(256)
 
-#define EXL3_FEW_D(M, FMT, T, PARTS)                                                      \
-  M(FMT, T, 64, 1, PARTS) M(FMT, T, 64, 2, PARTS) M(FMT, T, 128, 1, PARTS) M(FMT, T, 128, 2, PARTS) \
-  M(FMT, T, 256, 1, PARTS)
-#define EXL3_FEW(M)                                                                       \
-  EXL3_FEW_D(M, KV_F16, F16, 1) EXL3_FEW_D(M, KV_BF16, BF16, 1) EXL3_FEW_D(M, KV_Q8, F16, 1) \
-  EXL3_FEW_D(M, KV_Q8, F16, 2) EXL3_FEW_D(M, KV_Q4, F16, 1) EXL3_FEW_D(M, KV_Q4, F16, 2)
-#define EXL3_FEW_INST(FMT, T, D, RT, PARTS) \
-  template __global__ void attn_few_kernel<FMT, T, D, RT, PARTS>(AttnParams);
-EXL3_FEW(EXL3_FEW_INST)
-
-#define EXL3_MANY_D(M, FMT, T, PARTS) M(FMT, T, 64, PARTS) M(FMT, T, 128, PARTS) M(FMT, T, 256, PARTS)
-#define EXL3_MANY(M)                                                                      \
-  EXL3_MANY_D(M, KV_F16, F16, 1) EXL3_MANY_D(M, KV_BF16, BF16, 1) EXL3_MANY_D(M, KV_Q8, F16, 1) \
-  EXL3_MANY_D(M, KV_Q8, F16, 2) EXL3_MANY_D(M, KV_Q4, F16, 1) EXL3_MANY_D(M, KV_Q4, F16, 2)
-#define EXL3_MANY_INST(FMT, T, D, PARTS) \
-  template __global__ void attn_many_kernel<FMT, T, D, PARTS>(AttnParams, int);
-EXL3_MANY(EXL3_MANY_INST)
+EXL3_FEW(EXL3_FEW_INST, false)
+EXL3_MANY(EXL3_MANY_INST, false)
 
 }  // namespace exl3
 
@@ -137,16 +123,6 @@ using namespace exl3;
 namespace {
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
-
-struct Shape {
-  bool few;       // attn_few_kernel, else attn_many_kernel
-  int rows;       // rows of a workgroup
-  bool one_tile;  // every sequence's rows fit one workgroup
-  int64_t tiles;  // at most; the device counts the tiles that there are
-  int splits;     // even ranges of the tokens that a tile sees
-  int budget;     // else ranges by the batch's sum, about (as AttnParams')
-  int64_t slots;  // of partial results to join, `rows` rows each
-};
 
 // Few rows (decode, drafts) go to attn_few_kernel, up to 16 or 32 of them -- 32 of 256 channels
 // do not fit its registers -- others to attn_many_kernel.  Rows 17 to 32, us: 20 rows over
@@ -165,10 +141,10 @@ struct Shape {
 // Ranges by the sum cost every workgroup a look at all lengths, some 3 us a call (drafts 28.0
 // for 24.5), and save the wait for the longest sequence (8192 + 31 x 200 tokens 39 us to 24, 32
 // decodes of 1000 to 8192 99 to 95): from 1024 tokens a split on.
-Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int heads, int window) {
+AttnShape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int heads, int window) {
   const int group = heads / c.kv_heads;
   const int64_t rows = (int64_t)b.max_q * group;
-  Shape s;
+  AttnShape s;
   s.few = rows <= (c.head_dim == 256 ? 16 : 32);
   s.rows = s.few ? rows > 16 ? 32 : 16 : kManyRows;
   s.one_tile = rows <= s.rows;
@@ -190,40 +166,6 @@ Shape choose(const KvCacheView& c, const exl3_kv_batch& b, int64_t tokens, int h
   return s;
 }
 
-template <int FMT, typename T, int PARTS, int D, int RT>
-void launch_few(const AttnParams& p, hipStream_t s) {
-  const dim3 grid = p.budget ? dim3((unsigned)p.cache.kv_heads, (unsigned)(p.budget + p.batch.seqs + 1))
-                             : dim3((unsigned)p.cache.kv_heads, (unsigned)p.splits, (unsigned)p.batch.seqs);
-  constexpr size_t lds = 4 * (Few<FMT, T, D, RT, PARTS>::kWaveLds);
-  hipLaunchKernelGGL((attn_few_kernel<FMT, T, D, RT, PARTS>), grid, dim3(256), lds, s, p);
-}
-template <int FMT, typename T, int PARTS>
-void launch_few(const AttnParams& p, int rows, hipStream_t s) {
-  const int d = p.cache.head_dim;
-  if (rows == 16) {
-    d == 64 ? launch_few<FMT, T, PARTS, 64, 1>(p, s) : d == 128 ? launch_few<FMT, T, PARTS, 128, 1>(p, s)
-                                                                : launch_few<FMT, T, PARTS, 256, 1>(p, s);
-  } else {
-    d == 64 ? launch_few<FMT, T, PARTS, 64, 2>(p, s) : launch_few<FMT, T, PARTS, 128, 2>(p, s);
-  }
-}
-
-template <int FMT, typename T, int PARTS, int D>
-void launch_many(const AttnParams& p, int tiles, hipStream_t s) {
-  constexpr size_t lds = Many<FMT, T, D, PARTS>::kLds;
-  const dim3 grid((unsigned)tiles * p.splits * p.cache.kv_heads);
-  hipLaunchKernelGGL((attn_many_kernel<FMT, T, D, PARTS>), grid, dim3(256), lds, s, p, tiles);
-}
-template <int FMT, typename T, int PARTS>
-void launch(const AttnParams& p, const Shape& sh, hipStream_t s) {
-  const int d = p.cache.head_dim, tiles = (int)sh.tiles;
-  if (sh.few)
-    launch_few<FMT, T, PARTS>(p, sh.rows, s);
-  else
-    d == 64 ? launch_many<FMT, T, PARTS, 64>(p, tiles, s) : d == 128 ? launch_many<FMT, T, PARTS, 128>(p, tiles, s)
-                                                                     : launch_many<FMT, T, PARTS, 256>(p, tiles, s);
-}
-
 }  // namespace
 
 extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
@@ -232,7 +174,7 @@ extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
   if (!cache || !batch || tokens <= 0 || heads <= 0 || batch->seqs <= 0 || batch->max_q <= 0 ||
       batch->table_pages <= 0 || heads % cache->view.kv_heads)
     return 0;
-  const Shape sh = choose(cache->view, *batch, tokens, heads, 0);
+  const AttnShape sh = choose(cache->view, *batch, tokens, heads, 0);
   const size_t rows = (size_t)sh.slots * sh.rows;
   return align256(rows * cache->view.head_dim * 4) + align256(rows * 8);
 }
@@ -240,8 +182,9 @@ extern "C" size_t exl3_attention_workspace_bytes(const exl3_kv_cache* cache,
 // exl3_attention; without `run` its checks alone.
 static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const void* q,
                           int32_t q_type, int64_t tokens, int32_t heads, int64_t q_stride,
-                          float scale, int32_t causal, int32_t window, void* y, int64_t y_stride,
-                          void* workspace, size_t workspace_bytes, void* stream, bool run) {
+                          float scale, int32_t causal, int32_t window, const exl3_attn_scores* scores,
+                          void* y, int64_t y_stride, void* workspace, size_t workspace_bytes,
+                          void* stream, bool run) {
   if (!cache) return fail(EXL3_EINVAL, "null KV cache");
   AttnParams p{};
   p.cache = cache->view;
@@ -257,6 +200,15 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
   if (!(scale > 0.0f) || !std::isfinite(scale2))
     return fail(EXL3_EINVAL, "attention scale must be positive and finite");
   if (window < 0) return fail(EXL3_EINVAL, "negative attention window %d", window);
+  if (scores) {
+    const float cap = scores->softcap;
+    if (cap != 0.0f && !(cap >= 0x1p-64f && cap <= 0x1p64f))
+      return fail(EXL3_EINVAL, "attention softcap must be 0 or 2^-64 to 2^64, got %g", cap);
+    p.cap2 = cap * kLog2e;
+    p.slopes = scores->slopes;
+    p.prefix = causal ? scores->prefix : nullptr;
+  }
+  const bool shaped = p.cap2 != 0.0f || p.slopes || p.prefix;
   if (batch->max_q < 1) return fail(EXL3_EINVAL, "max_q must be positive");
   if (batch->seqs > 65535)
     return fail(EXL3_EUNSUPPORTED, "attention takes up to 65535 sequences, got %d", batch->seqs);
@@ -274,7 +226,8 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
     return fail(EXL3_EINVAL, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
   if (need && !aligned16(workspace))
     return fail(EXL3_EINVAL, "attention workspace must be 16-byte aligned");
-  const Shape sh = choose(p.cache, *batch, tokens, heads, window);
+  // (a prefix may lie any number of tokens behind a window)
+  const AttnShape sh = choose(p.cache, *batch, tokens, heads, p.prefix ? 0 : window);
   if (sh.tiles * sh.splits * p.cache.kv_heads > kMostBlocks)
     return fail(EXL3_EUNSUPPORTED, "attention of %lld tokens needs too many workgroups", (long long)tokens);
   if (!run) return EXL3_OK;
@@ -299,13 +252,10 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
   const int D = p.cache.head_dim;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = launch_gate("attention")) return rc;
-  const bool fine = q_type == EXL3_F16;  // coded values in two parts
-  switch (p.cache.format) {
-    case EXL3_KV_F16: launch<KV_F16, F16, 1>(p, sh, s); break;
-    case EXL3_KV_BF16: launch<KV_BF16, BF16, 1>(p, sh, s); break;
-    case EXL3_KV_Q8: fine ? launch<KV_Q8, F16, 2>(p, sh, s) : launch<KV_Q8, F16, 1>(p, sh, s); break;
-    default: fine ? launch<KV_Q4, F16, 2>(p, sh, s) : launch<KV_Q4, F16, 1>(p, sh, s);
-  }
+  if (shaped)
+    launch_attention_shaped(p, sh, s);
+  else
+    launch_attention<false>(p, sh, s);
   if (int rc = check_launch("attention")) return rc;
   if (!sh.slots) return EXL3_OK;
   if (int rc = launch_gate("attention join")) return rc;
@@ -317,12 +267,13 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
   const int per_block = groups >> shift;
   const dim3 grid((unsigned)((rows_most + per_block - 1) / per_block), (unsigned)p.cache.kv_heads,
                   (unsigned)sh.tiles);
-  if (D == 64)
-    hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(256), 0, s, p, sh.rows, shift);
-  else if (D == 128)
-    hipLaunchKernelGGL(attn_join_kernel<128>, grid, dim3(256), 0, s, p, sh.rows, shift);
+  auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, p, sh.rows, shift); };
+  if (shaped)
+    D == 64 ? join(attn_join_kernel<64, true>) : D == 128 ? join(attn_join_kernel<128, true>)
+                                                          : join(attn_join_kernel<256, true>);
   else
-    hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(256), 0, s, p, sh.rows, shift);
+    D == 64 ? join(attn_join_kernel<64, false>) : D == 128 ? join(attn_join_kernel<128, false>)
+                                                           : join(attn_join_kernel<256, false>);
   return check_launch("attention join");
 }
 
@@ -331,7 +282,16 @@ extern "C" int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* b
                               int64_t q_stride, float scale, int32_t causal, int32_t window,
                               void* y, int64_t y_stride, void* workspace, size_t workspace_bytes,
                               void* stream) {
-  return attention_call(cache, batch, q, q_type, tokens, heads, q_stride, scale, causal, window, y, y_stride,
+  return attention_call(cache, batch, q, q_type, tokens, heads, q_stride, scale, causal, window, nullptr, y, y_stride,
+                        workspace, workspace_bytes, stream, true);
+}
+
+extern "C" int exl3_attention_scores(const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                                     const void* q, int32_t q_type, int64_t tokens, int32_t heads,
+                                     int64_t q_stride, float scale, int32_t causal, int32_t window,
+                                     const exl3_attn_scores* scores, void* y, int64_t y_stride,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_call(cache, batch, q, q_type, tokens, heads, q_stride, scale, causal, window, scores, y, y_stride,
                         workspace, workspace_bytes, stream, true);
 }
 
@@ -388,12 +348,13 @@ extern "C" size_t exl3_attn_block_workspace_bytes(const exl3_linear* q, const ex
   return plan_block(q, k, v, o, cache, batch, x_type, rows, &b) ? 0 : b.total;
 }
 
-extern "C" int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* k,
-                                       const exl3_linear* v, const exl3_linear* o,
-                                       const exl3_kv_cache* cache, const exl3_kv_batch* batch,
-                                       const exl3_rope_spec* rope, float scale, int32_t window,
-                                       const void* x, int32_t x_type, int64_t rows, void* y,
-                                       void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int exl3_attn_block_forward_scores(const exl3_linear* q, const exl3_linear* k,
+                                              const exl3_linear* v, const exl3_linear* o,
+                                              const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                                              const exl3_rope_spec* rope, float scale, int32_t window,
+                                              const exl3_attn_scores* scores, const void* x,
+                                              int32_t x_type, int64_t rows, void* y, void* workspace,
+                                              size_t workspace_bytes, void* stream) {
   Block b;
   if (int rc = plan_block(q, k, v, o, cache, batch, x_type, rows, &b)) return rc;
   if (!x || !y) return fail(EXL3_EINVAL, "null attention block input or output");
@@ -419,7 +380,7 @@ extern "C" int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* 
     return append_call(cache, batch, qkv[1], narrow, qkv[2], narrow, b.types[1], rows, rope, stream, run);
   };
   auto attend = [&](bool run) {
-    return attention_call(cache, batch, query, x_type, rows, b.heads, wide, scale, 1, window, query, wide,
+    return attention_call(cache, batch, query, x_type, rows, b.heads, wide, scale, 1, window, scores, query, wide,
                           ws + b.attention, b.total - b.attention, stream, run);
   };
   // what a later part would refuse is refused before the first one's launch (the group's own
@@ -434,6 +395,16 @@ extern "C" int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* 
   if (int rc = attend(true)) return rc;
   return exl3_linear_forward(o, query, x_type, rows, y, exl3_linear_output_dtype(o, x_type), ws, b.linear,
                              stream);
+}
+
+extern "C" int exl3_attn_block_forward(const exl3_linear* q, const exl3_linear* k,
+                                       const exl3_linear* v, const exl3_linear* o,
+                                       const exl3_kv_cache* cache, const exl3_kv_batch* batch,
+                                       const exl3_rope_spec* rope, float scale, int32_t window,
+                                       const void* x, int32_t x_type, int64_t rows, void* y,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+  return exl3_attn_block_forward_scores(q, k, v, o, cache, batch, rope, scale, window, nullptr, x, x_type, rows, y,
+                                        workspace, workspace_bytes, stream);
 }
 
 #endif  // __HIP_DEVICE_COMPILE__

@@ -22,6 +22,10 @@ struct AttnParams {
   int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
   int q_vec, y_vec;  // rows of q are 16-byte, rows of y 8-byte aligned
   float scale2;   // scale * log2(e): scores in units of a factor of two
+  // of calls with shaped scores (the kernels' S): cap2 = cap * log2(e), 0 without a cap
+  float cap2;
+  const float* slopes;    // of every head, or null
+  const int32_t* prefix;  // of every sequence, or null
 };
 
 typedef float float16v __attribute__((ext_vector_type(16)));
@@ -161,25 +165,15 @@ __device__ __forceinline__ typename T::V8 query_operand(const u32x4& w, float fa
   return __builtin_bit_cast(typename T::V8, r);
 }
 
-// The tokens that row `row` (token row / group of the sequence) may see: [lo, hi).
-struct Seen {
-  int lo, hi;
-};
-__device__ __forceinline__ Seen row_sees(const AttnParams& p, int first, int len, int row) {
-  const int64_t pos = (int64_t)first + row / p.group;
-  Seen s{0, len};
-  if (p.causal) s.hi = (int)max((int64_t)0, min((int64_t)len, pos + 1));
-  if (p.window > 0) s.lo = (int)min((int64_t)len, max((int64_t)0, pos - p.window + 1));
-  return s;
-}
-
 // What a workgroup works on: sequence, its first row of the call's tensors, rows
 // (tokens x heads of the group), first new position, length cut to the table's room.  Rows
 // that q does not have are not touched, whatever q_starts says.
 struct Work {
   int seq, start, rows, first, len;
+  int prefix;            // tokens that all rows see (S)
   const int32_t* table;  // the sequence's row of the block table
 };
+template <bool S>
 __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
   Work w;
   w.seq = seq;
@@ -191,8 +185,22 @@ __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
   const int64_t room = (int64_t)p.batch.table_pages << p.cache.page_shift;
   w.len = (int)max((int64_t)0, min(min((int64_t)kv, room), (int64_t)INT32_MAX - 4095));
   w.first = (int)max((int64_t)INT32_MIN, (int64_t)kv - n);
+  w.prefix = S && p.prefix ? p.prefix[seq] : 0;
   w.table = p.batch.table + (int64_t)seq * p.batch.table_pages;
   return w;
+}
+
+// The tokens that row `row` (token row / group of the sequence) may see: [lo, hi).
+struct Seen {
+  int lo, hi;
+};
+template <bool S>
+__device__ __forceinline__ Seen row_sees(const AttnParams& p, const Work& w, int row) {
+  const int64_t pos = (int64_t)w.first + row / p.group, len = w.len;
+  Seen s{0, w.len};
+  if (p.causal) s.hi = (int)max((int64_t)0, min(len, S ? max(pos + 1, (int64_t)w.prefix) : pos + 1));
+  if (p.window > 0) s.lo = (int)min(len, max((int64_t)0, pos - p.window + 1));
+  return s;
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -207,12 +215,12 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // The sequence that item `i` belongs to, `items` telling how many each has; i becomes its
 // number there.  Behind the last item: no rows.  Every lane of a wave calls it with one i.
-template <typename F>
+template <bool S, typename F>
 __device__ __forceinline__ Work work_of(const AttnParams& p, int& i, F&& items) {
   const int lane = threadIdx.x & 63;
   for (int s0 = 0; s0 < p.batch.seqs; s0 += 64) {
     const int seq = s0 + lane;
-    const Work x = seq < p.batch.seqs ? sequence_work(p, seq) : Work{};
+    const Work x = seq < p.batch.seqs ? sequence_work<S>(p, seq) : Work{};
     const int mine = seq < p.batch.seqs ? items(x) : 0;
     int upto = mine;
 #pragma unroll
@@ -225,7 +233,7 @@ __device__ __forceinline__ Work work_of(const AttnParams& p, int& i, F&& items) 
       const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
       i -= __builtin_amdgcn_readlane(upto - mine, at);
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
-      return Work{s0 + at, of(x.start), of(x.rows), of(x.first), of(x.len),
+      return Work{s0 + at, of(x.start), of(x.rows), of(x.first), of(x.len), S ? of(x.prefix) : 0,
                   p.batch.table + (int64_t)(s0 + at) * p.batch.table_pages};
     }
     i -= __builtin_amdgcn_readlane(upto, 63);
@@ -235,10 +243,11 @@ __device__ __forceinline__ Work work_of(const AttnParams& p, int& i, F&& items) 
 
 // Sequence and first row of tile `tile`, sequences cut into tiles of `rows` rows; a tile
 // behind the last has no rows.
+template <bool S>
 __device__ __forceinline__ Work tile_work(const AttnParams& p, int tile, int rows, int& row0) {
   row0 = 0;
-  if (p.one_tile) return sequence_work(p, tile);
-  const Work w = work_of(p, tile, [&](const Work& x) { return (x.rows + rows - 1) / rows; });
+  if (p.one_tile) return sequence_work<S>(p, tile);
+  const Work w = work_of<S>(p, tile, [&](const Work& x) { return (x.rows + rows - 1) / rows; });
   row0 = tile * rows;
   return w;
 }
@@ -260,10 +269,11 @@ __device__ __forceinline__ int split_tokens(const AttnParams& p, int n) {
   return (int)max(((uint32_t)(n + p.splits - 1) / p.splits + 127) & ~127u, 128u);
 }
 // The tokens that a sequence's rows see, from a multiple of 16 on; a sequence with rows has one.
+template <bool S>
 __device__ __forceinline__ int seen_tokens(const AttnParams& p, const Work& w) {
   if (w.rows == 0) return 0;
-  const int lo = row_sees(p, w.first, w.len, 0).lo & ~15;
-  return max(row_sees(p, w.first, w.len, w.rows - 1).hi - lo, 1);
+  const int lo = row_sees<S>(p, w, 0).lo & ~15;
+  return max(row_sees<S>(p, w, w.rows - 1).hi - lo, 1);
 }
 
 // A batch of few rows split by its sum: ranges of equally many tokens for all sequences, longer
@@ -272,11 +282,12 @@ __device__ __forceinline__ int seen_tokens(const AttnParams& p, const Work& w) {
 // ranges, at most budget + seqs (a sequence's last one may be short).
 constexpr int kMostRanges = 32;  // of a sequence: a row's ranges are joined by few lanes
 // The tokens of a range, by the batch (a wave calls it) and by the sequence's own.
+template <bool S>
 __device__ __forceinline__ int range_tokens(const AttnParams& p) {
   float total = 0.0f;
   for (int s0 = 0; s0 < p.batch.seqs; s0 += 64) {
     const int seq = s0 + (threadIdx.x & 63);
-    if (seq < p.batch.seqs) total += (float)seen_tokens(p, sequence_work(p, seq));
+    if (seq < p.batch.seqs) total += (float)seen_tokens<S>(p, sequence_work<S>(p, seq));
   }
   total = wave_sum(total);
   return __builtin_amdgcn_readfirstlane(((int)fminf(total / p.budget, 2147483392.0f) + 128) & ~127);
@@ -315,10 +326,44 @@ __device__ __forceinline__ float slack_at(float m, float slack) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s)));
 }
 
+// Shaped scores: x is a score in factors of two, s scale log2(e).
+//
+// Capped it is cap2 tanh(x / cap2): a score z becomes cap tanh(z / cap).  tanh(u) = 1 - 2 / (1 + e^2u)
+// is off by 2^-23 or so whatever u, the capped score by cap2 times that, 1e-5 under a cap of 50.
+// Above a cap of 1024 that is too much for small scores: |u| < 1/4 takes tanh's series there.
+//
+// Where no |u| of a wave's scores is above kNear (scores up to 25 under a cap of 50) all of them are
+// x (1 + v (a + v (b + v c))), v = u^2, off by 6.5e-7 of themselves: six instructions instead of
+// two transcendentals, which go at a quarter of the rate, and three more.
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNear = 0.5f;
+struct Cap {
+  float cap2, inv, inv2, rate, near;
+  bool large;
+  __device__ __forceinline__ explicit Cap(float c)
+      : cap2(c), inv(1.0f / c), inv2(inv * inv), rate(2.0f * kLog2e * inv), near(c * kNear), large(c > 1024.0f * kLog2e) {
+    if (large) near = 0.0f;  // not taken
+  }
+  __device__ __forceinline__ float small(float x) const {
+    const float v = x * x * inv2;
+    return x * fmaf(v, fmaf(v, fmaf(v, -0.04475063f, 0.13205359f), -0.33328159f), 1.0f);
+  }
+  __device__ __forceinline__ float any(float x) const {
+    const float far = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * rate)), cap2);
+    if (!large) return far;
+    const float u = x * inv, v = u * u;
+    const float series =
+        fmaf(v, fmaf(v, fmaf(v, fmaf(v, 0.021869489f, -0.053968254f), 0.13333333f), -0.33333333f), 1.0f);
+    return fabsf(u) < 0.25f ? x * series : far;
+  }
+};
+// The bias by distance: slope2 = slope log2(e) times it off the score.
+__device__ __forceinline__ float biased(float x, float slope2, float away) { return fmaf(-slope2, fabsf(away), x); }
+
 // One row over the tokens [lo, hi) by one wave, its channels spread over the lanes (lane
 // l holds channels E l ..): running maximum m, sum l and weighted values acc.  Touches
 // only tokens that the row sees.
-template <int E>
+template <int E, bool S>
 __device__ __forceinline__ void row_pass(const AttnParams& p, const Work& w, int kvh, int row, int lo, int hi,
                                          int lane, float& m, float& l, float (&acc)[E]) {
   const KvCacheView& c = p.cache;
@@ -362,6 +407,10 @@ __device__ __forceinline__ void row_pass(const AttnParams& p, const Work& w, int
       s += q[e] * k;
     }
     s = wave_sum(s) * p.scale2;
+    if constexpr (S) {
+      if (p.cap2 > 0.0f) s = Cap(p.cap2).any(s);
+      if (p.slopes) s = biased(s, p.slopes[kvh * p.group + row % p.group] * kLog2e, (float)((int64_t)w.first + row / p.group - t));
+    }
     const float n = fmaxf(m, s);
     const float base = n == -__builtin_inff() ? 0.0f : n;
     const float f = exp2f(m - base), x = exp2f(s - base);

@@ -203,7 +203,7 @@ struct Few {
 
 // grid (kv heads, splits, sequences) or (kv heads, ranges by the batch's sum): ranges that there
 // are come before those left over, which would take the place of others on a CU
-template <int FMT, typename T, int D, int RT, int PARTS>
+template <int FMT, typename T, int D, int RT, int PARTS, bool S>
 __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_kernel(AttnParams p) {
   typedef Few<FMT, T, D, RT, PARTS> F;
   typedef typename T::V8 V8;
@@ -215,16 +215,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   int part = blockIdx.y, size = INT32_MAX & ~127;
   Work w;
   if (p.budget) {
-    size = range_tokens(p);
-    w = work_of(p, part, [&](const Work& x) { return range_count(size, seen_tokens(p, x)); });
+    size = range_tokens<S>(p);
+    w = work_of<S>(p, part, [&](const Work& x) { return range_count(size, seen_tokens<S>(p, x)); });
   } else {
-    w = sequence_work(p, blockIdx.z);
+    w = sequence_work<S>(p, blockIdx.z);
   }
   if (w.rows == 0) return;
-  const Seen top = row_sees(p, w.first, w.len, 0), end = row_sees(p, w.first, w.len, w.rows - 1);
+  const Seen top = row_sees<S>(p, w, 0), end = row_sees<S>(p, w, w.rows - 1);
   // rows see later tokens the later they are: the union is [top.lo, end.hi), what all see
   // [end.lo, top.hi)
-  const int seen = seen_tokens(p, w);
+  const int seen = seen_tokens<S>(p, w);
   size = p.budget ? range_tokens(size, seen) : p.splits > 1 ? split_tokens(p, seen) : size;
   const bool whole = p.budget ? seen <= size : p.splits == 1;  // the result is final
   const size_t slot0 = ((size_t)(blockIdx.z * gridDim.y + blockIdx.y) * p.cache.kv_heads + kvh) * (16 * RT);
@@ -243,13 +243,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   V8 q[RT][F::kSteps];
   float scale2[RT];  // the call's, of rows that were scaled times the inverse
   Seen see[RT];
+  float slope2[RT];  // of shaped scores: the row's bias,
+  int at[RT];        // its position less this lane's first token of a step
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int row = rt * 16 + n;
     const int r = row < w.rows ? row : 0;  // rows past the last repeat the first; nobody reads them
-    see[rt] = row_sees(p, w.first, w.len, r);
+    see[rt] = row_sees<S>(p, w, r);
     const size_t qi =
         (size_t)(w.start + r / p.group) * p.q_stride + (size_t)(kvh * p.group + r % p.group) * D;
+    if constexpr (S) {
+      slope2[rt] = p.slopes ? p.slopes[kvh * p.group + r % p.group] * kLog2e : 0.0f;
+      at[rt] = w.first + r / p.group - 4 * g;
+    }
     u32x4 raw[F::kSteps];
     float factor = 1.0f, most = 0.0f;
     scale2[rt] = p.scale2;
@@ -280,7 +286,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   // of the wave, and what scores are multiplied by as weights; far (kFar): less than 0 and 1
   float slack = kSlack + T::kRoom, unit[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) unit[rt] = scale2[rt];
+  for (int rt = 0; rt < RT; ++rt) unit[rt] = S ? 1.0f : scale2[rt];
+  const Cap cap(S ? p.cap2 : 1.0f);
 
   typename F::Keys k;
   typename F::Values v;
@@ -343,16 +350,38 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     for (int rt = 0; rt < RT; ++rt) {
       float x[8], most = -__builtin_inff();
 #pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = s[rt][i >> 2][i & 3];
+      if constexpr (S) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= scale2[rt];
+        if (p.cap2 > 0.0f) {
+          float far = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) far = fmaxf(far, fabsf(x[i]));
+          if (__any(far > cap.near)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = cap.any(x[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = cap.small(x[i]);
+          }
+        }
+        if (p.slopes) {
+          const float away = (float)(at[rt] - t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = biased(x[i], slope2[rt], away - (float)((i >> 2) * 16 + (i & 3)));
+        }
+      }
+#pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = s[rt][i >> 2][i & 3];
         if (edge) {
-          const int at = t + (i >> 2) * 16 + 4 * g + (i & 3);
-          const bool live = at >= see[rt].lo && at < min(see[rt].hi, t1) && ((i >> 2) ? on1 : on0);
+          const int token = t + (i >> 2) * 16 + 4 * g + (i & 3);
+          const bool live = token >= see[rt].lo && token < min(see[rt].hi, t1) && ((i >> 2) ? on1 : on0);
           x[i] = live ? x[i] : -__builtin_inff();
         }
         most = fmaxf(most, x[i]);
       }
-      most *= scale2[rt];
+      if constexpr (!S) most *= scale2[rt];
       if (__any(most - m[rt] > slack)) {
         most = fmaxf(most, xor_lanes<16>(most));
         most = fmaxf(most, xor_lanes<32>(most));
@@ -362,8 +391,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         l[rt] *= f;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
-        slack = slack_at(up, slack);
-        if (slack < 0.0f) {
+        if constexpr (!S) slack = slack_at(up, slack);
+        if (!S && slack < 0.0f) {
           unit[rt] = 1.0f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] *= scale2[rt];
@@ -419,8 +448,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     for (int row = wave; row < 16 * RT; row += 4) {
       float rm = -__builtin_inff(), rl = 0.0f, acc[E] = {};
       if (row < w.rows) {
-        const Seen s = row_sees(p, w.first, w.len, row);
-        row_pass<E>(p, w, kvh, row, max(s.lo, t0), min(s.hi, t1), lane, rm, rl, acc);
+        const Seen s = row_sees<S>(p, w, row);
+        row_pass<E, S>(p, w, kvh, row, max(s.lo, t0), min(s.hi, t1), lane, rm, rl, acc);
       }
       for (int o4 = 0; o4 < 4; ++o4) {
         if (lane == 0) {

@@ -159,7 +159,7 @@ struct Many {
 
 // One-dimensional grid of tiles x splits x kv heads, the heads fastest (blocks go to the
 // XCDs in turn, so a head's tiles share few L2s), a sequence's last and longest tiles first.
-template <int FMT, typename T, int D, int PARTS>
+template <int FMT, typename T, int D, int PARTS, bool S>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(Many<FMT, T, D, PARTS>::kGroups, Many<FMT, T, D, PARTS>::kGroups)))
 void attn_many_kernel(AttnParams p, int tiles) {
@@ -172,10 +172,10 @@ void attn_many_kernel(AttnParams p, int tiles) {
   const int kvh = blockIdx.x % p.cache.kv_heads, rest = blockIdx.x / p.cache.kv_heads;
   const int split = rest % p.splits, tile = tiles - 1 - rest / p.splits;
   int row0;
-  const Work w = tile_work(p, tile, kManyRows, row0);
+  const Work w = tile_work<S>(p, tile, kManyRows, row0);
   const int rows = min(w.rows - row0, kManyRows);
   if (rows <= 0) return;
-  const Seen top = row_sees(p, w.first, w.len, row0), end = row_sees(p, w.first, w.len, row0 + rows - 1);
+  const Seen top = row_sees<S>(p, w, row0), end = row_sees<S>(p, w, row0 + rows - 1);
   const int lo = top.lo & ~15, seen = max(end.hi - lo, 0), size = split_tokens(p, seen);
   const int t0 = (int)min((int64_t)lo + (int64_t)split * size, (int64_t)INT32_MAX - 4095);
   const int t1 = (int)min((int64_t)t0 + size, (int64_t)end.hi);
@@ -192,9 +192,9 @@ void attn_many_kernel(AttnParams p, int tiles) {
   const int wrow = row0 + 32 * wave;
   const bool busy = 32 * wave < rows;
   const int mine = min(wrow + n, row0 + rows - 1);  // rows past the last repeat it; nobody reads them
-  const Seen see = row_sees(p, w.first, w.len, mine);
-  const Seen wtop = row_sees(p, w.first, w.len, min(wrow, row0 + rows - 1));
-  const Seen wend = row_sees(p, w.first, w.len, min(wrow + 31, row0 + rows - 1));
+  const Seen see = row_sees<S>(p, w, mine);
+  const Seen wtop = row_sees<S>(p, w, min(wrow, row0 + rows - 1));
+  const Seen wend = row_sees<S>(p, w, min(wrow + 31, row0 + rows - 1));
   V8 q[D / 16];
   float scale2 = p.scale2;  // of rows that were scaled times the inverse
   {
@@ -216,13 +216,17 @@ void attn_many_kernel(AttnParams p, int tiles) {
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) q[s] = query_operand<FMT == KV_Q4 ? KV_Q8 : FMT, T, kScaled>(raw[s], factor);
   }
+  // of shaped scores: the row's bias, its position less this lane's first token of a tile
+  const float slope2 = S && p.slopes ? p.slopes[kvh * p.group + mine % p.group] * kLog2e : 0.0f;
+  const int at = w.first + mine / p.group - 4 * h;
+  const Cap cap(S ? p.cap2 : 1.0f);
   float16v o[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
   float m = kNothing, l = 0.0f;
   bool again = false;
   // of the wave, and what scores are multiplied by as weights; far (kFar): less than 0 and 1
-  float slack = kSlack + T::kRoom, unit = scale2;
+  float slack = kSlack + T::kRoom, unit = S ? 1.0f : scale2;
 
   typename F::Loads x;
   const int off = F::kMine * wave;  // of this wave's rows in a tile
@@ -313,6 +317,37 @@ void attn_many_kernel(AttnParams p, int tiles) {
       for (int i = 0; i < DT; ++i) vf[i] = value(i);
       pin();
       __builtin_amdgcn_s_setprio(0);
+      if constexpr (S) {
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[a][i] *= scale2;
+        if (p.cap2 > 0.0f) {
+          float far = 0.0f;
+#pragma unroll
+          for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) far = fmaxf(far, fabsf(s[a][i]));
+          if (__any(far > cap.near)) {
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[a][i] = cap.any(s[a][i]);
+          } else {
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[a][i] = cap.small(s[a][i]);
+          }
+        }
+        if (p.slopes) {
+          const float away = (float)(at - t);
+#pragma unroll
+          for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[a][i] = biased(s[a][i], slope2, away - (float)(32 * a + 8 * (i / 4) + i % 4));
+        }
+      }
       if (t < wend.lo || t + TK > min(wtop.hi, t1)) {
         // token r of the tile is one of the row's `n` from `lo` on
         const int lo = see.lo - t - 4 * h, n = max(min(see.hi, t1) - see.lo, 0);
@@ -338,7 +373,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
       for (int a = 0; a < NT; ++a)
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, s[a][i]);
-      most *= scale2;
+      if constexpr (!S) most *= scale2;
       if (__any(most - m > slack)) {
         most = fmaxf(most, xor_lanes<32>(most));
         const float up = fmaxf(m, most - T::kRoom);
@@ -347,8 +382,8 @@ void attn_many_kernel(AttnParams p, int tiles) {
         l *= f;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) o[dt] *= f;
-        slack = slack_at(up, slack);
-        if (slack < 0.0f) {
+        if constexpr (!S) slack = slack_at(up, slack);
+        if (!S && slack < 0.0f) {
           unit = 1.0f;
 #pragma unroll
           for (int a = 0; a < NT; ++a)
@@ -395,9 +430,9 @@ void attn_many_kernel(AttnParams p, int tiles) {
     constexpr int E = D / 64;
     for (int r = wave; r < rows; r += 4) {
       const int row = row0 + r;
-      const Seen s = row_sees(p, w.first, w.len, row);
+      const Seen s = row_sees<S>(p, w, row);
       float rm, rl, acc[E];
-      row_pass<E>(p, w, kvh, row, max(s.lo, t0), min(s.hi, t1), lane, rm, rl, acc);
+      row_pass<E, S>(p, w, kvh, row, max(s.lo, t0), min(s.hi, t1), lane, rm, rl, acc);
       const size_t yi = (size_t)(w.start + row / p.group) * p.y_stride +
                         (size_t)(kvh * p.group + row % p.group) * D + E * lane;
       for (int e = 0; e < E; ++e) {

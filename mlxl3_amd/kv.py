@@ -1,6 +1,7 @@
 """What lies between a layer's q/k/v projections and its output projection: rotary
 positions, the paged key/value cache and attention over it (``exl3_rope``,
-``exl3_kv_append``, ``exl3_kv_read``, ``exl3_attention`` of ``include/exl3_hip.h``).
+``exl3_kv_append``, ``exl3_kv_read``, ``exl3_attention``, ``exl3_attention_scores`` of
+``include/exl3_hip.h``).
 
 * :class:`KvBatch`   -- the sequences of a call: new tokens, lengths, block table
 * :class:`Rope`, :func:`rope_frequencies` -- rotary positions and their frequencies
@@ -43,6 +44,14 @@ class _RopeC(ctypes.Structure):
         ("rotary_dim", ctypes.c_int32),
         ("interleaved", ctypes.c_int32),
         ("scale", ctypes.c_double),
+    ]
+
+
+class _ScoresC(ctypes.Structure):
+    _fields_ = [
+        ("softcap", ctypes.c_float),
+        ("slopes", _vp),
+        ("prefix", _vp),
     ]
 
 
@@ -396,14 +405,40 @@ def _window(window) -> int:
     return int(window)
 
 
+def _scores(device, heads: int, seqs: int, softcap, slopes, prefix):
+    """The C form of shaped scores, or None without any."""
+    try:
+        softcap = float(softcap)
+    except (TypeError, ValueError):
+        raise Exl3Error(-1, f"attention softcap must be a number, got {softcap!r}") from None
+    if slopes is not None:
+        _plain(slopes, "slopes", (_torch().float32,), 1)
+        if slopes.numel() != heads:
+            raise Exl3Error(-1, f"{slopes.numel()} slopes for {heads} heads")
+        _same(device, slopes, "slopes")
+    if prefix is not None:
+        _plain(prefix, "prefix", (_torch().int32,), 1)
+        if prefix.numel() != seqs:
+            raise Exl3Error(-1, f"{prefix.numel()} prefixes for {seqs} sequences")
+        _same(device, prefix, "prefix")
+    if softcap == 0.0 and slopes is None and prefix is None:
+        return None
+    return _ScoresC(softcap, _ptr(slopes), _ptr(prefix))
+
+
 def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, causal: bool = True,
-              window: int = 0, out=None, workspace=None):
+              window: int = 0, out=None, workspace=None, softcap: float = 0.0, slopes=None, prefix=None):
     """Attention of the batch's new tokens over the cache (``exl3_attention``): q
     [tokens, heads, head_dim] (f16 or bf16, the cache's type where it is 16-bit) -> the
     same shape and type.  scale defaults to 1 / sqrt(head_dim); causal: a token sees the
     positions up to its own; window > 0: only the last `window` of them.  `out` may be q and is
     apart from it else.  Rows outside every sequence and past the batch's max_q are not
-    written (in a new tensor they hold anything)."""
+    written (in a new tensor they hold anything).
+
+    Shaped scores (``exl3_attention_scores``): softcap > 0: a score z = scale q.k becomes
+    softcap * tanh(z / softcap); slopes (f32 [heads], finite): then slope times the distance of
+    the token's position and the row's is taken off it; prefix (int32 [seqs], with causal): every
+    row sees the first prefix[b] tokens of its sequence too, as far as the window lets it."""
     torch = _torch()
     _floats()
     q = _heads(q, "q", _HALVES)
@@ -432,9 +467,17 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
         room = workspace.numel()
     if workspace is not None:
         space = workspace.data_ptr()
-    _launch(device, load_library().exl3_attention, cache._handle, batch._attended(n), q.data_ptr(), _HALVES[q.dtype],
-            n, heads, q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, window,
-            out.data_ptr(), out.stride(0), space, room)
+    shape = None
+    if slopes is not None or prefix is not None or softcap != 0.0:
+        shape = _scores(device, heads, batch.seqs, softcap, slopes, prefix)
+    if shape is None:
+        _launch(device, load_library().exl3_attention, cache._handle, batch._attended(n), q.data_ptr(), _HALVES[q.dtype],
+                n, heads, q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0, window,
+                out.data_ptr(), out.stride(0), space, room)
+    else:
+        _launch(device, load_library().exl3_attention_scores, cache._handle, batch._attended(n), q.data_ptr(),
+                _HALVES[q.dtype], n, heads, q.stride(0), dim**-0.5 if scale is None else float(scale), 1 if causal else 0,
+                window, ctypes.byref(shape), out.data_ptr(), out.stride(0), space, room)
     return out
 
 
@@ -444,10 +487,11 @@ _MOST_STREAMS = 40  # that a block keeps a workspace for; PyTorch's own pool has
 class Exl3Attention:
     """The attention block of a decoder layer (``exl3_attn_block_forward``): the q/k/v
     projections of x as a group, keys rotated and appended with the values, queries rotated,
-    causal attention over the cache, the o projection."""
+    causal attention over the cache (softcap and slopes as :func:`attention` takes them), the o
+    projection."""
 
     def __init__(self, q: Exl3Linear, k: Exl3Linear, v: Exl3Linear, o: Exl3Linear, rope: Optional[Rope] = None,
-                 scale: Optional[float] = None, window: int = 0):
+                 scale: Optional[float] = None, window: int = 0, softcap: float = 0.0, slopes=None):
         if len({(m.in_features, m.k, m.cb) for m in (q, k, v)}) != 1:
             raise Exl3Error(-1, "incompatible grouped projections")
         if o.in_features != q.out_features or k.out_features != v.out_features:
@@ -461,6 +505,7 @@ class Exl3Attention:
                     raise Exl3Error(-1, f"projection {name} is on {at}, others on {self.device}")
                 self.device = at
         self.rope, self.scale, self.window = rope, scale, _window(window)
+        self.softcap, self.slopes = softcap, slopes
         self._ws: dict = {}  # (lock, workspace) by stream, the last used one last
         self._ws_lock = threading.Lock()
 
@@ -485,13 +530,13 @@ class Exl3Attention:
                 del self._ws[next(iter(self._ws))]
         return kept
 
-    def forward(self, x, cache: KvCache, batch: KvBatch, workspace=None):
+    def forward(self, x, cache: KvCache, batch: KvBatch, workspace=None, prefix=None):
         """x [rows, in] (f16 or bf16) -> [rows, out] in the o projection's result dtype;
         the cache's pages get the rows' keys and values.  `workspace`: a zero-filled uint8
         tensor of :meth:`workspace_bytes`, of which two calls that run at once need one each;
         by default one that the block keeps for the stream (threads on one stream take turns), and
         in a captured graph one of the graph's, all of which every replay clears first (a given
-        one saves that)."""
+        one saves that).  `prefix`: as :func:`attention` takes it."""
         torch = _torch()
         _floats()
         x = _device_tensor(x, "x", _HALVES, 2).contiguous()
@@ -504,6 +549,9 @@ class Exl3Attention:
             _same(device, self, "projections")
         if self.rope is not None:
             _same(device, self.rope.inv_freq, "rope")
+        shape = None
+        if self.slopes is not None or prefix is not None or self.softcap != 0.0:
+            shape = _scores(device, self.q.out_features // cache.head_dim, batch.seqs, self.softcap, self.slopes, prefix)
         lib, code = load_library(), _HALVES[x.dtype]
         y = torch.empty(rows, self.o.out_features, device=device,
                         dtype=_code_dtype(lib.exl3_linear_output_dtype(self.o.handle, code)))
@@ -521,9 +569,13 @@ class Exl3Attention:
         with turn:
             if workspace is None:
                 workspace = kept.get(need, device)
-            _launch(device, lib.exl3_attn_block_forward, self.q.handle, self.k.handle, self.v.handle, self.o.handle,
-                    cache.handle, batch._attended(rows), None if self.rope is None else self.rope._ref, scale,
-                    self.window, x.data_ptr(), code, rows, y.data_ptr(), workspace.data_ptr(), workspace.numel())
+            args = (self.q.handle, self.k.handle, self.v.handle, self.o.handle, cache.handle, batch._attended(rows),
+                    None if self.rope is None else self.rope._ref, scale, self.window)
+            more = (x.data_ptr(), code, rows, y.data_ptr(), workspace.data_ptr(), workspace.numel())
+            if shape is None:
+                _launch(device, lib.exl3_attn_block_forward, *args, *more)
+            else:
+                _launch(device, lib.exl3_attn_block_forward_scores, *args, ctypes.byref(shape), *more)
         return y
 
     __call__ = forward
