@@ -28,7 +28,7 @@ namespace exl3 {
 // A split that saw nothing has a maximum of -inf and a sum of 0, and its sums, which are
 // not written, are not used.  Its latency bounds it: 5 us for 32 splits of 32 rows (a launch
 // alone takes 2 to 3), 53 before the loads went out together.
-template <int D, bool S>
+template <int D, int S>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows, int shift) {
   constexpr int L = D / 4, kGroups = 256 / L, kBatch = 8;
   __shared__ float4v sums[kGroups][L];
@@ -107,12 +107,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p, int rows, 
   for (int e = 0; e < 4; ++e) store1(p.y, p.q_type, yi + e, total != 0.0f ? acc[e] / total : 0.0f);
 }
 #define EXL3_JOIN_INST(D) \
-  template __global__ void attn_join_kernel<D, false>(AttnParams, int, int); \
-  template __global__ void attn_join_kernel<D, true>(AttnParams, int, int);
+  template __global__ void attn_join_kernel<D, kPlain>(AttnParams, int, int); \
+  template __global__ void attn_join_kernel<D, kEarly>(AttnParams, int, int);
 EXL3_JOIN_INST(64) EXL3_JOIN_INST(128) EXL3_JOIN_INST(256)
 
-EXL3_FEW(EXL3_FEW_INST, false)
-EXL3_MANY(EXL3_MANY_INST, false)
+EXL3_FEW(EXL3_FEW_INST, kPlain)
+EXL3_MANY(EXL3_MANY_INST, kPlain)
 
 }  // namespace exl3
 
@@ -200,6 +200,7 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
   if (!(scale > 0.0f) || !std::isfinite(scale2))
     return fail(EXL3_EINVAL, "attention scale must be positive and finite");
   if (window < 0) return fail(EXL3_EINVAL, "negative attention window %d", window);
+  int shaped = kPlain;
   if (scores) {
     const float cap = scores->softcap;
     if (cap != 0.0f && !(cap >= 0x1p-64f && cap <= 0x1p64f))
@@ -207,8 +208,11 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
     p.cap2 = cap * kLog2e;
     p.slopes = scores->slopes;
     p.prefix = causal ? scores->prefix : nullptr;
+    if (cap != 0.0f || (p.slopes && !(scale2 >= 0x1p-30f && scale2 <= 0x1p30f)))
+      shaped = kLate;
+    else if (p.slopes || p.prefix)
+      shaped = kEarly;
   }
-  const bool shaped = p.cap2 != 0.0f || p.slopes || p.prefix;
   if (batch->max_q < 1) return fail(EXL3_EINVAL, "max_q must be positive");
   if (batch->seqs > 65535)
     return fail(EXL3_EUNSUPPORTED, "attention takes up to 65535 sequences, got %d", batch->seqs);
@@ -247,15 +251,14 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
   p.q_vec = aligned16(q) && (tokens == 1 || q_stride % 8 == 0);
   p.y_vec = ((uintptr_t)y & 7) == 0 && (tokens == 1 || y_stride % 4 == 0);
   p.scale2 = scale2;
+  if (p.cap2 > 0.0f) cap_polynomials(p);
   p.part = (float*)workspace;
   p.stats = (float*)((uint8_t*)workspace + align256((size_t)sh.slots * sh.rows * p.cache.head_dim * 4));
   const int D = p.cache.head_dim;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = launch_gate("attention")) return rc;
-  if (shaped)
-    launch_attention_shaped(p, sh, s);
-  else
-    launch_attention<false>(p, sh, s);
+  shaped == kPlain ? launch_attention<kPlain>(p, sh, s)
+  : shaped == kEarly ? launch_attention_early(p, sh, s) : launch_attention_late(p, sh, s);
   if (int rc = check_launch("attention")) return rc;
   if (!sh.slots) return EXL3_OK;
   if (int rc = launch_gate("attention join")) return rc;
@@ -269,11 +272,11 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
                   (unsigned)sh.tiles);
   auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, p, sh.rows, shift); };
   if (shaped)
-    D == 64 ? join(attn_join_kernel<64, true>) : D == 128 ? join(attn_join_kernel<128, true>)
-                                                          : join(attn_join_kernel<256, true>);
+    D == 64 ? join(attn_join_kernel<64, kEarly>) : D == 128 ? join(attn_join_kernel<128, kEarly>)
+                                                          : join(attn_join_kernel<256, kEarly>);
   else
-    D == 64 ? join(attn_join_kernel<64, false>) : D == 128 ? join(attn_join_kernel<128, false>)
-                                                           : join(attn_join_kernel<256, false>);
+    D == 64 ? join(attn_join_kernel<64, kPlain>) : D == 128 ? join(attn_join_kernel<128, kPlain>)
+                                                           : join(attn_join_kernel<256, kPlain>);
   return check_launch("attention join");
 }
 

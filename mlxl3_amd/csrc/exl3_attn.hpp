@@ -22,8 +22,10 @@ struct AttnParams {
   int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
   int q_vec, y_vec;  // rows of q are 16-byte, rows of y 8-byte aligned
   float scale2;   // scale * log2(e): scores in units of a factor of two
-  // of calls with shaped scores (the kernels' S): cap2 = cap * log2(e), 0 without a cap
+  // of calls with shaped scores (the kernels' S): cap2 = cap * log2(e), 0 without a cap, and Cap's
+  // polynomials in squared products
   float cap2;
+  float cap_to[2], cap_near[4], cap_far[6];
   const float* slopes;    // of every head, or null
   const int32_t* prefix;  // of every sequence, or null
 };
@@ -134,8 +136,10 @@ __device__ __forceinline__ float largest_bf16(const u32x4& w, float most) {
   }
   return most;
 }
+// Shaped scores (S): from 2^-10 down, which leaves the queries' error far below a bias's.
+template <int S>
 __device__ __forceinline__ uint32_t fit_exponent(float most) {
-  return max(__builtin_bit_cast(uint32_t, most) >> 23, 16u);
+  return max(__builtin_bit_cast(uint32_t, most) >> 23, S ? 117u : 16u);
 }
 __device__ __forceinline__ float fit_factor(uint32_t e) { return __builtin_bit_cast(float, (269 - e) << 23); }
 // The scale times the inverse, a normal f32 too: a masked score, -inf, times zero would be NaN,
@@ -147,7 +151,7 @@ __device__ __forceinline__ float fit_scale(float scale2, uint32_t e) {
 
 // Eight query channels as T: T is the queries' own type for 16-bit caches, f16 for coded ones
 // (bf16 queries times `factor`; 4 bits: in codes4's order).
-template <int FMT, typename T, bool SCALED>
+template <int FMT, typename T, int SCALED>
 __device__ __forceinline__ typename T::V8 query_operand(const u32x4& w, float factor) {
   uint16_t h[8];
 #pragma unroll
@@ -173,7 +177,7 @@ struct Work {
   int prefix;            // tokens that all rows see (S)
   const int32_t* table;  // the sequence's row of the block table
 };
-template <bool S>
+template <int S>
 __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
   Work w;
   w.seq = seq;
@@ -194,7 +198,7 @@ __device__ __forceinline__ Work sequence_work(const AttnParams& p, int seq) {
 struct Seen {
   int lo, hi;
 };
-template <bool S>
+template <int S>
 __device__ __forceinline__ Seen row_sees(const AttnParams& p, const Work& w, int row) {
   const int64_t pos = (int64_t)w.first + row / p.group, len = w.len;
   Seen s{0, w.len};
@@ -215,7 +219,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // The sequence that item `i` belongs to, `items` telling how many each has; i becomes its
 // number there.  Behind the last item: no rows.  Every lane of a wave calls it with one i.
-template <bool S, typename F>
+template <int S, typename F>
 __device__ __forceinline__ Work work_of(const AttnParams& p, int& i, F&& items) {
   const int lane = threadIdx.x & 63;
   for (int s0 = 0; s0 < p.batch.seqs; s0 += 64) {
@@ -243,7 +247,7 @@ __device__ __forceinline__ Work work_of(const AttnParams& p, int& i, F&& items) 
 
 // Sequence and first row of tile `tile`, sequences cut into tiles of `rows` rows; a tile
 // behind the last has no rows.
-template <bool S>
+template <int S>
 __device__ __forceinline__ Work tile_work(const AttnParams& p, int tile, int rows, int& row0) {
   row0 = 0;
   if (p.one_tile) return sequence_work<S>(p, tile);
@@ -269,7 +273,7 @@ __device__ __forceinline__ int split_tokens(const AttnParams& p, int n) {
   return (int)max(((uint32_t)(n + p.splits - 1) / p.splits + 127) & ~127u, 128u);
 }
 // The tokens that a sequence's rows see, from a multiple of 16 on; a sequence with rows has one.
-template <bool S>
+template <int S>
 __device__ __forceinline__ int seen_tokens(const AttnParams& p, const Work& w) {
   if (w.rows == 0) return 0;
   const int lo = row_sees<S>(p, w, 0).lo & ~15;
@@ -282,7 +286,7 @@ __device__ __forceinline__ int seen_tokens(const AttnParams& p, const Work& w) {
 // ranges, at most budget + seqs (a sequence's last one may be short).
 constexpr int kMostRanges = 32;  // of a sequence: a row's ranges are joined by few lanes
 // The tokens of a range, by the batch (a wave calls it) and by the sequence's own.
-template <bool S>
+template <int S>
 __device__ __forceinline__ int range_tokens(const AttnParams& p) {
   float total = 0.0f;
   for (int s0 = 0; s0 < p.batch.seqs; s0 += 64) {
@@ -328,26 +332,37 @@ __device__ __forceinline__ float slack_at(float m, float slack) {
 
 // Shaped scores: x is a score in factors of two, s scale log2(e).
 //
-// Capped it is cap2 tanh(x / cap2): a score z becomes cap tanh(z / cap).  tanh(u) = 1 - 2 / (1 + e^2u)
-// is off by 2^-23 or so whatever u, the capped score by cap2 times that, 1e-5 under a cap of 50.
+// Capped it is cap2 tanh(u), u = x / cap2: a score z becomes cap tanh(z / cap).  tanh(u) = 1 - 2 / (1 +
+// e^2u) is off by 2^-23 or so whatever u, the capped score by cap2 times that, 1e-5 under a cap of 50.
 // Above a cap of 1024 that is too much for small scores: |u| < 1/4 takes tanh's series there.
 //
-// Where no |u| of a wave's scores is above kNear (scores up to 25 under a cap of 50) all of them are
-// x (1 + v (a + v (b + v c))), v = u^2, off by 6.5e-7 of themselves: six instructions instead of
-// two transcendentals, which go at a quarter of the rate, and three more.
+// Up to |u| = 1 (scores up to 50 under a cap of 50) tanh(u) is u times a polynomial in u^2, off by 7e-7
+// of itself (fitted to the least largest error, first coefficient 1): of degree 3 up to 1/2, of 5 up to
+// 1.  Where no score of a wave's tile is beyond that, it takes the place of two transcendentals, at a
+// quarter of the rate, and four more instructions: x = S c(S^2), S the product as it is, the host's
+// coefficients with the scale in them.
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNear = 0.5f;
+constexpr double kTanhNear[4] = {1.0, -0.33328159331842044, 0.13205359636370356, -0.044750641313108026};
+constexpr double kTanhFar[6] = {1.0, -0.33330279667160123, 0.13288490228334163, -0.05176828405213653,
+                                0.01690640684211184, -0.003126576844036082};
+// The largest products that the polynomials take (0: none do, a power of them leaves f32's range), and
+// their coefficients.
+inline void cap_polynomials(AttnParams& p) {
+  const double r = (double)p.scale2 / p.cap2;  // u / S
+  if (!(r >= 0x1p-12 && r <= 0x1p10) || p.cap2 > 1024.0f * kLog2e) return;
+  p.cap_to[0] = (float)(0.5 / r);
+  p.cap_to[1] = (float)(1.0 / r);
+  double power = p.scale2;
+  for (int i = 0; i < 6; ++i, power *= r * r) {
+    if (i < 4) p.cap_near[i] = (float)(kTanhNear[i] * power);
+    p.cap_far[i] = (float)(kTanhFar[i] * power);
+  }
+}
 struct Cap {
-  float cap2, inv, inv2, rate, near;
+  float cap2, inv, rate;
   bool large;
   __device__ __forceinline__ explicit Cap(float c)
-      : cap2(c), inv(1.0f / c), inv2(inv * inv), rate(2.0f * kLog2e * inv), near(c * kNear), large(c > 1024.0f * kLog2e) {
-    if (large) near = 0.0f;  // not taken
-  }
-  __device__ __forceinline__ float small(float x) const {
-    const float v = x * x * inv2;
-    return x * fmaf(v, fmaf(v, fmaf(v, -0.04475063f, 0.13205359f), -0.33328159f), 1.0f);
-  }
+      : cap2(c), inv(1.0f / c), rate(2.0f * kLog2e * inv), large(c > 1024.0f * kLog2e) {}
   __device__ __forceinline__ float any(float x) const {
     const float far = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * rate)), cap2);
     if (!large) return far;
@@ -357,13 +372,55 @@ struct Cap {
     return fabsf(u) < 0.25f ? x * series : far;
   }
 };
-// The bias by distance: slope2 = slope log2(e) times it off the score.
+// N products of every lane of a wave (of rows that were scaled, `unscale` less) as scores: times the
+// scale, and capped.
+template <bool SCALED, int N, typename G, typename P>
+__device__ __forceinline__ void scores_of(const AttnParams& p, const Cap& cap, float unscale, G&& get, P&& put) {
+  if (p.cap2 > 0.0f) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (SCALED) put(i, get(i) * unscale);
+      most = fmaxf(most, fabsf(get(i)));
+    }
+    if (!__any(most > p.cap_to[0])) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float x = get(i), v = x * x;
+        put(i, x * fmaf(v, fmaf(v, fmaf(v, p.cap_near[3], p.cap_near[2]), p.cap_near[1]), p.cap_near[0]));
+      }
+    } else if (!__any(most > p.cap_to[1])) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float x = get(i), v = x * x;
+        float c = fmaf(v, p.cap_far[5], p.cap_far[4]);
+#pragma unroll
+        for (int k = 3; k >= 0; --k) c = fmaf(v, c, p.cap_far[k]);
+        put(i, x * c);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) put(i, cap.any(get(i) * p.scale2));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) put(i, get(i) * (SCALED ? unscale * p.scale2 : p.scale2));
+  }
+}
+// The bias by distance: slope2 = slope log2(e) times it off the score.  Without a cap the sums of the
+// products start from it, divided by what scores are multiplied by (kEarly), and all else is as for
+// plain scores; that takes scales of 2^-30 to 2^30 and slopes up to 2^32.  Else (kLate) scores are
+// multiplied by the scale, capped, biased.
+enum : int { kPlain = 0, kEarly = 1, kLate = 2 };
 __device__ __forceinline__ float biased(float x, float slope2, float away) { return fmaf(-slope2, fabsf(away), x); }
+__device__ __forceinline__ float slope_of(const AttnParams& p, int head) {
+  return p.slopes ? __builtin_amdgcn_fmed3f(p.slopes[head], -4294967296.0f, 4294967296.0f) * kLog2e : 0.0f;
+}
 
 // One row over the tokens [lo, hi) by one wave, its channels spread over the lanes (lane
 // l holds channels E l ..): running maximum m, sum l and weighted values acc.  Touches
 // only tokens that the row sees.
-template <int E, bool S>
+template <int E, int S>
 __device__ __forceinline__ void row_pass(const AttnParams& p, const Work& w, int kvh, int row, int lo, int hi,
                                          int lane, float& m, float& l, float (&acc)[E]) {
   const KvCacheView& c = p.cache;
@@ -409,7 +466,7 @@ __device__ __forceinline__ void row_pass(const AttnParams& p, const Work& w, int
     s = wave_sum(s) * p.scale2;
     if constexpr (S) {
       if (p.cap2 > 0.0f) s = Cap(p.cap2).any(s);
-      if (p.slopes) s = biased(s, p.slopes[kvh * p.group + row % p.group] * kLog2e, (float)((int64_t)w.first + row / p.group - t));
+      if (p.slopes) s = biased(s, slope_of(p, kvh * p.group + row % p.group), (float)(w.first + row / p.group - t));
     }
     const float n = fmaxf(m, s);
     const float base = n == -__builtin_inff() ? 0.0f : n;

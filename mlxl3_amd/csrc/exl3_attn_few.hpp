@@ -203,7 +203,7 @@ struct Few {
 
 // grid (kv heads, splits, sequences) or (kv heads, ranges by the batch's sum): ranges that there
 // are come before those left over, which would take the place of others on a CU
-template <int FMT, typename T, int D, int RT, int PARTS, bool S>
+template <int FMT, typename T, int D, int RT, int PARTS, int S>
 __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_kernel(AttnParams p) {
   typedef Few<FMT, T, D, RT, PARTS> F;
   typedef typename T::V8 V8;
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   const int n = lane & 15, g = lane >> 4;
   uint8_t* my = lds + wave * F::kWaveLds;
   V8 q[RT][F::kSteps];
-  float scale2[RT];  // the call's, of rows that were scaled times the inverse
+  float scale2[RT], unscale[RT];  // the call's, of rows that were scaled times the inverse; that inverse
   Seen see[RT];
   float slope2[RT];  // of shaped scores: the row's bias,
   int at[RT];        // its position less this lane's first token of a step
@@ -253,12 +253,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     const size_t qi =
         (size_t)(w.start + r / p.group) * p.q_stride + (size_t)(kvh * p.group + r % p.group) * D;
     if constexpr (S) {
-      slope2[rt] = p.slopes ? p.slopes[kvh * p.group + r % p.group] * kLog2e : 0.0f;
+      slope2[rt] = slope_of(p, kvh * p.group + r % p.group);
       at[rt] = w.first + r / p.group - 4 * g;
     }
     u32x4 raw[F::kSteps];
     float factor = 1.0f, most = 0.0f;
     scale2[rt] = p.scale2;
+    unscale[rt] = 1.0f;
 #pragma unroll
     for (int s = 0; s < F::kSteps; ++s) raw[s] = load_q8(p, qi + F::channel(s, g));
     if constexpr (F::kScaled) {
@@ -266,9 +267,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
       for (int s = 0; s < F::kSteps; ++s) most = largest_bf16(raw[s], most);
       most = fmaxf(most, xor_lanes<16>(most));
       most = fmaxf(most, xor_lanes<32>(most));
-      const uint32_t e = fit_exponent(most);
+      const uint32_t e = fit_exponent<S>(most);
       factor = fit_factor(e);
       scale2[rt] = fit_scale(p.scale2, e);
+      unscale[rt] = fit_scale(1.0f, e);
     }
 #pragma unroll
     for (int s = 0; s < F::kSteps; ++s) q[rt][s] = query_operand<FMT, T, F::kScaled>(raw[s], factor);
@@ -286,8 +288,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   // of the wave, and what scores are multiplied by as weights; far (kFar): less than 0 and 1
   float slack = kSlack + T::kRoom, unit[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) unit[rt] = S ? 1.0f : scale2[rt];
-  const Cap cap(S ? p.cap2 : 1.0f);
+  for (int rt = 0; rt < RT; ++rt) unit[rt] = scale2[rt];
+  if constexpr (S) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (S == kLate)
+        unit[rt] = 1.0f;
+      else
+        slope2[rt] /= scale2[rt];
+    }
+  }
+  const Cap cap(S == kLate ? p.cap2 : 1.0f);
 
   typename F::Keys k;
   typename F::Values v;
@@ -314,7 +325,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int a = 0; a < 2; ++a) s[rt][a] = float4v{0, 0, 0, 0};
+      for (int a = 0; a < 2; ++a) {
+        s[rt][a] = float4v{0, 0, 0, 0};
+        if (S == kEarly) {
+          const float away = (float)(at[rt] - t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[rt][a][i] = -slope2[rt] * fabsf(away - (float)(16 * a + i));
+        }
+      }
 #pragma unroll
     for (int st = 0; st < F::kSteps; ++st)
 #pragma unroll
@@ -351,21 +369,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
       float x[8], most = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = s[rt][i >> 2][i & 3];
-      if constexpr (S) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= scale2[rt];
-        if (p.cap2 > 0.0f) {
-          float far = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) far = fmaxf(far, fabsf(x[i]));
-          if (__any(far > cap.near)) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = cap.any(x[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = cap.small(x[i]);
-          }
-        }
+      if constexpr (S == kLate) {
+        scores_of<F::kScaled, 8>(p, cap, unscale[rt], [&](int i) { return x[i]; }, [&](int i, float v) { x[i] = v; });
         if (p.slopes) {
           const float away = (float)(at[rt] - t);
 #pragma unroll
@@ -381,7 +386,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         }
         most = fmaxf(most, x[i]);
       }
-      if constexpr (!S) most *= scale2[rt];
+      if constexpr (S != kLate) most *= scale2[rt];
       if (__any(most - m[rt] > slack)) {
         most = fmaxf(most, xor_lanes<16>(most));
         most = fmaxf(most, xor_lanes<32>(most));
@@ -391,8 +396,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
         l[rt] *= f;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[rt][dt] *= f;
-        if constexpr (!S) slack = slack_at(up, slack);
-        if (!S && slack < 0.0f) {
+        if constexpr (S != kLate) slack = slack_at(up, slack);
+        if (S != kLate && slack < 0.0f) {
           unit[rt] = 1.0f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] *= scale2[rt];

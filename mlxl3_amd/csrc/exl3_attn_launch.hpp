@@ -1,6 +1,6 @@
 // Attention's kernels by format, width and rows: their instances, spelled out for the device
-// pass, and their launches.  S: scores that are capped or biased, or rows that see a prefix; those are
-// a translation unit of their own.
+// pass, and their launches.  S: scores that are capped or biased, or rows that see a prefix: translation
+// units of their own.
 #pragma once
 
 #include "exl3_attn_few.hpp"
@@ -36,14 +36,14 @@ struct AttnShape {
 
 #ifndef __HIP_DEVICE_COMPILE__
 
-template <bool S, int FMT, typename T, int PARTS, int D, int RT>
+template <int S, int FMT, typename T, int PARTS, int D, int RT>
 void launch_few(const AttnParams& p, hipStream_t s) {
   const dim3 grid = p.budget ? dim3((unsigned)p.cache.kv_heads, (unsigned)(p.budget + p.batch.seqs + 1))
                              : dim3((unsigned)p.cache.kv_heads, (unsigned)p.splits, (unsigned)p.batch.seqs);
   constexpr size_t lds = 4 * (Few<FMT, T, D, RT, PARTS>::kWaveLds);
   hipLaunchKernelGGL((attn_few_kernel<FMT, T, D, RT, PARTS, S>), grid, dim3(256), lds, s, p);
 }
-template <bool S, int FMT, typename T, int PARTS>
+template <int S, int FMT, typename T, int PARTS>
 void launch_few(const AttnParams& p, int rows, hipStream_t s) {
   const int d = p.cache.head_dim;
   if (rows == 16) {
@@ -54,13 +54,13 @@ void launch_few(const AttnParams& p, int rows, hipStream_t s) {
   }
 }
 
-template <bool S, int FMT, typename T, int PARTS, int D>
+template <int S, int FMT, typename T, int PARTS, int D>
 void launch_many(const AttnParams& p, int tiles, hipStream_t s) {
   constexpr size_t lds = Many<FMT, T, D, PARTS>::kLds;
   const dim3 grid((unsigned)tiles * p.splits * p.cache.kv_heads);
   hipLaunchKernelGGL((attn_many_kernel<FMT, T, D, PARTS, S>), grid, dim3(256), lds, s, p, tiles);
 }
-template <bool S, int FMT, typename T, int PARTS>
+template <int S, int FMT, typename T, int PARTS>
 void launch(const AttnParams& p, const AttnShape& sh, hipStream_t s) {
   const int d = p.cache.head_dim, tiles = (int)sh.tiles;
   if (sh.few)
@@ -71,7 +71,7 @@ void launch(const AttnParams& p, const AttnShape& sh, hipStream_t s) {
 }
 
 // The kernel of a call by the cache's format and the queries' type (f16 ones: coded values in two parts).
-template <bool S>
+template <int S>
 void launch_attention(const AttnParams& p, const AttnShape& sh, hipStream_t s) {
   const bool fine = p.q_type == DT_F16;
   switch (p.cache.format) {
@@ -84,7 +84,8 @@ void launch_attention(const AttnParams& p, const AttnShape& sh, hipStream_t s) {
 
 #endif  // __HIP_DEVICE_COMPILE__
 
-// launch_attention<true>, of the other translation unit.
-void launch_attention_shaped(const AttnParams& p, const AttnShape& sh, hipStream_t s);
+// launch_attention<kEarly> and <kLate>, of the other translation units.
+void launch_attention_early(const AttnParams& p, const AttnShape& sh, hipStream_t s);
+void launch_attention_late(const AttnParams& p, const AttnShape& sh, hipStream_t s);
 
 }  // namespace exl3

@@ -159,7 +159,7 @@ struct Many {
 
 // One-dimensional grid of tiles x splits x kv heads, the heads fastest (blocks go to the
 // XCDs in turn, so a head's tiles share few L2s), a sequence's last and longest tiles first.
-template <int FMT, typename T, int D, int PARTS, bool S>
+template <int FMT, typename T, int D, int PARTS, int S>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(Many<FMT, T, D, PARTS>::kGroups, Many<FMT, T, D, PARTS>::kGroups)))
 void attn_many_kernel(AttnParams p, int tiles) {
@@ -196,9 +196,9 @@ void attn_many_kernel(AttnParams p, int tiles) {
   const Seen wtop = row_sees<S>(p, w, min(wrow, row0 + rows - 1));
   const Seen wend = row_sees<S>(p, w, min(wrow + 31, row0 + rows - 1));
   V8 q[D / 16];
-  float scale2 = p.scale2;  // of rows that were scaled times the inverse
+  float scale2 = p.scale2, unscale = 1.0f;  // of rows that were scaled times the inverse; that inverse
+  constexpr bool kScaled = !F::kRaw && PARTS == 1;  // bf16 queries, to fit f16
   {
-    constexpr bool kScaled = !F::kRaw && PARTS == 1;  // bf16 queries, to fit f16
     const size_t qi = (size_t)(w.start + mine / p.group) * p.q_stride +
                       (size_t)(kvh * p.group + mine % p.group) * D;
     u32x4 raw[D / 16];
@@ -209,24 +209,26 @@ void attn_many_kernel(AttnParams p, int tiles) {
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) most = largest_bf16(raw[s], most);
       most = fmaxf(most, xor_lanes<32>(most));
-      const uint32_t e = fit_exponent(most);
+      const uint32_t e = fit_exponent<S>(most);
       factor = fit_factor(e);
       scale2 = fit_scale(p.scale2, e);
+      unscale = fit_scale(1.0f, e);
     }
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) q[s] = query_operand<FMT == KV_Q4 ? KV_Q8 : FMT, T, kScaled>(raw[s], factor);
   }
   // of shaped scores: the row's bias, its position less this lane's first token of a tile
-  const float slope2 = S && p.slopes ? p.slopes[kvh * p.group + mine % p.group] * kLog2e : 0.0f;
-  const int at = w.first + mine / p.group - 4 * h;
-  const Cap cap(S ? p.cap2 : 1.0f);
+  float slope2 = S ? slope_of(p, kvh * p.group + mine % p.group) : 0.0f;
+  const int at = w.first + mine / p.group - 4 * h, nearest = w.first + wrow / p.group;
+  if (S == kEarly) slope2 /= scale2;
+  const Cap cap(S == kLate ? p.cap2 : 1.0f);
   float16v o[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
   float m = kNothing, l = 0.0f;
   bool again = false;
   // of the wave, and what scores are multiplied by as weights; far (kFar): less than 0 and 1
-  float slack = kSlack + T::kRoom, unit = S ? 1.0f : scale2;
+  float slack = kSlack + T::kRoom, unit = S == kLate ? 1.0f : scale2;
 
   typename F::Loads x;
   const int off = F::kMine * wave;  // of this wave's rows in a tile
@@ -288,11 +290,31 @@ void attn_many_kernel(AttnParams p, int tiles) {
       V8 kf[kDepth];
 #pragma unroll
       for (int i = 0; i < kDepth; ++i) kf[i] = key(i);
+      if constexpr (S == kEarly) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = float16v{};
+        const float away = (float)(at - t);
+        // well behind all rows one instruction each: rounded at the tile's border, from where a
+        // token lies at most twice as far as the nearest one, it is off by 2^-23 of itself
+        if (t + 2 * TK <= nearest) {
+          const float from = -slope2 * away;
+#pragma unroll
+          for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[a][i] = fmaf(slope2, (float)(32 * a + 8 * (i / 4) + i % 4), from);
+        } else {
+#pragma unroll
+          for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              s[a][i] = -slope2 * fabsf(away - (float)(32 * a + 8 * (i / 4) + i % 4));
+        }
+    }
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < QK; ++i) {
         pin();
-        if (i < N) s[i] = float16v{};
+        if (S != kEarly && i < N) s[i] = float16v{};
         s[i % N] = T::mfma32(kf[i % kDepth], q[i / N], s[i % N]);
         if (i + kDepth < QK) kf[i % kDepth] = key(i + kDepth);
       }
@@ -317,35 +339,14 @@ void attn_many_kernel(AttnParams p, int tiles) {
       for (int i = 0; i < DT; ++i) vf[i] = value(i);
       pin();
       __builtin_amdgcn_s_setprio(0);
-      if constexpr (S) {
-#pragma unroll
-        for (int a = 0; a < NT; ++a)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[a][i] *= scale2;
-        if (p.cap2 > 0.0f) {
-          float far = 0.0f;
-#pragma unroll
-          for (int a = 0; a < NT; ++a)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) far = fmaxf(far, fabsf(s[a][i]));
-          if (__any(far > cap.near)) {
-#pragma unroll
-            for (int a = 0; a < NT; ++a)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) s[a][i] = cap.any(s[a][i]);
-          } else {
-#pragma unroll
-            for (int a = 0; a < NT; ++a)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) s[a][i] = cap.small(s[a][i]);
-          }
-        }
+      if constexpr (S == kLate) {
+        scores_of<kScaled, 16 * NT>(p, cap, unscale, [&](int i) { return s[i / 16][i % 16]; },
+                                    [&](int i, float v) { s[i / 16][i % 16] = v; });
         if (p.slopes) {
           const float away = (float)(at - t);
 #pragma unroll
-          for (int a = 0; a < NT; ++a)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[a][i] = biased(s[a][i], slope2, away - (float)(32 * a + 8 * (i / 4) + i % 4));
+          for (int i = 0; i < 16 * NT; ++i)
+            s[i / 16][i % 16] = biased(s[i / 16][i % 16], slope2, away - (float)(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4));
         }
       }
       if (t < wend.lo || t + TK > min(wtop.hi, t1)) {
@@ -373,7 +374,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
       for (int a = 0; a < NT; ++a)
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, s[a][i]);
-      if constexpr (!S) most *= scale2;
+      if constexpr (S != kLate) most *= scale2;
       if (__any(most - m > slack)) {
         most = fmaxf(most, xor_lanes<32>(most));
         const float up = fmaxf(m, most - T::kRoom);
@@ -382,8 +383,8 @@ void attn_many_kernel(AttnParams p, int tiles) {
         l *= f;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) o[dt] *= f;
-        if constexpr (!S) slack = slack_at(up, slack);
-        if (!S && slack < 0.0f) {
+        if constexpr (S != kLate) slack = slack_at(up, slack);
+        if (S != kLate && slack < 0.0f) {
           unit = 1.0f;
 #pragma unroll
           for (int a = 0; a < NT; ++a)

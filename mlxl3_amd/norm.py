@@ -4,7 +4,7 @@
 from __future__ import annotations
 
 from . import Exl3Error, _torch, load_library
-from . import kv as _kv
+from .kv import _floats, _launch, _rows_ok, _same
 
 
 def _laid(t):
@@ -15,29 +15,31 @@ def _laid(t):
         return 0, t.shape[-1]
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
         return 1, t.stride(0)
-    if t.dim() == 3 and _kv._rows_ok(t):
+    if t.dim() == 3 and _rows_ok(t):
         return t.shape[1], t.stride(0)
     return None
 
 
-def _floating(t, name: str):
-    torch = _torch()
+def _code(t, name: str) -> int:
+    """The type's code of a floating device tensor."""
+    torch, floats = _torch(), _floats()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise Exl3Error(-1, f"{name} must be a device tensor")
-    if t.dtype not in _kv._floats():
-        raise Exl3Error(-1, f"{name} has dtype {t.dtype}, expected one of {tuple(_kv._FLOATS)}")
-    return t
+    code = floats.get(t.dtype)
+    if code is None:
+        raise Exl3Error(-1, f"{name} has dtype {t.dtype}, expected one of {tuple(floats)}")
+    return code
 
 
-def _written(t, name: str, like, dtype):
-    """A tensor that the kernel writes: like's shape and device, rows that it can write in place."""
-    _floating(t, name)
-    if t.shape != like.shape or (dtype is not None and t.dtype != dtype):
-        raise Exl3Error(-1, f"{name} must have shape {tuple(like.shape)}" + (f" and dtype {dtype}" if dtype else ""))
-    _kv._same(like.device, t, name)
+def _written(t, name: str, shape, device, dtype) -> int:
+    """The type's code of a tensor that the kernel writes: rows that it can write in place."""
+    code = _code(t, name)
+    if t.shape != shape or (dtype is not None and t.dtype != dtype):
+        raise Exl3Error(-1, f"{name} must have shape {tuple(shape)}" + (f" and dtype {dtype}" if dtype else ""))
+    _same(device, t, name)
     if _laid(t) is None:
         raise Exl3Error(-1, f"{name} must have contiguous rows")
-    return t
+    return code
 
 
 def rms_norm(x, weight=None, eps: float = 1e-6, residual=None, total=None, out=None, dtype=None):
@@ -52,53 +54,70 @@ def rms_norm(x, weight=None, eps: float = 1e-6, residual=None, total=None, out=N
     heads); x, residual and weight are copied where their strides are others.  Outputs and inputs
     that are not the same tensor do not overlap."""
     torch = _torch()
-    x = _floating(x, "x")
-    floats, device = _kv._FLOATS, x.device
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise Exl3Error(-1, f"norms take rows of at least one value, got shape {tuple(x.shape)}")
-    if dtype is not None and dtype not in floats:
-        raise Exl3Error(-1, f"unsupported norm output dtype {dtype}")
-    try:
-        eps = float(eps)
-    except (TypeError, ValueError):
-        raise Exl3Error(-1, f"norm eps must be a number, got {eps!r}") from None
-    width = x.shape[-1]
+    x_code = _code(x, "x")
+    shape, device = x.shape, x.device
+    width = shape[-1] if shape else 0
+    if width < 1:
+        raise Exl3Error(-1, f"norms take rows of at least one value, got shape {tuple(shape)}")
+    if type(eps) is not float:
+        try:
+            eps = float(eps)
+        except (TypeError, ValueError):
+            raise Exl3Error(-1, f"norm eps must be a number, got {eps!r}") from None
+    w_code = r_code = 0
     if weight is not None:
-        _floating(weight, "weight")
-        if tuple(weight.shape) != (width,):
+        w_code = _code(weight, "weight")
+        if weight.dim() != 1 or weight.numel() != width:
             raise Exl3Error(-1, f"weight must have shape ({width},), got {tuple(weight.shape)}")
-        _kv._same(device, weight, "weight")
+        _same(device, weight, "weight")
         weight = weight.contiguous()
-    if residual is None:
-        if total is not None:
-            raise Exl3Error(-1, "a sum needs a residual")
-    else:
-        _floating(residual, "residual")
-        if residual.shape != x.shape:
-            raise Exl3Error(-1, f"residual must have shape {tuple(x.shape)}, got {tuple(residual.shape)}")
-        _kv._same(device, residual, "residual")
+    if residual is not None:
+        r_code = _code(residual, "residual")
+        if residual.shape != shape:
+            raise Exl3Error(-1, f"residual must have shape {tuple(shape)}, got {tuple(residual.shape)}")
+        _same(device, residual, "residual")
+    elif total is not None:
+        raise Exl3Error(-1, "a sum needs a residual")
     if out is not None:
-        _written(out, "out", x, dtype)
+        y_code = _written(out, "out", shape, device, dtype)
+    elif dtype is None or dtype == x.dtype:
+        y_code = x_code
+    else:
+        y_code = _floats().get(dtype)
+        if y_code is None:
+            raise Exl3Error(-1, f"unsupported norm output dtype {dtype}")
     if total is not None:
-        _written(total, "total", x, residual.dtype)
+        _written(total, "total", shape, device, residual.dtype)
         if total is out:
             raise Exl3Error(-1, "the sum and the norm are two outputs")
-    if _laid(x) is None:
+    if not x.is_contiguous() and _laid(x) is None:
         x = x.contiguous()
-    if residual is not None and _laid(residual) is None:
+    if residual is not None and not residual.is_contiguous() and _laid(residual) is None:
         residual = residual.contiguous()
+    # new tensors are contiguous (of contiguous ones the quicker way)
     if out is None:
-        out = torch.empty(x.shape, dtype=dtype or x.dtype, device=device)
+        if not x.is_contiguous():
+            out = torch.empty(shape, dtype=dtype or x.dtype, device=device)
+        else:
+            out = torch.empty_like(x) if y_code == x_code else torch.empty_like(x, dtype=dtype)
     if residual is not None and total is None:
-        total = torch.empty(x.shape, dtype=residual.dtype, device=device)
-    if x.numel() == 0:
+        if residual.is_contiguous():
+            total = torch.empty_like(residual)
+        else:
+            total = torch.empty(shape, dtype=residual.dtype, device=device)
+    count = x.numel()
+    if count == 0:
         return out if residual is None else (out, total)
-    laid = [(0, 0) if t is None else _laid(t) for t in (x, residual, total, out)]
-    heads = max(1, *(h for h, _ in laid))  # those that have gaps have x's
-    xs, rs, ts, ys = (stride * heads if h == 0 else stride for h, stride in laid)
-    _kv._launch(
-        device, load_library().exl3_rms_norm, x.data_ptr(), floats[x.dtype], x.numel() // (width * heads), heads, width, xs,
-        None if weight is None else weight.data_ptr(), 0 if weight is None else floats[weight.dtype], eps,
-        None if residual is None else residual.data_ptr(), 0 if residual is None else floats[residual.dtype], rs,
-        None if total is None else total.data_ptr(), ts, out.data_ptr(), floats[out.dtype], ys)
+    heads = 1
+    xs = rs = ts = ys = width
+    if not (x.is_contiguous() and out.is_contiguous()
+            and (residual is None or (residual.is_contiguous() and total.is_contiguous()))):
+        laid = [(0, 0) if t is None else _laid(t) for t in (x, residual, total, out)]
+        heads = max(1, max(laid)[0])  # those that have gaps have x's
+        xs, rs, ts, ys = (stride if h else stride * heads for h, stride in laid)
+    _launch(
+        device, load_library().exl3_rms_norm, x.data_ptr(), x_code, count // (width * heads), heads, width, xs,
+        None if weight is None else weight.data_ptr(), w_code, eps,
+        None if residual is None else residual.data_ptr(), r_code, rs,
+        None if total is None else total.data_ptr(), ts, out.data_ptr(), y_code, ys)
     return out if residual is None else (out, total)

@@ -18,8 +18,9 @@ def attend(q, k, v, first, scale, causal, window, softcap=0.0, slopes=None, pref
     own: 2^-21 of the cap -- 1 - 2 / (1 + e) with e off by 2^-22 or so of itself, which moves 1 / (1 + e) by
     at most a quarter of that, its sum and reciprocal rounded to 1.5 * 2^-24; or the polynomial's
     6.5e-7 of a score of up to half the cap, which is less; above a cap of 1024 the series', 2^-22 of
-    the score, up to a quarter of the cap; the bias: its factor log2(e) and itself rounded, the sum
-    rounded, 2^-22 of both.  The rest is as for plain
+    the score, up to a quarter of the cap; the bias: a slope over a scale, a distance and their product
+    rounded (2^-22 of it), and where it is what the f32 sum of the products starts from, as much of it as
+    of them is lost there, dim half steps.  The rest is as for plain
     scores: the exponential 2^-21, p rounded to 16 bits, coded values to f16, f32 sums over the tokens,
     the output's half step."""
     n, heads, dim = q.shape
@@ -47,7 +48,7 @@ def attend(q, k, v, first, scale, causal, window, softcap=0.0, slopes=None, pref
             z = softcap * torch.tanh(z / softcap)
         if slopes is not None:
             bias = float(slopes[h]) * away.abs().double()
-            e = e + 2.0**-22 * (bias.abs() + z.abs())
+            e = e + 2.0**-22 * z.abs() + bias.abs() * (2.0**-22 + dim * 2.0**-24)
             z = z - bias
         e = torch.where(seen, e + 2.0**-21 + 2.0**-23 * z.abs(), none)
         z = torch.where(seen, z, torch.tensor(-math.inf, dtype=torch.float64))
