@@ -90,29 +90,24 @@ def rms_norm(x, weight=None, eps: float = 1e-6, residual=None, total=None, out=N
         _written(total, "total", shape, device, residual.dtype)
         if total is out:
             raise Exl3Error(-1, "the sum and the norm are two outputs")
-    if not x.is_contiguous() and _laid(x) is None:
-        x = x.contiguous()
-    if residual is not None and not residual.is_contiguous() and _laid(residual) is None:
-        residual = residual.contiguous()
-    # new tensors are contiguous (of contiguous ones the quicker way)
+    # (heads, token stride) of x, residual, total and out where one of them has gaps
+    laid = None
+    if not (x.is_contiguous() and (residual is None or residual.is_contiguous())
+            and (total is None or total.is_contiguous()) and (out is None or out.is_contiguous())):
+        laid = [(0, width) if t is None else _laid(t) for t in (x, residual, total, out)]
+        if laid[0] is None:
+            x, laid[0] = x.contiguous(), (0, width)
+        if laid[1] is None:
+            residual, laid[1] = residual.contiguous(), (0, width)
     if out is None:
-        if not x.is_contiguous():
-            out = torch.empty(shape, dtype=dtype or x.dtype, device=device)
-        else:
-            out = torch.empty_like(x) if y_code == x_code else torch.empty_like(x, dtype=dtype)
+        out = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
     if residual is not None and total is None:
-        if residual.is_contiguous():
-            total = torch.empty_like(residual)
-        else:
-            total = torch.empty(shape, dtype=residual.dtype, device=device)
+        total = torch.empty_like(residual, memory_format=torch.contiguous_format)
     count = x.numel()
     if count == 0:
         return out if residual is None else (out, total)
-    heads = 1
-    xs = rs = ts = ys = width
-    if not (x.is_contiguous() and out.is_contiguous()
-            and (residual is None or (residual.is_contiguous() and total.is_contiguous()))):
-        laid = [(0, 0) if t is None else _laid(t) for t in (x, residual, total, out)]
+    heads, xs, rs, ts, ys = 1, width, width, width, width
+    if laid is not None:
         heads = max(1, max(laid)[0])  # those that have gaps have x's
         xs, rs, ts, ys = (stride if h else stride * heads for h, stride in laid)
     _launch(
