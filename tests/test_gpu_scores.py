@@ -104,6 +104,27 @@ def test_slopes_of_all_sizes(bits, cdtype, dtype, slope):
         check(pool, new, q, y, slopes=slopes)
 
 
+@pytest.mark.parametrize("bits, cdtype, dtype", FORMATS)
+@pytest.mark.parametrize("gain", [1e-30, 1e-12, 1e-5, 1e3])
+def test_biases_of_queries_of_all_sizes(bits, cdtype, dtype, gain):
+    """A bias counts as much whatever the queries' size (f16 ones down to zeros)."""
+    for new, lens in (([1, 2], [700, 33]), ([50], [300])):
+        pool = Pool(25, lens, 2, 64, 16, bits, cdtype, loud=1.0)
+        for kw in (dict(slopes=geometric(6)), dict(slopes=geometric(6), softcap=40.0)):
+            q, _, _, y, _ = run(pool, new, 6, dtype, gain=gain, **kw)
+            check(pool, new, q, y, **kw)
+
+
+@pytest.mark.parametrize("scale", [1e-36, 1e-12, 3.0, 1e9, 1e30])
+def test_scales_of_all_sizes(scale):
+    """Scales that a bias is not divided by, and others; queries of the inverse size."""
+    for new, lens in (([1, 2], [300, 33]), ([50], [200])):
+        pool = Pool(26, lens, 2, 128, 16, 16, BF16, loud=1.0)
+        for kw in (dict(slopes=geometric(4)), dict(softcap=4.0), dict(prefix=[20, 5][: len(new)])):
+            q, _, _, y, _ = run(pool, new, 4, BF16, gain=0.1 / scale, scale=scale, **kw)
+            check(pool, new, q, y, scale=scale, **kw)
+
+
 @pytest.mark.parametrize("bits, cdtype, dtype", FORMATS[:3])
 @pytest.mark.parametrize("causal", [True, False])
 def test_distances_count_both_ways(bits, cdtype, dtype, causal):
