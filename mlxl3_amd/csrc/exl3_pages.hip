@@ -4,7 +4,10 @@
 // One launch copies up to 224 pairs of pages in up to 32 caches of one shape -- a model's layers --
 // named in the kernel's arguments, so that nothing is uploaded.  Where a pair copies its first
 // n slots only, a head's n slots are one run of its page (its scales n of every group's run).
-// Memory bounds it: every byte is read and written once, 16 at a time.
+// Memory bounds it: every byte is read and written once, 16 at a time.  Measured, sources not in the
+// caches: 230 pages of 131 KB in 4 caches, 121 MB, 50 us, 4.8 TB/s read and written (a large copy: 5.1);
+// 48 partly filled 8-bit pages in 16 caches, 27 MB, 19 us (in the caches 11); one page's 9 slots in 32
+// caches 3.7 us, a launch and one round trip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,61 +34,76 @@ struct CopyParams {
   int page_shift, kv_heads, row, groups;  // row: bytes of a cached head; groups: of scales, 0 without
 };
 
-// A run of `runs` pieces of `length` 16-byte units, `pitch` units apart, copied by 256 threads from
-// unit `first` on.
-__device__ __forceinline__ void copy_units(const u32x4* from, u32x4* to, int runs, int length, int pitch, int first) {
-  const int n = runs * length;
-  u32x4 v[4];
-  int at[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t u = first + i * 256 + threadIdx.x;
-    at[i] = -1;
-    if (u >= (uint32_t)n) continue;
-    at[i] = length == pitch ? u : u / (uint32_t)length * pitch + u % (uint32_t)length;
-    v[i] = from[at[i]];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (at[i] >= 0) to[at[i]] = v[i];
+// STREAM: past the caches (copies that they do not hold).
+template <bool STREAM>
+__device__ __forceinline__ u32x4 read16(const u32x4* p) {
+  return STREAM ? __builtin_nontemporal_load(p) : *p;
+}
+template <bool STREAM>
+__device__ __forceinline__ void write16(u32x4* p, u32x4 v) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(v, p);
+  else
+    *p = v;
 }
 
+// n / d for n below 2^22 and d up to 1024, by a multiplication (once: 1, off by less than d 2^-32).
+struct Divisor {
+  uint32_t d, inv;
+  __device__ __forceinline__ explicit Divisor(uint32_t v) : d(v), inv(0xffffffffu / v + 1) {}
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return d == 1 ? n : __umulhi(n, inv); }
+};
+
 // grid (parts of a page, pairs, caches x sides): the parts of the codes, behind them those of the scales
+// (in workgroups of their own: 48 forks in 16 8-bit caches 19 us, with the codes' ones 24).  A thread
+// has four 16-byte units, all loaded before the first is stored.
+template <bool STREAM>
 __global__ __launch_bounds__(256) void kv_copy_kernel(CopyParams p, int parts) {
-  const int pair = blockIdx.y, cache = blockIdx.z >> 1, part = blockIdx.x;
+  const int pair = blockIdx.y, cache = blockIdx.z >> 1;
   const bool value = blockIdx.z & 1;
-  const int page = 1 << p.page_shift, slots = p.slots[pair];
+  const uint32_t page = 1u << p.page_shift, slots = p.slots[pair];
   const int64_t src = p.src[pair], dst = p.dst[pair];
-  if (part < parts) {
-    const int units = p.row / 16;  // of a slot
-    uint8_t* pool = value ? p.values[cache] : p.keys[cache];
-    const size_t bytes = (size_t)p.kv_heads * page * p.row;
-    copy_units((const u32x4*)(pool + src * bytes), (u32x4*)(pool + dst * bytes), p.kv_heads, slots * units,
-               page * units, part * kUnits);
+  if ((int)blockIdx.x < parts) {
+    // codes: the runs of all heads, `slots` slots each of 2^shift units, `page` slots apart
+    const int shift = __builtin_ctz(p.row) - 4;
+    const uint32_t units = (p.kv_heads * slots) << shift, first = blockIdx.x * kUnits + threadIdx.x;
+    const int64_t whole = ((int64_t)p.kv_heads * page) << shift;
+    u32x4* pool = (u32x4*)(value ? p.values[cache] : p.keys[cache]);
+    const u32x4* from = pool + src * whole;
+    u32x4* to = pool + dst * whole;
+    const Divisor by(slots);
+    u32x4 v[4];
+    uint32_t at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = first + i * 256;
+      at[i] = u + ((by.quotient(u >> shift) * (page - slots)) << shift);
+      if (u < units) v[i] = read16<STREAM>(from + at[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (first + i * 256 < units) write16<STREAM>(to + at[i], v[i]);
     return;
   }
+  // scales: the runs of all groups, eight slots at a time, the last ones of a run one by one
   uint16_t* pool = value ? p.value_scales[cache] : p.key_scales[cache];
-  const int runs = p.kv_heads * p.groups;
-  const uint16_t* from = pool + src * ((int64_t)runs << p.page_shift);
-  uint16_t* to = pool + dst * ((int64_t)runs << p.page_shift);
-  const int first = (part - parts) * kUnits;
-  if (slots == page) {
-    copy_units((const u32x4*)from, (u32x4*)to, runs, page / 8, page / 8, first);
-    return;
-  }
-  // eight slots at a time, the last ones of a run one by one
-  const uint32_t pieces = (slots + 7) / 8;
+  const uint32_t runs = p.kv_heads * p.groups, pieces = (slots + 7) / 8;
+  const uint16_t* from = pool + ((src * runs) << p.page_shift);
+  uint16_t* to = pool + ((dst * runs) << p.page_shift);
+  const Divisor by(pieces);
   for (int i = 0; i < 4; ++i) {
-    const uint32_t u = first + i * 256 + threadIdx.x;
+    const uint32_t u = (blockIdx.x - parts) * kUnits + i * 256 + threadIdx.x;
     if (u >= runs * pieces) return;
-    const int run = u / pieces, slot = u % pieces * 8, at = (run << p.page_shift) + slot;
+    const uint32_t run = by.quotient(u), slot = (u - run * pieces) * 8, at = (run << p.page_shift) + slot;
     if (slot + 8 <= slots) {
-      *(u32x4*)(to + at) = *(const u32x4*)(from + at);
+      write16<STREAM>((u32x4*)(to + at), read16<STREAM>((const u32x4*)(from + at)));
     } else {
-      for (int e = 0; e < slots - slot; ++e) to[at + e] = from[at + e];
+      for (uint32_t e = 0; e < slots - slot; ++e) to[at + e] = from[at + e];
     }
   }
 }
+template __global__ void kv_copy_kernel<false>(CopyParams, int);
+template __global__ void kv_copy_kernel<true>(CopyParams, int);
 
 }  // namespace exl3
 
@@ -93,7 +111,9 @@ using namespace exl3;
 
 #ifndef __HIP_DEVICE_COMPILE__
 
-static_assert(sizeof(CopyParams) + 16 <= 4096, "a launch takes 4 KB of arguments");
+constexpr double kCached = 64.0 * 1048576;  // bytes copied beyond which a copy goes past the caches
+
+static_assert(sizeof(CopyParams) + 8 <= 4096, "a launch takes 4 KB of arguments");
 
 // What a copy of pages refuses, before anything is launched: every page is in all pools, none is
 // written twice or written and read.
@@ -154,6 +174,18 @@ extern "C" int exl3_kv_copy_pages(const exl3_kv_cache* const* caches, int32_t co
     return a.format == b.format && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim;
   };
   if (int rc = launch_gate("KV page copy")) return rc;
+  // Copies that the caches (256 MB) do not hold with their source go past them.  Cold, us, 16-bit pages of
+  // four caches: 31 MB 14.3 past them, 18.5 through them; 63 MB 25.7, 30.8; 121 MB 50, 58.  But source and
+  // copy are read again soon where a sequence is forked: 48 forks in 16 caches and the attention of all
+  // layers after them 162 past them, 150 through them.
+  double bytes = 0.0;
+  for (int i = 0; i < count; ++i) {
+    const KvCacheView& v = caches[i]->view;
+    bytes += 2.0 * v.kv_heads * v.head_dim * (v.format == EXL3_KV_Q4 ? 0.5 : v.format == EXL3_KV_Q8 ? 1.0 : 2.0);
+  }
+  int64_t filled = 0;
+  for (int64_t i = 0; i < pairs; ++i) filled += slots ? slots[i] : 1 << caches[0]->view.page_shift;
+  const bool stream_past = bytes * filled > kCached;
   CopyParams p;
   for (int first = 0; first < count; ++first) {
     // the caches of one shape together, where its first one stands
@@ -180,18 +212,21 @@ extern "C" int exl3_kv_copy_pages(const exl3_kv_cache* const* caches, int32_t co
       for (int64_t at = 0; at < pairs;) {
         int m = 0, most = 0;
         for (; at < pairs && m < kMostPairs; ++at) {
-          const int filled = slots ? slots[at] : 1 << c.page_shift;
-          if (filled == 0) continue;
+          const int used = slots ? slots[at] : 1 << c.page_shift;
+          if (used == 0) continue;
           p.src[m] = src[at];
           p.dst[m] = dst[at];
-          p.slots[m++] = (uint16_t)filled;
-          most = std::max(most, filled);
+          p.slots[m++] = (uint16_t)used;
+          most = std::max(most, used);
         }
         if (m == 0) continue;
-        const int parts = (most * p.kv_heads * (p.row / 16) + kUnits - 1) / kUnits;
-        const int more = (p.kv_heads * p.groups * ((most + 7) / 8) + kUnits - 1) / kUnits;
-        hipLaunchKernelGGL(kv_copy_kernel, dim3((unsigned)(parts + more), (unsigned)m, 2u * (unsigned)n), dim3(256), 0,
-                           (hipStream_t)stream, p, parts);
+        const int codes = most * p.kv_heads * (p.row / 16), scales = p.kv_heads * p.groups * ((most + 7) / 8);
+        const int parts = (codes + kUnits - 1) / kUnits;
+        const dim3 grid((unsigned)(parts + (scales + kUnits - 1) / kUnits), (unsigned)m, 2u * (unsigned)n);
+        if (stream_past)
+          hipLaunchKernelGGL(kv_copy_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, p, parts);
+        else
+          hipLaunchKernelGGL(kv_copy_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, p, parts);
         if (int rc = check_launch("KV page copy")) return rc;
       }
     }
