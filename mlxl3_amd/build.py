@@ -25,7 +25,8 @@ LIB = HERE / "libexl3_hip.so"
 CODEC = HERE / "exl3_codec"  # the codec JSON-lines driver (links LIB)
 SOURCES = ["exl3_api.hip", "exl3_qmv.hip", "exl3_qmm.hip", "exl3_wide.hip", "exl3_moe.hip", "exl3_moe_wide.hip",
            "exl3_mapped.hip", "exl3_kv.hip", "exl3_pages.hip", "exl3_attn.hip",
-           "exl3_attn_early.hip", "exl3_attn_late.hip", "exl3_norm.hip", "exl3_checkpoint.cpp"]
+           "exl3_attn_early.hip", "exl3_attn_capped.hip", "exl3_attn_late.hip",
+           "exl3_norm.hip", "exl3_checkpoint.cpp"]
 ARCH = "gfx950"
 
 # -ffp-contract=off: every f32 multiply/add in the glue is rounded separately,

@@ -208,7 +208,11 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
     p.cap2 = cap * kLog2e;
     p.slopes = scores->slopes;
     p.prefix = causal ? scores->prefix : nullptr;
-    if (cap != 0.0f || (p.slopes && !(scale2 >= 0x1p-30f && scale2 <= 0x1p30f)))
+    // the factors of kCapped and kEarly far inside f32's range, else one after the other
+    const float rate = cap != 0.0f ? 2.0f * kLog2e / p.cap2 * scale2 : 0.0f;
+    if (cap != 0.0f && p.cap2 <= kLargeCap && rate >= 0x1p-100f && rate <= 0x1p100f)
+      shaped = kCapped;
+    else if (cap != 0.0f || (p.slopes && !(scale2 >= 0x1p-30f && scale2 <= 0x1p30f)))
       shaped = kLate;
     else if (p.slopes || p.prefix)
       shaped = kEarly;
@@ -251,14 +255,15 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
   p.q_vec = aligned16(q) && (tokens == 1 || q_stride % 8 == 0);
   p.y_vec = ((uintptr_t)y & 7) == 0 && (tokens == 1 || y_stride % 4 == 0);
   p.scale2 = scale2;
-  if (p.cap2 > 0.0f) cap_polynomials(p);
   p.part = (float*)workspace;
   p.stats = (float*)((uint8_t*)workspace + align256((size_t)sh.slots * sh.rows * p.cache.head_dim * 4));
   const int D = p.cache.head_dim;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = launch_gate("attention")) return rc;
-  shaped == kPlain ? launch_attention<kPlain>(p, sh, s)
-  : shaped == kEarly ? launch_attention_early(p, sh, s) : launch_attention_late(p, sh, s);
+  shaped == kPlain    ? launch_attention<kPlain>(p, sh, s)
+  : shaped == kEarly  ? launch_attention_early(p, sh, s)
+  : shaped == kCapped ? launch_attention_capped(p, sh, s)
+                      : launch_attention_late(p, sh, s);
   if (int rc = check_launch("attention")) return rc;
   if (!sh.slots) return EXL3_OK;
   if (int rc = launch_gate("attention join")) return rc;

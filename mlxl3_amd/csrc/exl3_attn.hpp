@@ -22,10 +22,8 @@ struct AttnParams {
   int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
   int q_vec, y_vec;  // rows of q are 16-byte, rows of y 8-byte aligned
   float scale2;   // scale * log2(e): scores in units of a factor of two
-  // of calls with shaped scores (the kernels' S): cap2 = cap * log2(e), 0 without a cap, and Cap's
-  // polynomials in squared products
+  // of calls with shaped scores (the kernels' S): cap2 = cap * log2(e), 0 without a cap
   float cap2;
-  float cap_to[2], cap_near[4], cap_far[6];
   const float* slopes;    // of every head, or null
   const int32_t* prefix;  // of every sequence, or null
 };
@@ -333,85 +331,40 @@ __device__ __forceinline__ float slack_at(float m, float slack) {
 // Shaped scores: x is a score in factors of two, s scale log2(e).
 //
 // Capped it is cap2 tanh(u), u = x / cap2: a score z becomes cap tanh(z / cap).  tanh(u) = 1 - 2 / (1 +
-// e^2u) is off by 2^-23 or so whatever u, the capped score by cap2 times that, 1e-5 under a cap of 50.
-// Above a cap of 1024 that is too much for small scores: |u| < 1/4 takes tanh's series there.
+// e^2u), and of all scores of a row softmax takes off what it likes: less cap2 a capped score is
+//   2 cap2 c,  c = -1 / (1 + 2^(rate x)),  rate = 2 log2(e) / cap2.
+// So a call with a cap (kCapped) puts c where the product was, in four instructions, and goes on as a
+// plain one whose scale is 2 cap2.  c is off by 2^-23 or so, the score by cap2 times that, 1e-5
+// under a cap of 50.  (tanh's polynomials in u^2 up to |u| = 1, in tiles where no score is beyond, are
+// as many instructions or more and a maximum: 2048 rows over 8192 bf16 tokens 335 us for 304, plain 256.)
 //
-// Up to |u| = 1 (scores up to 50 under a cap of 50) tanh(u) is u times a polynomial in u^2, off by 7e-7
-// of itself (fitted to the least largest error, first coefficient 1): of degree 3 up to 1/2, of 5 up to
-// 1.  Where no score of a wave's tile is beyond that, it takes the place of two transcendentals, at a
-// quarter of the rate, and four more instructions: x = S c(S^2), S the product as it is, the host's
-// coefficients with the scale in them.
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr double kTanhNear[4] = {1.0, -0.33328159331842044, 0.13205359636370356, -0.044750641313108026};
-constexpr double kTanhFar[6] = {1.0, -0.33330279667160123, 0.13288490228334163, -0.05176828405213653,
-                                0.01690640684211184, -0.003126576844036082};
-// The largest products that the polynomials take (0: none do, a power of them leaves f32's range), and
-// their coefficients.
-inline void cap_polynomials(AttnParams& p) {
-  const double r = (double)p.scale2 / p.cap2;  // u / S
-  if (!(r >= 0x1p-12 && r <= 0x1p10) || p.cap2 > 1024.0f * kLog2e) return;
-  p.cap_to[0] = (float)(0.5 / r);
-  p.cap_to[1] = (float)(1.0 / r);
-  double power = p.scale2;
-  for (int i = 0; i < 6; ++i, power *= r * r) {
-    if (i < 4) p.cap_near[i] = (float)(kTanhNear[i] * power);
-    p.cap_far[i] = (float)(kTanhFar[i] * power);
-  }
-}
-struct Cap {
-  float cap2, inv, rate;
-  bool large;
-  __device__ __forceinline__ explicit Cap(float c)
-      : cap2(c), inv(1.0f / c), rate(2.0f * kLog2e * inv), large(c > 1024.0f * kLog2e) {}
-  __device__ __forceinline__ float any(float x) const {
-    const float far = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * rate)), cap2);
-    if (!large) return far;
-    const float u = x * inv, v = u * u;
-    const float series =
-        fmaf(v, fmaf(v, fmaf(v, fmaf(v, 0.021869489f, -0.053968254f), 0.13333333f), -0.33333333f), 1.0f);
-    return fabsf(u) < 0.25f ? x * series : far;
-  }
-};
-// N products of every lane of a wave (of rows that were scaled, `unscale` less) as scores: times the
-// scale, and capped.
-template <bool SCALED, int N, typename G, typename P>
-__device__ __forceinline__ void scores_of(const AttnParams& p, const Cap& cap, float unscale, G&& get, P&& put) {
-  if (p.cap2 > 0.0f) {
-    float most = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if constexpr (SCALED) put(i, get(i) * unscale);
-      most = fmaxf(most, fabsf(get(i)));
-    }
-    if (!__any(most > p.cap_to[0])) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float x = get(i), v = x * x;
-        put(i, x * fmaf(v, fmaf(v, fmaf(v, p.cap_near[3], p.cap_near[2]), p.cap_near[1]), p.cap_near[0]));
-      }
-    } else if (!__any(most > p.cap_to[1])) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float x = get(i), v = x * x;
-        float c = fmaf(v, p.cap_far[5], p.cap_far[4]);
-#pragma unroll
-        for (int k = 3; k >= 0; --k) c = fmaf(v, c, p.cap_far[k]);
-        put(i, x * c);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) put(i, cap.any(get(i) * p.scale2));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) put(i, get(i) * (SCALED ? unscale * p.scale2 : p.scale2));
-  }
-}
-// The bias by distance: slope2 = slope log2(e) times it off the score.  Without a cap the sums of the
+// The bias by distance takes slope2 = slope log2(e) times it off the score.  Without a cap the sums of the
 // products start from it, divided by what scores are multiplied by (kEarly), and all else is as for
-// plain scores; that takes scales of 2^-30 to 2^30 and slopes up to 2^32.  Else (kLate) scores are
-// multiplied by the scale, capped, biased.
-enum : int { kPlain = 0, kEarly = 1, kLate = 2 };
+// plain scores; under a cap it is added to c, divided by 2 cap2.
+//
+// Caps above 1024, where the error above is too much for small scores (|u| < 1/4 takes tanh's series there,
+// and nothing is taken off), and factors whose quotients may leave f32's range go one step
+// after the other (kLate): times the scale, capped, biased.
+enum : int { kPlain = 0, kEarly = 1, kCapped = 2, kLate = 3 };
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLargeCap = 1024.0f * kLog2e;
+__device__ __forceinline__ float squashed(float x, float rate) {
+  return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * rate));
+}
+// What c's exponent is of a product, that of a score (both finite and positive).
+__device__ __forceinline__ float cap_rate(const AttnParams& p, float scale2) {
+  return fminf(2.0f * kLog2e / p.cap2 * scale2, 3.402823466e38f);
+}
+// A score capped, where there is a cap.
+__device__ __forceinline__ float capped(const AttnParams& p, float x) {
+  if (p.cap2 == 0.0f) return x;
+  const float c = 2.0f * p.cap2 * squashed(x, cap_rate(p, 1.0f));
+  if (p.cap2 <= kLargeCap) return c;
+  const float u = x / p.cap2, v = u * u;
+  const float series =
+      fmaf(v, fmaf(v, fmaf(v, fmaf(v, 0.021869489f, -0.053968254f), 0.13333333f), -0.33333333f), 1.0f);
+  return fabsf(u) < 0.25f ? x * series : p.cap2 + c;
+}
 __device__ __forceinline__ float biased(float x, float slope2, float away) { return fmaf(-slope2, fabsf(away), x); }
 __device__ __forceinline__ float slope_of(const AttnParams& p, int head) {
   return p.slopes ? __builtin_amdgcn_fmed3f(p.slopes[head], -4294967296.0f, 4294967296.0f) * kLog2e : 0.0f;
@@ -465,7 +418,7 @@ __device__ __forceinline__ void row_pass(const AttnParams& p, const Work& w, int
     }
     s = wave_sum(s) * p.scale2;
     if constexpr (S) {
-      if (p.cap2 > 0.0f) s = Cap(p.cap2).any(s);
+      s = capped(p, s);
       if (p.slopes) s = biased(s, slope_of(p, kvh * p.group + row % p.group), (float)(w.first + row / p.group - t));
     }
     const float n = fmaxf(m, s);

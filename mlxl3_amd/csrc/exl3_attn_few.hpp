@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   const int n = lane & 15, g = lane >> 4;
   uint8_t* my = lds + wave * F::kWaveLds;
   V8 q[RT][F::kSteps];
-  float scale2[RT], unscale[RT];  // the call's, of rows that were scaled times the inverse; that inverse
+  float scale2[RT], rate[RT];  // the call's, of rows that were scaled times the inverse; of capped scores
   Seen see[RT];
   float slope2[RT];  // of shaped scores: the row's bias,
   int at[RT];        // its position less this lane's first token of a step
@@ -259,7 +259,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
     u32x4 raw[F::kSteps];
     float factor = 1.0f, most = 0.0f;
     scale2[rt] = p.scale2;
-    unscale[rt] = 1.0f;
 #pragma unroll
     for (int s = 0; s < F::kSteps; ++s) raw[s] = load_q8(p, qi + F::channel(s, g));
     if constexpr (F::kScaled) {
@@ -270,7 +269,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
       const uint32_t e = fit_exponent<S>(most);
       factor = fit_factor(e);
       scale2[rt] = fit_scale(p.scale2, e);
-      unscale[rt] = fit_scale(1.0f, e);
     }
 #pragma unroll
     for (int s = 0; s < F::kSteps; ++s) q[rt][s] = query_operand<FMT, T, F::kScaled>(raw[s], factor);
@@ -288,17 +286,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
   // of the wave, and what scores are multiplied by as weights; far (kFar): less than 0 and 1
   float slack = kSlack + T::kRoom, unit[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) unit[rt] = scale2[rt];
-  if constexpr (S) {
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if (S == kLate)
-        unit[rt] = 1.0f;
-      else
-        slope2[rt] /= scale2[rt];
+  for (int rt = 0; rt < RT; ++rt) {
+    if constexpr (S == kEarly) slope2[rt] /= scale2[rt];
+    if constexpr (S == kCapped) {
+      rate[rt] = cap_rate(p, scale2[rt]);
+      scale2[rt] = 2.0f * p.cap2;
+      slope2[rt] /= scale2[rt];
     }
+    unit[rt] = S == kLate ? 1.0f : scale2[rt];
   }
-  const Cap cap(S == kLate ? p.cap2 : 1.0f);
 
   typename F::Keys k;
   typename F::Values v;
@@ -369,13 +365,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : RT == 1 ? 3 : 2) void attn_few_
       float x[8], most = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = s[rt][i >> 2][i & 3];
-      if constexpr (S == kLate) {
-        scores_of<F::kScaled, 8>(p, cap, unscale[rt], [&](int i) { return x[i]; }, [&](int i, float v) { x[i] = v; });
+      if constexpr (S == kCapped) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = squashed(x[i], rate[rt]);
         if (p.slopes) {
           const float away = (float)(at[rt] - t);
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = biased(x[i], slope2[rt], away - (float)((i >> 2) * 16 + (i & 3)));
         }
+      }
+      if constexpr (S == kLate) {
+        const float away = (float)(at[rt] - t);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[i] = biased(capped(p, x[i] * scale2[rt]), slope2[rt], away - (float)((i >> 2) * 16 + (i & 3)));
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {

@@ -84,8 +84,9 @@ void launch_attention(const AttnParams& p, const AttnShape& sh, hipStream_t s) {
 
 #endif  // __HIP_DEVICE_COMPILE__
 
-// launch_attention<kEarly> and <kLate>, of the other translation units.
+// launch_attention<kEarly>, <kCapped> and <kLate>, of the other translation units.
 void launch_attention_early(const AttnParams& p, const AttnShape& sh, hipStream_t s);
+void launch_attention_capped(const AttnParams& p, const AttnShape& sh, hipStream_t s);
 void launch_attention_late(const AttnParams& p, const AttnShape& sh, hipStream_t s);
 
 }  // namespace exl3

@@ -196,9 +196,9 @@ void attn_many_kernel(AttnParams p, int tiles) {
   const Seen wtop = row_sees<S>(p, w, min(wrow, row0 + rows - 1));
   const Seen wend = row_sees<S>(p, w, min(wrow + 31, row0 + rows - 1));
   V8 q[D / 16];
-  float scale2 = p.scale2, unscale = 1.0f;  // of rows that were scaled times the inverse; that inverse
-  constexpr bool kScaled = !F::kRaw && PARTS == 1;  // bf16 queries, to fit f16
+  float scale2 = p.scale2;  // of rows that were scaled times the inverse
   {
+    constexpr bool kScaled = !F::kRaw && PARTS == 1;  // bf16 queries, to fit f16
     const size_t qi = (size_t)(w.start + mine / p.group) * p.q_stride +
                       (size_t)(kvh * p.group + mine % p.group) * D;
     u32x4 raw[D / 16];
@@ -212,7 +212,6 @@ void attn_many_kernel(AttnParams p, int tiles) {
       const uint32_t e = fit_exponent<S>(most);
       factor = fit_factor(e);
       scale2 = fit_scale(p.scale2, e);
-      unscale = fit_scale(1.0f, e);
     }
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) q[s] = query_operand<FMT == KV_Q4 ? KV_Q8 : FMT, T, kScaled>(raw[s], factor);
@@ -220,8 +219,9 @@ void attn_many_kernel(AttnParams p, int tiles) {
   // of shaped scores: the row's bias, its position less this lane's first token of a tile
   float slope2 = S ? slope_of(p, kvh * p.group + mine % p.group) : 0.0f;
   const int at = w.first + mine / p.group - 4 * h, nearest = w.first + wrow / p.group;
-  if (S == kEarly) slope2 /= scale2;
-  const Cap cap(S == kLate ? p.cap2 : 1.0f);
+  const float rate = S == kCapped ? cap_rate(p, scale2) : 0.0f;
+  if (S == kCapped) scale2 = 2.0f * p.cap2;
+  if (S == kEarly || S == kCapped) slope2 /= scale2;
   float16v o[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
@@ -339,15 +339,22 @@ void attn_many_kernel(AttnParams p, int tiles) {
       for (int i = 0; i < DT; ++i) vf[i] = value(i);
       pin();
       __builtin_amdgcn_s_setprio(0);
-      if constexpr (S == kLate) {
-        scores_of<kScaled, 16 * NT>(p, cap, unscale, [&](int i) { return s[i / 16][i % 16]; },
-                                    [&](int i, float v) { s[i / 16][i % 16] = v; });
+      if constexpr (S == kCapped) {
+#pragma unroll
+        for (int i = 0; i < 16 * NT; ++i) s[i / 16][i % 16] = squashed(s[i / 16][i % 16], rate);
         if (p.slopes) {
           const float away = (float)(at - t);
 #pragma unroll
           for (int i = 0; i < 16 * NT; ++i)
             s[i / 16][i % 16] = biased(s[i / 16][i % 16], slope2, away - (float)(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4));
         }
+      }
+      if constexpr (S == kLate) {
+        const float away = (float)(at - t);
+#pragma unroll
+        for (int i = 0; i < 16 * NT; ++i)
+          s[i / 16][i % 16] = biased(capped(p, s[i / 16][i % 16] * scale2), slope2,
+                                     away - (float)(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4));
       }
       if (t < wend.lo || t + TK > min(wtop.hi, t1)) {
         // token r of the tile is one of the row's `n` from `lo` on
