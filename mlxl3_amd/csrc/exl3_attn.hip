@@ -208,14 +208,12 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
     p.cap2 = cap * kLog2e;
     p.slopes = scores->slopes;
     p.prefix = causal ? scores->prefix : nullptr;
-    // the factors of kCapped and kEarly far inside f32's range, else one after the other
+    // the factors of kCapped and kEarly far inside f32's range, else one step after the other
     const float rate = cap != 0.0f ? 2.0f * kLog2e / p.cap2 * scale2 : 0.0f;
-    if (cap != 0.0f && p.cap2 <= kLargeCap && rate >= 0x1p-100f && rate <= 0x1p100f)
-      shaped = kCapped;
-    else if (cap != 0.0f || (p.slopes && !(scale2 >= 0x1p-30f && scale2 <= 0x1p30f)))
-      shaped = kLate;
+    if (cap != 0.0f)
+      shaped = p.cap2 <= kLargeCap && rate >= 0x1p-100f && rate <= 0x1p100f ? kCapped : kLate;
     else if (p.slopes || p.prefix)
-      shaped = kEarly;
+      shaped = scale2 >= 0x1p-20f && scale2 <= 0x1p20f ? kEarly : kLate;
   }
   if (batch->max_q < 1) return fail(EXL3_EINVAL, "max_q must be positive");
   if (batch->seqs > 65535)

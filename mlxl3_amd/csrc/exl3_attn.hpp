@@ -6,6 +6,9 @@
 
 namespace exl3 {
 
+// What becomes of scores (the kernels' S; below).
+enum : int { kPlain = 0, kEarly = 1, kCapped = 2, kLate = 3 };
+
 struct AttnParams {
   KvCacheView cache;
   KvBatchView batch;
@@ -22,7 +25,7 @@ struct AttnParams {
   int one_tile;   // every sequence's rows fit one workgroup: tile = sequence
   int q_vec, y_vec;  // rows of q are 16-byte, rows of y 8-byte aligned
   float scale2;   // scale * log2(e): scores in units of a factor of two
-  // of calls with shaped scores (the kernels' S): cap2 = cap * log2(e), 0 without a cap
+  // of calls with shaped scores: cap2 = cap * log2(e), 0 without a cap
   float cap2;
   const float* slopes;    // of every head, or null
   const int32_t* prefix;  // of every sequence, or null
@@ -137,7 +140,7 @@ __device__ __forceinline__ float largest_bf16(const u32x4& w, float most) {
 // Shaped scores (S): from 2^-10 down, which leaves the queries' error far below a bias's.
 template <int S>
 __device__ __forceinline__ uint32_t fit_exponent(float most) {
-  return max(__builtin_bit_cast(uint32_t, most) >> 23, S ? 117u : 16u);
+  return max(__builtin_bit_cast(uint32_t, most) >> 23, S == kEarly ? 117u : 16u);
 }
 __device__ __forceinline__ float fit_factor(uint32_t e) { return __builtin_bit_cast(float, (269 - e) << 23); }
 // The scale times the inverse, a normal f32 too: a masked score, -inf, times zero would be NaN,
@@ -342,12 +345,11 @@ __device__ __forceinline__ float slack_at(float m, float slack) {
 // products start from it, divided by what scores are multiplied by (kEarly), and all else is as for
 // plain scores; under a cap it is added to c, divided by 2 cap2.
 //
-// Caps above 1024, where the error above is too much for small scores (|u| < 1/4 takes tanh's series there,
+// Caps above 256, where the error above is too much for small scores (|u| < 1/4 takes tanh's series there,
 // and nothing is taken off), and factors whose quotients may leave f32's range go one step
 // after the other (kLate): times the scale, capped, biased.
-enum : int { kPlain = 0, kEarly = 1, kCapped = 2, kLate = 3 };
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLargeCap = 1024.0f * kLog2e;
+constexpr float kLargeCap = 256.0f * kLog2e;
 __device__ __forceinline__ float squashed(float x, float rate) {
   return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * rate));
 }

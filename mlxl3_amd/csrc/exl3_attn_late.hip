@@ -1,4 +1,4 @@
-// Attention with caps above 1024 and with factors whose quotients may leave f32's range: the kernels of
+// Attention with caps above 256 and with factors whose quotients may leave f32's range: the kernels of
 // exl3_attn_few.hpp and exl3_attn_many.hpp with kLate (exl3_attn.hpp says what it adds).
 #include <hip/hip_runtime.h>
 

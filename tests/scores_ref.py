@@ -16,8 +16,7 @@ def attend(q, k, v, first, scale, causal, window, softcap=0.0, slopes=None, pref
     A score's error: that of a plain one (its f32 sum of dim products, the product with the scale;
     coded keys rounded to f16, 2^-11); a cap does not enlarge it (its slope is at most 1) and adds its
     own: 2^-21 of the cap -- 1 - 2 / (1 + e) with e off by 2^-22 or so of itself, which moves 1 / (1 + e) by
-    at most a quarter of that, its sum and reciprocal rounded to 1.5 * 2^-24; or the polynomial's
-    6.5e-7 of a score of up to half the cap, which is less; above a cap of 1024 the series', 2^-22 of
+    at most a quarter of that, its sum and reciprocal rounded to 1.5 * 2^-24; above a cap of 256 the series', 2^-22 of
     the score, up to a quarter of the cap; the bias: a slope over a scale, a distance and their product
     rounded (2^-22 of it), and where it is what the f32 sum of the products starts from, as much of it as
     of them is lost there, dim half steps.  The rest is as for plain
@@ -41,7 +40,7 @@ def attend(q, k, v, first, scale, causal, window, softcap=0.0, slopes=None, pref
         z = (q[:, h] @ kh.T) * scale
         e = (q[:, h].abs() @ kh.abs().T) * scale * (dim * 2.0**-24 + 2.0**-22 + (2.0**-11 if coded else 0.0))
         if softcap:
-            if softcap <= 1024:
+            if softcap <= 256:
                 e = e + softcap * 2.0**-21
             else:
                 e = e + torch.where(z.abs() < softcap / 4.01, 2.0**-22 * z.abs(), torch.full_like(z, softcap * 2.0**-21))

@@ -76,7 +76,7 @@ def test_shapes(bits, cdtype, dtype, dim, kv_heads, group, page, new, old, kind)
     check(pool, new, q, y, **kw)
 
 
-@pytest.mark.parametrize("softcap", [2.0**-64, 1e-6, 0.02, 1.0, 15.0, 50.0, 1000.0, 1025.0, 1e5, 2.0**64])
+@pytest.mark.parametrize("softcap", [2.0**-64, 1e-6, 0.02, 1.0, 15.0, 50.0, 255.0, 257.0, 1000.0, 1e5, 2.0**64])
 @pytest.mark.parametrize("gain", [0.05, 1.0, 20.0, 600.0])
 @pytest.mark.parametrize("new, old", [([1, 3], [200, 31]), ([40], [100])])
 def test_caps_and_scores_of_all_sizes(softcap, gain, new, old):
@@ -115,12 +115,14 @@ def test_biases_of_queries_of_all_sizes(bits, cdtype, dtype, gain):
             check(pool, new, q, y, **kw)
 
 
-@pytest.mark.parametrize("scale", [1e-36, 1e-12, 3.0, 1e9, 1e30])
-def test_scales_of_all_sizes(scale):
+@pytest.mark.parametrize("scale", [1e-36, 1e-12, 1e-5, 3.0, 1e5, 1e9, 1e30])
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_scales_of_all_sizes(bits, scale):
     """Scales that a bias is not divided by, and others; queries of the inverse size."""
     for new, lens in (([1, 2], [300, 33]), ([50], [200])):
-        pool = Pool(26, lens, 2, 128, 16, 16, BF16, loud=1.0)
-        for kw in (dict(slopes=geometric(4)), dict(softcap=4.0), dict(prefix=[20, 5][: len(new)])):
+        pool = Pool(26, lens, 2, 128, 16, bits, BF16, loud=1.0)
+        for kw in (dict(slopes=geometric(4)), dict(softcap=4.0), dict(softcap=4.0, slopes=geometric(4)),
+                   dict(softcap=300.0, slopes=geometric(4)), dict(prefix=[20, 5][: len(new)])):
             q, _, _, y, _ = run(pool, new, 4, BF16, gain=0.1 / scale, scale=scale, **kw)
             check(pool, new, q, y, scale=scale, **kw)
 
