@@ -1,11 +1,11 @@
 // Pages of the paged cache copied (layout: exl3_kv.hpp): forked sequences' last pages, pools
 // that are compacted.
 //
-// One launch copies up to 224 pairs of pages in up to 32 caches of one shape -- a model's layers --
+// One launch copies up to 300 pairs of pages in up to 32 caches of one shape -- a model's layers --
 // named in the kernel's arguments, so that nothing is uploaded.  Where a pair copies its first
 // n slots only, a head's n slots are one run of its page (its scales n of every group's run).
 // Memory bounds it: every byte is read and written once, 16 at a time.  Measured, sources not in the
-// caches: 230 pages of 131 KB in 4 caches, 121 MB, 50 us, 4.8 TB/s read and written (a large copy: 5.1);
+// caches: 230 pages of 131 KB in 4 caches, 121 MB, 47 us, 5.1 TB/s read and written (a large copy: 5.1);
 // 48 partly filled 8-bit pages in 16 caches, 27 MB, 19 us (in the caches 11); one page's 9 slots in 32
 // caches 3.7 us, a launch and one round trip.
 #include <hip/hip_runtime.h>
@@ -21,7 +21,7 @@
 
 namespace exl3 {
 
-constexpr int kMostCaches = 32, kMostPairs = 224;  // of a launch: 3.8 KB of arguments, of 4 that it takes
+constexpr int kMostCaches = 32, kMostPairs = 300;  // of a launch: 4.0 KB of arguments, as many as it takes
 constexpr int kUnits = 1024;                       // 16-byte units of a workgroup, four a thread
 
 struct CopyParams {
@@ -175,7 +175,7 @@ extern "C" int exl3_kv_copy_pages(const exl3_kv_cache* const* caches, int32_t co
   };
   if (int rc = launch_gate("KV page copy")) return rc;
   // Copies that the caches (256 MB) do not hold with their source go past them.  Cold, us, 16-bit pages of
-  // four caches: 31 MB 14.3 past them, 18.5 through them; 63 MB 25.7, 30.8; 121 MB 50, 58.  But source and
+  // four caches: 31 MB 14.3 past them, 18.5 through them; 63 MB 25.7, 30.8; 121 MB 47, 58.  But source and
   // copy are read again soon where a sequence is forked: 48 forks in 16 caches and the attention of all
   // layers after them 162 past them, 150 through them.
   double bytes = 0.0;

@@ -57,8 +57,8 @@ def test_formats_and_slots(bits, dtype, page, heads, dim):
 def test_more_pages_and_caches_than_a_launch_names():
     caches = [cache(i, 700, 16, 1, 64, 4) for i in range(70)]
     order = torch.randperm(700, generator=torch.Generator().manual_seed(1)).tolist()
-    check(caches, order[:300], order[300:600])
-    check(caches, order[:300], order[300:600], [i % 17 for i in range(300)])
+    check(caches, order[:340], order[340:680])
+    check(caches, order[:340], order[340:680], [i % 17 for i in range(340)])
     check(caches[:1], [5] * 600, [p for p in range(601) if p != 5])
 
 
