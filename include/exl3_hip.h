@@ -259,8 +259,9 @@ int exl3_finish_and_reduce(const float* raw, const uint16_t* svh, const void* sc
 
 /* ------------------------------------------------------------------------
  * Between a layer's q/k/v projections and its output projection: rotary
- * positions, the paged key/value cache, attention over it.  (No counterpart
- * in the reference's EXL3 operators; its engine has kernels per model.)
+ * positions, the paged key/value cache, attention over it; and the norm in
+ * front of them.  (No counterpart in the reference's EXL3 operators; its
+ * engine has kernels per model.)
  * ------------------------------------------------------------------------ */
 
 /* What a cache stores: f16 or bf16 values, or 8- or 4-bit codes with one f16
@@ -382,8 +383,8 @@ int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const
 
 /* exl3_attention with shaped scores.  A score z = scale q.k becomes softcap tanh(z / softcap)
  * where softcap is not 0 (2^-64 to 2^64), then slopes[head] times the distance of the
- * row's position and the token's is taken off it (slopes finite, the sum of a score and a bias
- * too); and with causal != 0 every row sees the first prefix[b] tokens of its sequence beside
+ * row's position and the token's is taken off it (slopes finite, and counted up to 2^32; the sum of
+ * a score and a bias finite too); and with causal != 0 every row sees the first prefix[b] tokens of its sequence beside
  * those up to its own position (t < kv_lens[b] and the window hold for them as for others).
  * slopes (f32 [heads]) and prefix (int32 [seqs]) are device memory, read at every call, and may
  * be NULL; so may `scores`. */
