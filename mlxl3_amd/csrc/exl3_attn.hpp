@@ -137,7 +137,8 @@ __device__ __forceinline__ float largest_bf16(const u32x4& w, float most) {
   }
   return most;
 }
-// Shaped scores (S): from 2^-10 down, which leaves the queries' error far below a bias's.
+// Where the products' sums start from a bias (kEarly): from 2^-10 down, so that the bias over the scale
+// stays inside f32's range; queries are off by 2^-50 or so then.
 template <int S>
 __device__ __forceinline__ uint32_t fit_exponent(float most) {
   return max(__builtin_bit_cast(uint32_t, most) >> 23, S == kEarly ? 117u : 16u);
@@ -152,7 +153,7 @@ __device__ __forceinline__ float fit_scale(float scale2, uint32_t e) {
 
 // Eight query channels as T: T is the queries' own type for 16-bit caches, f16 for coded ones
 // (bf16 queries times `factor`; 4 bits: in codes4's order).
-template <int FMT, typename T, int SCALED>
+template <int FMT, typename T, bool SCALED>
 __device__ __forceinline__ typename T::V8 query_operand(const u32x4& w, float factor) {
   uint16_t h[8];
 #pragma unroll
@@ -175,7 +176,7 @@ __device__ __forceinline__ typename T::V8 query_operand(const u32x4& w, float fa
 // that q does not have are not touched, whatever q_starts says.
 struct Work {
   int seq, start, rows, first, len;
-  int prefix;            // tokens that all rows see (S)
+  int prefix;            // tokens that all rows see (0 of a plain call)
   const int32_t* table;  // the sequence's row of the block table
 };
 template <int S>

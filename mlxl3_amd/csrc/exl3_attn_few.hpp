@@ -16,7 +16,8 @@
 // inside 16 bits' and f32's range), so a step usually has no exchange between lanes
 // at all; the sum l is kept per lane and reduced once at the end.
 // The waves' results meet in LDS; with more than one range per sequence they are joined
-// by attn_join_kernel.
+// by attn_join_kernel.  Shaped scores (S, exl3_attn.hpp) take their instructions from S, before the
+// mask, or start the products' sums: within 2 % of plain ones at every size measured.
 //
 // P rounded to 16 bits is the product's operand type; its sum l is of the unrounded ones.
 // The loop's only waits are for its own loads: the next step's keys and values are on the

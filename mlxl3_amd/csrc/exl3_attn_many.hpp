@@ -10,6 +10,8 @@
 //   P             rounded to 16 bits, already the next product's B operand, its sum f32 of the
 //                 unrounded ones, the maximum with kSlack, as in attn_few_kernel;
 //   O^T += V^T P^T  V read from LDS transposed.
+// Shaped scores (S, exl3_attn.hpp): a bias is where S^T's sums start; a cap puts four instructions a
+// score behind the first product.
 // The next tile's loads are in flight meanwhile, straight into the other half of LDS or,
 // coded ones, into registers and from there decoded behind the products: one barrier per
 // tile.  Two workgroups share a CU (heads of 64: three), so that one's exponentials run beside
@@ -27,6 +29,9 @@
 // of 64 733 to 757, 610 / 431, 514 / 370 (half the products per exponential); of 256 630, 475 / 348,
 // 486 / 337 (one workgroup a CU: its registers).  Six prompts of 496 to 1500 tokens, heads of 64,
 // window 512: 46 us, 432 TFLOP/s, masked tiles and two rounds of short workgroups.
+// Shaped, 2048 tokens over 8192, us (plain 256 to 285): bf16 heads of 128 biased 250 to 257, capped 304 to
+// 324, both 317, with a prefix only 262 to 277; f16 heads of 64 (159) 161, 217 to 228, 242, 169;
+// bf16 heads of 256 (742) 762, 846, 827, 809; over 8 bits (335) 294, 366, 366, 327.
 // Where rows are done one by one (below, values that are not finite and some rows do not see) a
 // workgroup takes its rows times its tokens: one NaN in the newest of 8192 tokens makes 2048 rows'
 // 0.29 ms 268 ms.

@@ -436,9 +436,10 @@ def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, 
     written (in a new tensor they hold anything).
 
     Shaped scores (``exl3_attention_scores``): softcap > 0: a score z = scale q.k becomes
-    softcap * tanh(z / softcap); slopes (f32 [heads], finite, counted up to 2^32): then slope times
-    the distance of the token's position and the row's is taken off it; prefix (int32 [seqs], with causal): every
-    row sees the first prefix[b] tokens of its sequence too, as far as the window lets it."""
+    softcap * tanh(z / softcap); slopes (f32 [heads], finite, counted up to 2^32): then slope
+    times the distance of the token's position and the row's is taken off it; prefix (int32
+    [seqs], with causal): every row sees the first prefix[b] tokens of its sequence too, as far
+    as the window lets it."""
     torch = _torch()
     _floats()
     q = _heads(q, "q", _HALVES)
