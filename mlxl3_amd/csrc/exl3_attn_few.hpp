@@ -17,7 +17,7 @@
 // at all; the sum l is kept per lane and reduced once at the end.
 // The waves' results meet in LDS; with more than one range per sequence they are joined
 // by attn_join_kernel.  Shaped scores (S, exl3_attn.hpp) take their instructions from S, before the
-// mask, or start the products' sums: within 2 % of plain ones at every size measured.
+// mask, or start the products' sums: within 6 % of plain ones (one token over 1000: 11.3 us for 10.8).
 //
 // P rounded to 16 bits is the product's operand type; its sum l is of the unrounded ones.
 // The loop's only waits are for its own loads: the next step's keys and values are on the
