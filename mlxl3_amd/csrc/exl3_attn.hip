@@ -232,8 +232,8 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
     return fail(EXL3_EINVAL, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
   if (need && !aligned16(workspace))
     return fail(EXL3_EINVAL, "attention workspace must be 16-byte aligned");
-  // (a prefix may lie any number of tokens behind a window)
-  const AttnShape sh = choose(p.cache, *batch, tokens, heads, p.prefix ? 0 : window);
+  // (rows inside a prefix may see more than their window: the launch is shaped for the others)
+  const AttnShape sh = choose(p.cache, *batch, tokens, heads, window);
   if (sh.tiles * sh.splits * p.cache.kv_heads > kMostBlocks)
     return fail(EXL3_EUNSUPPORTED, "attention of %lld tokens needs too many workgroups", (long long)tokens);
   if (!run) return EXL3_OK;
