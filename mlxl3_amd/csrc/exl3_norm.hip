@@ -5,7 +5,7 @@
 //
 // s is f32 and not rounded on the way to y, the sum of squares is f32: up to 8 V squares in
 // a lane, then a tree.  Memory bounds it (every value is read and written once), so a row stays in
-// registers between its sum and its outputs: T threads hold 8 V values each.  Rows of more
+// registers between its sum and its outputs: T threads hold 8 V values each, as few as do.  Rows of more
 // than 32768 values are read again instead (from the caches).
 //
 // Measured, inputs not in the caches: 4096 rows of 4096 bf16 values with an f32 residual 36 us, 5.6 TB/s
@@ -43,11 +43,9 @@ __device__ __forceinline__ float row_sum(float v, float* parts) {
   v += xor_lanes<1>(v);
   v += xor_lanes<2>(v);
   v += xor_lanes<4>(v);
-  v += xor_lanes<8>(v);
-  if constexpr (T >= 64) {
-    v += xor_lanes<16>(v);
-    v += xor_lanes<32>(v);
-  }
+  if constexpr (T >= 16) v += xor_lanes<8>(v);
+  if constexpr (T >= 32) v += xor_lanes<16>(v);
+  if constexpr (T >= 64) v += xor_lanes<32>(v);
   if constexpr (T > 64) {
     if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -204,7 +202,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(NormParams 
 }
 
 #define EXL3_NORM_T(M, WHOLE, XB, RB)                                                                \
-  M(WHOLE, XB, RB, 16, 1, false) M(WHOLE, XB, RB, 64, 1, false) M(WHOLE, XB, RB, 256, 1, false)      \
+  M(WHOLE, XB, RB, 8, 1, false) M(WHOLE, XB, RB, 16, 1, false) M(WHOLE, XB, RB, 32, 1, false)        \
+  M(WHOLE, XB, RB, 64, 1, false) M(WHOLE, XB, RB, 256, 1, false)                                     \
   M(WHOLE, XB, RB, 256, 2, false) M(WHOLE, XB, RB, 256, 4, false) M(WHOLE, XB, RB, 1024, 2, false)   \
   M(WHOLE, XB, RB, 1024, 4, false) M(WHOLE, XB, RB, 1024, 4, true)
 #define EXL3_NORM_B(M, WHOLE)                                                                        \
@@ -233,7 +232,9 @@ void launch(const NormParams& p, hipStream_t s) {
 template <bool WHOLE, int XB, int RB>
 void launch(const NormParams& p, hipStream_t s) {
   const int w = p.width;
-  w <= 128     ? launch<WHOLE, XB, RB, 16, 1>(p, s)
+  w <= 64      ? launch<WHOLE, XB, RB, 8, 1>(p, s)
+  : w <= 128   ? launch<WHOLE, XB, RB, 16, 1>(p, s)
+  : w <= 256   ? launch<WHOLE, XB, RB, 32, 1>(p, s)
   : w <= 512   ? launch<WHOLE, XB, RB, 64, 1>(p, s)
   : w <= 2048  ? launch<WHOLE, XB, RB, 256, 1>(p, s)
   : w <= 4096  ? launch<WHOLE, XB, RB, 256, 2>(p, s)
@@ -294,7 +295,7 @@ extern "C" int exl3_rms_norm(const void* x, int32_t x_type, int64_t tokens, int3
       (total && (!in_place(total, residual_type, ts, x, x_type, xs) ||
                  !in_place(total, residual_type, ts, residual, residual_type, rs))))
     return fail(EXL3_EINVAL, "a norm in place keeps the type and the stride");
-  const int64_t per = width <= 128 ? 16 : width <= 512 ? 4 : 1, most = width > 8192 ? kMostBlocks / 4 : kMostBlocks;
+  const int64_t per = width <= 64 ? 32 : width <= 128 ? 16 : width <= 256 ? 8 : width <= 512 ? 4 : 1, most = width > 8192 ? kMostBlocks / 4 : kMostBlocks;
   if (tokens > INT64_MAX / need || (tokens * heads + per - 1) / per > most)
     return fail(EXL3_EUNSUPPORTED, "too many tokens: %lld", (long long)tokens);
   NormParams p{};

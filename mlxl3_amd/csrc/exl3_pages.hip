@@ -1,8 +1,8 @@
 // Pages of the paged cache copied (layout: exl3_kv.hpp): forked sequences' last pages, pools
 // that are compacted.
 //
-// One launch copies up to 300 pairs of pages in up to 32 caches of one shape -- a model's layers --
-// named in the kernel's arguments, so that nothing is uploaded.  Where a pair copies its first
+// One launch copies some 200 to 400 pairs of pages in up to 64 caches of one shape -- a model's
+// layers -- named in the kernel's arguments, so that nothing is uploaded.  Where a pair copies its first
 // n slots only, a head's n slots are one run of its page (its scales n of every group's run).
 // Memory bounds it: every byte is read and written once, 16 at a time.  Measured, sources not in the
 // caches: 230 pages of 131 KB in 4 caches, 121 MB, 47 us, 5.1 TB/s read and written (a large copy: 5.1);
@@ -21,26 +21,28 @@
 
 namespace exl3 {
 
-constexpr int kMostCaches = 32, kMostPairs = 300;  // of a launch: 4.0 KB of arguments, as many as it takes
-constexpr int kUnits = 1024;                       // 16-byte units of a workgroup, four a thread
+constexpr int kWords = 504;      // of their pools and the pairs: 4 KB of arguments, as many as a launch takes
+constexpr int kUnits = 1024;     // 16-byte units of a workgroup, four a thread
 
 struct CopyParams {
-  uint8_t* keys[kMostCaches];
-  uint8_t* values[kMostCaches];
-  uint16_t* key_scales[kMostCaches];
-  uint16_t* value_scales[kMostCaches];
-  int32_t src[kMostPairs], dst[kMostPairs];
-  uint16_t slots[kMostPairs];
+  // the pools of every cache (keys, values and, where there are groups, the scales of both), the pages of
+  // every pair (low half: copied, high half: copied to), the slots of every pair, four a word
+  uint64_t words[kWords];
   int page_shift, kv_heads, row, groups;  // row: bytes of a cached head; groups: of scales, 0 without
+  int caches, parts;                      // parts: workgroups of a page's codes
 };
 
+// Pools are named by numbers, so that their memory has to be called global (else the compiler's accesses
+// wait for LDS too).
+typedef __attribute__((address_space(1))) u32x4 Unit;
+typedef __attribute__((address_space(1))) uint16_t Scale;
 // STREAM: past the caches (copies that they do not hold).
 template <bool STREAM>
-__device__ __forceinline__ u32x4 read16(const u32x4* p) {
+__device__ __forceinline__ u32x4 read16(const Unit* p) {
   return STREAM ? __builtin_nontemporal_load(p) : *p;
 }
 template <bool STREAM>
-__device__ __forceinline__ void write16(u32x4* p, u32x4 v) {
+__device__ __forceinline__ void write16(Unit* p, u32x4 v) {
   if constexpr (STREAM)
     __builtin_nontemporal_store(v, p);
   else
@@ -58,19 +60,20 @@ struct Divisor {
 // (in workgroups of their own: 48 forks in 16 8-bit caches 19 us, with the codes' ones 24).  A thread
 // has four 16-byte units, all loaded before the first is stored.
 template <bool STREAM>
-__global__ __launch_bounds__(256) void kv_copy_kernel(CopyParams p, int parts) {
-  const int pair = blockIdx.y, cache = blockIdx.z >> 1;
-  const bool value = blockIdx.z & 1;
-  const uint32_t page = 1u << p.page_shift, slots = p.slots[pair];
-  const int64_t src = p.src[pair], dst = p.dst[pair];
-  if ((int)blockIdx.x < parts) {
+__global__ __launch_bounds__(256) void kv_copy_kernel(CopyParams p) {
+  const int pair = blockIdx.y, cache = blockIdx.z >> 1, side = blockIdx.z & 1;
+  const int pools = p.groups ? 4 : 2, pages_at = p.caches * pools, slots_at = pages_at + gridDim.y;
+  const uint32_t page = 1u << p.page_shift, slots = (uint32_t)(p.words[slots_at + pair / 4] >> (16 * (pair % 4))) & 0xffff;
+  const uint64_t pages = p.words[pages_at + pair];
+  const int64_t src = (uint32_t)pages, dst = pages >> 32;
+  if ((int)blockIdx.x < p.parts) {
     // codes: the runs of all heads, `slots` slots each of 2^shift units, `page` slots apart
     const int shift = __builtin_ctz(p.row) - 4;
     const uint32_t units = (p.kv_heads * slots) << shift, first = blockIdx.x * kUnits + threadIdx.x;
     const int64_t whole = ((int64_t)p.kv_heads * page) << shift;
-    u32x4* pool = (u32x4*)(value ? p.values[cache] : p.keys[cache]);
-    const u32x4* from = pool + src * whole;
-    u32x4* to = pool + dst * whole;
+    Unit* pool = (Unit*)p.words[cache * pools + side];
+    const Unit* from = pool + src * whole;
+    Unit* to = pool + dst * whole;
     const Divisor by(slots);
     u32x4 v[4];
     uint32_t at[4];
@@ -86,24 +89,24 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(CopyParams p, int parts) {
     return;
   }
   // scales: the runs of all groups, eight slots at a time, the last ones of a run one by one
-  uint16_t* pool = value ? p.value_scales[cache] : p.key_scales[cache];
+  Scale* pool = (Scale*)p.words[cache * pools + 2 + side];
   const uint32_t runs = p.kv_heads * p.groups, pieces = (slots + 7) / 8;
-  const uint16_t* from = pool + ((src * runs) << p.page_shift);
-  uint16_t* to = pool + ((dst * runs) << p.page_shift);
+  const Scale* from = pool + ((src * runs) << p.page_shift);
+  Scale* to = pool + ((dst * runs) << p.page_shift);
   const Divisor by(pieces);
   for (int i = 0; i < 4; ++i) {
-    const uint32_t u = (blockIdx.x - parts) * kUnits + i * 256 + threadIdx.x;
+    const uint32_t u = (blockIdx.x - p.parts) * kUnits + i * 256 + threadIdx.x;
     if (u >= runs * pieces) return;
     const uint32_t run = by.quotient(u), slot = (u - run * pieces) * 8, at = (run << p.page_shift) + slot;
     if (slot + 8 <= slots) {
-      write16<STREAM>((u32x4*)(to + at), read16<STREAM>((const u32x4*)(from + at)));
+      write16<STREAM>((Unit*)(to + at), read16<STREAM>((const Unit*)(from + at)));
     } else {
       for (uint32_t e = 0; e < slots - slot; ++e) to[at + e] = from[at + e];
     }
   }
 }
-template __global__ void kv_copy_kernel<false>(CopyParams, int);
-template __global__ void kv_copy_kernel<true>(CopyParams, int);
+template __global__ void kv_copy_kernel<false>(CopyParams);
+template __global__ void kv_copy_kernel<true>(CopyParams);
 
 }  // namespace exl3
 
@@ -111,9 +114,10 @@ using namespace exl3;
 
 #ifndef __HIP_DEVICE_COMPILE__
 
+constexpr int kMostCaches = 64;  // of a launch, twice of a grid's z
 constexpr double kCached = 64.0 * 1048576;  // bytes copied beyond which a copy goes past the caches
 
-static_assert(sizeof(CopyParams) + 8 <= 4096, "a launch takes 4 KB of arguments");
+static_assert(sizeof(CopyParams) <= 4096, "a launch takes 4 KB of arguments");
 
 // What a copy of pages refuses, before anything is launched: every page is in all pools, none is
 // written twice or written and read.
@@ -203,30 +207,40 @@ extern "C" int exl3_kv_copy_pages(const exl3_kv_cache* const* caches, int32_t co
       for (; next < count && n < kMostCaches; ++next) {
         const KvCacheView& v = caches[next]->view;
         if (!alike(v, c)) continue;
-        p.keys[n] = v.k;
-        p.values[n] = v.v;
-        p.key_scales[n] = v.ks;
-        p.value_scales[n++] = v.vs;
+        uint64_t* pools = p.words + (coded ? 4 : 2) * n++;
+        pools[0] = (uintptr_t)v.k;
+        pools[1] = (uintptr_t)v.v;
+        if (coded) {
+          pools[2] = (uintptr_t)v.ks;
+          pools[3] = (uintptr_t)v.vs;
+        }
       }
       if (n == 0) break;
+      p.caches = n;
+      uint64_t* words = p.words + (coded ? 4 : 2) * n;
+      const int room = (int)(p.words + kWords - words) * 4 / 5;
       for (int64_t at = 0; at < pairs;) {
+        uint16_t filled_slots[kWords];
         int m = 0, most = 0;
-        for (; at < pairs && m < kMostPairs; ++at) {
+        for (; at < pairs && m < room; ++at) {
           const int used = slots ? slots[at] : 1 << c.page_shift;
           if (used == 0) continue;
-          p.src[m] = src[at];
-          p.dst[m] = dst[at];
-          p.slots[m++] = (uint16_t)used;
+          words[m] = (uint64_t)(uint32_t)src[at] | (uint64_t)(uint32_t)dst[at] << 32;
+          filled_slots[m++] = (uint16_t)used;
           most = std::max(most, used);
         }
         if (m == 0) continue;
+        for (int i = 0; i < m; ++i) {
+          uint64_t& four = words[m + i / 4];
+          four = (i % 4 ? four : 0) | (uint64_t)filled_slots[i] << (16 * (i % 4));
+        }
         const int codes = most * p.kv_heads * (p.row / 16), scales = p.kv_heads * p.groups * ((most + 7) / 8);
-        const int parts = (codes + kUnits - 1) / kUnits;
-        const dim3 grid((unsigned)(parts + (scales + kUnits - 1) / kUnits), (unsigned)m, 2u * (unsigned)n);
+        p.parts = (codes + kUnits - 1) / kUnits;
+        const dim3 grid((unsigned)(p.parts + (scales + kUnits - 1) / kUnits), (unsigned)m, 2u * (unsigned)n);
         if (stream_past)
-          hipLaunchKernelGGL(kv_copy_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, p, parts);
+          hipLaunchKernelGGL(kv_copy_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, p);
         else
-          hipLaunchKernelGGL(kv_copy_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, p, parts);
+          hipLaunchKernelGGL(kv_copy_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, p);
         if (int rc = check_launch("KV page copy")) return rc;
       }
     }
