@@ -210,10 +210,13 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
     p.prefix = causal ? scores->prefix : nullptr;
     // the factors of kCapped and kEarly far inside f32's range, else one step after the other
     const float rate = cap != 0.0f ? 2.0f * kLog2e / p.cap2 * scale2 : 0.0f;
+    const bool near = scale2 >= 0x1p-20f && scale2 <= 0x1p20f;
     if (cap != 0.0f)
-      shaped = p.cap2 <= kLargeCap && rate >= 0x1p-100f && rate <= 0x1p100f ? kCapped : kLate;
-    else if (p.slopes || p.prefix)
-      shaped = scale2 >= 0x1p-20f && scale2 <= 0x1p20f ? kEarly : kLate;
+      shaped = p.cap2 > kLargeCap || !(rate >= 0x1p-100f && rate <= 0x1p100f) ? kLate : p.slopes ? kBoth : kCapped;
+    else if (p.slopes)
+      shaped = near ? kEarly : kLate;
+    else if (p.prefix)
+      shaped = near ? kSeen : kLate;
   }
   if (batch->max_q < 1) return fail(EXL3_EINVAL, "max_q must be positive");
   if (batch->seqs > 65535)
@@ -258,10 +261,12 @@ static int attention_call(const exl3_kv_cache* cache, const exl3_kv_batch* batch
   const int D = p.cache.head_dim;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = launch_gate("attention")) return rc;
-  shaped == kPlain    ? launch_attention<kPlain>(p, sh, s)
-  : shaped == kEarly  ? launch_attention_early(p, sh, s)
-  : shaped == kCapped ? launch_attention_capped(p, sh, s)
-                      : launch_attention_late(p, sh, s);
+  switch (shaped) {
+    case kPlain: launch_attention<kPlain>(p, sh, s); break;
+    case kSeen: case kEarly: launch_attention_early(p, sh, shaped == kSeen, s); break;
+    case kCapped: case kBoth: launch_attention_capped(p, sh, shaped == kBoth, s); break;
+    default: launch_attention_late(p, sh, s);
+  }
   if (int rc = check_launch("attention")) return rc;
   if (!sh.slots) return EXL3_OK;
   if (int rc = launch_gate("attention join")) return rc;

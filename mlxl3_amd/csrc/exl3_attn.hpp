@@ -6,8 +6,9 @@
 
 namespace exl3 {
 
-// What becomes of scores (the kernels' S; below).
-enum : int { kPlain = 0, kEarly = 1, kCapped = 2, kLate = 3 };
+// What becomes of scores (the kernels' S; below).  For few rows, which memory bounds, kEarly does for
+// kSeen and kCapped for kBoth.
+enum : int { kPlain = 0, kEarly = 1, kCapped = 2, kLate = 3, kSeen = 4, kBoth = 5 };
 
 struct AttnParams {
   KvCacheView cache;
@@ -337,9 +338,9 @@ __device__ __forceinline__ float slack_at(float m, float slack) {
 // Capped it is cap2 tanh(u), u = x / cap2: a score z becomes cap tanh(z / cap).  tanh(u) = 1 - 2 / (1 +
 // e^2u), and of all scores of a row softmax takes off what it likes: less cap2 a capped score is
 //   2 cap2 c,  c = -1 / (1 + 2^(rate x)),  rate = 2 log2(e) / cap2.
-// So a call with a cap (kCapped) puts c where the product was, in four instructions, and goes on as a
-// plain one whose scale is 2 cap2.  c is off by 2^-23 or so, the score by cap2 times that, 1e-5
-// under a cap of 50.  (tanh's polynomials in u^2 up to |u| = 1, in tiles where no score is beyond, are
+// So a call with a cap (kCapped, with a bias kBoth) puts c where the product was, in four instructions,
+// and goes on as a plain one whose scale is 2 cap2.  c is off by 2^-23 or so, the score by cap2 times
+// that, 1e-5 under a cap of 50.  (tanh's polynomials in u^2 up to |u| = 1, in tiles where no score is beyond, are
 // as many instructions or more and a maximum: 2048 rows over 8192 bf16 tokens 335 us for 304, plain 256.)
 //
 // The bias by distance takes slope2 = slope log2(e) times it off the score.  Without a cap the sums of the
@@ -349,6 +350,8 @@ __device__ __forceinline__ float slack_at(float m, float slack) {
 // Caps above 256, where the error above is too much for small scores (|u| < 1/4 takes tanh's series there,
 // and nothing is taken off), and factors whose quotients may leave f32's range go one step
 // after the other (kLate): times the scale, capped, biased.
+//
+// A prefix only moves the end of what a row sees (kSeen: without a cap and a bias).
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLargeCap = 256.0f * kLog2e;
 __device__ __forceinline__ float squashed(float x, float rate) {

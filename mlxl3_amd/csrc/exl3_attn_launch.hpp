@@ -64,7 +64,7 @@ template <int S, int FMT, typename T, int PARTS>
 void launch(const AttnParams& p, const AttnShape& sh, hipStream_t s) {
   const int d = p.cache.head_dim, tiles = (int)sh.tiles;
   if (sh.few)
-    launch_few<S, FMT, T, PARTS>(p, sh.rows, s);
+    launch_few<S == kSeen ? kEarly : S == kBoth ? kCapped : S, FMT, T, PARTS>(p, sh.rows, s);
   else
     d == 64 ? launch_many<S, FMT, T, PARTS, 64>(p, tiles, s) : d == 128 ? launch_many<S, FMT, T, PARTS, 128>(p, tiles, s)
                                                                      : launch_many<S, FMT, T, PARTS, 256>(p, tiles, s);
@@ -84,9 +84,9 @@ void launch_attention(const AttnParams& p, const AttnShape& sh, hipStream_t s) {
 
 #endif  // __HIP_DEVICE_COMPILE__
 
-// launch_attention<kEarly>, <kCapped> and <kLate>, of the other translation units.
-void launch_attention_early(const AttnParams& p, const AttnShape& sh, hipStream_t s);
-void launch_attention_capped(const AttnParams& p, const AttnShape& sh, hipStream_t s);
+// launch_attention<kEarly> and <kSeen>, <kCapped> and <kBoth>, <kLate>, of the other translation units.
+void launch_attention_early(const AttnParams& p, const AttnShape& sh, bool seen, hipStream_t s);
+void launch_attention_capped(const AttnParams& p, const AttnShape& sh, bool both, hipStream_t s);
 void launch_attention_late(const AttnParams& p, const AttnShape& sh, hipStream_t s);
 
 }  // namespace exl3

@@ -29,9 +29,11 @@
 // of 64 733 to 757, 610 / 431, 514 / 370 (half the products per exponential); of 256 630, 475 / 348,
 // 486 / 337 (one workgroup a CU: its registers).  Six prompts of 496 to 1500 tokens, heads of 64,
 // window 512: 46 us, 432 TFLOP/s, masked tiles and two rounds of short workgroups.
-// Shaped, 2048 tokens over 8192, us (plain 256 to 285): bf16 heads of 128 biased 250 to 257, capped 304 to
-// 324, both 317, with a prefix only 262 to 277; f16 heads of 64 (159) 161, 217 to 228, 242, 169;
-// bf16 heads of 256 (742) 762, 846, 827, 809; over 8 bits (335) 294, 366, 366, 327.
+// Shaped, 2048 tokens over 8192, us (plain 259 to 277): bf16 heads of 128 biased 248 to 257, capped 298 to
+// 314, both 312, with a prefix only 259 to 262; f16 heads of 64 (162) 164, 216 to 222, 235, 161;
+// bf16 heads of 256 (745) 760, 777 to 830, 813, 776; over 8 bits (337) 295, 363, 364, 307.  Kernels that
+// looked for a bias under each cap and started a prefix' sums from a bias of zero: capped 318, heads of
+// 64 229, of 256 845; with a prefix only 267, 173, 808.
 // Where rows are done one by one (below, values that are not finite and some rows do not see) a
 // workgroup takes its rows times its tokens: one NaN in the newest of 8192 tokens makes 2048 rows'
 // 0.29 ms 268 ms.
@@ -222,11 +224,12 @@ void attn_many_kernel(AttnParams p, int tiles) {
     for (int s = 0; s < D / 16; ++s) q[s] = query_operand<FMT == KV_Q4 ? KV_Q8 : FMT, T, kScaled>(raw[s], factor);
   }
   // of shaped scores: the row's bias, its position less this lane's first token of a tile
-  float slope2 = S ? slope_of(p, kvh * p.group + mine % p.group) : 0.0f;
+  constexpr bool kCap = S == kCapped || S == kBoth;
+  float slope2 = S == kEarly || S == kBoth || S == kLate ? slope_of(p, kvh * p.group + mine % p.group) : 0.0f;
   const int at = w.first + mine / p.group - 4 * h, nearest = w.first + wrow / p.group;
-  const float rate = S == kCapped ? cap_rate(p, scale2) : 0.0f;
-  if (S == kCapped) scale2 = 2.0f * p.cap2;
-  if (S == kEarly || S == kCapped) slope2 /= scale2;
+  const float rate = kCap ? cap_rate(p, scale2) : 0.0f;
+  if (kCap) scale2 = 2.0f * p.cap2;
+  if (S == kEarly || S == kBoth) slope2 /= scale2;
   float16v o[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) o[dt] = float16v{};
@@ -240,7 +243,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
   // biased scores mostly rise towards the row's own position: newest tiles first, so that the running
   // maximum rarely moves (2048 biased rows over 8192 tokens, us: heads of 128 the other way 279, this one
   // 250; of 64 183 and 159; of 256 993 and 755)
-  constexpr bool kBack = S != kPlain;
+  constexpr bool kBack = S == kEarly || S == kBoth || S == kLate;
   const int first = kBack && t0 < t1 ? t0 + (t1 - t0 - 1) / TK * TK : t0, step = kBack ? -TK : TK;
   auto entry_at = [&](int t) { return table_entry(p, w, kBack ? max((t + off) & ~15, 0) : (t + off) & ~15, t1); };
   auto page_at = [&](int entry, int t) { return page_ok(p, entry, (t + off) & ~15, t1); };
@@ -344,15 +347,16 @@ void attn_many_kernel(AttnParams p, int tiles) {
       for (int i = 0; i < DT; ++i) vf[i] = value(i);
       pin();
       __builtin_amdgcn_s_setprio(0);
-      if constexpr (S == kCapped) {
+      if constexpr (kCap) {
 #pragma unroll
         for (int i = 0; i < 16 * NT; ++i) s[i / 16][i % 16] = squashed(s[i / 16][i % 16], rate);
-        if (p.slopes) {
-          const float away = (float)(at - t);
+      }
+      if constexpr (S == kBoth) {
+        pin();  // caps first: both at once 320 us for 311 (2048 rows over 8192, heads of 128), 240 for 235 (of 64)
+        const float away = (float)(at - t);
 #pragma unroll
-          for (int i = 0; i < 16 * NT; ++i)
-            s[i / 16][i % 16] = biased(s[i / 16][i % 16], slope2, away - (float)(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4));
-        }
+        for (int i = 0; i < 16 * NT; ++i)
+          s[i / 16][i % 16] = biased(s[i / 16][i % 16], slope2, away - (float)(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4));
       }
       if constexpr (S == kLate) {
         const float away = (float)(at - t);

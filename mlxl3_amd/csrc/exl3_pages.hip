@@ -114,7 +114,7 @@ using namespace exl3;
 
 #ifndef __HIP_DEVICE_COMPILE__
 
-constexpr int kMostCaches = 64;  // of a launch, twice of a grid's z
+constexpr int kMostCaches = 64;  // of a launch: keys and values of each are a grid's z
 constexpr double kCached = 64.0 * 1048576;  // bytes copied beyond which a copy goes past the caches
 
 static_assert(sizeof(CopyParams) <= 4096, "a launch takes 4 KB of arguments");

@@ -154,6 +154,8 @@ def test_prefixes(prefix, window, new):
     ([1], [20000], dict(softcap=50.0)), ([1], [9001], dict(slopes=geometric(8))), ([2, 1], [5000, 300], dict(softcap=20.0, slopes=geometric(8))),
     ([1] * 5, [9000, 200, 1, 64, 3000], dict(slopes=geometric(8) / 50)), ([70], [3000], dict(softcap=50.0, prefix=[2990])),
     ([200, 130], [2500, 130], dict(slopes=geometric(8) / 100, prefix=[100, 70], window=900)),
+    ([60, 70], [700, 3000], dict(prefix=[650, 2990])), ([1, 2], [9000, 700], dict(prefix=[0, 700])),
+    ([90], [2800], dict(softcap=20.0, slopes=geometric(8) / 30)),
 ])
 def test_long_contexts(bits, cdtype, dtype, new, lens, kw):
     """Tokens split over workgroups, evenly and by the batch's sum, and joined."""
