@@ -49,7 +49,8 @@ __device__ __forceinline__ void write16(Unit* p, u32x4 v) {
     *p = v;
 }
 
-// n / d for n below 2^22 and d up to 1024, by a multiplication (once: 1, off by less than d 2^-32).
+// n / d for n below 2^22 and d up to 1024, by a multiplication: inv is 2^32 / d rounded up, off by less
+// than 1, the quotient by less than n 2^-32 < 1 / d.  (2^32 / 1 is past 32 bits: d of 1 is no division.)
 struct Divisor {
   uint32_t d, inv;
   __device__ __forceinline__ explicit Divisor(uint32_t v) : d(v), inv(0xffffffffu / v + 1) {}

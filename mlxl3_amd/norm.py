@@ -57,8 +57,8 @@ def rms_norm(x, weight=None, eps: float = 1e-6, residual=None, total=None, out=N
     x_code = _code(x, "x")
     shape, device = x.shape, x.device
     width = shape[-1] if shape else 0
-    if width < 1:
-        raise Exl3Error(-1, f"norms take rows of at least one value, got shape {tuple(shape)}")
+    if not 0 < width < 2**31:
+        raise Exl3Error(-1, f"norms take rows of at least one value and fewer than 2^31, got shape {tuple(shape)}")
     if type(eps) is not float:
         try:
             eps = float(eps)
@@ -109,6 +109,8 @@ def rms_norm(x, weight=None, eps: float = 1e-6, residual=None, total=None, out=N
     heads, xs, rs, ts, ys = 1, width, width, width, width
     if laid is not None:
         heads = max(1, max(laid)[0])  # those that have gaps have x's
+        if heads >= 2**31:
+            raise Exl3Error(-1, f"norms take fewer than 2^31 heads, got {heads}")
         xs, rs, ts, ys = (stride if h else stride * heads for h, stride in laid)
     _launch(
         device, load_library().exl3_rms_norm, x.data_ptr(), x_code, count // (width * heads), heads, width, xs,

@@ -223,3 +223,16 @@ def test_refusals():
             mlxl3_amd.rms_norm(bad)
     with pytest.raises(err, match="two outputs"):
         mlxl3_amd.rms_norm(x, residual=x.clone(), out=(o := x.clone()), total=o)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Not cut to 32 bits: 2^32 + 128 values are no rows of 128, 2^32 + 1 heads not one."""
+    for make, msg in (
+        (lambda: torch.empty(1, 2**32 + 128, dtype=F16, device="cuda"), "fewer than 2\\^31, got shape"),
+        (lambda: torch.empty(2, 2**32 + 2, 1, dtype=F16, device="cuda")[:, 1:], "fewer than 2\\^31 heads"),
+    ):
+        x = make()
+        with pytest.raises(mlxl3_amd.Exl3Error, match=msg):
+            mlxl3_amd.rms_norm(x, out=x)  # in place: x stays the only one of its size
+        del x
+        torch.cuda.empty_cache()
