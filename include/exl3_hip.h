@@ -383,11 +383,11 @@ int exl3_attention(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const
 
 /* exl3_attention with shaped scores.  A score z = scale q.k becomes softcap tanh(z / softcap)
  * where softcap is not 0 (2^-64 to 2^64), then slopes[head] times the distance of the
- * row's position and the token's is taken off it (slopes finite, and counted up to 2^32; the sum of
- * a score and a bias finite too); and with causal != 0 every row sees the first prefix[b] tokens of its sequence beside
- * those up to its own position (t < kv_lens[b] and the window hold for them as for others).
- * slopes (f32 [heads]) and prefix (int32 [seqs]) are device memory, read at every call, and may
- * be NULL; so may `scores`. */
+ * row's position and the token's is taken off it (slopes finite, and counted up to 2^32; the sum
+ * of a score and a bias finite too); and with causal != 0 every row sees the first prefix[b]
+ * tokens of its sequence beside those up to its own position (t < kv_lens[b] and the window hold
+ * for them as for others).  slopes (f32 [heads]) and prefix (int32 [seqs]) are device memory, read
+ * at every call, and may be NULL; so may `scores`. */
 typedef struct {
   float softcap;
   const float* slopes;

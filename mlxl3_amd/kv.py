@@ -423,7 +423,10 @@ def _scores(device, heads: int, seqs: int, softcap, slopes, prefix):
         _same(device, prefix, "prefix")
     if softcap == 0.0 and slopes is None and prefix is None:
         return None
-    return _ScoresC(softcap, _ptr(slopes), _ptr(prefix))
+    scores = _ScoresC(softcap, _ptr(slopes), _ptr(prefix))
+    if softcap != 0.0 and scores.softcap == 0.0:  # (what else is out of range the call refuses)
+        raise Exl3Error(-1, f"attention softcap must be 0 or 2^-64 to 2^64, got {softcap:g}")
+    return scores
 
 
 def attention(q, cache: KvCache, batch: KvBatch, scale: Optional[float] = None, causal: bool = True,

@@ -70,3 +70,9 @@ def test_the_block_refuses_before_its_first_launch():
         for p in made:
             lib.exl3_linear_destroy(p)
         lib.exl3_kv_cache_destroy(h)
+
+
+@pytest.mark.parametrize("cap", [1e-60, -1e-60, 5e-324])
+def test_a_cap_that_f32_does_not_hold_is_no_call_without_one(cap):
+    with pytest.raises(mlxl3_amd.Exl3Error, match="softcap must be 0 or 2\\^-64 to 2\\^64"):
+        kv._scores(None, 4, 1, cap, None, None)
