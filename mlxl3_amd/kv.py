@@ -183,6 +183,13 @@ class KvBatch:
         return sized[1]
 
 
+def _ask(batch) -> None:
+    """Whether the batch's pages are its sequences' to append to: KvPages knows of those that it made."""
+    asked = getattr(batch, "_asked", None)
+    if asked is not None:
+        asked()
+
+
 # rope_scaling by type: the keys it needs, and those it may have
 _SCALING = {
     "default": (set(), set()),
@@ -377,6 +384,7 @@ class KvCache:
         _same(device, batch.kv_lens, "batch")
         if rope is not None:
             _same(device, rope.inv_freq, "rope")
+        _ask(batch)
         _launch(device, load_library().exl3_kv_append, self._handle, batch._ref, k.data_ptr(), k.stride(0),
                 v.data_ptr(), v.stride(0), _FLOATS[k.dtype], k.shape[0], None if rope is None else rope._ref)
 
@@ -553,6 +561,7 @@ class Exl3Attention:
             _same(device, self, "projections")
         if self.rope is not None:
             _same(device, self.rope.inv_freq, "rope")
+        _ask(batch)
         shape = None
         if self.slopes is not None or prefix is not None or self.softcap != 0.0:
             shape = _scores(device, self.q.out_features // cache.head_dim, batch.seqs, self.softcap, self.slopes, prefix)

@@ -51,14 +51,32 @@ class _Held:
         self.pages, self.tokens = pages, tokens
 
 
+class _Appended:
+    """What an append of a batch is asked: the pages that it writes, (sequence, number of the first
+    page, pages), and the state of the bookkeeping in which they were found to be right."""
+
+    __slots__ = ("owner", "parts", "right")
+
+    def __init__(self, owner, parts):
+        self.owner, self.parts, self.right = owner, parts, None
+
+    def __call__(self) -> None:
+        if self.right != self.owner._changes:  # asked once, not by every layer
+            self.right = self.owner._check_appended(self.parts)
+
+
 class KvPages:
     """The pages of `caches`, one :class:`KvCache` per layer (as many pages of as many tokens each,
     on one device), handed out to sequences, which are named by numbers.
 
-    A sequence's pages are the same in every cache.  :meth:`fork` shares them; a shared page that
-    is only partly filled is copied before :meth:`grow` lets it be written, so that what appending
-    writes belongs to one sequence.  Copies go to the current stream, like the calls that write
-    and read the caches.  Methods may be called from any thread."""
+    A sequence's pages are the same in every cache.  Its tokens are those that it has room for:
+    :meth:`new` and :meth:`grow` count them before they are appended, and nothing here knows whether
+    they were.  :meth:`fork` shares the pages; a shared page that is only partly filled is copied before
+    :meth:`grow` makes room in it, so that room belongs to one sequence.  Room that was made before a
+    fork is in shared pages: the oldest of the sequences that share a page fills it, once, for all of
+    them and before one of them grows (a copy takes what is there), and an append through another one's
+    :meth:`batch` is refused.  Copies go to the current stream, like the calls that write and read the
+    caches.  Methods may be called from any thread."""
 
     def __init__(self, caches: Sequence[KvCache]):
         caches = [caches] if isinstance(caches, KvCache) else list(caches)
@@ -77,6 +95,7 @@ class KvPages:
         self._free = list(range(self.pages))  # a heap: the first free page is taken first
         self._held: dict = {}
         self._next = 0
+        self._changes = 0  # of which pages belong to whom
         self._lock = threading.RLock()
 
     # -- copies ---------------------------------------------------------------
@@ -170,6 +189,7 @@ class KvPages:
                 at += n
             if src:
                 self.copy(src, dst, slots)
+            self._changes += 1
             for _ in taken:
                 heapq.heappop(self._free)
             at = 0
@@ -182,9 +202,11 @@ class KvPages:
                 held.tokens, at = total, at + n
 
     def fork(self, seq) -> int:
-        """A new sequence with the tokens of `seq`, whose pages it shares."""
+        """A new sequence with the tokens of `seq`, whose pages it shares: append those that there is
+        room for first."""
         with self._lock:
             held = self._sequence(seq)
+            self._changes += 1
             for p in held.pages:
                 self._uses[p] += 1
             self._held[self._next] = _Held(list(held.pages), held.tokens)
@@ -199,6 +221,7 @@ class KvPages:
             if not 0 <= tokens <= held.tokens:
                 raise Exl3Error(-1, f"{tokens} of {held.tokens} tokens kept")
             keep = -(-tokens // self.page_tokens)
+            self._changes += 1
             self._drop(held.pages[keep:])
             del held.pages[keep:]
             held.tokens = tokens
@@ -207,6 +230,7 @@ class KvPages:
         """Ends a sequence; its pages that no other one shares are free."""
         with self._lock:
             self._drop(self._sequence(seq).pages)
+            self._changes += 1
             del self._held[seq]
 
     def _drop(self, pages) -> None:
@@ -217,7 +241,8 @@ class KvPages:
 
     def compact(self) -> int:
         """Moves pages to the front of the pool, so that the pages in use are its first ones;
-        returns how many moved.  Batches made before name the old ones."""
+        returns how many moved.  Batches made before name the old ones; nothing is appended through
+        them."""
         with self._lock:
             used = self.pages - len(self._free)
             src = [p for p in range(used, self.pages) if self._uses[p]]
@@ -230,6 +255,7 @@ class KvPages:
                     if p in filled:
                         filled[p] = max(filled[p], min(page, held.tokens - i * page))
             self.copy(src, dst, [filled[p] for p in src])
+            self._changes += 1
             to = dict(zip(src, dst))
             for held in self._held.values():
                 held.pages = [to.get(p, p) for p in held.pages]
@@ -240,7 +266,10 @@ class KvPages:
 
     def batch(self, seqs, new=1, max_kv: Optional[int] = None) -> KvBatch:
         """The :class:`KvBatch` of a call with the `new` newest tokens (a number, or one per
-        sequence) of each of the sequences `seqs`."""
+        sequence) of each of the sequences `seqs`, to read or to append them.  An append through it
+        asks whether their pages are the sequences' to write, as they are then.  A captured graph asks
+        at its capture, and nobody looks at what the program writes to the batch's tensors: one that
+        makes room ahead and captures a step sets kv_lens to the tokens of each replay."""
         torch = _torch()
         with self._lock:
             seqs = _several(seqs, "sequences")
@@ -256,8 +285,29 @@ class KvPages:
             wide = max(1, max(len(h.pages) for h in held))
             rows = [p for h in held for p in h.pages + [0] * (wide - len(h.pages))]
             lens = [h.tokens for h in held]
+            page = self.page_tokens
+            parts = [(s, (h.tokens - n) // page, h.pages[(h.tokens - n) // page :]) for s, n, h in zip(seqs, new, held) if n]
         # one transfer: starts, lengths, table
         both = torch.frombuffer(_ints(starts + lens + rows, "tokens"), dtype=torch.int32).to(self.device)
         n = len(seqs)
-        return KvBatch(both[: n + 1], both[n + 1 : 2 * n + 1], both[2 * n + 1 :].view(n, wide), max_q=max(1, max(new)),
-                       max_kv=max(lens) if max_kv is None else max_kv)
+        batch = KvBatch(both[: n + 1], both[n + 1 : 2 * n + 1], both[2 * n + 1 :].view(n, wide), max_q=max(1, max(new)),
+                        max_kv=max(lens) if max_kv is None else max_kv)
+        batch._asked = _Appended(self, parts)
+        return batch
+
+    def _check_appended(self, parts) -> int:
+        """Refuses an append to `parts` (:class:`_Appended`) that would write what another sequence
+        has, or a slot twice; returns the state that it was asked in."""
+        with self._lock:
+            if len({seq for seq, _, _ in parts}) != len(parts):
+                raise Exl3Error(-1, "a sequence whose tokens are appended is listed twice")
+            for seq, first, pages in parts:
+                held = self._held.get(seq)
+                if held is None or held.pages[first : first + len(pages)] != pages:
+                    raise Exl3Error(-1, f"a batch that was made before the pages of sequence {seq} changed")
+                for i, p in enumerate(pages, first):
+                    # (a shared page has one place in all that share it; the oldest come first)
+                    if self._uses[p] > 1 and seq != next(
+                            s for s, h in self._held.items() if i < len(h.pages) and h.pages[i] == p):
+                        raise Exl3Error(-1, f"page {p} is shared: an older sequence than {seq} appends to it")
+            return self._changes
