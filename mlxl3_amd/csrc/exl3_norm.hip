@@ -297,7 +297,7 @@ extern "C" int exl3_rms_norm(const void* x, int32_t x_type, int64_t tokens, int3
     return fail(EXL3_EINVAL, "a norm in place keeps the type and the stride");
   const int64_t per = width <= 64 ? 32 : width <= 128 ? 16 : width <= 256 ? 8 : width <= 512 ? 4 : 1;
   const int64_t most = width > 8192 ? kMostBlocks / 4 : kMostBlocks;
-  if (tokens > INT64_MAX / need || (tokens * heads + per - 1) / per > most)
+  if (tokens > INT64_MAX / need || tokens * heads > most * per)
     return fail(EXL3_EUNSUPPORTED, "too many tokens: %lld", (long long)tokens);
   NormParams p{};
   p.x = x;
