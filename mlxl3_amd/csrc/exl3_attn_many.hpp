@@ -283,7 +283,7 @@ void attn_many_kernel(AttnParams p, int tiles) {
 #pragma unroll
   for (int st = 0; st < D / 16; ++st) asm volatile("" : "+v"(q[st]));
   int cur = 0;
-  for (int t = first; t < t1 && t >= t0; t += step, cur ^= 1) {
+  for (int t = first; t < t1 && (!kBack || t >= t0); t += step, cur ^= 1) {
     __syncthreads();
     const uint8_t* keys = lds + cur * F::kHalf;
     const uint8_t* values = keys + PARTS * F::kTile;
