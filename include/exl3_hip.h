@@ -343,7 +343,8 @@ int exl3_rope(const exl3_rope_spec* rope, const void* x, int32_t x_type, int64_t
 /* Writes the batch's new tokens, k and v [tokens][kv_heads][head_dim] of
  * `type` (f16, bf16 or f32; token strides in elements), to their pages, keys
  * rotated first where rope is not NULL (as exl3_rope, but rounded only to the
- * cache's format).  A sequence is listed once. */
+ * cache's format).  A sequence is listed once, and no two have a new token in one
+ * slot (of a page that they share): a slot is written once. */
 int exl3_kv_append(const exl3_kv_cache* cache, const exl3_kv_batch* batch, const void* k,
                    int64_t k_stride, const void* v, int64_t v_stride, int32_t type,
                    int64_t tokens, const exl3_rope_spec* rope, void* stream);

@@ -29,11 +29,16 @@
 // of 64 733 to 757, 610 / 431, 514 / 370 (half the products per exponential); of 256 630, 475 / 348,
 // 486 / 337 (one workgroup a CU: its registers).  Six prompts of 496 to 1500 tokens, heads of 64,
 // window 512: 46 us, 432 TFLOP/s, masked tiles and two rounds of short workgroups.
-// Shaped, 2048 tokens over 8192, us (plain 259 to 277): bf16 heads of 128 biased 248 to 257, capped 298 to
-// 314, both 312, with a prefix only 259 to 262; f16 heads of 64 (162) 164, 216 to 222, 235, 161;
-// bf16 heads of 256 (745) 760, 777 to 830, 813, 776; over 8 bits (337) 295, 363, 364, 307.  Kernels that
-// looked for a bias under each cap and started a prefix' sums from a bias of zero: capped 318, heads of
-// 64 229, of 256 845; with a prefix only 267, 173, 808.
+// Shaped, 2048 tokens over 8192, us on two machines, plain | biased | capped | both | with a prefix only:
+//   bf16 heads of 128       239, 252 | 248, 260 | 288, 302 | 311, 326 | 240, 252
+//   f16 heads of 64         153, 159 | 161, 167 | 208, 222 | 232, 233 | 154, 159
+//   bf16 heads of 256       684, 678 | 750, 743 | 781, 746 | 806, 798 | 709, 720
+//   bf16 over 8 bits        294, 308 | 292, 306 | 350, 365 | 363, 376 | 295, 309
+//   f16 over 8 bits         504, 526 | 490, 512 | 554, 578 | 547, 570 | 507, 528
+//   bf16 over 4 bits        293, 305 | 292, 304 | 348, 364 | 362, 370 | 294, 305
+//   f16 over 4 bits         593, 603 | 606, 602 | 659, 662 | 682, 677 | 593, 601
+// Kernels that looked for a bias under each cap and started a prefix' sums from a bias of zero (another
+// machine): capped 318 for 310, heads of 64 229, of 256 845; with a prefix only 267 for 259, 173, 808.
 // Where rows are done one by one (below, values that are not finite and some rows do not see) a
 // workgroup takes its rows times its tokens: one NaN in the newest of 8192 tokens makes 2048 rows'
 // 0.29 ms 268 ms.

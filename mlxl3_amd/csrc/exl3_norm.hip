@@ -8,8 +8,8 @@
 // registers between its sum and its outputs: T threads hold 8 V values each, as few as do.  Rows of more
 // than 32768 values are read again instead (from the caches).
 //
-// Measured, inputs not in the caches: 4096 rows of 4096 bf16 values with an f32 residual 36 us, 5.6 TB/s
-// (a large copy: 5.1), of 8192 with half the rows 39, of 2048 with twice as many 35, of 1024 35; with a
+// Measured in a graph, inputs not in the caches: 4096 rows of 4096 bf16 values with an f32 residual 36 us,
+// 5.6 TB/s (a large copy: 5.1; a call from Python among others 39.9, of which the kernel 33.7), of 8192 with half the rows 39, of 2048 with twice as many 35, of 1024 35; with a
 // bf16 residual 26; 20000 tokens' 32 heads of 128 f16 values, without one, 65 us, 5.0 TB/s, 2001 tokens'
 // 9.5.  One row of 4096 takes 3.4, a launch and one round trip to memory.
 //

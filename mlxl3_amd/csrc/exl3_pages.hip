@@ -179,7 +179,7 @@ extern "C" int exl3_kv_copy_pages(const exl3_kv_cache* const* caches, int32_t co
     return a.format == b.format && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim;
   };
   if (int rc = launch_gate("KV page copy")) return rc;
-  // Copies that the caches (256 MB) do not hold with their source go past them.  Cold, us, 16-bit pages of
+  // Copies of more than 64 MB -- with their source half of what the caches hold -- go past them.  Cold, us, 16-bit pages of
   // four caches: 31 MB 14.3 past them, 18.5 through them; 63 MB 25.7, 30.8; 121 MB 47, 58.  But source and
   // copy are read again soon where a sequence is forked: 48 forks in 16 caches and the attention of all
   // layers after them 162 past them, 150 through them.

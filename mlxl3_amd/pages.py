@@ -266,10 +266,11 @@ class KvPages:
 
     def batch(self, seqs, new=1, max_kv: Optional[int] = None) -> KvBatch:
         """The :class:`KvBatch` of a call with the `new` newest tokens (a number, or one per
-        sequence) of each of the sequences `seqs`, to read or to append them.  An append through it
-        asks whether their pages are the sequences' to write, as they are then.  A captured graph asks
-        at its capture, and nobody looks at what the program writes to the batch's tensors: one that
-        makes room ahead and captures a step sets kv_lens to the tokens of each replay."""
+        sequence) of each of the sequences `seqs`, to read or to append them: made and uploaded anew by
+        every call, so one of a step is for all its layers.  An append through it asks whether their
+        pages are the sequences' to write, as they are then.  A captured graph asks at its capture, and
+        nobody looks at what the program writes to the batch's tensors: one that makes room ahead and
+        captures a step sets kv_lens to the tokens of each replay."""
         torch = _torch()
         with self._lock:
             seqs = _several(seqs, "sequences")
